@@ -2,7 +2,8 @@
 
 Modules mirror the reference's layout: ``kv_cache.storage`` (KVStorage),
 ``attn.metadata`` (AttentionMetadata) and ``attn.core`` (decode / mixed
-attention host functions, the ``inference::*`` ops and the Qwen2 drop-in).
+attention host functions, the ``inference::*`` ops and the Qwen2 drop-in);
+``kv_cache.quant`` and ``attn.quant`` are their forms for a cache held in 8 bits.
 The kernels live in ``libcie_paged.so`` (``csrc/``, C ABI in
 ``include/cie_paged_attention.h``), built by ``_build.build()``.
 """
@@ -29,5 +30,14 @@ from .attn.core import (  # noqa: F401
     reset_split_counters,
     use_triton_attention,
 )
+from .attn.quant import (  # noqa: F401
+    append_tokens_qkv_rope_q8,
+    decode_append_gqa_attention_q8,
+    decode_gqa_attention_q8,
+    decode_qkv_rope_gqa_attention_q8,
+    mixed_gqa_attention_q8,
+    mixed_plan_q8,
+)
 from .attn.metadata import AttentionMetadata  # noqa: F401
+from .kv_cache.quant import kv_append_decode_q8, kv_append_tokens_q8, kv_read_tokens_q8  # noqa: F401
 from .kv_cache.storage import KVStorage, kv_append_decode, kv_append_tokens  # noqa: F401

@@ -27,7 +27,8 @@ INCLUDE = os.path.join(REPO_DIR, "include")
 BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_NAME = "libcie_paged.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
-SOURCES = ("capi.hip", "kv_append.hip", "paged_decode.hip", "mixed_attention.hip")
+SOURCES = ("capi.hip", "kv_append.hip", "paged_decode.hip", "mixed_attention.hip", "q8_append.hip", "q8_decode.hip",
+           "q8_mixed.hip")
 # bench.py's measurement helpers: a library of their own, never linked into the product
 BENCH_SOURCES = ("bench/gather_probe.hip",)
 BENCH_LIB_PATH = os.path.join(PKG_DIR, "libcie_bench.so")

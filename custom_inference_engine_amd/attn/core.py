@@ -662,6 +662,9 @@ def _(k_cache, cu_seqlens, kv_lens, slot_ids, block_table, max_seqlen, total_T, 
     return k_cache.new_empty((n // 4,), dtype=torch.int32)
 
 
+from . import quant as _q8  # noqa: E402  (it takes this module's helpers, above)
+
+
 class TritonQwen2Attention(torch.nn.Module):
     """Drop-in for HF ``Qwen2Attention`` over the paged pool (attn/core.py:139-236).
 
@@ -713,24 +716,30 @@ class TritonQwen2Attention(torch.nn.Module):
         total_T = hidden_states.shape[1]
         hidden_shape = (1, total_T, -1, self.head_dim)
         keys, values = kv_manager.keys[self.layer_idx], kv_manager.values[self.layer_idx]
+        scales = kv_manager.scales[self.layer_idx] if getattr(kv_manager, "scales", None) is not None else None
         if self.fuse_qkv and self.fuse_rope and (self.fuse_append or not metadata.full_decode):
             qkv = torch.nn.functional.linear(hidden_states, self.qkv_weight, self.qkv_bias)
             cos, sin = position_embeddings
-            if metadata.full_decode:
+            if metadata.full_decode and scales is not None:
+                o = _q8.gqa_decode_qkv_rope_attention_q8_op(
+                    qkv, cos, sin, keys, values, scales, kv_manager.lens, metadata.slot_ids,
+                    kv_manager.block_table, self.num_heads, plan=getattr(metadata, "decode_plan", None),
+                )
+            elif metadata.full_decode:
                 o = gqa_decode_qkv_rope_attention_op(
                     qkv, cos, sin, keys, values, kv_manager.lens, metadata.slot_ids,
                     kv_manager.block_table, self.num_heads, plan=getattr(metadata, "decode_plan", None),
                 )
             else:
-                query_states = kv_append_tokens_qkv_rope_op(
-                    qkv, cos, sin, keys, values, metadata.pages, metadata.offsets, self.num_heads,
-                )
-                o = gqa_mixed_attention_op(
-                    query_states, keys, values,
-                    kv_lens=kv_manager.lens[metadata.slot_ids], max_seqlen=metadata.max_seqlen,
-                    cu_seqlens=metadata.cu_seqlens, slot_ids=metadata.slot_ids,
-                    block_table=kv_manager.block_table, plan=getattr(metadata, "mixed_plan", None),
-                )
+                if scales is not None:
+                    query_states = _q8.kv_append_tokens_qkv_rope_q8_op(
+                        qkv, cos, sin, keys, values, scales, metadata.pages, metadata.offsets, self.num_heads,
+                    )
+                else:
+                    query_states = kv_append_tokens_qkv_rope_op(
+                        qkv, cos, sin, keys, values, metadata.pages, metadata.offsets, self.num_heads,
+                    )
+                o = self._mixed(query_states, kv_manager, metadata, scales)
             attn_output = attn.o_proj(o.reshape(1, total_T, self.num_heads * self.head_dim))
             return attn_output, None
 
@@ -746,7 +755,12 @@ class TritonQwen2Attention(torch.nn.Module):
         query_states, key_states = apply_rotary_pos_emb(query_states, key_states, cos, sin,
                                                         unsqueeze_dim=2)
 
-        if metadata.full_decode and self.fuse_append:
+        if metadata.full_decode and self.fuse_append and scales is not None:
+            o = _q8.gqa_decode_append_attention_q8_op(
+                query_states, keys, values, scales, key_states, value_states, kv_manager.lens,
+                metadata.slot_ids, kv_manager.block_table, plan=getattr(metadata, "decode_plan", None),
+            )
+        elif metadata.full_decode and self.fuse_append:
             o = gqa_decode_append_attention_op(
                 query_states, kv_manager.keys[self.layer_idx], kv_manager.values[self.layer_idx],
                 key_states, value_states, kv_manager.lens, metadata.slot_ids, kv_manager.block_table,
@@ -754,22 +768,41 @@ class TritonQwen2Attention(torch.nn.Module):
             )
         elif metadata.full_decode:
             kv_manager.decode_update(self.layer_idx, metadata.slot_ids, key_states, value_states)
-            o = gqa_decode_attention_op(
-                query_states, kv_manager.keys[self.layer_idx], kv_manager.values[self.layer_idx],
-                kv_manager.lens[metadata.slot_ids] + 1,
-                slot_ids=metadata.slot_ids, block_table=kv_manager.block_table,
-            )
+            if scales is not None:
+                o = _q8.gqa_decode_attention_q8_op(
+                    query_states, keys, values, scales, kv_manager.lens[metadata.slot_ids] + 1,
+                    slot_ids=metadata.slot_ids, block_table=kv_manager.block_table,
+                )
+            else:
+                o = gqa_decode_attention_op(
+                    query_states, kv_manager.keys[self.layer_idx], kv_manager.values[self.layer_idx],
+                    kv_manager.lens[metadata.slot_ids] + 1,
+                    slot_ids=metadata.slot_ids, block_table=kv_manager.block_table,
+                )
         else:
             kv_manager.mixed_update(self.layer_idx, metadata.pages, metadata.offsets,
                                     key_states, value_states)
-            o = gqa_mixed_attention_op(
-                query_states, kv_manager.keys[self.layer_idx], kv_manager.values[self.layer_idx],
-                kv_lens=kv_manager.lens[metadata.slot_ids], max_seqlen=metadata.max_seqlen,
-                cu_seqlens=metadata.cu_seqlens, slot_ids=metadata.slot_ids,
-                block_table=kv_manager.block_table, plan=getattr(metadata, "mixed_plan", None),
-            )
+            o = self._mixed(query_states, kv_manager, metadata, scales)
         attn_output = attn.o_proj(o.reshape(1, total_T, self.num_heads * self.head_dim))
         return attn_output, None
+
+    def _mixed(self, query_states, kv_manager, metadata, scales):
+        """The step's varlen attention on this layer's pools (16-bit, or 8-bit with ``scales``)."""
+        keys, values = kv_manager.keys[self.layer_idx], kv_manager.values[self.layer_idx]
+        plan = getattr(metadata, "mixed_plan", None)
+        if scales is not None:
+            return _q8.gqa_mixed_attention_q8_op(
+                query_states, keys, values, scales,
+                kv_lens=kv_manager.lens[metadata.slot_ids], max_seqlen=metadata.max_seqlen,
+                cu_seqlens=metadata.cu_seqlens, slot_ids=metadata.slot_ids,
+                block_table=kv_manager.block_table, plan=plan,
+            )
+        return gqa_mixed_attention_op(
+            query_states, keys, values,
+            kv_lens=kv_manager.lens[metadata.slot_ids], max_seqlen=metadata.max_seqlen,
+            cu_seqlens=metadata.cu_seqlens, slot_ids=metadata.slot_ids,
+            block_table=kv_manager.block_table, plan=plan,
+        )
 
 
 HipQwen2Attention = TritonQwen2Attention

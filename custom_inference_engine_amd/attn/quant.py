@@ -1,0 +1,328 @@
+"""Paged GQA attention over the 8-bit cache (``kv_cache/quant.py``).
+
+The forms of ``core.py`` with one argument more, the cache's ``scales``: decode
+(plain, with the append of the new row, and from the fused QKV projection with
+RoPE; on their own or from a step's ``decode_plan``, which does not depend on the
+pools' type) and varlen mixed attention.  Queries, new rows and outputs are
+float16; the attended values are the cache's own (byte times scale), the sums
+float32, as in ``core.py``.  ``TritonQwen2Attention`` calls these where its
+``KVStorage`` holds 8 bits.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from .. import _native
+from ..kv_cache.quant import check_cache_q8, int64_index, int64_table, new_rows, on_device
+from .core import (GQA_DECODE_CONFIG, _plan_workgroups, _qkv_rows, _require, _rope_rows, default_decode_splits,
+                   split_counters)
+
+
+def _decode(entry, o, q_args, cache, row_args, lens, slot_ids, block_table, H_q, append, num_programs, err, counters,
+            plan, dev):
+    """One decode launch of the C entry ``entry`` (cie_q8_decode*): its shared arguments and buffers."""
+    k, v, scales = cache
+    N_PAGES, H_kv, PAGE_SIZE, D = k.shape
+    B = slot_ids.shape[0]
+    lens, slot_ids, block_table = int64_index(lens), int64_index(slot_ids), int64_table(block_table)
+    lib = _native.load()
+    if plan is not None:  # a step's plan (decode_plan, same append mode)
+        P = _plan_workgroups(plan)
+        n_wg = P
+    else:
+        P = int(num_programs) if num_programs else default_decode_splits(B, H_kv, dev)
+        _require(1 <= P <= lib.cie_paged_decode_max_splits(), "num_programs outside [1, the kernel's split limit]")
+        n_wg = P * B * H_kv
+    partials = None
+    if n_wg > B * H_kv:
+        partials = torch.empty(lib.cie_paged_decode_planned_partials_bytes(n_wg, H_q, H_kv, D), dtype=torch.uint8,
+                               device=dev)
+        if counters is None:
+            counters = split_counters(dev, 2 * B * H_kv)
+        _require(counters.dtype == torch.int32 and counters.numel() >= 2 * B * H_kv, "counters too small")
+    n_slots = min(lens.shape[0], block_table.shape[0]) if append else block_table.shape[0]
+    with on_device(dev):
+        _native.check(
+            getattr(lib, entry)(
+                o.data_ptr(), *q_args, k.data_ptr(), v.data_ptr(), scales.data_ptr(), *row_args,
+                lens.data_ptr(), slot_ids.data_ptr(), block_table.data_ptr(), _native.ptr(plan),
+                _native.ptr(partials), _native.ptr(counters), B, H_q, H_kv, D, PAGE_SIZE, N_PAGES,
+                k.stride(0), k.stride(1), block_table.stride(0), block_table.shape[1], n_slots, P,
+                _native.ptr(err), _native.stream_handle(dev),
+            ),
+            entry,
+        )
+    return o
+
+
+def _check_decode(H_q, cache, slot_ids, block_table, rows: int) -> None:
+    k, v, scales = cache
+    check_cache_q8(k, v, scales)
+    _require(H_q % k.shape[1] == 0, "H_q must be a multiple of H_kv")
+    _require(k.shape[0] == block_table.shape[1], "block_table width must equal n_pages")
+    _require(rows == slot_ids.shape[0], "decode takes one query token per sequence")
+
+
+def _check_q(q: torch.Tensor, d: int) -> None:
+    _require(q.dim() == 4 and q.shape[0] == 1 and q.shape[3] == d, "q must be (1, T, H_q, D)")
+    _require(q.dtype == torch.float16, "q must be float16")
+    _require(q.is_contiguous(), "q must be contiguous")
+
+
+def decode_gqa_attention_q8(q, k, v, scales, lens, slot_ids, block_table, num_programs=None, err=None, counters=None,
+                            plan=None):
+    """``decode_gqa_attention`` over an 8-bit cache: q (1, B, H_q, D) against ``lens[b]`` tokens of each slot.
+
+    ``plan``: the step's ``decode_plan`` (``append=False``)."""
+    _check_q(q, k.shape[3])
+    H_q = q.shape[2]
+    _check_decode(H_q, (k, v, scales), slot_ids, block_table, q.shape[1])
+    _require(tuple(lens.shape) == (slot_ids.shape[0],), "lens must be (B,)")
+    dev = _native.require_device(q, k, v, scales, lens, slot_ids, block_table)
+    o = torch.empty_like(q)
+    if q.shape[1] == 0:
+        return o
+    return _decode("cie_q8_decode", o, (q.data_ptr(),), (k, v, scales), (), lens, slot_ids, block_table, H_q, False,
+                   num_programs, err, counters, plan, dev)
+
+
+def decode_append_gqa_attention_q8(q, k_cache, v_cache, scales, k, v, lens, slot_ids, block_table, num_programs=None,
+                                   err=None, counters=None, plan=None):
+    """``decode_append_gqa_attention`` over an 8-bit cache, one launch.
+
+    The cache and the result are those of ``kv_append_decode_q8`` followed by
+    ``decode_gqa_attention_q8`` over ``lens[slot_ids] + 1`` tokens.  Slots other
+    than the padding slot must be distinct."""
+    _check_q(q, k_cache.shape[3])
+    H_q, B = q.shape[2], slot_ids.shape[0]
+    cache = (k_cache, v_cache, scales)
+    _check_decode(H_q, cache, slot_ids, block_table, q.shape[1])
+    dev = _native.require_device(q, k_cache, v_cache, scales, k, v, lens, slot_ids, block_table)
+    kr, vr = new_rows(k, k_cache.shape[1], k_cache.shape[3]), new_rows(v, k_cache.shape[1], k_cache.shape[3])
+    _require(kr.shape[0] == B and vr.shape[0] == B, "one new K/V row per sequence")
+    o = torch.empty_like(q)
+    if B == 0:
+        return o
+    rows = (kr.data_ptr(), vr.data_ptr(), kr.stride(0), kr.stride(1), vr.stride(0), vr.stride(1))
+    return _decode("cie_q8_decode_append", o, (q.data_ptr(),), cache, rows, lens, slot_ids, block_table, H_q, True,
+                   num_programs, err, counters, plan, dev)
+
+
+def decode_qkv_rope_gqa_attention_q8(qkv, cos, sin, k_cache, v_cache, scales, lens, slot_ids, block_table,
+                                     num_heads: int, num_programs=None, err=None, counters=None, plan=None):
+    """``decode_qkv_rope_gqa_attention`` over an 8-bit cache, one launch.
+
+    The new K row is rotated in float32, rounded to float16 as the float16
+    cache's is, then quantised: the cache and the result are those of the split,
+    ``apply_rotary_pos_emb`` and ``decode_append_gqa_attention_q8``."""
+    H_q, (_, H_kv, _, D), B = int(num_heads), k_cache.shape, slot_ids.shape[0]
+    cache = (k_cache, v_cache, scales)
+    rows = _qkv_rows(qkv, (H_q + 2 * H_kv) * D)
+    _check_decode(H_q, cache, slot_ids, block_table, rows.shape[0])
+    dev = _native.require_device(rows, cos, sin, k_cache, v_cache, scales, lens, slot_ids, block_table)
+    cr, sr = _rope_rows(cos, B, D), _rope_rows(sin, B, D)
+    _require(cr.stride(0) == sr.stride(0), "cos and sin need the same row stride")
+    o = rows.new_empty((1, B, H_q, D))
+    if B == 0:
+        return o
+    q_args = (rows.data_ptr(), rows.stride(0), cr.data_ptr(), sr.data_ptr(), cr.stride(0))
+    return _decode("cie_q8_decode_qkv_rope", o, q_args, cache, (), lens, slot_ids, block_table, H_q, True,
+                   num_programs, err, counters, plan, dev)
+
+
+def append_tokens_qkv_rope_q8(qkv, cos, sin, k_cache, v_cache, scales, pages, offsets, num_heads: int, err=None):
+    """``append_tokens_qkv_rope`` into an 8-bit cache, one launch: returns the rotated q (1, T, H_q, D)."""
+    check_cache_q8(k_cache, v_cache, scales)
+    N_PAGES, H_kv, PAGE_SIZE, D = k_cache.shape
+    H_q = int(num_heads)
+    rows = _qkv_rows(qkv, (H_q + 2 * H_kv) * D)
+    T = rows.shape[0]
+    _require(tuple(pages.shape) == (T,) and tuple(offsets.shape) == (T,), "pages / offsets must be (T,)")
+    dev = _native.require_device(rows, cos, sin, k_cache, v_cache, scales, pages, offsets)
+    cr, sr = _rope_rows(cos, T, D), _rope_rows(sin, T, D)
+    _require(cr.stride(0) == sr.stride(0), "cos and sin need the same row stride")
+    pages, offsets = int64_index(pages), int64_index(offsets)
+    q = rows.new_empty((1, T, H_q, D))
+    if T == 0:
+        return q
+    lib = _native.load()
+    with on_device(dev):
+        _native.check(
+            lib.cie_q8_append_tokens_qkv_rope(
+                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr(), rows.data_ptr(),
+                rows.stride(0), cr.data_ptr(), sr.data_ptr(), cr.stride(0), pages.data_ptr(), offsets.data_ptr(),
+                T, H_q, H_kv, PAGE_SIZE, D, N_PAGES, k_cache.stride(0), k_cache.stride(1),
+                _native.ptr(err), _native.stream_handle(dev),
+            ),
+            "cie_q8_append_tokens_qkv_rope",
+        )
+    return q
+
+
+def mixed_plan_q8(k_cache, cu_seqlens, kv_lens, slot_ids, block_table, max_seqlen: int, total_T: int, num_heads: int,
+                  err=None):
+    """One mixed step's plan for ``mixed_gqa_attention_q8``, made once and used by every layer (as ``mixed_plan``).
+
+    Returns an int32 device tensor; pass it as ``plan=`` to calls with the same
+    batch, ``total_T`` (q's packed rows), heads and block table."""
+    N_PAGES, H_kv, PAGE_SIZE, D = k_cache.shape
+    B = slot_ids.shape[0]
+    _require(num_heads % H_kv == 0, "H_q must be a multiple of H_kv")
+    _require(tuple(cu_seqlens.shape) == (B + 1,) and tuple(kv_lens.shape) == (B,),
+             "cu_seqlens must be (B+1,) and kv_lens (B,)")
+    _require(N_PAGES == block_table.shape[1], "block_table width must equal n_pages")
+    dev = _native.require_device(k_cache, cu_seqlens, kv_lens, slot_ids, block_table)
+    cu_seqlens, kv_lens, slot_ids = int64_index(cu_seqlens), int64_index(kv_lens), int64_index(slot_ids)
+    lib = _native.load()
+    n = lib.cie_q8_mixed_plan_bytes(B, int(total_T), num_heads, H_kv)
+    _require(n > 0, "batch too large for a mixed plan")
+    plan = torch.empty(n // 4, dtype=torch.int32, device=dev)
+    with on_device(dev):
+        _native.check(
+            lib.cie_q8_mixed_plan(
+                plan.data_ptr(), n, cu_seqlens.data_ptr(), kv_lens.data_ptr(), slot_ids.data_ptr(), B, int(total_T),
+                int(max_seqlen), num_heads, H_kv, D, PAGE_SIZE, block_table.shape[1], block_table.shape[0],
+                _native.ptr(err), _native.stream_handle(dev),
+            ),
+            "cie_q8_mixed_plan",
+        )
+    return plan
+
+
+def mixed_gqa_attention_q8(q, k, v, scales, max_seqlen: int, cu_seqlens, kv_lens, slot_ids, block_table, err=None,
+                           counters=None, plan=None):
+    """``mixed_gqa_attention`` over an 8-bit cache: row i of sequence b attends keys [0, kv_lens[b] + i].
+
+    q (1, total_T, H_q, D); rows outside every sequence, and those at or past
+    ``max_seqlen`` in theirs (reported in ``err``), are left as
+    ``torch.empty_like`` leaves them.  ``plan``: the step's ``mixed_plan_q8``;
+    without one the call makes its own (a second, small launch).
+    """
+    _check_q(q, k.shape[3])
+    total_T, H_q, D = q.shape[1:]
+    check_cache_q8(k, v, scales)
+    N_PAGES, H_kv, PAGE_SIZE, _ = k.shape
+    B = slot_ids.shape[0]
+    _require(H_q % H_kv == 0, "H_q must be a multiple of H_kv")
+    _require(tuple(kv_lens.shape) == (B,), "kv_lens must be (B,)")
+    _require(tuple(cu_seqlens.shape) == (B + 1,), "cu_seqlens must be (B+1,)")
+    _require(N_PAGES == block_table.shape[1], "block_table width must equal n_pages")
+    dev = _native.require_device(q, k, v, scales, cu_seqlens, kv_lens, slot_ids, block_table)
+    o = torch.empty_like(q)
+    if B == 0 or total_T == 0 or int(max_seqlen) == 0:
+        return o
+    block_table = int64_table(block_table)
+    if plan is None:
+        plan = mixed_plan_q8(k, cu_seqlens, kv_lens, slot_ids, block_table, max_seqlen, total_T, H_q, err=err)
+    lib = _native.load()
+    _require(plan.dtype == torch.int32 and plan.is_contiguous()
+             and plan.numel() * 4 >= lib.cie_q8_mixed_plan_bytes(B, total_T, H_q, H_kv),
+             "plan must come from mixed_plan_q8 for this batch")
+    n = lib.cie_q8_mixed_partials_bytes(total_T, H_q, D)
+    partials = torch.empty(n, dtype=torch.uint8, device=dev)
+    n_ctr = lib.cie_q8_mixed_counters()
+    if counters is None:
+        counters = split_counters(dev, n_ctr)
+    _require(counters.dtype == torch.int32 and counters.numel() >= n_ctr, "counters too small")
+    with on_device(dev):
+        _native.check(
+            lib.cie_q8_mixed(
+                o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), scales.data_ptr(), plan.data_ptr(),
+                plan.numel() * 4, block_table.data_ptr(), partials.data_ptr(), n, counters.data_ptr(), B, total_T,
+                H_q, H_kv, D, PAGE_SIZE, N_PAGES, k.stride(0), k.stride(1), block_table.stride(0),
+                block_table.shape[1], block_table.shape[0], _native.ptr(err), _native.stream_handle(dev),
+            ),
+            "cie_q8_mixed",
+        )
+    return o
+
+
+def _decode_config(plan):
+    return {"plan": plan} if plan is not None else GQA_DECODE_CONFIG
+
+
+@torch.library.custom_op("inference::gqa_decode_attention_q8", mutates_args=())
+def gqa_decode_attention_q8_op(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor,
+    lens: torch.Tensor, slot_ids: torch.Tensor, block_table: torch.Tensor,
+) -> torch.Tensor:
+    return decode_gqa_attention_q8(q, k, v, scales, lens, slot_ids, block_table, **GQA_DECODE_CONFIG)
+
+
+@gqa_decode_attention_q8_op.register_fake
+def _(q, k, v, scales, lens, slot_ids, block_table):
+    return torch.empty_like(q)
+
+
+@torch.library.custom_op("inference::gqa_decode_append_attention_q8", mutates_args=("k_cache", "v_cache", "scales"))
+def gqa_decode_append_attention_q8_op(
+    q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor, k: torch.Tensor,
+    v: torch.Tensor, lens: torch.Tensor, slot_ids: torch.Tensor, block_table: torch.Tensor,
+    plan: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    return decode_append_gqa_attention_q8(q, k_cache, v_cache, scales, k, v, lens, slot_ids, block_table,
+                                          **_decode_config(plan))
+
+
+@gqa_decode_append_attention_q8_op.register_fake
+def _(q, k_cache, v_cache, scales, k, v, lens, slot_ids, block_table, plan=None):
+    return torch.empty_like(q)
+
+
+@torch.library.custom_op("inference::gqa_decode_qkv_rope_attention_q8",
+                         mutates_args=("k_cache", "v_cache", "scales"))
+def gqa_decode_qkv_rope_attention_q8_op(
+    qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+    scales: torch.Tensor, lens: torch.Tensor, slot_ids: torch.Tensor, block_table: torch.Tensor,
+    num_heads: int, plan: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    return decode_qkv_rope_gqa_attention_q8(qkv, cos, sin, k_cache, v_cache, scales, lens, slot_ids, block_table,
+                                            num_heads, **_decode_config(plan))
+
+
+@gqa_decode_qkv_rope_attention_q8_op.register_fake
+def _(qkv, cos, sin, k_cache, v_cache, scales, lens, slot_ids, block_table, num_heads, plan=None):
+    return qkv.new_empty((1, qkv.shape[1], num_heads, k_cache.shape[-1]))
+
+
+@torch.library.custom_op("inference::kv_append_tokens_qkv_rope_q8", mutates_args=("k_cache", "v_cache", "scales"))
+def kv_append_tokens_qkv_rope_q8_op(
+    qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+    scales: torch.Tensor, pages: torch.Tensor, offsets: torch.Tensor, num_heads: int,
+) -> torch.Tensor:
+    return append_tokens_qkv_rope_q8(qkv, cos, sin, k_cache, v_cache, scales, pages, offsets, num_heads)
+
+
+@kv_append_tokens_qkv_rope_q8_op.register_fake
+def _(qkv, cos, sin, k_cache, v_cache, scales, pages, offsets, num_heads):
+    return qkv.new_empty((1, qkv.shape[1], num_heads, k_cache.shape[-1]))
+
+
+@torch.library.custom_op("inference::gqa_mixed_attention_q8", mutates_args=())
+def gqa_mixed_attention_q8_op(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor,
+    max_seqlen: int, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
+    slot_ids: torch.Tensor, block_table: torch.Tensor, plan: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    return mixed_gqa_attention_q8(q, k, v, scales, max_seqlen, cu_seqlens, kv_lens, slot_ids, block_table, plan=plan)
+
+
+@gqa_mixed_attention_q8_op.register_fake
+def _(q, k, v, scales, max_seqlen, cu_seqlens, kv_lens, slot_ids, block_table, plan=None):
+    return torch.empty_like(q)
+
+
+@torch.library.custom_op("inference::gqa_mixed_plan_q8", mutates_args=())
+def gqa_mixed_plan_q8_op(k_cache: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
+                         slot_ids: torch.Tensor, block_table: torch.Tensor, max_seqlen: int, total_T: int,
+                         num_heads: int) -> torch.Tensor:
+    """A mixed step's plan for its layers' mixed attention (mixed_plan_q8)."""
+    return mixed_plan_q8(k_cache, cu_seqlens, kv_lens, slot_ids, block_table, max_seqlen, total_T, num_heads)
+
+
+@gqa_mixed_plan_q8_op.register_fake
+def _(k_cache, cu_seqlens, kv_lens, slot_ids, block_table, max_seqlen, total_T, num_heads):
+    n = _native.load().cie_q8_mixed_plan_bytes(slot_ids.shape[0], total_T, num_heads, k_cache.shape[1])
+    return k_cache.new_empty((n // 4,), dtype=torch.int32)

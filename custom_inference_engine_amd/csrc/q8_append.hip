@@ -1,0 +1,422 @@
+// Writing the 8-bit paged cache (q8_cache.h) and reading it back.
+//
+// Append.  The unit of work is a block: 16 rows of one kv head, K or V, with one
+// scale.  A wave takes one (block, head, K or V) at a time, a lane 16 values of a
+// row (8 dims and their rotate_half partners, D / 2 further on), so RoPE, the
+// block's amax (one wave maximum) and the rounding stay in registers: new rows are
+// read once and written once, and the block's other rows are read only where it is
+// not started anew, written only where its scale grows.
+//
+// Which rows of a call fall into a block: token mode takes any list of (page,
+// offset) pairs.  A workgroup belongs to a token and goes on only if the token's
+// block is not the one before its (a run's first token).  It then looks through the
+// whole list for the block: an earlier token with it makes that one's workgroup the
+// owner; otherwise the last token of each row is the one written.  So a list in any
+// order, or with the same index twice, gives one result, with no race on a block.
+// The search reads T page ids (L2 hits) and is shared by all heads of the block.
+//
+// What bounds it: memory at many tokens, the start's chain (index, then rows) at
+// few.
+#include "q8_cache.h"
+
+namespace cie {
+
+constexpr int kAppendThreads = 256;
+constexpr int kAppendWaves = kAppendThreads / kWave;
+
+struct Q8Params {
+  uint8_t* k_pool;
+  uint8_t* v_pool;
+  float* scales;
+  const f16* k_new;
+  const f16* v_new;
+  int64_t k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
+  // decode mode
+  const int64_t* slot_ids;
+  const int64_t* lens;
+  const int64_t* block_table;
+  int64_t bt_stride, bt_width, n_slots;
+  // token mode
+  const int64_t* pages;
+  const int64_t* offsets;
+  // rope (token mode from the fused QKV projection): k_new / v_new point into its rows
+  f16* q_out;
+  const f16* qkv;
+  const f16* cos;
+  const f16* sin;
+  int64_t qkv_stride, cs_stride;
+  int32_t H_q;
+  int32_t n_append_wg;  // workgroups that append; those after them rotate q
+  // common
+  int64_t n_rows, n_pages, pool_page_stride, pool_head_stride;
+  int32_t H_kv, page_size, tokens_per_wg;
+  int32_t* err;
+};
+
+// Rows of one block, and where the rows written come from.
+struct Q8Rows {
+  int64_t page;
+  int block;        // block of the page
+  bool fresh;       // row 0 is written: the block starts anew
+  const int* last;  // [16] token of each row, -1: not written
+};
+
+// One wave's (block, head, K or V).
+template <int D, bool kRope>
+__device__ __forceinline__ void append_block(const Q8Params& p, const Q8Rows& b, int h, bool is_v, int lane) {
+  constexpr int NU = D / 64;    // units of 16 values a lane
+  constexpr int kPer = D / 16;  // units a row
+  uint8_t* const pool = (is_v ? p.v_pool : p.k_pool) + b.page * p.pool_page_stride + h * p.pool_head_stride +
+                        (int64_t)b.block * kQ8Block * D;
+  float* const scale = p.scales + 2 * ((b.page * p.H_kv + h) * (p.page_size / kQ8Block) + b.block) + (is_v ? 1 : 0);
+  const f16* const src = is_v ? p.v_new + h * p.v_head_stride : p.k_new + h * p.k_head_stride;
+  const int64_t stride = is_v ? p.v_tok_stride : p.k_tok_stride;
+  const int e_old = b.fresh ? kQ8EMin : q8_scale_exponent(*scale);
+  f16x8 x[NU][2];
+  u32x2 old[NU][2];
+  bool written[NU];
+  uint32_t mag = 0;
+#pragma unroll
+  for (int u = 0; u < NU; ++u) {
+    const int unit = lane + u * kWave;
+    const int row = unit / kPer, d0 = 8 * (unit % kPer);
+    const int t = b.last[row];
+    written[u] = t >= 0;
+    if (written[u]) {
+      const f16* const r = src + t * stride + d0;
+      x[u][0] = *reinterpret_cast<const f16x8*>(r);
+      x[u][1] = *reinterpret_cast<const f16x8*>(r + D / 2);
+      if constexpr (kRope) {
+        if (!is_v) {
+          const f16* const c = p.cos + t * p.cs_stride + d0;
+          const f16* const s = p.sin + t * p.cs_stride + d0;
+          rope8(x[u][0], x[u][1], *reinterpret_cast<const f16x8*>(c), *reinterpret_cast<const f16x8*>(c + D / 2),
+                *reinterpret_cast<const f16x8*>(s), *reinterpret_cast<const f16x8*>(s + D / 2));
+        }
+      }
+      mag = q8_mag8(x[u][0], q8_mag8(x[u][1], mag));
+    } else if (!b.fresh) {
+      old[u][0] = *reinterpret_cast<const u32x2*>(pool + row * D + d0);
+      old[u][1] = *reinterpret_cast<const u32x2*>(pool + row * D + d0 + D / 2);
+    }
+  }
+  const int e = max(e_old, q8_exponent(q8_wave_mag(mag)));
+  const float inv = q8_pow2(-e), factor = q8_pow2(e_old - e);
+#pragma unroll
+  for (int u = 0; u < NU; ++u) {
+    const int unit = lane + u * kWave;
+    uint8_t* const dst = pool + (unit / kPer) * D + 8 * (unit % kPer);
+    if (written[u]) {
+      *reinterpret_cast<u32x2*>(dst) = q8_round8(x[u][0], inv);
+      *reinterpret_cast<u32x2*>(dst + D / 2) = q8_round8(x[u][1], inv);
+    } else if (!b.fresh && e != e_old) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<u32x2*>(dst + i * (D / 2)) =
+            u32x2{q8_rescale4(old[u][i][0], factor), q8_rescale4(old[u][i][1], factor)};
+    }
+  }
+  if (lane == 0) *scale = q8_pow2(e);
+}
+
+// The q heads of the rope form: a lane rotates 8 dims and their partners.
+template <int D>
+__device__ __forceinline__ void rotate_q(const Q8Params& p, int64_t gid) {
+  constexpr int kPer = D / 16;
+  if (gid >= p.n_rows * p.H_q * kPer) return;
+  const int d0 = 8 * (int)(gid % kPer);
+  const int64_t row = gid / kPer;
+  const int h = (int)(row % p.H_q);
+  const int64_t t = row / p.H_q;
+  const f16* const x = p.qkv + t * p.qkv_stride + (int64_t)h * D + d0;
+  const f16* const c = p.cos + t * p.cs_stride + d0;
+  const f16* const s = p.sin + t * p.cs_stride + d0;
+  f16x8 lo = *reinterpret_cast<const f16x8*>(x), hi = *reinterpret_cast<const f16x8*>(x + D / 2);
+  rope8(lo, hi, *reinterpret_cast<const f16x8*>(c), *reinterpret_cast<const f16x8*>(c + D / 2),
+        *reinterpret_cast<const f16x8*>(s), *reinterpret_cast<const f16x8*>(s + D / 2));
+  f16* const dst = p.q_out + row * D + d0;
+  *reinterpret_cast<f16x8*>(dst) = lo;
+  *reinterpret_cast<f16x8*>(dst + D / 2) = hi;
+}
+
+template <int D, bool kDecode, bool kRope>
+__global__ __launch_bounds__(kAppendThreads) void q8_append_kernel(Q8Params p) {
+  __shared__ int last[kQ8Block];
+  __shared__ int earlier;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  if constexpr (kRope) {
+    if ((int)blockIdx.x >= p.n_append_wg) {
+      rotate_q<D>(p, (int64_t)(blockIdx.x - p.n_append_wg) * kAppendThreads + threadIdx.x);
+      return;
+    }
+  }
+  const int64_t t_end = min(p.n_rows, (int64_t)(blockIdx.x + 1) * p.tokens_per_wg);
+  for (int64_t t = (int64_t)blockIdx.x * p.tokens_per_wg; t < t_end; ++t) {  // (every branch below is uniform)
+    int64_t page, off;
+    if constexpr (kDecode) {
+      const int64_t slot = p.slot_ids[t];
+      if (slot < 0 || slot >= p.n_slots) {
+        if (threadIdx.x == 0) set_err(p.err, CIE_ERRBIT_PAGE);
+        continue;
+      }
+      const int64_t pos = p.lens[slot];
+      if (pos < 0 || pos >= p.bt_width * p.page_size) {
+        if (threadIdx.x == 0) set_err(p.err, CIE_ERRBIT_LEN);
+        continue;
+      }
+      page = p.block_table[slot * p.bt_stride + pos / p.page_size];
+      off = pos % p.page_size;
+    } else {
+      page = p.pages[t];
+      off = p.offsets[t];
+      if (off < 0 || off >= p.page_size) {
+        if (threadIdx.x == 0) set_err(p.err, CIE_ERRBIT_OFFSET);
+        continue;
+      }
+    }
+    if (page < 0 || page >= p.n_pages) {
+      if (threadIdx.x == 0) set_err(p.err, CIE_ERRBIT_PAGE);
+      continue;
+    }
+    const int block = (int)off / kQ8Block;
+    if (!kDecode && t > 0 && p.pages[t - 1] == page) {
+      const int64_t o = p.offsets[t - 1];
+      if (o >= 0 && o < p.page_size && (int)o / kQ8Block == block) continue;  // not its run's first token
+    }
+    __syncthreads();  // (the last token's block is done with `last`)
+    if (threadIdx.x < kQ8Block) last[threadIdx.x] = -1;
+    if (threadIdx.x == 0) earlier = 0;
+    __syncthreads();
+    if constexpr (kDecode) {
+      // a slot that comes again later in the batch writes the row
+      const int64_t slot = p.slot_ids[t];
+      bool again = false;
+      for (int64_t i = t + 1 + threadIdx.x; i < p.n_rows; i += kAppendThreads) again |= p.slot_ids[i] == slot;
+      if (again) earlier = 1;
+      if (threadIdx.x == 0) last[off % kQ8Block] = (int)t;
+    } else {
+      for (int64_t i = threadIdx.x; i < p.n_rows; i += kAppendThreads) {
+        if (p.pages[i] != page) continue;
+        const int64_t o = p.offsets[i];
+        if (o < 0 || o >= p.page_size || (int)o / kQ8Block != block) continue;
+        if (i < t) earlier = 1;
+        atomicMax(&last[o % kQ8Block], (int)i);
+      }
+    }
+    __syncthreads();
+    if (earlier) continue;
+    const Q8Rows rows{page, block, last[0] >= 0, last};
+    for (int task = wave; task < 2 * p.H_kv; task += kAppendWaves)
+      append_block<D, kRope>(p, rows, task >> 1, task & 1, lane);
+  }
+}
+
+// ---- reading back ----
+
+struct Q8ReadParams {
+  f16* k_out;  // (T, H_kv, D) dense
+  f16* v_out;
+  const uint8_t* k_pool;
+  const uint8_t* v_pool;
+  const float* scales;
+  const int64_t* pages;
+  const int64_t* offsets;
+  int64_t T, n_pages, pool_page_stride, pool_head_stride;
+  int32_t H_kv, page_size;
+  int32_t* err;
+};
+
+// Row t of the outputs = the cache's row (pages[t], offsets[t]): a lane converts 16 values of K and of V.
+// Bound by memory.  A bad index reads as zeros and is reported.
+template <int D>
+__global__ __launch_bounds__(256) void q8_read_kernel(Q8ReadParams p) {
+  constexpr int kPer = D / 16;
+  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (gid >= p.T * p.H_kv * kPer) return;
+  const int d0 = 16 * (int)(gid % kPer);
+  const int64_t row = gid / kPer;
+  const int h = (int)(row % p.H_kv);
+  const int64_t t = row / p.H_kv;
+  const int64_t page = p.pages[t], off = p.offsets[t];
+  f16x8 k[2] = {}, v[2] = {};
+  const bool off_ok = off >= 0 && off < p.page_size, page_ok = page >= 0 && page < p.n_pages;
+  if (off_ok && page_ok) {
+    const int64_t at = page * p.pool_page_stride + h * p.pool_head_stride + off * D + d0;
+    const u32x4 kb = *reinterpret_cast<const u32x4*>(p.k_pool + at);
+    const u32x4 vb = *reinterpret_cast<const u32x4*>(p.v_pool + at);
+    const float* const s = p.scales + 2 * ((page * p.H_kv + h) * (p.page_size / kQ8Block) + off / kQ8Block);
+    const float ks = s[0], vs = s[1];
+    k[0] = q8_values8(kb[0], kb[1], ks);
+    k[1] = q8_values8(kb[2], kb[3], ks);
+    v[0] = q8_values8(vb[0], vb[1], vs);
+    v[1] = q8_values8(vb[2], vb[3], vs);
+  } else {
+    set_err(p.err, off_ok ? CIE_ERRBIT_PAGE : CIE_ERRBIT_OFFSET);
+  }
+  f16* const ko = p.k_out + row * D + d0;
+  f16* const vo = p.v_out + row * D + d0;
+  *reinterpret_cast<f16x8*>(ko) = k[0];
+  *reinterpret_cast<f16x8*>(ko + 8) = k[1];
+  *reinterpret_cast<f16x8*>(vo) = v[0];
+  *reinterpret_cast<f16x8*>(vo + 8) = v[1];
+}
+
+static bool q8_aligned(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
+
+// What every entry point asks of the pools (D: 64 or 128, the attention kernels').
+static int q8_check_pools(const void* k_pool, const void* v_pool, const void* scales, int64_t H_kv,
+                          int64_t page_size, int64_t D, int64_t n_pages, int64_t page_stride, int64_t head_stride) {
+  if (H_kv <= 0 || page_size <= 0 || D <= 0 || n_pages <= 0) return CIE_EINVAL;
+  if ((D != 64 && D != 128) || page_size % kQ8Block != 0 || H_kv > 65535 || page_size > (1 << 20))
+    return CIE_EUNSUPPORTED;
+  if (!k_pool || !v_pool || !scales || !q8_aligned(k_pool) || !q8_aligned(v_pool) || !q8_aligned(scales) ||
+      page_stride % 16 != 0 || head_stride % 16 != 0)
+    return CIE_EINVAL;
+  return CIE_OK;
+}
+
+// Tokens a workgroup looks at: one, so that the rows of a decode batch, each a block of its own, run side
+// by side; four at more tokens than the chip holds workgroups at once (2,048), where most belong to a run
+// that another workgroup owns and only their number costs.
+template <bool kDecode, bool kRope>
+static int q8_launch_append(Q8Params& p, int64_t D, hipStream_t stream) {
+  if (p.n_rows > 0x7fffffff / 512) return CIE_EUNSUPPORTED;
+  p.tokens_per_wg = !kDecode && p.n_rows > 2048 ? 4 : 1;
+  p.n_append_wg = (int32_t)((p.n_rows + p.tokens_per_wg - 1) / p.tokens_per_wg);
+  int64_t blocks = p.n_append_wg;
+  if (kRope) blocks += (p.n_rows * p.H_q * (D / 16) + kAppendThreads - 1) / kAppendThreads;
+  if (blocks > 0x7fffffff) return CIE_EUNSUPPORTED;
+  if (D == 64)
+    hipLaunchKernelGGL((q8_append_kernel<64, kDecode, kRope>), dim3((unsigned)blocks), dim3(kAppendThreads), 0, stream, p);
+  else
+    hipLaunchKernelGGL((q8_append_kernel<128, kDecode, kRope>), dim3((unsigned)blocks), dim3(kAppendThreads), 0, stream, p);
+  return (int)hipGetLastError();
+}
+
+static Q8Params q8_params(void* k_pool, void* v_pool, void* scales, int64_t n_rows, int64_t H_kv, int64_t page_size,
+                          int64_t n_pages, int64_t page_stride, int64_t head_stride, int32_t* err) {
+  Q8Params p{};
+  p.k_pool = static_cast<uint8_t*>(k_pool);
+  p.v_pool = static_cast<uint8_t*>(v_pool);
+  p.scales = static_cast<float*>(scales);
+  p.n_rows = n_rows;
+  p.H_kv = (int32_t)H_kv;
+  p.page_size = (int32_t)page_size;
+  p.n_pages = n_pages;
+  p.pool_page_stride = page_stride;
+  p.pool_head_stride = head_stride;
+  p.err = err;
+  return p;
+}
+
+static int q8_new_rows(Q8Params& p, const void* k_new, const void* v_new, int64_t k_tok, int64_t k_head,
+                       int64_t v_tok, int64_t v_head) {
+  if (!k_new || !v_new || !q8_aligned(k_new) || !q8_aligned(v_new) || k_tok % 8 != 0 || k_head % 8 != 0 ||
+      v_tok % 8 != 0 || v_head % 8 != 0)
+    return CIE_EINVAL;
+  p.k_new = static_cast<const f16*>(k_new);
+  p.v_new = static_cast<const f16*>(v_new);
+  p.k_tok_stride = k_tok;
+  p.k_head_stride = k_head;
+  p.v_tok_stride = v_tok;
+  p.v_head_stride = v_head;
+  return CIE_OK;
+}
+
+}  // namespace cie
+
+using namespace cie;
+
+extern "C" int cie_q8_append_decode(void* k_pool, void* v_pool, void* scales, const void* k_new, const void* v_new,
+                                    int64_t k_tok_stride, int64_t k_head_stride, int64_t v_tok_stride,
+                                    int64_t v_head_stride, const int64_t* slot_ids, const int64_t* lens,
+                                    const int64_t* block_table, int64_t B, int64_t H_kv, int64_t page_size, int64_t D,
+                                    int64_t n_pages, int64_t pool_page_stride, int64_t pool_head_stride,
+                                    int64_t bt_stride, int64_t bt_width, int64_t n_slots, int32_t* err, void* stream) {
+  if (B < 0 || bt_width <= 0 || bt_stride < bt_width || n_slots <= 0) return CIE_EINVAL;
+  if (int rc = q8_check_pools(k_pool, v_pool, scales, H_kv, page_size, D, n_pages, pool_page_stride, pool_head_stride))
+    return rc;
+  if (bt_width > 0x7fffffff / page_size) return CIE_EUNSUPPORTED;
+  if (B == 0) return CIE_OK;
+  if (!slot_ids || !lens || !block_table) return CIE_EINVAL;
+  Q8Params p = q8_params(k_pool, v_pool, scales, B, H_kv, page_size, n_pages, pool_page_stride, pool_head_stride, err);
+  if (int rc = q8_new_rows(p, k_new, v_new, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride)) return rc;
+  p.slot_ids = slot_ids;
+  p.lens = lens;
+  p.block_table = block_table;
+  p.bt_stride = bt_stride;
+  p.bt_width = bt_width;
+  p.n_slots = n_slots;
+  return q8_launch_append<true, false>(p, D, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int cie_q8_append_tokens(void* k_pool, void* v_pool, void* scales, const void* k_new, const void* v_new,
+                                    int64_t k_tok_stride, int64_t k_head_stride, int64_t v_tok_stride,
+                                    int64_t v_head_stride, const int64_t* pages, const int64_t* offsets, int64_t T,
+                                    int64_t H_kv, int64_t page_size, int64_t D, int64_t n_pages,
+                                    int64_t pool_page_stride, int64_t pool_head_stride, int32_t* err, void* stream) {
+  if (T < 0) return CIE_EINVAL;
+  if (int rc = q8_check_pools(k_pool, v_pool, scales, H_kv, page_size, D, n_pages, pool_page_stride, pool_head_stride))
+    return rc;
+  if (T == 0) return CIE_OK;
+  if (!pages || !offsets) return CIE_EINVAL;
+  Q8Params p = q8_params(k_pool, v_pool, scales, T, H_kv, page_size, n_pages, pool_page_stride, pool_head_stride, err);
+  if (int rc = q8_new_rows(p, k_new, v_new, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride)) return rc;
+  p.pages = pages;
+  p.offsets = offsets;
+  return q8_launch_append<false, false>(p, D, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int cie_q8_append_tokens_qkv_rope(void* q_out, void* k_pool, void* v_pool, void* scales, const void* qkv,
+                                             int64_t qkv_row_stride, const void* cos, const void* sin,
+                                             int64_t cs_row_stride, const int64_t* pages, const int64_t* offsets,
+                                             int64_t T, int64_t H_q, int64_t H_kv, int64_t page_size, int64_t D,
+                                             int64_t n_pages, int64_t pool_page_stride, int64_t pool_head_stride,
+                                             int32_t* err, void* stream) {
+  if (T < 0 || H_q <= 0) return CIE_EINVAL;
+  if (int rc = q8_check_pools(k_pool, v_pool, scales, H_kv, page_size, D, n_pages, pool_page_stride, pool_head_stride))
+    return rc;
+  if (H_q > 65535) return CIE_EUNSUPPORTED;
+  if (T == 0) return CIE_OK;
+  if (!q_out || !qkv || !cos || !sin || !pages || !offsets || !q8_aligned(q_out) || !q8_aligned(qkv) ||
+      !q8_aligned(cos) || !q8_aligned(sin) || qkv_row_stride % 8 != 0 || cs_row_stride % 8 != 0 ||
+      qkv_row_stride < (H_q + 2 * H_kv) * D || cs_row_stride < D)
+    return CIE_EINVAL;
+  Q8Params p = q8_params(k_pool, v_pool, scales, T, H_kv, page_size, n_pages, pool_page_stride, pool_head_stride, err);
+  const f16* const row = static_cast<const f16*>(qkv);
+  p.k_new = row + H_q * D;
+  p.v_new = row + (H_q + H_kv) * D;
+  p.k_tok_stride = p.v_tok_stride = qkv_row_stride;
+  p.k_head_stride = p.v_head_stride = D;
+  p.q_out = static_cast<f16*>(q_out);
+  p.qkv = row;
+  p.cos = static_cast<const f16*>(cos);
+  p.sin = static_cast<const f16*>(sin);
+  p.qkv_stride = qkv_row_stride;
+  p.cs_stride = cs_row_stride;
+  p.pages = pages;
+  p.offsets = offsets;
+  p.H_q = (int32_t)H_q;
+  return q8_launch_append<false, true>(p, D, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int cie_q8_read_tokens(void* k_out, void* v_out, const void* k_pool, const void* v_pool,
+                                  const void* scales, const int64_t* pages, const int64_t* offsets, int64_t T,
+                                  int64_t H_kv, int64_t page_size, int64_t D, int64_t n_pages,
+                                  int64_t pool_page_stride, int64_t pool_head_stride, int32_t* err, void* stream) {
+  if (T < 0) return CIE_EINVAL;
+  if (int rc = q8_check_pools(k_pool, v_pool, scales, H_kv, page_size, D, n_pages, pool_page_stride, pool_head_stride))
+    return rc;
+  if (T == 0) return CIE_OK;
+  if (!k_out || !v_out || !pages || !offsets || !q8_aligned(k_out) || !q8_aligned(v_out)) return CIE_EINVAL;
+  Q8ReadParams p{static_cast<f16*>(k_out), static_cast<f16*>(v_out), static_cast<const uint8_t*>(k_pool),
+                 static_cast<const uint8_t*>(v_pool), static_cast<const float*>(scales), pages, offsets, T, n_pages,
+                 pool_page_stride, pool_head_stride, (int32_t)H_kv, (int32_t)page_size, err};
+  if (T > 0x7fffffffLL * 256 / (H_kv * (D / 16))) return CIE_EUNSUPPORTED;
+  const int64_t blocks = (T * H_kv * (D / 16) + 255) / 256;
+  if (D == 64)
+    hipLaunchKernelGGL(q8_read_kernel<64>, dim3((unsigned)blocks), dim3(256), 0, static_cast<hipStream_t>(stream), p);
+  else
+    hipLaunchKernelGGL(q8_read_kernel<128>, dim3((unsigned)blocks), dim3(256), 0, static_cast<hipStream_t>(stream), p);
+  return (int)hipGetLastError();
+}

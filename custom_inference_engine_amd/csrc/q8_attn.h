@@ -1,0 +1,205 @@
+// Attention over 8-bit key tiles (q8_cache.h): tile loads, conversion and the
+// 32-key step, shared by the decode and mixed kernels.
+//
+// As in attn_engine.h a wave computes S^T = K . Q^T and O^T = V^T . P^T with
+// v_mfma_f32_16x16x32_f16, up to 16 query columns per column tile.  Operand layout
+// (lane l, r16 = l % 16, grp = l / 16), chosen for byte rows:
+//   K tile: lane holds bytes [64 j + 16 grp, + 16) of key r16, j < D / 64: one
+//     16-byte load per 64 dims (a wave reads 1 KiB in one piece).  The order of the
+//     dims in the dot product is free, so k-step 2 j + i takes bytes 8 i .. 8 i + 7 of
+//     them, and Q is loaded in that order (q8_dim).
+//   V tile: lane holds bytes [NT r16, + NT) of rows 4 grp + e, e < 4 (a group reads
+//     whole rows).  Bytes of two rows are brought side by side (v_perm), so one
+//     conversion gives the two keys of an operand register.
+// The converted values are the cache's own, exactly (its scales are applied by the
+// conversion), so what follows is the fp16 kernels' arithmetic: P rounded to fp16
+// (2^-11 of each weight, the cache's own rounding is 2^-4), sums in fp32.
+#pragma once
+
+#include "attn_engine.h"
+#include "q8_cache.h"
+
+namespace cie {
+
+// First dim of the 8 that k-step ks takes in lane group grp.
+__device__ __forceinline__ int q8_dim(int ks, int grp) { return 64 * (ks >> 1) + 16 * grp + 8 * (ks & 1); }
+
+// Raw bytes of one 16-key tile.
+template <int D>
+struct Q8Tile {
+  static constexpr int NJ = D / 64;
+  typedef uint32_t vrow_t __attribute__((ext_vector_type(NJ)));
+  u32x4 k[NJ];
+  vrow_t v[4];
+};
+
+// Lane's byte offsets in a tile.
+template <int D>
+struct Q8Lane {
+  uint32_t k, v;
+  __device__ __forceinline__ Q8Lane(int r16, int grp)
+      : k((uint32_t)(r16 * D + 16 * grp)), v((uint32_t)(4 * grp * D + Geo<D>::NT * r16)) {}
+};
+
+// A tile's rows as a raw buffer (attn_engine.h, tile_rsrc): rows at or past `rows` read as zeros and
+// touch no memory, so a sequence's last tile costs its rows only and an absent tile (0 rows) nothing.
+// All arguments wave-uniform.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t q8_rsrc(const uint8_t* pool, int64_t off, int rows, int D) {
+  return coherent_rsrc(pool + off, (uint32_t)__builtin_amdgcn_readfirstlane(rows * D));
+}
+
+// A call reads each K/V byte once per workgroup: past the caches' reuse (nt).
+template <int D, int POL>
+__device__ __forceinline__ void q8_load(Q8Tile<D>& t, __amdgpu_buffer_rsrc_t rk, __amdgpu_buffer_rsrc_t rv,
+                                        const Q8Lane<D>& lo) {
+  typedef typename Q8Tile<D>::vrow_t vrow_t;
+#pragma unroll
+  for (int j = 0; j < Q8Tile<D>::NJ; ++j)
+    t.k[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, lo.k + 64 * j, 0, POL));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (D == 64)
+      t.v[e] = __builtin_bit_cast(vrow_t, __builtin_amdgcn_raw_buffer_load_b32(rv, lo.v + e * D, 0, POL));
+    else
+      t.v[e] = __builtin_bit_cast(vrow_t, __builtin_amdgcn_raw_buffer_load_b64(rv, lo.v + e * D, 0, POL));
+  }
+}
+
+// A tile's K operands.
+template <int D>
+__device__ __forceinline__ void q8_k_operand(f16x8 (&k)[Geo<D>::KS], const Q8Tile<D>& t, float scale) {
+#pragma unroll
+  for (int j = 0; j < Q8Tile<D>::NJ; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) k[2 * j + i] = q8_values8(t.k[j][2 * i], t.k[j][2 * i + 1], scale);
+}
+
+// Rows 4 grp + e at or past n_rows become zeros: a masked key's weight is 0, but its bytes may hold
+// anything (NaN among it).
+template <int D>
+__device__ __forceinline__ void q8_zero_rows(Q8Tile<D>& t, int n_rows, int grp) {
+  typedef typename Q8Tile<D>::vrow_t vrow_t;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (4 * grp + e >= n_rows) t.v[e] = vrow_t{};
+}
+
+// Keys 4 grp + 0 .. 3 of a tile as elements 4 half .. 4 half + 3 of the V^T operands (dim NT r16 + nt).
+template <int D>
+__device__ __forceinline__ void q8_v_operand(f16x8 (&va)[Geo<D>::NT], int half, const Q8Tile<D>& t, float scale) {
+#pragma unroll
+  for (int w = 0; w < Q8Tile<D>::NJ; ++w) {
+#pragma unroll
+    for (int pr = 0; pr < 2; ++pr) {  // keys 2 pr, 2 pr + 1
+      const uint32_t a = t.v[2 * pr][w], b = t.v[2 * pr + 1][w];
+      const uint32_t d01 = __builtin_amdgcn_perm(b, a, 0x05010400);  // {a0, b0, a1, b1}
+      const uint32_t d23 = __builtin_amdgcn_perm(b, a, 0x07030602);
+      const f16x2 x[4] = {q8_pair<false>(d01, scale), q8_pair<true>(d01, scale), q8_pair<false>(d23, scale),
+                          q8_pair<true>(d23, scale)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        va[4 * w + i][4 * half + 2 * pr] = x[i][0];
+        va[4 * w + i][4 * half + 2 * pr + 1] = x[i][1];
+      }
+    }
+  }
+}
+
+// One 32-key step of NCT column tiles: K operands ka / kb of tiles a and b, whose first keys are key0a / key0b
+// (kNoKey: absent, all masked); v(va) gives the V^T operands once the weights are known.  lim[c]: keys the
+// lane's column attends; mask: some key of the step may be at or past one of them.  Phase by phase over the
+// column tiles, so that a wave overlaps their VALU work and MFMAs; attend_pair_body's softmax.
+template <int D, int NCT, class V>
+__device__ __forceinline__ void q8_step(SoftmaxAcc<D, NCT>& st, const f16x8 (&ka)[Geo<D>::KS],
+                                        const f16x8 (&kb)[Geo<D>::KS], V v, const f16x8 (&q)[NCT][Geo<D>::KS],
+                                        int key0a, int key0b, const int (&lim)[NCT], bool mask, float scale_log2,
+                                        int grp) {
+  constexpr int KS = Geo<D>::KS;
+  constexpr int NT = Geo<D>::NT;
+  f32x4 s[NCT][2];
+#pragma unroll
+  for (int c = 0; c < NCT; ++c) {
+    s[c][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    s[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      s[c][0] = mfma16x16x32(ka[ks], q[c][ks], s[c][0]);
+      s[c][1] = mfma16x16x32(kb[ks], q[c][ks], s[c][1]);
+    }
+  }
+  if (mask) {
+#pragma unroll
+    for (int c = 0; c < NCT; ++c)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[c][0][r] = key0a + 4 * grp + r < lim[c] ? s[c][0][r] : kNegInf;
+        s[c][1][r] = key0b + 4 * grp + r < lim[c] ? s[c][1][r] : kNegInf;
+      }
+  }
+  float xb[NCT];
+  bool need = false;
+#pragma unroll
+  for (int c = 0; c < NCT; ++c) {
+    xb[c] = fmaxf(fmaxf(fmaxf(s[c][0][0], s[c][0][1]), fmaxf(s[c][0][2], s[c][0][3])),
+                  fmaxf(fmaxf(s[c][1][0], s[c][1][1]), fmaxf(s[c][1][2], s[c][1][3])));
+    need |= xb[c] > st.thr[c];
+  }
+  if (__any(need)) {  // rare: move the reference max
+#pragma unroll
+    for (int c = 0; c < NCT; ++c) {
+      const float m_new = fmaxf(st.m[c], col_max4(xb[c]) * scale_log2);
+      const float alpha = fast_exp2(st.m[c] - m_new);
+      st.m[c] = m_new;
+      st.thr[c] = (m_new + kRescaleSlack) / scale_log2;
+      st.lsum[c][0] *= alpha;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) st.acc[c][nt] *= alpha;
+    }
+  }
+  f16x8 p[NCT];
+#pragma unroll
+  for (int c = 0; c < NCT; ++c)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[c][e] = (f16)fast_exp2(__builtin_fmaf(s[c][e / 4][e % 4], scale_log2, -st.m[c]));
+  f16x8 va[NT];
+  v(va);
+  const f16x8 ones = {(f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f};
+#pragma unroll
+  for (int c = 0; c < NCT; ++c) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) st.acc[c][nt] = mfma16x16x32(va[nt], p[c], st.acc[c][nt]);
+    st.lsum[c] = mfma16x16x32(ones, p[c], st.lsum[c]);
+  }
+}
+
+// The same for one column tile from raw tiles.
+template <int D>
+__device__ __forceinline__ void q8_attend(SoftmaxAcc<D, 1>& st, const Q8Tile<D>& a, const Q8Tile<D>& b, float ksa,
+                                          float vsa, float ksb, float vsb, const f16x8 (&q)[1][Geo<D>::KS], int key0a,
+                                          int key0b, const int (&lim)[1], bool mask, float scale_log2, int grp) {
+  f16x8 ka[Geo<D>::KS], kb[Geo<D>::KS];
+  q8_k_operand<D>(ka, a, ksa);
+  q8_k_operand<D>(kb, b, ksb);
+  auto v = [&](f16x8 (&va)[Geo<D>::NT]) {
+    q8_v_operand<D>(va, 0, a, vsa);
+    q8_v_operand<D>(va, 1, b, vsb);
+  };
+  q8_step<D, 1>(st, ka, kb, v, q, key0a, key0b, lim, mask, scale_log2, grp);
+}
+
+// Where a wave's tiles live: kv head g of the pools and of the scales.
+struct Q8Src {
+  const uint8_t* k_pool;
+  const uint8_t* v_pool;
+  const float* scales;
+  int64_t page_stride, head_off;  // bytes
+  int32_t H_kv, g, per;           // per: blocks a page
+  __device__ __forceinline__ int64_t tile(int page, int block, int D) const {
+    return (int64_t)page * page_stride + head_off + (int64_t)block * (kQ8Block * D);
+  }
+  __device__ __forceinline__ const float* scale(int page, int block) const {
+    return scales + 2 * (((int64_t)page * H_kv + g) * per + block);
+  }
+};
+
+}  // namespace cie

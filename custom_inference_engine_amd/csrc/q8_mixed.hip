@@ -1,0 +1,802 @@
+// Varlen causal attention over the 8-bit paged cache (q8_cache.h): chunked prefill
+// and decode rows in one launch, from a plan made once per step.
+//
+// Sequence b owns query rows [cu_seqlens[b], cu_seqlens[b + 1]); its row i sits at
+// position kv_lens[b] + i and attends keys 0 .. kv_lens[b] + i of slot slot_ids[b].
+// Rows outside every sequence are left untouched.
+//
+// Work.  A query tile is up to R rows of a sequence and one kv head: R * G <= 64 CT
+// (row, head) columns.  An item is a tile and a range of its key tiles.
+//  * Wide items (more than 16 columns): every wave has up to CT column tiles of 16
+//    and all keys of the item.  Keys go by stages of 64: wave w loads the stage's
+//    16-key tile w as bytes (so its page and its two scales are scalars), converts it
+//    once and leaves it in LDS in MFMA operand order (K: slot [tile][k-step][lane];
+//    V^T: [pair][dim tile][lane]), where a lane writes its own slots and every wave
+//    reads the same ones: 16-byte accesses without bank conflicts.  Converting in the
+//    loader costs each value once per workgroup instead of once per wave.  Two
+//    buffers, one barrier a stage, the next stage's bytes in flight in registers.
+//  * Narrow items (a decode row and its like: 16 columns or fewer): one column tile,
+//    its keys dealt over the four waves, straight from registers as the decode
+//    kernel does; the waves fold through LDS.
+// A tile whose keys exceed the plan's share is split over several items; each
+// leaves its state (m, l, acc) in `partials` and the last to arrive merges them.
+//
+// The plan (q8_mixed_plan_kernel, one workgroup) sizes that share so that the
+// launch has about kQ8Slots items' worth of work, and lists the items, wide ones
+// first.  It depends on the step's sequences only, so a step makes it once for all
+// its layers.
+//
+// What bounds it: prefill, the softmax's VALU work between the MFMAs (a step of 32
+// keys costs a wave 18 MFMAs and 16 exponentials at D = 64 and CT = 2); decode rows,
+// the K/V reads.
+#include "q8_attn.h"
+
+namespace cie {
+
+constexpr int kMW = 4;  // waves a workgroup
+constexpr int kMThreads = kMW * kWave;
+constexpr int kQ8Slots = 512;        // items a launch's work is cut into, about
+constexpr int kMaxSplitItems = 2 * kQ8Slots;  // (see plan_share)
+constexpr int kQ8MinShare = 32;  // key tiles (512 keys): below, an item's start costs more than its keys
+constexpr int kQ8MaxSeqs = 2048;
+constexpr int kItemWords = 12;
+constexpr int kHeadWords = 12;
+constexpr int kQ8MaxChunks = 64;  // items of a split tile at most (one workgroup merges them)
+constexpr int kPlanThreadsM = 1024;
+constexpr int kPlanMagic = 0x71386d31;
+
+// Column tiles of a wave, and columns of a wide tile, at most.
+constexpr int kQ8Ct = 2;
+static __host__ __device__ constexpr int q8_tile_cols() { return 16 * kMW * kQ8Ct; }
+
+struct Q8Item {
+  int tok0;    // packed row of the tile's first row
+  int rows;    // rows, negative: a narrow item
+  int g, slot;
+  int pos0;    // position of the first row
+  int t0, t1;  // key tiles
+  int chunk, n_chunks;
+  int pbase;   // first partial row of the tile (split tiles): row pbase + chunk * columns + column
+  int ctr;     // its arrival word
+  int pad;
+};
+static_assert(sizeof(Q8Item) == kItemWords * 4, "item layout");
+
+struct Q8MixedParams {
+  f16* o;
+  const f16* q;
+  const uint8_t* k_pool;
+  const uint8_t* v_pool;
+  const float* scales;
+  const int64_t* block_table;
+  const int32_t* plan;
+  float* part_m;
+  float* part_l;
+  float* part_acc;
+  int32_t* counters;
+  int64_t pool_page_stride, pool_head_stride, bt_stride, n_pages, total_T;
+  int32_t part_cap, n_ctr, plan_cap, B, bt_width, n_slots, H_q, H_kv, G, page_size;
+  uint32_t g_magic;
+  float scale_log2;
+  int32_t* err;
+};
+
+// ---- the plan ----
+
+struct Q8PlanParams {
+  int32_t* plan;
+  const int64_t* cu_seqlens;
+  const int64_t* kv_lens;
+  const int64_t* slot_ids;
+  int64_t total_T, cap;  // cap: keys a block-table row holds
+  int32_t B, bt_width, n_slots, H_q, H_kv, G, page_size, D, max_rows, part_cap, plan_cap;
+  int32_t* err;
+};
+
+// What a plan was made for (its first words, after the item count): a call with other sizes writes nothing.
+template <class P>
+__device__ __forceinline__ int plan_word(const P& p, int i, int D) {
+  const int w[kHeadWords - 1] = {kPlanMagic, p.B, (int)p.total_T, p.H_q, p.H_kv, D, p.page_size, p.bt_width,
+                                 p.n_slots, p.part_cap, p.plan_cap};
+  return w[i];
+}
+
+struct Q8Seq {
+  int64_t t0;
+  int slot, L, c;
+};
+
+__device__ __forceinline__ Q8Seq q8_seq(const Q8PlanParams& p, int b, bool report) {
+  Q8Seq s{0, 0, 0, 0};
+  const int64_t t0 = p.cu_seqlens[b], t1 = p.cu_seqlens[b + 1], slot = p.slot_ids[b], c = p.kv_lens[b];
+  if (t1 == t0) return s;
+  if (t0 < 0 || t1 < t0 || t1 > p.total_T || slot < 0 || slot >= p.n_slots) {
+    if (report) set_err(p.err, CIE_ERRBIT_PAGE);
+    return s;
+  }
+  if (c < 0 || c > p.cap || c + (t1 - t0) > p.cap) {
+    if (report) set_err(p.err, CIE_ERRBIT_LEN);
+    return s;
+  }
+  if (t1 - t0 > p.max_rows && report) set_err(p.err, CIE_ERRBIT_LEN);
+  s.t0 = t0;
+  s.slot = (int)slot;
+  s.L = (int)min((int64_t)p.max_rows, t1 - t0);
+  s.c = (int)c;
+  return s;
+}
+
+// How a sequence is cut: its tiles' rows, and key tiles an item at most.
+struct Q8Cut {
+  bool narrow;
+  int R, n_rt, share;
+  __device__ __forceinline__ Q8Cut(const Q8PlanParams& p, const Q8Seq& s, int want) {
+    narrow = (int64_t)s.L * p.G <= 16;
+    R = narrow ? max(1, s.L) : q8_tile_cols() / p.G;
+    n_rt = (s.L + R - 1) / R;
+    share = (max(kQ8MinShare, narrow ? 4 * want : want) + 3) & ~3;
+  }
+  __device__ __forceinline__ int rows(const Q8Seq& s, int r) const { return min(R, s.L - r * R); }
+  __device__ __forceinline__ int key_tiles(const Q8Seq& s, int r) const {
+    return (s.c + r * R + rows(s, r) + 15) >> 4;
+  }
+  __device__ __forceinline__ int chunks(const Q8Seq& s, int r, bool split) const {
+    return split ? min(kQ8MaxChunks, (key_tiles(s, r) + share - 1) / share) : 1;
+  }
+};
+
+__device__ __forceinline__ int64_t plan_wave_sum(int64_t v) {
+  for (int off = 1; off < kWave; off <<= 1) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+__device__ __forceinline__ int plan_wave_sum(int v) {
+  for (int off = 1; off < kWave; off <<= 1) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+
+// Exclusive prefix sums of x[0 .. n) in place, in LDS, by the whole workgroup; the total.
+__device__ __forceinline__ int plan_scan(int* x, int n, int* red) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  int carry = 0;
+  for (int i0 = 0; i0 < n; i0 += kPlanThreadsM) {
+    const int i = i0 + threadIdx.x;
+    const int v = i < n ? x[i] : 0;
+    const int inc = wave_inclusive_sum(v);
+    __syncthreads();
+    if (lane == kWave - 1) red[wave] = inc;
+    __syncthreads();
+    int base = carry, all = carry;
+    for (int w = 0; w < kPlanThreadsM / kWave; ++w) {
+      if (w < wave) base += red[w];
+      all += red[w];
+    }
+    if (i < n) x[i] = base + inc - v;
+    carry = all;
+  }
+  __syncthreads();
+  return carry;
+}
+
+// A wave takes a sequence at a time, a lane one of its query tiles.
+//
+// Key tiles an item holds at most: with W the launch's work in key tiles of wide items (a narrow item's key tile
+// counts a quarter), want = W / kQ8Slots, 4 want for narrow items, and kQ8MinShare at least.  A tile of kt > share
+// key tiles becomes ceil(kt / share) items, so the items beyond one a tile are at most kQ8Slots, split tiles at most
+// that many, and their items at most kMaxSplitItems.
+__global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanParams p) {
+  __shared__ int sm_items[kQ8MaxSeqs];   // items, then their first index (narrow ones: among narrow)
+  __shared__ int sm_narrow[kQ8MaxSeqs];
+  __shared__ int sm_rows[kQ8MaxSeqs];    // partial rows
+  __shared__ int sm_ctr[kQ8MaxSeqs];     // split (tile, kv head)s
+  __shared__ int sm_red[kPlanThreadsM / kWave];
+  __shared__ unsigned long long sm_work;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  constexpr int kWaves = kPlanThreadsM / kWave;
+  if (threadIdx.x == 0) sm_work = 0;
+  __syncthreads();
+  for (int b = wave; b < p.B; b += kWaves) {
+    const Q8Seq s = q8_seq(p, b, lane == 0);
+    const Q8Cut cut(p, s, 0);
+    int64_t w = 0;
+    for (int r = lane; r < cut.n_rt; r += kWave) w += cut.narrow ? (cut.key_tiles(s, r) + 3) / 4 : cut.key_tiles(s, r);
+    w = plan_wave_sum(w);
+    if (lane == 0) atomicAdd(&sm_work, (unsigned long long)w * p.H_kv);
+  }
+  __syncthreads();
+  const int want = (int)min((int64_t)1 << 26, ((int64_t)sm_work + kQ8Slots - 1) / kQ8Slots);
+  for (int b = wave; b < p.B; b += kWaves) {
+    const Q8Seq s = q8_seq(p, b, false);
+    const Q8Cut cut(p, s, want);
+    int rows = 0;
+    for (int r = lane; r < cut.n_rt; r += kWave) {
+      const int n = cut.chunks(s, r, true);
+      if (n > 1) rows += n * cut.rows(s, r) * p.G;
+    }
+    rows = plan_wave_sum(rows);
+    if (lane == 0) sm_rows[b] = rows * p.H_kv;
+  }
+  __syncthreads();
+  plan_scan(sm_rows, p.B, sm_red);
+  // sequences whose partial rows would end past the buffer run unsplit
+  auto splits = [&](int b, const Q8Seq& s, const Q8Cut& cut) {
+    int rows = 0;
+    for (int r = lane; r < cut.n_rt; r += kWave) {
+      const int n = cut.chunks(s, r, true);
+      if (n > 1) rows += n * cut.rows(s, r) * p.G;
+    }
+    return (int64_t)sm_rows[b] + (int64_t)plan_wave_sum(rows) * p.H_kv <= p.part_cap;
+  };
+  for (int b = wave; b < p.B; b += kWaves) {
+    const Q8Seq s = q8_seq(p, b, false);
+    const Q8Cut cut(p, s, want);
+    const bool split = splits(b, s, cut);
+    int items = 0, ctr = 0;
+    for (int r = lane; r < cut.n_rt; r += kWave) {
+      const int n = cut.chunks(s, r, split);
+      items += n;
+      ctr += n > 1;
+    }
+    items = plan_wave_sum(items) * p.H_kv;
+    ctr = plan_wave_sum(ctr) * p.H_kv;
+    if (lane == 0) {
+      sm_items[b] = cut.narrow ? 0 : items;
+      sm_narrow[b] = cut.narrow ? items : 0;
+      sm_ctr[b] = ctr;
+    }
+  }
+  __syncthreads();
+  const int n_wide = plan_scan(sm_items, p.B, sm_red);
+  const int n_items = n_wide + plan_scan(sm_narrow, p.B, sm_red);
+  plan_scan(sm_ctr, p.B, sm_red);
+  const bool fits = n_items <= p.plan_cap;
+  if (threadIdx.x == 0) {
+    p.plan[0] = fits ? n_items : 0;
+#pragma unroll
+    for (int i = 1; i < kHeadWords; ++i) p.plan[i] = plan_word(p, i - 1, p.D);
+    if (!fits) set_err(p.err, CIE_ERRBIT_PLAN);
+  }
+  if (!fits) return;
+  Q8Item* const items = reinterpret_cast<Q8Item*>(p.plan + kHeadWords);
+  for (int b = wave; b < p.B; b += kWaves) {
+    const Q8Seq s = q8_seq(p, b, false);
+    const Q8Cut cut(p, s, want);
+    const bool split = splits(b, s, cut);
+    int at = cut.narrow ? n_wide + sm_narrow[b] : sm_items[b];
+    int row_at = sm_rows[b], ctr_at = sm_ctr[b];
+    for (int r0 = 0; r0 < cut.n_rt; r0 += kWave) {
+      const int r = cut.n_rt - 1 - (r0 + lane);  // the longest tiles first
+      const bool live = r >= 0;
+      const int n = live ? cut.chunks(s, r, split) : 0;
+      const int rows = live ? cut.rows(s, r) : 0, cols = rows * p.G;
+      const int mine = n * p.H_kv, my_rows = n > 1 ? n * cols * p.H_kv : 0, my_ctr = n > 1 ? p.H_kv : 0;
+      const int i_inc = wave_inclusive_sum(mine), r_inc = wave_inclusive_sum(my_rows), c_inc = wave_inclusive_sum(my_ctr);
+      if (live) {
+        const int kt = cut.key_tiles(s, r);
+        Q8Item it;
+        it.tok0 = (int)(s.t0 + r * cut.R);
+        it.rows = cut.narrow ? -rows : rows;
+        it.slot = s.slot;
+        it.pos0 = s.c + r * cut.R;
+        it.n_chunks = n;
+        it.pad = 0;
+        // near-equal chunks in whole stages (4 tiles): their share of the tile's stages, rounded up
+        const int per = 4 * ((((kt + 3) >> 2) + n - 1) / n);
+        int i = at + i_inc - mine, pr = row_at + r_inc - my_rows;
+        for (int g = 0; g < p.H_kv; ++g) {
+          it.g = g;
+          it.pbase = pr;
+          it.ctr = n > 1 ? ctr_at + c_inc - my_ctr + g : 0;
+          for (int c = 0; c < n; ++c, ++i) {
+            it.chunk = c;
+            it.t0 = min(kt, c * per);
+            it.t1 = min(kt, it.t0 + per);
+            items[i] = it;
+          }
+          pr += n * cols;
+        }
+      }
+      at += __builtin_amdgcn_readlane(i_inc, kWave - 1);
+      row_at += __builtin_amdgcn_readlane(r_inc, kWave - 1);
+      ctr_at += __builtin_amdgcn_readlane(c_inc, kWave - 1);
+    }
+  }
+}
+
+// ---- the attention ----
+
+template <int D>
+struct Q8Lds {
+  static constexpr int kK = 4 * Geo<D>::KS * kWave;  // operand slots of a stage
+  static constexpr int kV = 2 * Geo<D>::NT * kWave;
+  static constexpr int kStage = kK + kV;
+  static constexpr int kFold = kMW * 16 * (D / 4 + 1) + 2 * kMW * 16 / 4;
+  static constexpr int kSlots = 2 * kStage > kFold ? 2 * kStage : kFold;
+};
+
+// Column cc of an item: its row and head, and where its output goes.
+struct Q8Col {
+  int row, head;
+  __device__ __forceinline__ Q8Col(const Q8MixedParams& p, int cc)
+      : row(magic_div(cc, p.g_magic)), head(cc - magic_div(cc, p.g_magic) * p.G) {}
+};
+template <int D>
+__device__ __forceinline__ int64_t out_row(const Q8MixedParams& p, const Q8Item& it, const Q8Col& c) {
+  return ((int64_t)(it.tok0 + c.row) * p.H_q + it.g * p.G + c.head) * D;
+}
+
+// The wave's tiles: t0 + wave + 4 k, byte offsets and scales of 64 of them in its lanes.
+template <int D>
+struct WaveTiles {
+  const Q8MixedParams& p;
+  const Q8Src src;
+  const int64_t* bt_row;
+  int t0, n, tpp, lane;
+  int64_t off;
+  f32x2 sc;
+  __device__ __forceinline__ WaveTiles(const Q8MixedParams& p_, const Q8Item& it, int wave, int lane_)
+      : p(p_),
+        src{p_.k_pool, p_.v_pool, p_.scales, p_.pool_page_stride, (int64_t)it.g * p_.pool_head_stride, p_.H_kv, it.g,
+            p_.page_size >> 4},
+        bt_row(p_.block_table + (int64_t)it.slot * p_.bt_stride),
+        t0(uniform(it.t0 + wave)),
+        n(uniform(max(0, (it.t1 - it.t0 - wave + 3) >> 2))),
+        tpp(p_.page_size >> 4),
+        lane(lane_),
+        off(0),
+        sc{1.f, 1.f} {}
+  __device__ __forceinline__ void gather(int c0) {
+    if (c0 + lane < n) {
+      const int t = t0 + 4 * (c0 + lane);
+      int64_t page = bt_row[t / tpp];
+      if (page < 0 || page >= p.n_pages) {
+        set_err(p.err, CIE_ERRBIT_PAGE);
+        page = 0;
+      }
+      off = src.tile((int)page, t % tpp, D);
+      sc = *reinterpret_cast<const f32x2*>(src.scale((int)page, t % tpp));
+    }
+  }
+  // tile k (of the gathered 64), rows below key_end; a k past the last: no rows
+  template <int POL>
+  __device__ __forceinline__ void load(Q8Tile<D>& t, int c0, int k, int key_end, const Q8Lane<D>& lo) const {
+    const bool real = c0 + k < n;
+    const int rows = real ? min(16, key_end - 16 * (t0 + 4 * (c0 + k))) : 0;
+    const int64_t o = readlane64(off, real ? k : 0);
+    q8_load<D, POL>(t, q8_rsrc(p.k_pool, o, rows, D), q8_rsrc(p.v_pool, o, rows, D), lo);
+  }
+  __device__ __forceinline__ float scale(int i, int k) const {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[i]), k));
+  }
+};
+
+// Merge a split tile's chunk states into o: a thread owns 4 dims of a column and takes the chunks in groups,
+// their loads all issued before any is used.
+template <int D>
+__device__ __forceinline__ void q8_mixed_merge(const Q8MixedParams& p, const Q8Item& it, int cols) {
+  constexpr int D4 = D / 4, kGroup = 8;
+  const __amdgpu_buffer_rsrc_t racc =
+      coherent_rsrc(p.part_acc + (int64_t)it.pbase * D, (uint32_t)(cols * it.n_chunks * D * sizeof(float)));
+  for (int u = threadIdx.x; u < cols * D4; u += kMThreads) {
+    const int cc = u / D4, d4 = u - cc * D4;
+    float M = kEmptyMax, den = 0.f;
+    f32x4 num = {0.f, 0.f, 0.f, 0.f};
+    for (int c0 = 0; c0 < it.n_chunks; c0 += kGroup) {
+      float ms[kGroup], ls[kGroup];
+      f32x4 as[kGroup];
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        const bool live = c0 + i < it.n_chunks;
+        const int row = (live ? c0 + i : 0) * cols + cc;
+        ms[i] = agent_load(&p.part_m[it.pbase + row]);
+        ls[i] = agent_load(&p.part_l[it.pbase + row]);
+        as[i] = agent_load4(racc, (uint32_t)((row * D + 4 * d4) * sizeof(float)));
+        if (!live) {
+          ms[i] = kEmptyMax;
+          ls[i] = 0.f;
+          as[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+      }
+      float Mn = M;
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) Mn = fmaxf(Mn, ms[i]);
+      const float k = fast_exp2(M - Mn);
+      num *= k;
+      den *= k;
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        const float a = fast_exp2(ms[i] - Mn);
+        num += a * as[i];
+        den += a * ls[i];
+      }
+      M = Mn;
+    }
+    f16x4 o4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o4[i] = (f16)(den > 0.f ? num[i] / den : 0.f);
+    *reinterpret_cast<f16x4*>(p.o + out_row<D>(p, it, Q8Col(p, cc)) + 4 * d4) = o4;
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void load_col_q(f16x8 (&q)[Geo<D>::KS], int& lim, const Q8MixedParams& p, const Q8Item& it,
+                                           int cols, int cc, int grp) {
+  const bool live = cc < cols;
+  const Q8Col c(p, live ? cc : 0);
+  const f16* const row = p.q + out_row<D>(p, it, c);
+#pragma unroll
+  for (int ks = 0; ks < Geo<D>::KS; ++ks) {
+    q[ks] = *reinterpret_cast<const f16x8*>(row + q8_dim(ks, grp));
+    if (!live) q[ks] = f16x8{};
+  }
+  lim = live ? it.pos0 + c.row + 1 : kNoKey;  // (an absent column attends everything, for no one)
+}
+
+// Wide item, NA column tiles in this wave (0: it only loads).
+template <int D, int NA>
+__device__ __forceinline__ void wide_item(const Q8MixedParams& p, const Q8Item& it, int cols, f32x4* lds, int wave,
+                                          int lane) {
+  constexpr int KS = Geo<D>::KS, NT = Geo<D>::NT;
+  constexpr int NC = NA > 0 ? NA : 1;
+  const int r16 = lane & 15, grp = lane >> 4;
+  const Q8Lane<D> lo(r16, grp);
+  const int key_end = it.pos0 + it.rows;
+  WaveTiles<D> tiles(p, it, wave, lane);
+  f16x8 q[NC][KS];
+  int lim[NC];
+  tiles.gather(0);
+  if constexpr (NA > 0) {
+#pragma unroll
+    for (int c = 0; c < NA; ++c) load_col_q<D>(q[c], lim[c], p, it, cols, 16 * (wave + kMW * c) + r16, grp);
+  }
+  int mask_from = kNoKey;
+  if constexpr (NA > 0) {
+#pragma unroll
+    for (int c = 0; c < NA; ++c) mask_from = min(mask_from, lim[c]);
+    for (int off = 1; off < kWave; off <<= 1) mask_from = min(mask_from, __shfl_xor(mask_from, off, kWave));
+    mask_from = uniform(mask_from);
+  }
+  SoftmaxAcc<D, NC> st;
+  st.init();
+  const int n_stages = uniform((it.t1 - it.t0 + 3) >> 2);
+  Q8Tile<D> raw;
+  tiles.template load<0>(raw, 0, 0, key_end, lo);
+  for (int sg = 0; sg < n_stages; ++sg) {
+    f16x8* const kbuf = reinterpret_cast<f16x8*>(lds) + (sg & 1) * Q8Lds<D>::kStage;
+    f16x8* const vbuf = kbuf + Q8Lds<D>::kK;
+    {  // this wave's tile, converted into operand slots
+      const int k = sg & (kWave - 1);
+      const float ks = tiles.scale(0, k), vs = tiles.scale(1, k);
+      f16x8 ko[KS];
+      q8_k_operand<D>(ko, raw, ks);
+#pragma unroll
+      for (int i = 0; i < KS; ++i) kbuf[(wave * KS + i) * kWave + lane] = ko[i];
+      f16x8 va[NT];
+      q8_v_operand<D>(va, 0, raw, vs);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        reinterpret_cast<f16x4*>(vbuf + ((wave >> 1) * NT + nt) * kWave + lane)[wave & 1] =
+            f16x4{va[nt][0], va[nt][1], va[nt][2], va[nt][3]};
+    }
+    if (sg + 1 < n_stages) {
+      const int k = (sg + 1) & (kWave - 1);
+      if (k == 0) tiles.gather(sg + 1);
+      tiles.template load<0>(raw, sg + 1 - k, k, key_end, lo);
+    }
+    __syncthreads();
+    if constexpr (NA > 0) {
+#pragma unroll
+      for (int pr = 0; pr < 2; ++pr) {
+        const int key0 = 16 * (it.t0 + 4 * sg + 2 * pr);
+        if (key0 < key_end) {  // uniform
+          f16x8 ka[KS], kb[KS];
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            ka[i] = kbuf[(2 * pr * KS + i) * kWave + lane];
+            kb[i] = kbuf[((2 * pr + 1) * KS + i) * kWave + lane];
+          }
+          auto v = [&](f16x8 (&va)[NT]) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) va[nt] = vbuf[(pr * NT + nt) * kWave + lane];
+          };
+          q8_step<D, NC>(st, ka, kb, v, q, key0, key0 + 16, lim, key0 + 32 > mask_from, p.scale_log2, grp);
+        }
+      }
+    }
+  }
+  if constexpr (NA > 0) {
+    const __amdgpu_buffer_rsrc_t racc =
+        coherent_rsrc(p.part_acc + (int64_t)it.pbase * D,
+                      it.n_chunks > 1 ? (uint32_t)(cols * it.n_chunks * D * sizeof(float)) : 0);
+#pragma unroll
+    for (int c = 0; c < NA; ++c) {
+      const int cc = 16 * (wave + kMW * c) + r16;
+      if (cc >= cols) continue;
+      const float l = st.lsum[c][0];
+      if (it.n_chunks == 1) {
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        f16* const o = p.o + out_row<D>(p, it, Q8Col(p, cc)) + NT * 4 * grp;
+#pragma unroll
+        for (int i = 0; i < NT / 2; ++i) {  // the lane's 4 NT dims, 8 at a time
+          f16x8 x;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = (f16)(st.acc[c][(8 * i + j) % NT][(8 * i + j) / NT] * inv);
+          *reinterpret_cast<f16x8*>(o + 8 * i) = x;
+        }
+      } else {
+        const int row = it.chunk * cols + cc;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          agent_store4(racc, (uint32_t)((row * D + NT * 4 * grp + 4 * i) * sizeof(float)),
+                       f32x4{st.acc[c][(4 * i) % NT][(4 * i) / NT], st.acc[c][(4 * i + 1) % NT][(4 * i + 1) / NT],
+                             st.acc[c][(4 * i + 2) % NT][(4 * i + 2) / NT],
+                             st.acc[c][(4 * i + 3) % NT][(4 * i + 3) / NT]});
+        if (grp == 0) {
+          agent_store(&p.part_m[it.pbase + row], st.m[c]);
+          agent_store(&p.part_l[it.pbase + row], l);
+        }
+      }
+    }
+  }
+}
+
+// Narrow item: one column tile, the keys dealt over the waves.
+template <int D>
+__device__ __forceinline__ void narrow_item(const Q8MixedParams& p, const Q8Item& it, int cols, f32x4* lds, int wave,
+                                            int lane) {
+  constexpr int KS = Geo<D>::KS, NT = Geo<D>::NT, D4 = D / 4;
+  constexpr int PF = D == 64 ? 3 : 2;
+  const int r16 = lane & 15, grp = lane >> 4;
+  const Q8Lane<D> lo(r16, grp);
+  const int key_end = it.pos0 - it.rows;  // (rows: negative here)
+  WaveTiles<D> tiles(p, it, wave, lane);
+  tiles.gather(0);
+  f16x8 q[1][KS];
+  int lim[1];
+  load_col_q<D>(q[0], lim[0], p, it, cols, r16, grp);
+  const int mask_from = it.pos0 + 1;  // the first row's keys
+  SoftmaxAcc<D, 1> st;
+  st.init();
+  for (int c0 = 0; c0 < tiles.n; c0 += kWave) {
+    if (c0 > 0) tiles.gather(c0);
+    const int n_chunk = min(kWave, tiles.n - c0);
+    const int n_steps = (n_chunk + 1) >> 1;
+    Q8Tile<D> ring[PF + 1][2];
+    auto issue = [&](int i, int j) {  // (tiles past the last: no rows)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        tiles.template load<kBufNt>(ring[i][u], c0, 2 * j + u < n_chunk ? 2 * j + u : tiles.n, key_end, lo);
+    };
+#pragma unroll
+    for (int j = 0; j < PF; ++j) issue(j, j);
+    for (int j0 = 0; j0 < n_steps; j0 += PF + 1) {
+#pragma unroll
+      for (int u = 0; u <= PF; ++u) {
+        const int j = j0 + u;
+        issue((u + PF) % (PF + 1), j + PF);
+        if (j < n_steps) {
+          const int ka = 2 * j, kb = min(ka + 1, n_chunk - 1);
+          const int key0a = 16 * (tiles.t0 + 4 * (c0 + ka));
+          const int key0b = ka + 1 < n_chunk ? key0a + 64 : kNoKey;
+          q8_attend<D>(st, ring[u][0], ring[u][1], tiles.scale(0, ka), tiles.scale(1, ka), tiles.scale(0, kb),
+                       tiles.scale(1, kb), q, key0a, key0b, lim, max(key0a, key0b) + 16 > mask_from, p.scale_log2, grp);
+        }
+      }
+    }
+  }
+  // fold the waves
+  f32x4(*const sm_acc)[16][D4 + 1] = reinterpret_cast<f32x4(*)[16][D4 + 1]>(lds);
+  float(*const sm_m)[16] = reinterpret_cast<float(*)[16]>(lds + kMW * 16 * (D4 + 1));
+  float(*const sm_l)[16] = sm_m + kMW;
+  if (grp == 0) {
+    sm_m[wave][r16] = st.m[0];
+    sm_l[wave][r16] = st.lsum[0][0];
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int n4 = 0; n4 < NT / 4; ++n4)
+      sm_acc[wave][r16][(NT * (4 * grp + r)) / 4 + n4] = f32x4{st.acc[0][4 * n4][r], st.acc[0][4 * n4 + 1][r],
+                                                              st.acc[0][4 * n4 + 2][r], st.acc[0][4 * n4 + 3][r]};
+  __syncthreads();
+  const __amdgpu_buffer_rsrc_t racc =
+      coherent_rsrc(p.part_acc + (int64_t)it.pbase * D,
+                    it.n_chunks > 1 ? (uint32_t)(cols * it.n_chunks * D * sizeof(float)) : 0);
+  for (int u = threadIdx.x; u < cols * D4; u += kMThreads) {
+    const int cc = u / D4, d4 = u - cc * D4;
+    float M = kEmptyMax, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < kMW; ++w) M = fmaxf(M, sm_m[w][cc]);
+    f32x4 num = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kMW; ++w) {
+      const float a = fast_exp2(sm_m[w][cc] - M);
+      num += a * sm_acc[w][cc][d4];
+      den += a * sm_l[w][cc];
+    }
+    if (it.n_chunks == 1) {
+      f16x4 o4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o4[i] = (f16)(den > 0.f ? num[i] / den : 0.f);
+      *reinterpret_cast<f16x4*>(p.o + out_row<D>(p, it, Q8Col(p, cc)) + 4 * d4) = o4;
+    } else {
+      const int row = it.chunk * cols + cc;
+      agent_store4(racc, (uint32_t)((row * D + 4 * d4) * sizeof(float)), num);
+      if (d4 == 0) {
+        agent_store(&p.part_m[it.pbase + row], M);
+        agent_store(&p.part_l[it.pbase + row], den);
+      }
+    }
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(kMThreads) __attribute__((amdgpu_waves_per_eu(2)))
+void q8_mixed_kernel(Q8MixedParams p) {
+  __shared__ f32x4 lds[Q8Lds<D>::kSlots];
+  __shared__ int sm_last;
+  const int32_t* const head = p.plan;
+  bool same = true;
+#pragma unroll
+  for (int i = 1; i < kHeadWords; ++i) same &= head[i] == plan_word(p, i - 1, D);
+  if (!same) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) set_err(p.err, CIE_ERRBIT_PLAN);
+    return;
+  }
+  if ((int)blockIdx.x >= head[0]) return;
+  const Q8Item it = reinterpret_cast<const Q8Item*>(p.plan + kHeadWords)[blockIdx.x];
+  const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave);
+  const bool narrow = it.rows < 0;
+  const int cols = (narrow ? -it.rows : it.rows) * p.G;
+  if (narrow) {
+    narrow_item<D>(p, it, cols, lds, wave, lane);
+  } else {
+    const int n_ct = (cols + 15) >> 4;
+    const int na = n_ct > wave ? (n_ct - wave + kMW - 1) / kMW : 0;  // column tiles wave, wave + 4
+    if (na >= 2)
+      wide_item<D, 2>(p, it, cols, lds, wave, lane);
+    else if (na == 1)
+      wide_item<D, 1>(p, it, cols, lds, wave, lane);
+    else
+      wide_item<D, 0>(p, it, cols, lds, wave, lane);
+  }
+  if (it.n_chunks == 1) return;
+  int32_t* const arrival = p.counters + it.ctr;
+  if (!arrive_last(arrival, p.n_ctr, it.n_chunks, &sm_last, p.err)) return;
+  q8_mixed_merge<D>(p, it, cols);
+  if (threadIdx.x == 0) counter_reset(arrival);
+}
+
+// Items a plan can hold: one a query tile and kv head, and kQ8Slots more from splitting.
+static int64_t q8_plan_items(int64_t B, int64_t total_T, int64_t H_q, int64_t H_kv) {
+  const int64_t R = q8_tile_cols() / (H_q / H_kv);
+  return H_kv * (total_T / R + B) + kQ8Slots;
+}
+
+// Partial rows a launch can need: its split items' columns, and no more than kQ8MaxChunks a query row and head.
+static int64_t q8_part_rows(int64_t total_T, int64_t H_q) {
+  const int64_t most = (int64_t)kMaxSplitItems * q8_tile_cols();
+  return total_T > most / (kQ8MaxChunks * H_q) ? most : kQ8MaxChunks * total_T * H_q;
+}
+
+static int q8_mixed_check(int64_t B, int64_t total_T, int64_t max_seqlen, int64_t H_q, int64_t H_kv, int64_t D,
+                          int64_t page_size, int64_t bt_width, int64_t n_slots) {
+  if (B < 0 || total_T < 0 || max_seqlen < 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || page_size <= 0 ||
+      bt_width <= 0 || n_slots <= 0)
+    return CIE_EINVAL;
+  if (H_q / H_kv > 16 || (D != 64 && D != 128) || page_size % 16 != 0 || B > kQ8MaxSeqs || H_kv > 4096 ||
+      total_T > (1 << 24) || bt_width > 0x3fffffff / page_size ||
+      q8_plan_items(B, total_T, H_q, H_kv) > 0x7fffffff / kItemWords)
+    return CIE_EUNSUPPORTED;
+  return CIE_OK;
+}
+
+}  // namespace cie
+
+using namespace cie;
+
+extern "C" int64_t cie_q8_mixed_plan_bytes(int64_t B, int64_t total_T, int64_t H_q, int64_t H_kv) {
+  if (B < 0 || total_T < 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || H_q / H_kv > 16 || B > kQ8MaxSeqs ||
+      H_kv > 4096 || total_T > (1 << 24))
+    return -1;
+  return (kHeadWords + q8_plan_items(B, total_T, H_q, H_kv) * kItemWords) * 4;
+}
+
+extern "C" int64_t cie_q8_mixed_partials_bytes(int64_t total_T, int64_t H_q, int64_t D) {
+  if (total_T < 0 || H_q <= 0 || H_q > 65536 || D <= 0) return -1;
+  const int64_t rows = q8_part_rows(total_T, H_q);
+  auto up = [](int64_t x) { return (x + 255) & ~int64_t(255); };
+  return 2 * up(rows * 4) + rows * D * 4;
+}
+
+extern "C" int64_t cie_q8_mixed_counters(void) { return 2 * kQ8Slots; }
+
+extern "C" int cie_q8_mixed_plan(int32_t* plan, int64_t plan_bytes, const int64_t* cu_seqlens, const int64_t* kv_lens,
+                                 const int64_t* slot_ids, int64_t B, int64_t total_T, int64_t max_seqlen, int64_t H_q,
+                                 int64_t H_kv, int64_t D, int64_t page_size, int64_t bt_width, int64_t n_slots,
+                                 int32_t* err, void* stream) {
+  if (int rc = q8_mixed_check(B, total_T, max_seqlen, H_q, H_kv, D, page_size, bt_width, n_slots)) return rc;
+  if (!plan || (reinterpret_cast<uintptr_t>(plan) & 15) || (B > 0 && (!cu_seqlens || !kv_lens || !slot_ids)) ||
+      plan_bytes < cie_q8_mixed_plan_bytes(B, total_T, H_q, H_kv))
+    return CIE_EINVAL;
+  Q8PlanParams p{};
+  p.plan = plan;
+  p.cu_seqlens = cu_seqlens;
+  p.kv_lens = kv_lens;
+  p.slot_ids = slot_ids;
+  p.total_T = total_T;
+  p.cap = bt_width * page_size;
+  p.B = (int32_t)B;
+  p.n_slots = (int32_t)(n_slots > 0x7fffffff ? 0x7fffffff : n_slots);
+  p.H_q = (int32_t)H_q;
+  p.H_kv = (int32_t)H_kv;
+  p.G = (int32_t)(H_q / H_kv);
+  p.D = (int32_t)D;
+  p.page_size = (int32_t)page_size;
+  p.bt_width = (int32_t)bt_width;
+  p.max_rows = (int32_t)(max_seqlen > total_T ? total_T : max_seqlen);
+  p.part_cap = (int32_t)q8_part_rows(total_T, H_q);
+  p.plan_cap = (int32_t)q8_plan_items(B, total_T, H_q, H_kv);
+  p.err = err;
+  hipLaunchKernelGGL(q8_mixed_plan_kernel, dim3(1), dim3(kPlanThreadsM), 0, static_cast<hipStream_t>(stream), p);
+  return (int)hipGetLastError();
+}
+
+extern "C" int cie_q8_mixed(void* o, const void* q, const void* k_pool, const void* v_pool, const void* scales,
+                            const int32_t* plan, int64_t plan_bytes, const int64_t* block_table, void* partials,
+                            int64_t partials_bytes, int32_t* counters, int64_t B, int64_t total_T, int64_t H_q,
+                            int64_t H_kv, int64_t D, int64_t page_size, int64_t n_pages, int64_t pool_page_stride,
+                            int64_t pool_head_stride, int64_t bt_stride, int64_t bt_width, int64_t n_slots,
+                            int32_t* err, void* stream) {
+  if (int rc = q8_mixed_check(B, total_T, total_T, H_q, H_kv, D, page_size, bt_width, n_slots)) return rc;
+  if (n_pages <= 0 || n_pages > 0x7fffffff || bt_stride < bt_width || pool_page_stride % 16 != 0 ||
+      pool_head_stride % 16 != 0)
+    return CIE_EINVAL;
+  if (B == 0 || total_T == 0) return CIE_OK;
+  if (!o || !q || !k_pool || !v_pool || !scales || !plan || !block_table || !partials || !counters ||
+      plan_bytes < cie_q8_mixed_plan_bytes(B, total_T, H_q, H_kv) ||
+      partials_bytes < cie_q8_mixed_partials_bytes(total_T, H_q, D))
+    return CIE_EINVAL;
+  if ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) |
+       reinterpret_cast<uintptr_t>(v_pool) | reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(plan) |
+       reinterpret_cast<uintptr_t>(partials) | reinterpret_cast<uintptr_t>(counters)) & 15)
+    return CIE_EINVAL;
+  Q8MixedParams p{};
+  p.o = static_cast<f16*>(o);
+  p.q = static_cast<const f16*>(q);
+  p.k_pool = static_cast<const uint8_t*>(k_pool);
+  p.v_pool = static_cast<const uint8_t*>(v_pool);
+  p.scales = static_cast<const float*>(scales);
+  p.block_table = block_table;
+  p.plan = plan;
+  const int64_t rows = q8_part_rows(total_T, H_q);
+  auto up = [](int64_t x) { return (x + 255) & ~int64_t(255); };
+  char* const ws = static_cast<char*>(partials);
+  p.part_m = reinterpret_cast<float*>(ws);
+  p.part_l = reinterpret_cast<float*>(ws + up(rows * 4));
+  p.part_acc = reinterpret_cast<float*>(ws + 2 * up(rows * 4));
+  p.counters = counters;
+  p.pool_page_stride = pool_page_stride;
+  p.pool_head_stride = pool_head_stride;
+  p.bt_stride = bt_stride;
+  p.n_pages = n_pages;
+  p.total_T = total_T;
+  p.part_cap = (int32_t)rows;
+  p.n_ctr = kQ8Slots;
+  p.plan_cap = (int32_t)q8_plan_items(B, total_T, H_q, H_kv);
+  p.B = (int32_t)B;
+  p.bt_width = (int32_t)bt_width;
+  p.n_slots = (int32_t)(n_slots > 0x7fffffff ? 0x7fffffff : n_slots);
+  p.H_q = (int32_t)H_q;
+  p.H_kv = (int32_t)H_kv;
+  p.G = (int32_t)(H_q / H_kv);
+  p.page_size = (int32_t)page_size;
+  p.g_magic = div_magic((uint32_t)p.G);
+  p.scale_log2 = kLog2e / __builtin_sqrtf((float)D);
+  p.err = err;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (D == 64)
+    hipLaunchKernelGGL(q8_mixed_kernel<64>, dim3((unsigned)p.plan_cap), dim3(kMThreads), 0, s, p);
+  else
+    hipLaunchKernelGGL(q8_mixed_kernel<128>, dim3((unsigned)p.plan_cap), dim3(kMThreads), 0, s, p);
+  return (int)hipGetLastError();
+}

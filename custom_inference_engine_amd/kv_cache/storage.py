@@ -20,6 +20,7 @@ import math
 import torch
 
 from .. import _native
+from . import quant
 
 
 def _as_rows(x: torch.Tensor, h_kv: int, d: int) -> torch.Tensor:
@@ -138,6 +139,8 @@ class KVStorage:
     """Paged per-layer K/V pools plus per-slot lengths and block tables.
 
     Same constructor and attributes as the reference (kv_cache/storage.py:6-60).
+    ``dtype=torch.float8_e4m3fn`` holds the rows in 8 bits (``quant.py``), at half
+    the bytes: ``scales[l]`` (None for 16-bit pools) is layer l's block scales.
     """
 
     def __init__(self, config, max_cache_len, page_size, n_slots, device, dtype):
@@ -162,22 +165,48 @@ class KVStorage:
         self.keys = list(self._k_storage.unbind(0))
         self.values = list(self._v_storage.unbind(0))
 
+        self.scales = None
+        if dtype == torch.float8_e4m3fn:
+            if page_size % quant.BLOCK or self.head_dim not in (64, 128):
+                raise AssertionError("an 8-bit cache needs a page_size that is a multiple of 16 and head_dim 64 or 128")
+            self._scales = torch.ones(shape[:3] + (page_size // quant.BLOCK, 2), device=device, dtype=torch.float32)
+            self.scales = list(self._scales.unbind(0))
+
         self.lens = torch.zeros((n_slots,), dtype=torch.long, device=self.device)
         self.block_table = torch.zeros((n_slots, self.n_pages), dtype=torch.long, device=self.device)
         self.last_generated = torch.zeros((n_slots,), dtype=torch.long, device=self.device)
 
     def mixed_update(self, layer_num: int, pages: torch.Tensor, offsets: torch.Tensor,
                      k_proj: torch.Tensor, v_proj: torch.Tensor) -> None:
+        if self.scales is not None:
+            torch.ops.inference.kv_append_tokens_q8(
+                self.keys[layer_num], self.values[layer_num], self.scales[layer_num], k_proj, v_proj, pages, offsets
+            )
+            return
         torch.ops.inference.kv_append_tokens(
             self.keys[layer_num], self.values[layer_num], k_proj, v_proj, pages, offsets
         )
 
     def decode_update(self, layer_num: int, slot_ids: torch.Tensor,
                       k_proj: torch.Tensor, v_proj: torch.Tensor) -> None:
+        if self.scales is not None:
+            torch.ops.inference.kv_append_decode_q8(
+                self.keys[layer_num], self.values[layer_num], self.scales[layer_num], k_proj, v_proj,
+                slot_ids, self.lens, self.block_table,
+            )
+            return
         torch.ops.inference.kv_append_decode(
             self.keys[layer_num], self.values[layer_num], k_proj, v_proj,
             slot_ids, self.lens, self.block_table,
         )
+
+    def read_tokens(self, layer_num: int, pages: torch.Tensor, offsets: torch.Tensor):
+        """The held rows ``(pages[t], :, offsets[t])``: K and V, each (1, T, H_kv, D), as
+        ``mixed_update`` takes them (what an 8-bit cache holds comes back as float16)."""
+        if self.scales is not None:
+            return quant.kv_read_tokens_q8(self.keys[layer_num], self.values[layer_num], self.scales[layer_num],
+                                           pages, offsets)
+        return tuple(pool[layer_num][pages, :, offsets][None] for pool in (self.keys, self.values))
 
     # lens[unused_idx] = 0 as a device kernel (a 1-element multiply), not a
     # host scalar copy, so a decode step that contains it can be graph-captured

@@ -16,11 +16,14 @@ from __future__ import annotations
 import torch
 from torch.fx.passes.split_module import split_module
 
+from ..attn import quant as _quant  # noqa: F401  (registers the 8-bit cache's op)
+
 MIXED_ATTENTION = torch.ops.inference.gqa_mixed_attention.default
+MIXED_ATTENTION_Q8 = torch.ops.inference.gqa_mixed_attention_q8.default  # the same over an 8-bit cache
 
 
 def is_attention(node) -> bool:
-    return node.op == "call_function" and node.target is MIXED_ATTENTION
+    return node.op == "call_function" and node.target in (MIXED_ATTENTION, MIXED_ATTENTION_Q8)
 
 
 def create_partition(gm: torch.fx.GraphModule) -> dict:

@@ -45,6 +45,7 @@ import contextlib
 import torch
 
 from ..attn.core import gqa_mixed_plan_op
+from ..attn.quant import gqa_mixed_plan_q8_op
 from ..attn.metadata import AttentionMetadata
 from ..graphs import StepGraph, StepInputs
 from ..piecewise import get_piecewise_backend
@@ -93,7 +94,8 @@ class MixedModule:
         # step prepared on the CPU — traced, never run — has none.)
         if kv.keys[0].is_cuda:
             T = self.token_count
-            self.metadata.mixed_plan = gqa_mixed_plan_op(
+            make_plan = gqa_mixed_plan_op if getattr(kv, "scales", None) is None else gqa_mixed_plan_q8_op
+            self.metadata.mixed_plan = make_plan(
                 kv.keys[0], self.cu_seqlens, kv.lens[self.slots], self.slots, kv.block_table, T, T,
                 self.model.config.num_attention_heads)
 

@@ -150,7 +150,7 @@ class ModuleExecutor:
         piecewise = [t for t in self.token_counts if piecewise_above is not None and t > piecewise_above]
         if graph_mixed and piecewise:
             self.buffer = torch.zeros((1, max(piecewise), kv_cache.num_q_heads, kv_cache.head_dim),
-                                      dtype=kv_cache.dtype, device=kv_cache.device)
+                                      dtype=model.dtype, device=kv_cache.device)
         if graph_mixed:
             for t in sorted(self.token_counts, reverse=True):
                 if t in piecewise:

@@ -414,6 +414,133 @@ int cie_mixed_attention_planned(void* o, const void* q,
                                 int64_t bt_stride, int64_t bt_width, int64_t n_slots,
                                 int32_t* err, void* stream);
 
+/*
+ * The 8-bit cache: K and V rows in e4m3 (OCP: finite, largest 448), with a
+ * power-of-two scale for each block of 16 tokens, kv head and K / V.
+ *   pools      : (n_pages, H_kv, page_size, D) bytes, last two dims dense, 16-byte
+ *                aligned, page and head strides multiples of 16 (in elements);
+ *                page_size a multiple of 16, D 64 or 128
+ *   scales     : (n_pages, H_kv, page_size / 16, 2) dense fp32, 16-byte aligned;
+ *                [..., 0] K's and [..., 1] V's, 2^e with -15 <= e <= 8, written by the
+ *                appends.  A held value is byte * 2^e, always an fp16 value.
+ * A block's e is the least with amax <= 448 * 2^e over the rows written since its
+ * row 0 last was: writing row 0 starts the block anew (the bytes of its other rows
+ * then mean nothing until written), writing another row keeps the others, rounded
+ * again where e grows.  Values are rounded to nearest even; beyond +-61440 (240 *
+ * 2^8; infinities too) they are held as that; NaN is held as NaN and not in amax.
+ * Nothing else is shared with the fp16 pools' entry points: strides, indices, err,
+ * counters and partials behave as theirs do.  No call allocates or synchronises.
+ *
+ * Append, as cie_kv_append_decode / _tokens / _tokens_qkv_rope:
+ *  - decode: slots other than padding must not share the page they append to; of a
+ *    slot that comes several times in the batch the last row is written.
+ *  - tokens: (pages[t], offsets[t]) in any order; of an index that comes several
+ *    times the last token is written.  Bad indices are skipped and reported.
+ * Read back: k_out / v_out (T, H_kv, D) dense fp16 = the values of the rows
+ * (pages[t], offsets[t]), exactly; zeros (and a report) for a bad index.
+ */
+int cie_q8_append_decode(void* k_pool, void* v_pool, void* scales,
+                         const void* k_new, const void* v_new,
+                         int64_t k_tok_stride, int64_t k_head_stride,
+                         int64_t v_tok_stride, int64_t v_head_stride,
+                         const int64_t* slot_ids, const int64_t* lens,
+                         const int64_t* block_table, int64_t B, int64_t H_kv,
+                         int64_t page_size, int64_t D, int64_t n_pages,
+                         int64_t pool_page_stride, int64_t pool_head_stride,
+                         int64_t bt_stride, int64_t bt_width, int64_t n_slots,
+                         int32_t* err, void* stream);
+int cie_q8_append_tokens(void* k_pool, void* v_pool, void* scales,
+                         const void* k_new, const void* v_new,
+                         int64_t k_tok_stride, int64_t k_head_stride,
+                         int64_t v_tok_stride, int64_t v_head_stride,
+                         const int64_t* pages, const int64_t* offsets, int64_t T,
+                         int64_t H_kv, int64_t page_size, int64_t D, int64_t n_pages,
+                         int64_t pool_page_stride, int64_t pool_head_stride,
+                         int32_t* err, void* stream);
+int cie_q8_append_tokens_qkv_rope(void* q_out, void* k_pool, void* v_pool, void* scales,
+                                  const void* qkv, int64_t qkv_row_stride,
+                                  const void* cos, const void* sin, int64_t cs_row_stride,
+                                  const int64_t* pages, const int64_t* offsets, int64_t T,
+                                  int64_t H_q, int64_t H_kv, int64_t page_size, int64_t D,
+                                  int64_t n_pages, int64_t pool_page_stride,
+                                  int64_t pool_head_stride, int32_t* err, void* stream);
+int cie_q8_read_tokens(void* k_out, void* v_out, const void* k_pool, const void* v_pool,
+                       const void* scales, const int64_t* pages, const int64_t* offsets,
+                       int64_t T, int64_t H_kv, int64_t page_size, int64_t D,
+                       int64_t n_pages, int64_t pool_page_stride,
+                       int64_t pool_head_stride, int32_t* err, void* stream);
+
+/*
+ * Decode over the 8-bit cache, as cie_paged_decode / _append / _qkv_rope, one launch.
+ * plan: NULL, with n_splits splits per (sequence, kv head), or a step's
+ * cie_paged_decode_plan (same append mode; lens / slot_ids / n_slots are then not
+ * read), with n_splits its n_workgroups.  partials:
+ * cie_paged_decode_planned_partials_bytes(workgroups, H_q, H_kv, D), workgroups =
+ * B * H_kv * n_splits or the plan's; counters: 2 * B * H_kv words; both may be NULL
+ * where workgroups == B * H_kv.  The appending forms leave the same bytes and scales
+ * as cie_q8_append_decode, and attend them.  n_pages < 2^31.
+ */
+int cie_q8_decode(void* o, const void* q, const void* k_pool, const void* v_pool,
+                  const void* scales, const int64_t* lens, const int64_t* slot_ids,
+                  const int64_t* block_table, const int32_t* plan,
+                  void* partials, int32_t* counters,
+                  int64_t B, int64_t H_q, int64_t H_kv, int64_t D, int64_t page_size,
+                  int64_t n_pages, int64_t pool_page_stride, int64_t pool_head_stride,
+                  int64_t bt_stride, int64_t bt_width, int64_t n_slots,
+                  int64_t n_splits, int32_t* err, void* stream);
+int cie_q8_decode_append(void* o, const void* q, void* k_pool, void* v_pool, void* scales,
+                         const void* k_new, const void* v_new,
+                         int64_t k_tok_stride, int64_t k_head_stride,
+                         int64_t v_tok_stride, int64_t v_head_stride,
+                         const int64_t* lens, const int64_t* slot_ids,
+                         const int64_t* block_table, const int32_t* plan,
+                         void* partials, int32_t* counters,
+                         int64_t B, int64_t H_q, int64_t H_kv, int64_t D, int64_t page_size,
+                         int64_t n_pages, int64_t pool_page_stride, int64_t pool_head_stride,
+                         int64_t bt_stride, int64_t bt_width, int64_t n_slots,
+                         int64_t n_splits, int32_t* err, void* stream);
+int cie_q8_decode_qkv_rope(void* o, const void* qkv, int64_t qkv_row_stride,
+                           const void* cos, const void* sin, int64_t cs_row_stride,
+                           void* k_pool, void* v_pool, void* scales,
+                           const int64_t* lens, const int64_t* slot_ids,
+                           const int64_t* block_table, const int32_t* plan,
+                           void* partials, int32_t* counters,
+                           int64_t B, int64_t H_q, int64_t H_kv, int64_t D, int64_t page_size,
+                           int64_t n_pages, int64_t pool_page_stride, int64_t pool_head_stride,
+                           int64_t bt_stride, int64_t bt_width, int64_t n_slots,
+                           int64_t n_splits, int32_t* err, void* stream);
+
+/*
+ * Varlen causal attention over the 8-bit cache, as cie_mixed_attention, from a plan:
+ *   cie_q8_mixed_plan   once per step: the work items of its sequences, into `plan`
+ *                       (cie_q8_mixed_plan_bytes bytes, 16-byte aligned, any
+ *                       contents).  Index errors, and rows at or past max_seqlen
+ *                       (not computed), are reported here.
+ *   cie_q8_mixed        per layer.  A plan made for other sizes (B, total_T, heads,
+ *                       D, page_size, block table) writes nothing and raises
+ *                       CIE_ERRBIT_PLAN; so does a batch of overlapping sequences
+ *                       whose items exceed the plan.
+ * partials: cie_q8_mixed_partials_bytes bytes, 16-byte aligned; counters:
+ * cie_q8_mixed_counters() words, zero before the call and after it.
+ * B <= 2048, H_q / H_kv <= 16, total_T <= 2^24.
+ */
+int64_t cie_q8_mixed_plan_bytes(int64_t B, int64_t total_T, int64_t H_q, int64_t H_kv);
+int64_t cie_q8_mixed_partials_bytes(int64_t total_T, int64_t H_q, int64_t D);
+int64_t cie_q8_mixed_counters(void);
+int cie_q8_mixed_plan(int32_t* plan, int64_t plan_bytes,
+                      const int64_t* cu_seqlens, const int64_t* kv_lens, const int64_t* slot_ids,
+                      int64_t B, int64_t total_T, int64_t max_seqlen,
+                      int64_t H_q, int64_t H_kv, int64_t D, int64_t page_size,
+                      int64_t bt_width, int64_t n_slots, int32_t* err, void* stream);
+int cie_q8_mixed(void* o, const void* q, const void* k_pool, const void* v_pool,
+                 const void* scales, const int32_t* plan, int64_t plan_bytes,
+                 const int64_t* block_table, void* partials, int64_t partials_bytes,
+                 int32_t* counters, int64_t B, int64_t total_T,
+                 int64_t H_q, int64_t H_kv, int64_t D, int64_t page_size, int64_t n_pages,
+                 int64_t pool_page_stride, int64_t pool_head_stride,
+                 int64_t bt_stride, int64_t bt_width, int64_t n_slots,
+                 int32_t* err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
