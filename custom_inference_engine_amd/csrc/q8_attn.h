@@ -105,43 +105,49 @@ __device__ __forceinline__ void q8_v_operand(f16x8 (&va)[Geo<D>::NT], int half, 
   }
 }
 
-// One 32-key step of NCT column tiles: K operands ka / kb of tiles a and b, whose first keys are key0a / key0b
-// (kNoKey: absent, all masked); v(va) gives the V^T operands once the weights are known.  lim[c]: keys the
-// lane's column attends; mask: some key of the step may be at or past one of them.  Phase by phase over the
-// column tiles, so that a wave overlaps their VALU work and MFMAs; attend_pair_body's softmax.
-template <int D, int NCT, class V>
-__device__ __forceinline__ void q8_step(SoftmaxAcc<D, NCT>& st, const f16x8 (&ka)[Geo<D>::KS],
-                                        const f16x8 (&kb)[Geo<D>::KS], V v, const f16x8 (&q)[NCT][Geo<D>::KS],
-                                        int key0a, int key0b, const int (&lim)[NCT], bool mask, float scale_log2,
+// One step of NP 32-key pairs of tiles for NCT column tiles.  k(i, ka) gives the K operands of tile i (< 2 NP), whose
+// first key is key0[i] (kNoKey: absent, all masked), v(p, va) the V^T operands of pair p once the weights are known.
+// lim[c]: keys the lane's column attends; mask: some key of the step may be at or past one of them.  Phase by phase,
+// so that a wave overlaps the VALU work and the MFMAs of its column tiles and pairs; attend_pair_body's softmax.
+template <int D, int NCT, int NP, class K, class V>
+__device__ __forceinline__ void q8_step(SoftmaxAcc<D, NCT>& st, K k, V v, const f16x8 (&q)[NCT][Geo<D>::KS],
+                                        const int (&key0)[2 * NP], const int (&lim)[NCT], bool mask, float scale_log2,
                                         int grp) {
   constexpr int KS = Geo<D>::KS;
   constexpr int NT = Geo<D>::NT;
-  f32x4 s[NCT][2];
+  f32x4 s[NCT][2 * NP];
+  f16x8 ka[2][KS];  // a tile's operands are fetched while the one before it is multiplied
+  k(0, ka[0]);
 #pragma unroll
-  for (int c = 0; c < NCT; ++c) {
-    s[c][0] = f32x4{0.f, 0.f, 0.f, 0.f};
-    s[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < 2 * NP; ++i) {
+    if (i + 1 < 2 * NP) k(i + 1, ka[(i + 1) % 2]);
+    if (NP > 1) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      s[c][0] = mfma16x16x32(ka[ks], q[c][ks], s[c][0]);
-      s[c][1] = mfma16x16x32(kb[ks], q[c][ks], s[c][1]);
-    }
+    for (int c = 0; c < NCT; ++c) s[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int c = 0; c < NCT; ++c) s[c][i] = mfma16x16x32(ka[i % 2][ks], q[c][ks], s[c][i]);
+    if (NP > 1) __builtin_amdgcn_sched_barrier(0);
   }
   if (mask) {
 #pragma unroll
     for (int c = 0; c < NCT; ++c)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[c][0][r] = key0a + 4 * grp + r < lim[c] ? s[c][0][r] : kNegInf;
-        s[c][1][r] = key0b + 4 * grp + r < lim[c] ? s[c][1][r] : kNegInf;
+      for (int i = 0; i < 2 * NP; ++i) {
+        // (the asm keeps this a branch: most steps mask nothing, and selects nearly double a step's VALU work)
+        asm volatile("" : "+v"(s[c][i]));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[c][i][r] = key0[i] + 4 * grp + r < lim[c] ? s[c][i][r] : kNegInf;
       }
   }
   float xb[NCT];
   bool need = false;
 #pragma unroll
   for (int c = 0; c < NCT; ++c) {
-    xb[c] = fmaxf(fmaxf(fmaxf(s[c][0][0], s[c][0][1]), fmaxf(s[c][0][2], s[c][0][3])),
-                  fmaxf(fmaxf(s[c][1][0], s[c][1][1]), fmaxf(s[c][1][2], s[c][1][3])));
+    xb[c] = s[c][0][0];
+#pragma unroll
+    for (int i = 0; i < 8 * NP; ++i) xb[c] = fmaxf(xb[c], s[c][i / 4][i % 4]);
     need |= xb[c] > st.thr[c];
   }
   if (__any(need)) {  // rare: move the reference max
@@ -156,19 +162,27 @@ __device__ __forceinline__ void q8_step(SoftmaxAcc<D, NCT>& st, const f16x8 (&ka
       for (int nt = 0; nt < NT; ++nt) st.acc[c][nt] *= alpha;
     }
   }
-  f16x8 p[NCT];
-#pragma unroll
-  for (int c = 0; c < NCT; ++c)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) p[c][e] = (f16)fast_exp2(__builtin_fmaf(s[c][e / 4][e % 4], scale_log2, -st.m[c]));
-  f16x8 va[NT];
-  v(va);
   const f16x8 ones = {(f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f, (f16)1.f};
 #pragma unroll
-  for (int c = 0; c < NCT; ++c) {
+  for (int pr = 0; pr < NP; ++pr) {
+    f16x8 va[NT];
+    if (NP > 1) {
+      v(pr, va);  // (from LDS: fetched while the exponentials run)
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    f16x8 p[NCT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) st.acc[c][nt] = mfma16x16x32(va[nt], p[c], st.acc[c][nt]);
-    st.lsum[c] = mfma16x16x32(ones, p[c], st.lsum[c]);
+    for (int c = 0; c < NCT; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        p[c][e] = (f16)fast_exp2(__builtin_fmaf(s[c][2 * pr + e / 4][e % 4], scale_log2, -st.m[c]));
+    if (NP == 1) v(pr, va);
+#pragma unroll
+    for (int c = 0; c < NCT; ++c) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) st.acc[c][nt] = mfma16x16x32(va[nt], p[c], st.acc[c][nt]);
+      st.lsum[c] = mfma16x16x32(ones, p[c], st.lsum[c]);
+    }
   }
 }
 
@@ -177,14 +191,13 @@ template <int D>
 __device__ __forceinline__ void q8_attend(SoftmaxAcc<D, 1>& st, const Q8Tile<D>& a, const Q8Tile<D>& b, float ksa,
                                           float vsa, float ksb, float vsb, const f16x8 (&q)[1][Geo<D>::KS], int key0a,
                                           int key0b, const int (&lim)[1], bool mask, float scale_log2, int grp) {
-  f16x8 ka[Geo<D>::KS], kb[Geo<D>::KS];
-  q8_k_operand<D>(ka, a, ksa);
-  q8_k_operand<D>(kb, b, ksb);
-  auto v = [&](f16x8 (&va)[Geo<D>::NT]) {
+  auto k = [&](int i, f16x8 (&ka)[Geo<D>::KS]) { q8_k_operand<D>(ka, i ? b : a, i ? ksb : ksa); };
+  auto v = [&](int, f16x8 (&va)[Geo<D>::NT]) {
     q8_v_operand<D>(va, 0, a, vsa);
     q8_v_operand<D>(va, 1, b, vsb);
   };
-  q8_step<D, 1>(st, ka, kb, v, q, key0a, key0b, lim, mask, scale_log2, grp);
+  const int key0[2] = {key0a, key0b};
+  q8_step<D, 1, 1>(st, k, v, q, key0, lim, mask, scale_log2, grp);
 }
 
 // Where a wave's tiles live: kv head g of the pools and of the scales.

@@ -22,7 +22,7 @@
 // leaves its state (m, l, acc) in `partials` and the last to arrive merges them.
 //
 // The plan (q8_mixed_plan_kernel, one workgroup) sizes that share so that the
-// launch has about kQ8Slots items' worth of work, and lists the items, wide ones
+// launch has about kQ8Slots items' worth of work, and lists the items, longest
 // first.  It depends on the step's sequences only, so a step makes it once for all
 // its layers.
 //
@@ -42,7 +42,7 @@ constexpr int kQ8MaxSeqs = 2048;
 constexpr int kItemWords = 12;
 constexpr int kHeadWords = 12;
 constexpr int kQ8MaxChunks = 64;  // items of a split tile at most (one workgroup merges them)
-constexpr int kPlanThreadsM = 1024;
+constexpr int kPlanThreadsM = 512;
 constexpr int kPlanMagic = 0x71386d31;
 
 // Column tiles of a wave, and columns of a wide tile, at most.
@@ -126,178 +126,173 @@ __device__ __forceinline__ Q8Seq q8_seq(const Q8PlanParams& p, int b, bool repor
   return s;
 }
 
-// How a sequence is cut: its tiles' rows, and key tiles an item at most.
+// How a sequence is cut: its tiles' rows, and key tiles an item at most (once the launch's `want` is known).
 struct Q8Cut {
   bool narrow;
   int R, n_rt, share;
-  __device__ __forceinline__ Q8Cut(const Q8PlanParams& p, const Q8Seq& s, int want) {
-    narrow = (int64_t)s.L * p.G <= 16;
-    R = narrow ? max(1, s.L) : q8_tile_cols() / p.G;
-    n_rt = (s.L + R - 1) / R;
+  __device__ __forceinline__ Q8Cut(const Q8PlanParams& p, int L, int want) {
+    narrow = (int64_t)L * p.G <= 16;
+    R = narrow ? max(1, L) : q8_tile_cols() / p.G;
+    n_rt = (L + R - 1) / R;
     share = (max(kQ8MinShare, narrow ? 4 * want : want) + 3) & ~3;
-  }
-  __device__ __forceinline__ int rows(const Q8Seq& s, int r) const { return min(R, s.L - r * R); }
-  __device__ __forceinline__ int key_tiles(const Q8Seq& s, int r) const {
-    return (s.c + r * R + rows(s, r) + 15) >> 4;
-  }
-  __device__ __forceinline__ int chunks(const Q8Seq& s, int r, bool split) const {
-    return split ? min(kQ8MaxChunks, (key_tiles(s, r) + share - 1) / share) : 1;
   }
 };
 
-__device__ __forceinline__ int64_t plan_wave_sum(int64_t v) {
-  for (int off = 1; off < kWave; off <<= 1) v += __shfl_xor(v, off, kWave);
-  return v;
-}
-__device__ __forceinline__ int plan_wave_sum(int v) {
-  for (int off = 1; off < kWave; off <<= 1) v += __shfl_xor(v, off, kWave);
-  return v;
-}
+constexpr int kPlanWavesM = kPlanThreadsM / kWave;
 
-// Exclusive prefix sums of x[0 .. n) in place, in LDS, by the whole workgroup; the total.
-__device__ __forceinline__ int plan_scan(int* x, int n, int* red) {
+// Exclusive prefix sum of v over the workgroup's threads, and the sum; red: a word a wave.
+__device__ __forceinline__ int plan_block_scan(int v, int* red, int& all) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  int carry = 0;
-  for (int i0 = 0; i0 < n; i0 += kPlanThreadsM) {
-    const int i = i0 + threadIdx.x;
-    const int v = i < n ? x[i] : 0;
-    const int inc = wave_inclusive_sum(v);
-    __syncthreads();
-    if (lane == kWave - 1) red[wave] = inc;
-    __syncthreads();
-    int base = carry, all = carry;
-    for (int w = 0; w < kPlanThreadsM / kWave; ++w) {
-      if (w < wave) base += red[w];
-      all += red[w];
-    }
-    if (i < n) x[i] = base + inc - v;
-    carry = all;
-  }
+  const int inc = wave_inclusive_sum(v);
   __syncthreads();
-  return carry;
+  if (lane == kWave - 1) red[wave] = inc;
+  __syncthreads();
+  int base = 0;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWavesM; ++w) {
+    if (w < wave) base += red[w];
+    all += red[w];
+  }
+  return base + inc - v;
 }
 
-// A wave takes a sequence at a time, a lane one of its query tiles.
+// One workgroup: a thread a sequence, then a thread a query tile.
 //
 // Key tiles an item holds at most: with W the launch's work in key tiles of wide items (a narrow item's key tile
 // counts a quarter), want = W / kQ8Slots, 4 want for narrow items, and kQ8MinShare at least.  A tile of kt > share
 // key tiles becomes ceil(kt / share) items, so the items beyond one a tile are at most kQ8Slots, split tiles at most
-// that many, and their items at most kMaxSplitItems.
+// that many, and their items at most kMaxSplitItems.  (W is taken from closed forms that are no smaller.)
+//
+// Items are listed the longest first, to kPlanLevels of length: the workgroups of a launch start in order, so what
+// starts last is short.
+constexpr int kPlanLevels = 64;
 __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanParams p) {
-  __shared__ int sm_items[kQ8MaxSeqs];   // items, then their first index (narrow ones: among narrow)
-  __shared__ int sm_narrow[kQ8MaxSeqs];
-  __shared__ int sm_rows[kQ8MaxSeqs];    // partial rows
-  __shared__ int sm_ctr[kQ8MaxSeqs];     // split (tile, kv head)s
-  __shared__ int sm_red[kPlanThreadsM / kWave];
+  __shared__ int64_t sm_t0[kQ8MaxSeqs];
+  __shared__ int sm_slot[kQ8MaxSeqs], sm_L[kQ8MaxSeqs], sm_c[kQ8MaxSeqs];
+  __shared__ int sm_first[kQ8MaxSeqs];  // a sequence's first tile
+  __shared__ int sm_level[kPlanLevels];
+  __shared__ int sm_red[kPlanWavesM];
   __shared__ unsigned long long sm_work;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  constexpr int kWaves = kPlanThreadsM / kWave;
-  if (threadIdx.x == 0) sm_work = 0;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  if (tid == 0) sm_work = 0;
+  if (tid < kPlanLevels) sm_level[tid] = 0;
   __syncthreads();
-  for (int b = wave; b < p.B; b += kWaves) {
-    const Q8Seq s = q8_seq(p, b, lane == 0);
-    const Q8Cut cut(p, s, 0);
-    int64_t w = 0;
-    for (int r = lane; r < cut.n_rt; r += kWave) w += cut.narrow ? (cut.key_tiles(s, r) + 3) / 4 : cut.key_tiles(s, r);
-    w = plan_wave_sum(w);
-    if (lane == 0) atomicAdd(&sm_work, (unsigned long long)w * p.H_kv);
+  int n_tiles = 0;
+  int64_t work = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kPlanThreadsM) {
+    const int b = b0 + tid;
+    int n = 0;
+    if (b < p.B) {
+      const Q8Seq s = q8_seq(p, b, true);
+      const Q8Cut cut(p, s.L, 0);
+      n = cut.n_rt;
+      sm_t0[b] = s.t0;
+      sm_slot[b] = s.slot;
+      sm_L[b] = s.L;
+      sm_c[b] = s.c;
+      if (s.L > 0)
+        work += cut.narrow ? (int64_t)((s.c + s.L) >> 6) + 1
+                           : (int64_t)n * ((s.c >> 4) + 2) + (int64_t)cut.R * n * (n + 1) / 32 + 1;
+    }
+    int all;
+    const int first = plan_block_scan(n, sm_red, all);
+    if (b < p.B) sm_first[b] = n_tiles + first;
+    n_tiles += all;
   }
+  for (int off = 1; off < kWave; off <<= 1) work += __shfl_xor(work, off, kWave);
+  if (lane == 0 && work > 0) atomicAdd(&sm_work, (unsigned long long)work);
   __syncthreads();
-  const int want = (int)min((int64_t)1 << 26, ((int64_t)sm_work + kQ8Slots - 1) / kQ8Slots);
-  for (int b = wave; b < p.B; b += kWaves) {
-    const Q8Seq s = q8_seq(p, b, false);
-    const Q8Cut cut(p, s, want);
-    int rows = 0;
-    for (int r = lane; r < cut.n_rt; r += kWave) {
-      const int n = cut.chunks(s, r, true);
-      if (n > 1) rows += n * cut.rows(s, r) * p.G;
-    }
-    rows = plan_wave_sum(rows);
-    if (lane == 0) sm_rows[b] = rows * p.H_kv;
-  }
-  __syncthreads();
-  plan_scan(sm_rows, p.B, sm_red);
-  // sequences whose partial rows would end past the buffer run unsplit
-  auto splits = [&](int b, const Q8Seq& s, const Q8Cut& cut) {
-    int rows = 0;
-    for (int r = lane; r < cut.n_rt; r += kWave) {
-      const int n = cut.chunks(s, r, true);
-      if (n > 1) rows += n * cut.rows(s, r) * p.G;
-    }
-    return (int64_t)sm_rows[b] + (int64_t)plan_wave_sum(rows) * p.H_kv <= p.part_cap;
-  };
-  for (int b = wave; b < p.B; b += kWaves) {
-    const Q8Seq s = q8_seq(p, b, false);
-    const Q8Cut cut(p, s, want);
-    const bool split = splits(b, s, cut);
-    int items = 0, ctr = 0;
-    for (int r = lane; r < cut.n_rt; r += kWave) {
-      const int n = cut.chunks(s, r, split);
-      items += n;
-      ctr += n > 1;
-    }
-    items = plan_wave_sum(items) * p.H_kv;
-    ctr = plan_wave_sum(ctr) * p.H_kv;
-    if (lane == 0) {
-      sm_items[b] = cut.narrow ? 0 : items;
-      sm_narrow[b] = cut.narrow ? items : 0;
-      sm_ctr[b] = ctr;
-    }
-  }
-  __syncthreads();
-  const int n_wide = plan_scan(sm_items, p.B, sm_red);
-  const int n_items = n_wide + plan_scan(sm_narrow, p.B, sm_red);
-  plan_scan(sm_ctr, p.B, sm_red);
-  const bool fits = n_items <= p.plan_cap;
-  if (threadIdx.x == 0) {
-    p.plan[0] = fits ? n_items : 0;
-#pragma unroll
-    for (int i = 1; i < kHeadWords; ++i) p.plan[i] = plan_word(p, i - 1, p.D);
-    if (!fits) set_err(p.err, CIE_ERRBIT_PLAN);
-  }
-  if (!fits) return;
-  Q8Item* const items = reinterpret_cast<Q8Item*>(p.plan + kHeadWords);
-  for (int b = wave; b < p.B; b += kWaves) {
-    const Q8Seq s = q8_seq(p, b, false);
-    const Q8Cut cut(p, s, want);
-    const bool split = splits(b, s, cut);
-    int at = cut.narrow ? n_wide + sm_narrow[b] : sm_items[b];
-    int row_at = sm_rows[b], ctr_at = sm_ctr[b];
-    for (int r0 = 0; r0 < cut.n_rt; r0 += kWave) {
-      const int r = cut.n_rt - 1 - (r0 + lane);  // the longest tiles first
-      const bool live = r >= 0;
-      const int n = live ? cut.chunks(s, r, split) : 0;
-      const int rows = live ? cut.rows(s, r) : 0, cols = rows * p.G;
-      const int mine = n * p.H_kv, my_rows = n > 1 ? n * cols * p.H_kv : 0, my_ctr = n > 1 ? p.H_kv : 0;
-      const int i_inc = wave_inclusive_sum(mine), r_inc = wave_inclusive_sum(my_rows), c_inc = wave_inclusive_sum(my_ctr);
-      if (live) {
-        const int kt = cut.key_tiles(s, r);
-        Q8Item it;
-        it.tok0 = (int)(s.t0 + r * cut.R);
-        it.rows = cut.narrow ? -rows : rows;
-        it.slot = s.slot;
-        it.pos0 = s.c + r * cut.R;
-        it.n_chunks = n;
-        it.pad = 0;
-        // near-equal chunks in whole stages (4 tiles): their share of the tile's stages, rounded up
-        const int per = 4 * ((((kt + 3) >> 2) + n - 1) / n);
-        int i = at + i_inc - mine, pr = row_at + r_inc - my_rows;
-        for (int g = 0; g < p.H_kv; ++g) {
-          it.g = g;
-          it.pbase = pr;
-          it.ctr = n > 1 ? ctr_at + c_inc - my_ctr + g : 0;
-          for (int c = 0; c < n; ++c, ++i) {
-            it.chunk = c;
-            it.t0 = min(kt, c * per);
-            it.t1 = min(kt, it.t0 + per);
-            items[i] = it;
-          }
-          pr += n * cols;
-        }
+  const int want = (int)min((int64_t)1 << 26, ((int64_t)sm_work * p.H_kv + kQ8Slots - 1) / kQ8Slots);
+
+  // A thread's tile: sequence, rows, chunks, partial rows and arrival words before it.
+  int b = 0, r = 0, n = 0, rows = 0, kt = 0, pbase = 0, ctr = 0, level = 0;
+  int rows_at = 0, ctr_at = 0;
+  auto tile = [&](int i0) {
+    const int i = i0 + tid;
+    n = rows = 0;
+    int R = 1, share = 1;
+    bool narrow = false;
+    if (i < n_tiles) {
+      int lo = 0, hi = p.B - 1;  // the last sequence whose first tile is at or before i
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (sm_first[mid] <= i)
+          lo = mid;
+        else
+          hi = mid - 1;
       }
-      at += __builtin_amdgcn_readlane(i_inc, kWave - 1);
-      row_at += __builtin_amdgcn_readlane(r_inc, kWave - 1);
-      ctr_at += __builtin_amdgcn_readlane(c_inc, kWave - 1);
+      b = lo;
+      const Q8Cut cut(p, sm_L[b], want);
+      r = i - sm_first[b];
+      R = cut.R;
+      share = cut.share;
+      narrow = cut.narrow;
+      rows = min(R, sm_L[b] - r * R);
+      kt = (sm_c[b] + r * R + rows + 15) >> 4;
+      n = min(kQ8MaxChunks, (kt + share - 1) / share);
+    }
+    int all;
+    const int mine = n > 1 ? n * rows * p.G * p.H_kv : 0;
+    pbase = rows_at + plan_block_scan(mine, sm_red, all);
+    rows_at += all;
+    if ((int64_t)pbase + mine > p.part_cap) n = 1;  // its partial rows would end past the buffer: unsplit
+    ctr = ctr_at + plan_block_scan(n > 1 ? p.H_kv : 0, sm_red, all);
+    ctr_at += all;
+    if (n > 0) {
+      const int len = (kt + n - 1) / n;  // an item's key tiles, in a wide item's
+      level = kPlanLevels - 1 - min(kPlanLevels - 1, (int)((int64_t)len * kPlanLevels / (share + 1)));
+      if (narrow) rows = -rows;
+    }
+  };
+  const bool once = n_tiles <= kPlanThreadsM;
+  for (int i0 = 0; i0 < n_tiles; i0 += kPlanThreadsM) {
+    tile(i0);
+    if (n > 0) atomicAdd(&sm_level[level], n * p.H_kv);
+  }
+  __syncthreads();
+  if (tid < kWave) {  // levels' first items
+    const int v = sm_level[tid], inc = wave_inclusive_sum(v);
+    sm_level[tid] = inc - v;
+    const int n_items = __builtin_amdgcn_readlane(inc, kWave - 1);
+    if (tid == 0) {
+      const bool fits = n_items <= p.plan_cap;
+      if (!fits) set_err(p.err, CIE_ERRBIT_PLAN);
+      sm_red[0] = fits;
+      p.plan[0] = fits ? n_items : 0;
+#pragma unroll
+      for (int i = 1; i < kHeadWords; ++i) p.plan[i] = plan_word(p, i - 1, p.D);
+    }
+  }
+  __syncthreads();
+  if (!sm_red[0]) return;
+  Q8Item* const items = reinterpret_cast<Q8Item*>(p.plan + kHeadWords);
+  __syncthreads();
+  rows_at = ctr_at = 0;
+  for (int i0 = 0; i0 < n_tiles; i0 += kPlanThreadsM) {
+    if (!once) tile(i0);
+    if (n == 0) continue;
+    const int abs_rows = rows < 0 ? -rows : rows;
+    const int R = rows < 0 ? 0 : q8_tile_cols() / p.G;  // (a narrow sequence has one tile)
+    int at = atomicAdd(&sm_level[level], n * p.H_kv);
+    Q8Item it;
+    it.tok0 = (int)sm_t0[b] + r * R;
+    it.rows = rows;
+    it.slot = sm_slot[b];
+    it.pos0 = sm_c[b] + r * R;
+    it.n_chunks = n;
+    it.pad = 0;
+    const int per = 4 * ((((kt + 3) >> 2) + n - 1) / n);  // near-equal chunks in whole stages (4 tiles)
+    for (int g = 0; g < p.H_kv; ++g) {
+      it.g = g;
+      it.pbase = n > 1 ? pbase + g * n * abs_rows * p.G : 0;
+      it.ctr = n > 1 ? ctr + g : 0;
+      for (int c = 0; c < n; ++c) {
+        it.chunk = c;
+        it.t0 = min(kt, c * per);
+        it.t1 = min(kt, it.t0 + per);
+        items[at++] = it;
+      }
     }
   }
 }
@@ -484,23 +479,18 @@ __device__ __forceinline__ void wide_item(const Q8MixedParams& p, const Q8Item& 
     }
     __syncthreads();
     if constexpr (NA > 0) {
+      int key0[4];
 #pragma unroll
-      for (int pr = 0; pr < 2; ++pr) {
-        const int key0 = 16 * (it.t0 + 4 * sg + 2 * pr);
-        if (key0 < key_end) {  // uniform
-          f16x8 ka[KS], kb[KS];
+      for (int i = 0; i < 4; ++i) key0[i] = 16 * (it.t0 + 4 * sg + i);
+      auto k = [&](int i, f16x8 (&ka)[KS]) {
 #pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            ka[i] = kbuf[(2 * pr * KS + i) * kWave + lane];
-            kb[i] = kbuf[((2 * pr + 1) * KS + i) * kWave + lane];
-          }
-          auto v = [&](f16x8 (&va)[NT]) {
+        for (int ks = 0; ks < KS; ++ks) ka[ks] = kbuf[(i * KS + ks) * kWave + lane];
+      };
+      auto v = [&](int pr, f16x8 (&va)[NT]) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) va[nt] = vbuf[(pr * NT + nt) * kWave + lane];
-          };
-          q8_step<D, NC>(st, ka, kb, v, q, key0, key0 + 16, lim, key0 + 32 > mask_from, p.scale_log2, grp);
-        }
-      }
+        for (int nt = 0; nt < NT; ++nt) va[nt] = vbuf[(pr * NT + nt) * kWave + lane];
+      };
+      q8_step<D, NC, 2>(st, k, v, q, key0, lim, key0[3] + 16 > mask_from, p.scale_log2, grp);
     }
   }
   if constexpr (NA > 0) {
