@@ -106,11 +106,12 @@ __device__ __forceinline__ void q8_v_operand(f16x8 (&va)[Geo<D>::NT], int half, 
 }
 
 // One step of NP 32-key pairs of tiles for NCT column tiles.  k(i, ka) gives the K operands of tile i (< 2 NP), whose
-// first key is key0[i] (kNoKey: absent, all masked), v(p, va) the V^T operands of pair p once the weights are known.
+// first key is key0[i] (kNoKey: absent, all masked), v(p, va) the V^T operands of pair p once the weights are known;
+// meanwhile() is work that needs nothing of the step, done while its S MFMAs run.
 // lim[c]: keys the lane's column attends; mask: some key of the step may be at or past one of them.  Phase by phase,
 // so that a wave overlaps the VALU work and the MFMAs of its column tiles and pairs; attend_pair_body's softmax.
-template <int D, int NCT, int NP, class K, class V>
-__device__ __forceinline__ void q8_step(SoftmaxAcc<D, NCT>& st, K k, V v, const f16x8 (&q)[NCT][Geo<D>::KS],
+template <int D, int NCT, int NP, bool LDS, class K, class V, class M>
+__device__ __forceinline__ void q8_step(SoftmaxAcc<D, NCT>& st, K k, V v, M meanwhile, const f16x8 (&q)[NCT][Geo<D>::KS],
                                         const int (&key0)[2 * NP], const int (&lim)[NCT], bool mask, float scale_log2,
                                         int grp) {
   constexpr int KS = Geo<D>::KS;
@@ -121,15 +122,16 @@ __device__ __forceinline__ void q8_step(SoftmaxAcc<D, NCT>& st, K k, V v, const 
 #pragma unroll
   for (int i = 0; i < 2 * NP; ++i) {
     if (i + 1 < 2 * NP) k(i + 1, ka[(i + 1) % 2]);
-    if (NP > 1) __builtin_amdgcn_sched_barrier(0);
+    if (LDS) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int c = 0; c < NCT; ++c) s[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int c = 0; c < NCT; ++c) s[c][i] = mfma16x16x32(ka[i % 2][ks], q[c][ks], s[c][i]);
-    if (NP > 1) __builtin_amdgcn_sched_barrier(0);
+    if (LDS) __builtin_amdgcn_sched_barrier(0);
   }
+  meanwhile();
   if (mask) {
 #pragma unroll
     for (int c = 0; c < NCT; ++c)
@@ -166,7 +168,7 @@ __device__ __forceinline__ void q8_step(SoftmaxAcc<D, NCT>& st, K k, V v, const 
 #pragma unroll
   for (int pr = 0; pr < NP; ++pr) {
     f16x8 va[NT];
-    if (NP > 1) {
+    if (LDS) {
       v(pr, va);  // (from LDS: fetched while the exponentials run)
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -176,7 +178,7 @@ __device__ __forceinline__ void q8_step(SoftmaxAcc<D, NCT>& st, K k, V v, const 
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         p[c][e] = (f16)fast_exp2(__builtin_fmaf(s[c][2 * pr + e / 4][e % 4], scale_log2, -st.m[c]));
-    if (NP == 1) v(pr, va);
+    if (!LDS) v(pr, va);
 #pragma unroll
     for (int c = 0; c < NCT; ++c) {
 #pragma unroll
@@ -197,7 +199,7 @@ __device__ __forceinline__ void q8_attend(SoftmaxAcc<D, 1>& st, const Q8Tile<D>&
     q8_v_operand<D>(va, 1, b, vsb);
   };
   const int key0[2] = {key0a, key0b};
-  q8_step<D, 1, 1>(st, k, v, q, key0, lim, mask, scale_log2, grp);
+  q8_step<D, 1, 1, false>(st, k, v, [] {}, q, key0, lim, mask, scale_log2, grp);
 }
 
 // Where a wave's tiles live: kv head g of the pools and of the scales.

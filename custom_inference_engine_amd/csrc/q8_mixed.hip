@@ -35,19 +35,19 @@ namespace cie {
 
 constexpr int kMW = 4;  // waves a workgroup
 constexpr int kMThreads = kMW * kWave;
-constexpr int kQ8Slots = 512;        // items a launch's work is cut into, about
+constexpr int kQ8Slots = 256;        // items a launch's work is cut into, about
 constexpr int kMaxSplitItems = 2 * kQ8Slots;  // (see plan_share)
 constexpr int kQ8MinShare = 32;  // key tiles (512 keys): below, an item's start costs more than its keys
 constexpr int kQ8MaxSeqs = 2048;
 constexpr int kItemWords = 12;
 constexpr int kHeadWords = 12;
-constexpr int kQ8MaxChunks = 64;  // items of a split tile at most (one workgroup merges them)
+constexpr int kQ8MaxChunks = 48;  // items of a split tile at most (one workgroup merges them)
 constexpr int kPlanThreadsM = 512;
 constexpr int kPlanMagic = 0x71386d31;
 
 // Column tiles of a wave, and columns of a wide tile, at most.
 constexpr int kQ8Ct = 2;
-static __host__ __device__ constexpr int q8_tile_cols() { return 16 * kMW * kQ8Ct; }
+constexpr int kTileCols = 16 * kMW * kQ8Ct;
 
 struct Q8Item {
   int tok0;    // packed row of the tile's first row
@@ -132,7 +132,7 @@ struct Q8Cut {
   int R, n_rt, share;
   __device__ __forceinline__ Q8Cut(const Q8PlanParams& p, int L, int want) {
     narrow = (int64_t)L * p.G <= 16;
-    R = narrow ? max(1, L) : q8_tile_cols() / p.G;
+    R = narrow ? max(1, L) : kTileCols / p.G;
     n_rt = (L + R - 1) / R;
     share = (max(kQ8MinShare, narrow ? 4 * want : want) + 3) & ~3;
   }
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
     if (!once) tile(i0);
     if (n == 0) continue;
     const int abs_rows = rows < 0 ? -rows : rows;
-    const int R = rows < 0 ? 0 : q8_tile_cols() / p.G;  // (a narrow sequence has one tile)
+    const int R = rows < 0 ? 0 : kTileCols / p.G;  // (a narrow sequence has one tile)
     int at = atomicAdd(&sm_level[level], n * p.H_kv);
     Q8Item it;
     it.tok0 = (int)sm_t0[b] + r * R;
@@ -305,7 +305,10 @@ struct Q8Lds {
   static constexpr int kV = 2 * Geo<D>::NT * kWave;
   static constexpr int kStage = kK + kV;
   static constexpr int kFold = kMW * 16 * (D / 4 + 1) + 2 * kMW * 16 / 4;
+  static constexpr int kMerge = (kTileCols * kQ8MaxChunks + 2 * kMThreads) / 4 + kMThreads;
   static constexpr int kSlots = 2 * kStage > kFold ? 2 * kStage : kFold;
+  static_assert(kSlots >= kMerge, "the merge's scratch");
+  static_assert(kMThreads >= kTileCols && kTileCols * (D / 4) <= 16 * kMThreads, "the merge's threads");
 };
 
 // Column cc of an item: its row and head, and where its output goes.
@@ -364,52 +367,130 @@ struct WaveTiles {
   }
 };
 
-// Merge a split tile's chunk states into o: a thread owns 4 dims of a column and takes the chunks in groups,
-// their loads all issued before any is used.
+// A partial row's order: the 16-byte piece of dims 4 d4 .. 4 d4 + 3 sits at piece (d4 % NT) * 4 + d4 / NT, so that the
+// four lanes of a column (each NT pieces of consecutive dims) write 64 bytes in one piece at a time.
 template <int D>
-__device__ __forceinline__ void q8_mixed_merge(const Q8MixedParams& p, const Q8Item& it, int cols) {
-  constexpr int D4 = D / 4, kGroup = 8;
+__device__ __forceinline__ int part_piece(int d4) {
+  return (d4 % Geo<D>::NT) * 4 + d4 / Geo<D>::NT;
+}
+
+// The chunks' pieces of a split tile, summed with their weights and stored: a thread owns UN pieces (4 dims of a
+// column; pieces tid + 256 i), kMergeLoads loads in flight.  Where the pieces are fewer than the threads, R threads
+// share one, each taking every R-th chunk, and are summed through LDS.
+constexpr int kMergeLoads = 16;
+template <int D, int UN>
+__device__ __forceinline__ void merge_pieces(const Q8MixedParams& p, const Q8Item& it, int cols, const float* sm_w,
+                                             f32x4* sm_sum) {
+  constexpr int D4 = D / 4, CG = kMergeLoads / UN;
+  const int n = it.n_chunks, n_units = cols * D4;
   const __amdgpu_buffer_rsrc_t racc =
-      coherent_rsrc(p.part_acc + (int64_t)it.pbase * D, (uint32_t)(cols * it.n_chunks * D * sizeof(float)));
-  for (int u = threadIdx.x; u < cols * D4; u += kMThreads) {
-    const int cc = u / D4, d4 = u - cc * D4;
-    float M = kEmptyMax, den = 0.f;
-    f32x4 num = {0.f, 0.f, 0.f, 0.f};
-    for (int c0 = 0; c0 < it.n_chunks; c0 += kGroup) {
+      coherent_rsrc(p.part_acc + (int64_t)it.pbase * D, (uint32_t)(n_units * n * sizeof(f32x4)));
+  const int R = UN == 1 ? max(1, kMThreads / n_units) : 1;
+  const int r = R > 1 ? (int)threadIdx.x / n_units : 0;
+  const int u0 = threadIdx.x - r * n_units;
+  f32x4 num[UN];
+#pragma unroll
+  for (int i = 0; i < UN; ++i) num[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int c0 = r; c0 < n; c0 += R * CG) {
+    f32x4 x[CG][UN];
+#pragma unroll
+    for (int k = 0; k < CG; ++k)
+#pragma unroll
+      for (int i = 0; i < UN; ++i) {  // (past the last piece or chunk: beyond the descriptor, zeros)
+        const int u = u0 + i * kMThreads, c = c0 + k * R;
+        x[k][i] = agent_load4(racc, r < R && u < n_units && c < n ? (uint32_t)((c * n_units + u) * sizeof(f32x4))
+                                                                  : 0x7ffffff0u);
+      }
+#pragma unroll
+    for (int k = 0; k < CG; ++k)
+#pragma unroll
+      for (int i = 0; i < UN; ++i) {
+        const int u = u0 + i * kMThreads, c = c0 + k * R;
+        if (u < n_units && c < n) num[i] += sm_w[c * cols + u / D4] * x[k][i];
+      }
+  }
+  if (R > 1) {
+    sm_sum[threadIdx.x] = num[0];
+    __syncthreads();
+    if (r == 0)
+      for (int i = 1; i < R; ++i) num[0] += sm_sum[u0 + i * n_units];
+  }
+#pragma unroll
+  for (int i = 0; i < UN; ++i) {
+    const int u = u0 + i * kMThreads;
+    if (r == 0 && u < n_units) {
+      const int cc = u / D4, piece = u % D4;
+      const int d4 = (piece % 4) * Geo<D>::NT + piece / 4;
+      f16x4 o4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o4[j] = (f16)num[i][j];
+      *reinterpret_cast<f16x4*>(p.o + out_row<D>(p, it, Q8Col(p, cc)) + 4 * d4) = o4;
+    }
+  }
+}
+
+// Merge a split tile's chunk states into o.  One workgroup does it, so memory round trips bound it: the chunks'
+// weights 2^(m - M) / l first (LDS), then the pieces.
+template <int D>
+__device__ __forceinline__ void q8_mixed_merge(const Q8MixedParams& p, const Q8Item& it, int cols, f32x4* lds) {
+  constexpr int kGroup = 8;
+  const int n = it.n_chunks;
+  float* const sm_w = reinterpret_cast<float*>(lds);
+  float* const sm_m = sm_w + kTileCols * kQ8MaxChunks;  // [2][thread]: threads' maxima, sums
+  // threads share a column's chunks: tpc of them, chunk k * tpc + j
+  const int tpc = kMThreads / cols;
+  const int j = (int)threadIdx.x / cols, cc = threadIdx.x - j * cols;
+  float M = kEmptyMax, den = 0.f;
+  if (j < tpc) {
+    for (int c0 = j; c0 < n; c0 += kGroup * tpc) {
       float ms[kGroup], ls[kGroup];
-      f32x4 as[kGroup];
 #pragma unroll
       for (int i = 0; i < kGroup; ++i) {
-        const bool live = c0 + i < it.n_chunks;
-        const int row = (live ? c0 + i : 0) * cols + cc;
-        ms[i] = agent_load(&p.part_m[it.pbase + row]);
-        ls[i] = agent_load(&p.part_l[it.pbase + row]);
-        as[i] = agent_load4(racc, (uint32_t)((row * D + 4 * d4) * sizeof(float)));
-        if (!live) {
-          ms[i] = kEmptyMax;
-          ls[i] = 0.f;
-          as[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        const int row = it.pbase + min(c0 + i * tpc, n - 1) * cols + cc;
+        ms[i] = agent_load(&p.part_m[row]);
+        ls[i] = agent_load(&p.part_l[row]);
       }
       float Mn = M;
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) Mn = fmaxf(Mn, ms[i]);
-      const float k = fast_exp2(M - Mn);
-      num *= k;
-      den *= k;
+      for (int i = 0; i < kGroup; ++i) Mn = fmaxf(Mn, ms[i]);  // (the last chunk again past the end: no matter)
+      den *= fast_exp2(M - Mn);
+      M = Mn;
 #pragma unroll
       for (int i = 0; i < kGroup; ++i) {
-        const float a = fast_exp2(ms[i] - Mn);
-        num += a * as[i];
-        den += a * ls[i];
+        const int c = c0 + i * tpc;
+        if (c < n) {
+          den += fast_exp2(ms[i] - M) * ls[i];
+          sm_w[c * cols + cc] = ms[i];
+        }
       }
-      M = Mn;
     }
-    f16x4 o4;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o4[i] = (f16)(den > 0.f ? num[i] / den : 0.f);
-    *reinterpret_cast<f16x4*>(p.o + out_row<D>(p, it, Q8Col(p, cc)) + 4 * d4) = o4;
+    sm_m[threadIdx.x] = M;
+    sm_m[kMThreads + threadIdx.x] = den;
   }
+  __syncthreads();
+  if (j < tpc) {
+    float top = kEmptyMax, sum = 0.f;
+    for (int i = 0; i < tpc; ++i) top = fmaxf(top, sm_m[i * cols + cc]);
+    for (int i = 0; i < tpc; ++i) sum += fast_exp2(sm_m[i * cols + cc] - top) * sm_m[kMThreads + i * cols + cc];
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    for (int c = j; c < n; c += tpc) {
+      float* const w = &sm_w[c * cols + cc];
+      *w = fast_exp2(*w - top) * inv;
+    }
+  }
+  __syncthreads();
+  f32x4* const sm_sum = lds + (kTileCols * kQ8MaxChunks + 2 * kMThreads) / 4;
+  const int n_units = cols * (D / 4);
+  if (n_units <= kMThreads)
+    merge_pieces<D, 1>(p, it, cols, sm_w, sm_sum);
+  else if (n_units <= 2 * kMThreads)
+    merge_pieces<D, 2>(p, it, cols, sm_w, sm_sum);
+  else if (n_units <= 4 * kMThreads)
+    merge_pieces<D, 4>(p, it, cols, sm_w, sm_sum);
+  else if (n_units <= 8 * kMThreads)
+    merge_pieces<D, 8>(p, it, cols, sm_w, sm_sum);
+  else
+    merge_pieces<D, 16>(p, it, cols, sm_w, sm_sum);
 }
 
 template <int D>
@@ -454,30 +535,34 @@ __device__ __forceinline__ void wide_item(const Q8MixedParams& p, const Q8Item& 
   st.init();
   const int n_stages = uniform((it.t1 - it.t0 + 3) >> 2);
   Q8Tile<D> raw;
-  tiles.template load<0>(raw, 0, 0, key_end, lo);
-  for (int sg = 0; sg < n_stages; ++sg) {
-    f16x8* const kbuf = reinterpret_cast<f16x8*>(lds) + (sg & 1) * Q8Lds<D>::kStage;
+  f16x8* const buf = reinterpret_cast<f16x8*>(lds);
+  // this wave's tile of stage sg (its bytes in raw), converted into operand slots; then stage sg + 1's loads
+  auto stage = [&](int sg) {
+    f16x8* const kbuf = buf + (sg & 1) * Q8Lds<D>::kStage;
     f16x8* const vbuf = kbuf + Q8Lds<D>::kK;
-    {  // this wave's tile, converted into operand slots
-      const int k = sg & (kWave - 1);
-      const float ks = tiles.scale(0, k), vs = tiles.scale(1, k);
-      f16x8 ko[KS];
-      q8_k_operand<D>(ko, raw, ks);
+    const int k = sg & (kWave - 1);
+    const float ks = tiles.scale(0, k), vs = tiles.scale(1, k);
+    f16x8 ko[KS];
+    q8_k_operand<D>(ko, raw, ks);
 #pragma unroll
-      for (int i = 0; i < KS; ++i) kbuf[(wave * KS + i) * kWave + lane] = ko[i];
-      f16x8 va[NT];
-      q8_v_operand<D>(va, 0, raw, vs);
+    for (int i = 0; i < KS; ++i) kbuf[(wave * KS + i) * kWave + lane] = ko[i];
+    f16x8 va[NT];
+    q8_v_operand<D>(va, 0, raw, vs);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        reinterpret_cast<f16x4*>(vbuf + ((wave >> 1) * NT + nt) * kWave + lane)[wave & 1] =
-            f16x4{va[nt][0], va[nt][1], va[nt][2], va[nt][3]};
-    }
-    if (sg + 1 < n_stages) {
-      const int k = (sg + 1) & (kWave - 1);
-      if (k == 0) tiles.gather(sg + 1);
-      tiles.template load<0>(raw, sg + 1 - k, k, key_end, lo);
-    }
+    for (int nt = 0; nt < NT; ++nt)
+      reinterpret_cast<f16x4*>(vbuf + ((wave >> 1) * NT + nt) * kWave + lane)[wave & 1] =
+          f16x4{va[nt][0], va[nt][1], va[nt][2], va[nt][3]};
+    const int next = (sg + 1) & (kWave - 1);
+    if (next == 0) tiles.gather(sg + 1);
+    tiles.template load<0>(raw, sg + 1 - next, next, key_end, lo);  // (past the last: no rows)
+  };
+  tiles.template load<0>(raw, 0, 0, key_end, lo);
+  stage(0);
+  for (int sg = 0; sg < n_stages; ++sg) {
+    // stage sg is written, and stage sg - 1's buffer free: the next one is converted while sg's S MFMAs run
     __syncthreads();
+    const f16x8* const kbuf = buf + (sg & 1) * Q8Lds<D>::kStage;
+    const f16x8* const vbuf = kbuf + Q8Lds<D>::kK;
     if constexpr (NA > 0) {
       int key0[4];
 #pragma unroll
@@ -490,9 +575,13 @@ __device__ __forceinline__ void wide_item(const Q8MixedParams& p, const Q8Item& 
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) va[nt] = vbuf[(pr * NT + nt) * kWave + lane];
       };
-      q8_step<D, NC, 2>(st, k, v, q, key0, lim, key0[3] + 16 > mask_from, p.scale_log2, grp);
+      q8_step<D, NC, 2, true>(st, k, v, [&] { stage(sg + 1); }, q, key0, lim, key0[3] + 16 > mask_from, p.scale_log2,
+                              grp);
+    } else {
+      stage(sg + 1);
     }
   }
+  __syncthreads();  // (the merge takes the buffers)
   if constexpr (NA > 0) {
     const __amdgpu_buffer_rsrc_t racc =
         coherent_rsrc(p.part_acc + (int64_t)it.pbase * D,
@@ -516,7 +605,7 @@ __device__ __forceinline__ void wide_item(const Q8MixedParams& p, const Q8Item& 
         const int row = it.chunk * cols + cc;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-          agent_store4(racc, (uint32_t)((row * D + NT * 4 * grp + 4 * i) * sizeof(float)),
+          agent_store4(racc, (uint32_t)((row * D + 4 * part_piece<D>(NT * grp + i)) * sizeof(float)),
                        f32x4{st.acc[c][(4 * i) % NT][(4 * i) / NT], st.acc[c][(4 * i + 1) % NT][(4 * i + 1) / NT],
                              st.acc[c][(4 * i + 2) % NT][(4 * i + 2) / NT],
                              st.acc[c][(4 * i + 3) % NT][(4 * i + 3) / NT]});
@@ -610,7 +699,7 @@ __device__ __forceinline__ void narrow_item(const Q8MixedParams& p, const Q8Item
       *reinterpret_cast<f16x4*>(p.o + out_row<D>(p, it, Q8Col(p, cc)) + 4 * d4) = o4;
     } else {
       const int row = it.chunk * cols + cc;
-      agent_store4(racc, (uint32_t)((row * D + 4 * d4) * sizeof(float)), num);
+      agent_store4(racc, (uint32_t)((row * D + 4 * part_piece<D>(d4)) * sizeof(float)), num);
       if (d4 == 0) {
         agent_store(&p.part_m[it.pbase + row], M);
         agent_store(&p.part_l[it.pbase + row], den);
@@ -625,6 +714,7 @@ void q8_mixed_kernel(Q8MixedParams p) {
   __shared__ f32x4 lds[Q8Lds<D>::kSlots];
   __shared__ int sm_last;
   const int32_t* const head = p.plan;
+  const Q8Item it = reinterpret_cast<const Q8Item*>(head + kHeadWords)[blockIdx.x];  // (read with the head)
   bool same = true;
 #pragma unroll
   for (int i = 1; i < kHeadWords; ++i) same &= head[i] == plan_word(p, i - 1, D);
@@ -633,7 +723,6 @@ void q8_mixed_kernel(Q8MixedParams p) {
     return;
   }
   if ((int)blockIdx.x >= head[0]) return;
-  const Q8Item it = reinterpret_cast<const Q8Item*>(p.plan + kHeadWords)[blockIdx.x];
   const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave);
   const bool narrow = it.rows < 0;
   const int cols = (narrow ? -it.rows : it.rows) * p.G;
@@ -641,8 +730,8 @@ void q8_mixed_kernel(Q8MixedParams p) {
     narrow_item<D>(p, it, cols, lds, wave, lane);
   } else {
     const int n_ct = (cols + 15) >> 4;
-    const int na = n_ct > wave ? (n_ct - wave + kMW - 1) / kMW : 0;  // column tiles wave, wave + 4
-    if (na >= 2)
+    const int na = n_ct > wave ? (n_ct - wave + kMW - 1) / kMW : 0;  // column tiles wave, wave + 4, ..
+    if (na == 2)
       wide_item<D, 2>(p, it, cols, lds, wave, lane);
     else if (na == 1)
       wide_item<D, 1>(p, it, cols, lds, wave, lane);
@@ -652,19 +741,19 @@ void q8_mixed_kernel(Q8MixedParams p) {
   if (it.n_chunks == 1) return;
   int32_t* const arrival = p.counters + it.ctr;
   if (!arrive_last(arrival, p.n_ctr, it.n_chunks, &sm_last, p.err)) return;
-  q8_mixed_merge<D>(p, it, cols);
+  q8_mixed_merge<D>(p, it, cols, lds);
   if (threadIdx.x == 0) counter_reset(arrival);
 }
 
 // Items a plan can hold: one a query tile and kv head, and kQ8Slots more from splitting.
 static int64_t q8_plan_items(int64_t B, int64_t total_T, int64_t H_q, int64_t H_kv) {
-  const int64_t R = q8_tile_cols() / (H_q / H_kv);
+  const int64_t R = kTileCols / (H_q / H_kv);
   return H_kv * (total_T / R + B) + kQ8Slots;
 }
 
 // Partial rows a launch can need: its split items' columns, and no more than kQ8MaxChunks a query row and head.
 static int64_t q8_part_rows(int64_t total_T, int64_t H_q) {
-  const int64_t most = (int64_t)kMaxSplitItems * q8_tile_cols();
+  const int64_t most = (int64_t)kMaxSplitItems * kTileCols;
   return total_T > most / (kQ8MaxChunks * H_q) ? most : kQ8MaxChunks * total_T * H_q;
 }
 
@@ -692,7 +781,7 @@ extern "C" int64_t cie_q8_mixed_plan_bytes(int64_t B, int64_t total_T, int64_t H
 }
 
 extern "C" int64_t cie_q8_mixed_partials_bytes(int64_t total_T, int64_t H_q, int64_t D) {
-  if (total_T < 0 || H_q <= 0 || H_q > 65536 || D <= 0) return -1;
+  if (total_T < 0 || H_q <= 0 || H_q > 65536 || (D != 64 && D != 128)) return -1;
   const int64_t rows = q8_part_rows(total_T, H_q);
   auto up = [](int64_t x) { return (x + 255) & ~int64_t(255); };
   return 2 * up(rows * 4) + rows * D * 4;
