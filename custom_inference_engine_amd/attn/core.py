@@ -28,6 +28,7 @@ does the split, RoPE and ``KVStorage.mixed_update`` of a mixed step in one.
 """
 from __future__ import annotations
 
+import functools
 import threading
 from typing import Optional
 
@@ -171,6 +172,7 @@ def _planned_buffers(lib, dev, B, H_q, H_kv, D, n_wg, counters):
     return partials, counters
 
 
+@functools.lru_cache(maxsize=None)
 def _cu_count(dev: torch.device | None) -> int:
     if dev is not None and dev.type == "cuda":
         return torch.cuda.get_device_properties(dev).multi_processor_count

@@ -15,60 +15,61 @@ from typing import Optional
 import torch
 
 from .. import _native
-from ..kv_cache.quant import check_cache_q8, int64_index, int64_table, new_rows, on_device
-from .core import (GQA_DECODE_CONFIG, _plan_workgroups, _qkv_rows, _require, _rope_rows, default_decode_splits,
-                   split_counters)
+from ..kv_cache.quant import check_cache_q8, int64_index, int64_table, launch, new_rows, one_device
+from .core import (DECODE_MAX_SPLITS, GQA_DECODE_CONFIG, _plan_workgroups, _qkv_rows, _require, _rope_rows,
+                   default_decode_splits, split_counters)
 
 
-def _decode(entry, o, q_args, cache, row_args, lens, slot_ids, block_table, H_q, append, num_programs, err, counters,
-            plan, dev):
+def _decode(entry, o, q_args, cache, geometry, row_args, lens, slot_ids, block_table, H_q, append, num_programs, err,
+            counters, plan, dev):
     """One decode launch of the C entry ``entry`` (cie_q8_decode*): its shared arguments and buffers."""
     k, v, scales = cache
-    N_PAGES, H_kv, PAGE_SIZE, D = k.shape
+    (N_PAGES, H_kv, PAGE_SIZE, D), (s_page, s_head, _, _) = geometry
     B = slot_ids.shape[0]
     lens, slot_ids, block_table = int64_index(lens), int64_index(slot_ids), int64_table(block_table)
-    lib = _native.load()
+    n_groups = B * H_kv
     if plan is not None:  # a step's plan (decode_plan, same append mode)
-        P = _plan_workgroups(plan)
-        n_wg = P
+        n_wg = P = _plan_workgroups(plan)
     else:
         P = int(num_programs) if num_programs else default_decode_splits(B, H_kv, dev)
-        _require(1 <= P <= lib.cie_paged_decode_max_splits(), "num_programs outside [1, the kernel's split limit]")
-        n_wg = P * B * H_kv
-    partials = None
-    if n_wg > B * H_kv:
-        partials = torch.empty(lib.cie_paged_decode_planned_partials_bytes(n_wg, H_q, H_kv, D), dtype=torch.uint8,
-                               device=dev)
+        _require(1 <= P <= DECODE_MAX_SPLITS, "num_programs outside [1, the kernel's split limit]")
+        n_wg = P * n_groups
+    partials = 0
+    if n_wg > n_groups:
+        n = _native.load().cie_paged_decode_planned_partials_bytes(n_wg, H_q, H_kv, D)
+        buffer = torch.empty(n, dtype=torch.uint8, device=dev)
+        partials = buffer.data_ptr()
         if counters is None:
-            counters = split_counters(dev, 2 * B * H_kv)
-        _require(counters.dtype == torch.int32 and counters.numel() >= 2 * B * H_kv, "counters too small")
-    n_slots = min(lens.shape[0], block_table.shape[0]) if append else block_table.shape[0]
-    with on_device(dev):
-        _native.check(
-            getattr(lib, entry)(
-                o.data_ptr(), *q_args, k.data_ptr(), v.data_ptr(), scales.data_ptr(), *row_args,
-                lens.data_ptr(), slot_ids.data_ptr(), block_table.data_ptr(), _native.ptr(plan),
-                _native.ptr(partials), _native.ptr(counters), B, H_q, H_kv, D, PAGE_SIZE, N_PAGES,
-                k.stride(0), k.stride(1), block_table.stride(0), block_table.shape[1], n_slots, P,
-                _native.ptr(err), _native.stream_handle(dev),
-            ),
-            entry,
-        )
+            counters = split_counters(dev, 2 * n_groups)
+        _require(counters.dtype == torch.int32 and counters.numel() >= 2 * n_groups, "counters too small")
+    slots, width = block_table.shape
+    launch(dev, entry, o.data_ptr(), *q_args, k.data_ptr(), v.data_ptr(), scales.data_ptr(), *row_args,
+           lens.data_ptr(), slot_ids.data_ptr(), block_table.data_ptr(), None if plan is None else plan.data_ptr(),
+           partials or None, None if counters is None else counters.data_ptr(), B, H_q, H_kv, D, PAGE_SIZE, N_PAGES,
+           s_page, s_head, block_table.stride(0), width, min(lens.shape[0], slots) if append else slots, P, err=err)
     return o
 
 
-def _check_decode(H_q, cache, slot_ids, block_table, rows: int) -> None:
-    k, v, scales = cache
-    check_cache_q8(k, v, scales)
-    _require(H_q % k.shape[1] == 0, "H_q must be a multiple of H_kv")
-    _require(k.shape[0] == block_table.shape[1], "block_table width must equal n_pages")
-    _require(rows == slot_ids.shape[0], "decode takes one query token per sequence")
+def _check_decode(H_q, cache, slot_ids, block_table, rows: int):
+    geometry = check_cache_q8(*cache)
+    if H_q % geometry[0][1]:
+        raise AssertionError("H_q must be a multiple of H_kv")
+    if geometry[0][0] != block_table.shape[1]:
+        raise AssertionError("block_table width must equal n_pages")
+    if rows != slot_ids.shape[0]:
+        raise AssertionError("decode takes one query token per sequence")
+    return geometry
 
 
-def _check_q(q: torch.Tensor, d: int) -> None:
-    _require(q.dim() == 4 and q.shape[0] == 1 and q.shape[3] == d, "q must be (1, T, H_q, D)")
-    _require(q.dtype == torch.float16, "q must be float16")
-    _require(q.is_contiguous(), "q must be contiguous")
+def _check_q(q: torch.Tensor, d: int) -> torch.Size:
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != 1 or shape[3] != d:
+        raise AssertionError("q must be (1, T, H_q, D)")
+    if q.dtype != torch.float16:
+        raise AssertionError("q must be float16")
+    if not q.is_contiguous():
+        raise AssertionError("q must be contiguous")
+    return shape
 
 
 def decode_gqa_attention_q8(q, k, v, scales, lens, slot_ids, block_table, num_programs=None, err=None, counters=None,
@@ -76,15 +77,14 @@ def decode_gqa_attention_q8(q, k, v, scales, lens, slot_ids, block_table, num_pr
     """``decode_gqa_attention`` over an 8-bit cache: q (1, B, H_q, D) against ``lens[b]`` tokens of each slot.
 
     ``plan``: the step's ``decode_plan`` (``append=False``)."""
-    _check_q(q, k.shape[3])
-    H_q = q.shape[2]
-    _check_decode(H_q, (k, v, scales), slot_ids, block_table, q.shape[1])
-    _require(tuple(lens.shape) == (slot_ids.shape[0],), "lens must be (B,)")
-    dev = _native.require_device(q, k, v, scales, lens, slot_ids, block_table)
+    _, B, H_q, _ = _check_q(q, k.shape[3])
+    geometry = _check_decode(H_q, (k, v, scales), slot_ids, block_table, B)
+    _require(lens.shape == (B,), "lens must be (B,)")
+    dev = one_device(q, k, v, scales, lens, slot_ids, block_table)
     o = torch.empty_like(q)
-    if q.shape[1] == 0:
+    if B == 0:
         return o
-    return _decode("cie_q8_decode", o, (q.data_ptr(),), (k, v, scales), (), lens, slot_ids, block_table, H_q, False,
+    return _decode("cie_q8_decode", o, (q.data_ptr(),), (k, v, scales), geometry, (), lens, slot_ids, block_table, H_q, False,
                    num_programs, err, counters, plan, dev)
 
 
@@ -95,18 +95,17 @@ def decode_append_gqa_attention_q8(q, k_cache, v_cache, scales, k, v, lens, slot
     The cache and the result are those of ``kv_append_decode_q8`` followed by
     ``decode_gqa_attention_q8`` over ``lens[slot_ids] + 1`` tokens.  Slots other
     than the padding slot must be distinct."""
-    _check_q(q, k_cache.shape[3])
-    H_q, B = q.shape[2], slot_ids.shape[0]
+    _, B, H_q, D = _check_q(q, k_cache.shape[3])
     cache = (k_cache, v_cache, scales)
-    _check_decode(H_q, cache, slot_ids, block_table, q.shape[1])
-    dev = _native.require_device(q, k_cache, v_cache, scales, k, v, lens, slot_ids, block_table)
-    kr, vr = new_rows(k, k_cache.shape[1], k_cache.shape[3]), new_rows(v, k_cache.shape[1], k_cache.shape[3])
-    _require(kr.shape[0] == B and vr.shape[0] == B, "one new K/V row per sequence")
+    geometry = _check_decode(H_q, cache, slot_ids, block_table, B)
+    H_kv = geometry[0][1]
+    dev = one_device(q, k_cache, v_cache, scales, k, v, lens, slot_ids, block_table)
+    (k, k_row, k_head), (v, v_row, v_head) = new_rows(k, B, H_kv, D), new_rows(v, B, H_kv, D)
     o = torch.empty_like(q)
     if B == 0:
         return o
-    rows = (kr.data_ptr(), vr.data_ptr(), kr.stride(0), kr.stride(1), vr.stride(0), vr.stride(1))
-    return _decode("cie_q8_decode_append", o, (q.data_ptr(),), cache, rows, lens, slot_ids, block_table, H_q, True,
+    rows = (k.data_ptr(), v.data_ptr(), k_row, k_head, v_row, v_head)
+    return _decode("cie_q8_decode_append", o, (q.data_ptr(),), cache, geometry, rows, lens, slot_ids, block_table, H_q, True,
                    num_programs, err, counters, plan, dev)
 
 
@@ -120,44 +119,35 @@ def decode_qkv_rope_gqa_attention_q8(qkv, cos, sin, k_cache, v_cache, scales, le
     H_q, (_, H_kv, _, D), B = int(num_heads), k_cache.shape, slot_ids.shape[0]
     cache = (k_cache, v_cache, scales)
     rows = _qkv_rows(qkv, (H_q + 2 * H_kv) * D)
-    _check_decode(H_q, cache, slot_ids, block_table, rows.shape[0])
-    dev = _native.require_device(rows, cos, sin, k_cache, v_cache, scales, lens, slot_ids, block_table)
+    geometry = _check_decode(H_q, cache, slot_ids, block_table, rows.shape[0])
+    dev = one_device(rows, cos, sin, k_cache, v_cache, scales, lens, slot_ids, block_table)
     cr, sr = _rope_rows(cos, B, D), _rope_rows(sin, B, D)
     _require(cr.stride(0) == sr.stride(0), "cos and sin need the same row stride")
     o = rows.new_empty((1, B, H_q, D))
     if B == 0:
         return o
     q_args = (rows.data_ptr(), rows.stride(0), cr.data_ptr(), sr.data_ptr(), cr.stride(0))
-    return _decode("cie_q8_decode_qkv_rope", o, q_args, cache, (), lens, slot_ids, block_table, H_q, True,
+    return _decode("cie_q8_decode_qkv_rope", o, q_args, cache, geometry, (), lens, slot_ids, block_table, H_q, True,
                    num_programs, err, counters, plan, dev)
 
 
 def append_tokens_qkv_rope_q8(qkv, cos, sin, k_cache, v_cache, scales, pages, offsets, num_heads: int, err=None):
     """``append_tokens_qkv_rope`` into an 8-bit cache, one launch: returns the rotated q (1, T, H_q, D)."""
-    check_cache_q8(k_cache, v_cache, scales)
-    N_PAGES, H_kv, PAGE_SIZE, D = k_cache.shape
+    (N_PAGES, H_kv, PAGE_SIZE, D), (s_page, s_head, _, _) = check_cache_q8(k_cache, v_cache, scales)
     H_q = int(num_heads)
     rows = _qkv_rows(qkv, (H_q + 2 * H_kv) * D)
     T = rows.shape[0]
     _require(tuple(pages.shape) == (T,) and tuple(offsets.shape) == (T,), "pages / offsets must be (T,)")
-    dev = _native.require_device(rows, cos, sin, k_cache, v_cache, scales, pages, offsets)
+    dev = one_device(rows, cos, sin, k_cache, v_cache, scales, pages, offsets)
     cr, sr = _rope_rows(cos, T, D), _rope_rows(sin, T, D)
     _require(cr.stride(0) == sr.stride(0), "cos and sin need the same row stride")
     pages, offsets = int64_index(pages), int64_index(offsets)
     q = rows.new_empty((1, T, H_q, D))
     if T == 0:
         return q
-    lib = _native.load()
-    with on_device(dev):
-        _native.check(
-            lib.cie_q8_append_tokens_qkv_rope(
-                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr(), rows.data_ptr(),
-                rows.stride(0), cr.data_ptr(), sr.data_ptr(), cr.stride(0), pages.data_ptr(), offsets.data_ptr(),
-                T, H_q, H_kv, PAGE_SIZE, D, N_PAGES, k_cache.stride(0), k_cache.stride(1),
-                _native.ptr(err), _native.stream_handle(dev),
-            ),
-            "cie_q8_append_tokens_qkv_rope",
-        )
+    launch(dev, "cie_q8_append_tokens_qkv_rope", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+           scales.data_ptr(), rows.data_ptr(), rows.stride(0), cr.data_ptr(), sr.data_ptr(), cr.stride(0),
+           pages.data_ptr(), offsets.data_ptr(), T, H_q, H_kv, PAGE_SIZE, D, N_PAGES, s_page, s_head, err=err)
     return q
 
 
@@ -173,21 +163,15 @@ def mixed_plan_q8(k_cache, cu_seqlens, kv_lens, slot_ids, block_table, max_seqle
     _require(tuple(cu_seqlens.shape) == (B + 1,) and tuple(kv_lens.shape) == (B,),
              "cu_seqlens must be (B+1,) and kv_lens (B,)")
     _require(N_PAGES == block_table.shape[1], "block_table width must equal n_pages")
-    dev = _native.require_device(k_cache, cu_seqlens, kv_lens, slot_ids, block_table)
+    dev = one_device(k_cache, cu_seqlens, kv_lens, slot_ids, block_table)
     cu_seqlens, kv_lens, slot_ids = int64_index(cu_seqlens), int64_index(kv_lens), int64_index(slot_ids)
     lib = _native.load()
     n = lib.cie_q8_mixed_plan_bytes(B, int(total_T), num_heads, H_kv)
     _require(n > 0, "batch too large for a mixed plan")
     plan = torch.empty(n // 4, dtype=torch.int32, device=dev)
-    with on_device(dev):
-        _native.check(
-            lib.cie_q8_mixed_plan(
-                plan.data_ptr(), n, cu_seqlens.data_ptr(), kv_lens.data_ptr(), slot_ids.data_ptr(), B, int(total_T),
-                int(max_seqlen), num_heads, H_kv, D, PAGE_SIZE, block_table.shape[1], block_table.shape[0],
-                _native.ptr(err), _native.stream_handle(dev),
-            ),
-            "cie_q8_mixed_plan",
-        )
+    launch(dev, "cie_q8_mixed_plan", plan.data_ptr(), n, cu_seqlens.data_ptr(), kv_lens.data_ptr(),
+           slot_ids.data_ptr(), B, int(total_T), int(max_seqlen), num_heads, H_kv, D, PAGE_SIZE, N_PAGES,
+           block_table.shape[0], err=err)
     return plan
 
 
@@ -200,42 +184,35 @@ def mixed_gqa_attention_q8(q, k, v, scales, max_seqlen: int, cu_seqlens, kv_lens
     ``torch.empty_like`` leaves them.  ``plan``: the step's ``mixed_plan_q8``;
     without one the call makes its own (a second, small launch).
     """
-    _check_q(q, k.shape[3])
-    total_T, H_q, D = q.shape[1:]
-    check_cache_q8(k, v, scales)
-    N_PAGES, H_kv, PAGE_SIZE, _ = k.shape
+    _, total_T, H_q, D = _check_q(q, k.shape[3])
+    (N_PAGES, H_kv, PAGE_SIZE, _), (s_page, s_head, _, _) = check_cache_q8(k, v, scales)
     B = slot_ids.shape[0]
     _require(H_q % H_kv == 0, "H_q must be a multiple of H_kv")
-    _require(tuple(kv_lens.shape) == (B,), "kv_lens must be (B,)")
-    _require(tuple(cu_seqlens.shape) == (B + 1,), "cu_seqlens must be (B+1,)")
-    _require(N_PAGES == block_table.shape[1], "block_table width must equal n_pages")
-    dev = _native.require_device(q, k, v, scales, cu_seqlens, kv_lens, slot_ids, block_table)
+    _require(kv_lens.shape == (B,), "kv_lens must be (B,)")
+    _require(cu_seqlens.shape == (B + 1,), "cu_seqlens must be (B+1,)")
+    slots, width = block_table.shape
+    _require(N_PAGES == width, "block_table width must equal n_pages")
+    dev = one_device(q, k, v, scales, cu_seqlens, kv_lens, slot_ids, block_table)
     o = torch.empty_like(q)
     if B == 0 or total_T == 0 or int(max_seqlen) == 0:
         return o
     block_table = int64_table(block_table)
+    lib = _native.load()
     if plan is None:
         plan = mixed_plan_q8(k, cu_seqlens, kv_lens, slot_ids, block_table, max_seqlen, total_T, H_q, err=err)
-    lib = _native.load()
-    _require(plan.dtype == torch.int32 and plan.is_contiguous()
-             and plan.numel() * 4 >= lib.cie_q8_mixed_plan_bytes(B, total_T, H_q, H_kv),
-             "plan must come from mixed_plan_q8 for this batch")
+    else:
+        _require(plan.dtype == torch.int32 and plan.is_contiguous()
+                 and plan.numel() * 4 >= lib.cie_q8_mixed_plan_bytes(B, total_T, H_q, H_kv),
+                 "plan must come from mixed_plan_q8 for this batch")
     n = lib.cie_q8_mixed_partials_bytes(total_T, H_q, D)
     partials = torch.empty(n, dtype=torch.uint8, device=dev)
     n_ctr = lib.cie_q8_mixed_counters()
     if counters is None:
         counters = split_counters(dev, n_ctr)
     _require(counters.dtype == torch.int32 and counters.numel() >= n_ctr, "counters too small")
-    with on_device(dev):
-        _native.check(
-            lib.cie_q8_mixed(
-                o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), scales.data_ptr(), plan.data_ptr(),
-                plan.numel() * 4, block_table.data_ptr(), partials.data_ptr(), n, counters.data_ptr(), B, total_T,
-                H_q, H_kv, D, PAGE_SIZE, N_PAGES, k.stride(0), k.stride(1), block_table.stride(0),
-                block_table.shape[1], block_table.shape[0], _native.ptr(err), _native.stream_handle(dev),
-            ),
-            "cie_q8_mixed",
-        )
+    launch(dev, "cie_q8_mixed", o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), scales.data_ptr(),
+           plan.data_ptr(), plan.numel() * 4, block_table.data_ptr(), partials.data_ptr(), n, counters.data_ptr(), B,
+           total_T, H_q, H_kv, D, PAGE_SIZE, N_PAGES, s_page, s_head, block_table.stride(0), width, slots, err=err)
     return o
 
 

@@ -23,6 +23,7 @@ namespace cie {
 
 constexpr int kAppendThreads = 256;
 constexpr int kAppendWaves = kAppendThreads / kWave;
+constexpr int kScan = 8;
 
 struct Q8Params {
   uint8_t* k_pool;
@@ -61,63 +62,84 @@ struct Q8Rows {
   const int* last;  // [16] token of each row, -1: not written
 };
 
-// One wave's (block, head, K or V).
+// One wave's (block, head, K or V): loaded, then rounded and stored, so that a wave can load its next one between.
 template <int D, bool kRope>
-__device__ __forceinline__ void append_block(const Q8Params& p, const Q8Rows& b, int h, bool is_v, int lane) {
-  constexpr int NU = D / 64;    // units of 16 values a lane
-  constexpr int kPer = D / 16;  // units a row
-  uint8_t* const pool = (is_v ? p.v_pool : p.k_pool) + b.page * p.pool_page_stride + h * p.pool_head_stride +
-                        (int64_t)b.block * kQ8Block * D;
-  float* const scale = p.scales + 2 * ((b.page * p.H_kv + h) * (p.page_size / kQ8Block) + b.block) + (is_v ? 1 : 0);
-  const f16* const src = is_v ? p.v_new + h * p.v_head_stride : p.k_new + h * p.k_head_stride;
-  const int64_t stride = is_v ? p.v_tok_stride : p.k_tok_stride;
-  const int e_old = b.fresh ? kQ8EMin : q8_scale_exponent(*scale);
+struct BlockTask {
+  static constexpr int NU = D / 64;    // units of 16 values a lane
+  static constexpr int kPer = D / 16;  // units a row
+  uint8_t* pool;
+  float* scale;
+  float old_scale;
   f16x8 x[NU][2];
+  f16x8 cs[kRope ? NU : 1][4];  // cos and sin of the dims, of their partners
   u32x2 old[NU][2];
-  bool written[NU];
-  uint32_t mag = 0;
+  bool written[NU], rope;
+
+  __device__ __forceinline__ void load(const Q8Params& p, const Q8Rows& b, int task, int lane) {
+    const int h = task >> 1;
+    const bool is_v = task & 1;
+    pool = (is_v ? p.v_pool : p.k_pool) + b.page * p.pool_page_stride + h * p.pool_head_stride +
+           (int64_t)b.block * kQ8Block * D;
+    scale = p.scales + 2 * ((b.page * p.H_kv + h) * (p.page_size / kQ8Block) + b.block) + (is_v ? 1 : 0);
+    const f16* const src = is_v ? p.v_new + h * p.v_head_stride : p.k_new + h * p.k_head_stride;
+    const int64_t stride = is_v ? p.v_tok_stride : p.k_tok_stride;
+    rope = kRope && !is_v;
+    old_scale = 0.f;
+    if (!b.fresh) old_scale = *scale;
 #pragma unroll
-  for (int u = 0; u < NU; ++u) {
-    const int unit = lane + u * kWave;
-    const int row = unit / kPer, d0 = 8 * (unit % kPer);
-    const int t = b.last[row];
-    written[u] = t >= 0;
-    if (written[u]) {
-      const f16* const r = src + t * stride + d0;
-      x[u][0] = *reinterpret_cast<const f16x8*>(r);
-      x[u][1] = *reinterpret_cast<const f16x8*>(r + D / 2);
-      if constexpr (kRope) {
-        if (!is_v) {
+    for (int u = 0; u < NU; ++u) {
+      const int unit = lane + u * kWave;
+      const int row = unit / kPer, d0 = 8 * (unit % kPer);
+      const int t = b.last[row];
+      written[u] = t >= 0;
+      if (written[u]) {
+        const f16* const r = src + t * stride + d0;
+        x[u][0] = *reinterpret_cast<const f16x8*>(r);
+        x[u][1] = *reinterpret_cast<const f16x8*>(r + D / 2);
+        if (rope) {
           const f16* const c = p.cos + t * p.cs_stride + d0;
           const f16* const s = p.sin + t * p.cs_stride + d0;
-          rope8(x[u][0], x[u][1], *reinterpret_cast<const f16x8*>(c), *reinterpret_cast<const f16x8*>(c + D / 2),
-                *reinterpret_cast<const f16x8*>(s), *reinterpret_cast<const f16x8*>(s + D / 2));
+          cs[u][0] = *reinterpret_cast<const f16x8*>(c);
+          cs[u][1] = *reinterpret_cast<const f16x8*>(c + D / 2);
+          cs[u][2] = *reinterpret_cast<const f16x8*>(s);
+          cs[u][3] = *reinterpret_cast<const f16x8*>(s + D / 2);
         }
+      } else if (!b.fresh) {
+        old[u][0] = *reinterpret_cast<const u32x2*>(pool + row * D + d0);
+        old[u][1] = *reinterpret_cast<const u32x2*>(pool + row * D + d0 + D / 2);
       }
-      mag = q8_mag8(x[u][0], q8_mag8(x[u][1], mag));
-    } else if (!b.fresh) {
-      old[u][0] = *reinterpret_cast<const u32x2*>(pool + row * D + d0);
-      old[u][1] = *reinterpret_cast<const u32x2*>(pool + row * D + d0 + D / 2);
     }
   }
-  const int e = max(e_old, q8_exponent(q8_wave_mag(mag)));
-  const float inv = q8_pow2(-e), factor = q8_pow2(e_old - e);
+
+  __device__ __forceinline__ void store(bool fresh, int lane) {
+    uint32_t mag = 0;
 #pragma unroll
-  for (int u = 0; u < NU; ++u) {
-    const int unit = lane + u * kWave;
-    uint8_t* const dst = pool + (unit / kPer) * D + 8 * (unit % kPer);
-    if (written[u]) {
-      *reinterpret_cast<u32x2*>(dst) = q8_round8(x[u][0], inv);
-      *reinterpret_cast<u32x2*>(dst + D / 2) = q8_round8(x[u][1], inv);
-    } else if (!b.fresh && e != e_old) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<u32x2*>(dst + i * (D / 2)) =
-            u32x2{q8_rescale4(old[u][i][0], factor), q8_rescale4(old[u][i][1], factor)};
+    for (int u = 0; u < NU; ++u) {
+      if (written[u]) {
+        if (rope) rope8(x[u][0], x[u][1], cs[u][0], cs[u][1], cs[u][2], cs[u][3]);
+        mag = q8_mag8(x[u][0], q8_mag8(x[u][1], mag));
+      }
     }
+    const int e_old = fresh ? kQ8EMin : q8_scale_exponent(old_scale);
+    const int e = max(e_old, q8_exponent(q8_wave_mag(mag)));
+    const float inv = q8_pow2(-e), factor = q8_pow2(e_old - e);
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int unit = lane + u * kWave;
+      uint8_t* const dst = pool + (unit / kPer) * D + 8 * (unit % kPer);
+      if (written[u]) {
+        *reinterpret_cast<u32x2*>(dst) = q8_round8(x[u][0], inv);
+        *reinterpret_cast<u32x2*>(dst + D / 2) = q8_round8(x[u][1], inv);
+      } else if (!fresh && e != e_old) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          *reinterpret_cast<u32x2*>(dst + i * (D / 2)) =
+              u32x2{q8_rescale4(old[u][i][0], factor), q8_rescale4(old[u][i][1], factor)};
+      }
+    }
+    if (lane == 0) *scale = q8_pow2(e);
   }
-  if (lane == 0) *scale = q8_pow2(e);
-}
+};
 
 // The q heads of the rope form: a lane rotates 8 dims and their partners.
 template <int D>
@@ -150,39 +172,49 @@ __global__ __launch_bounds__(kAppendThreads) void q8_append_kernel(Q8Params p) {
       return;
     }
   }
-  const int64_t t_end = min(p.n_rows, (int64_t)(blockIdx.x + 1) * p.tokens_per_wg);
-  for (int64_t t = (int64_t)blockIdx.x * p.tokens_per_wg; t < t_end; ++t) {  // (every branch below is uniform)
-    int64_t page, off;
+  // The workgroup's tokens, a lane each (every wave the same): which of them start a run.
+  // A prompt's run starts lie 16 tokens apart.  Workgroups go round the XCDs and their CUs in turn, so dealt in order
+  // the ones with work would share a few CUs: the list is dealt with stride 16 tokens instead, which makes them
+  // neighbours (4 x 2,048 rows, D = 128: 29 us dealt in order).
+  const int stride = kQ8Block / p.tokens_per_wg, per = p.n_append_wg / stride;
+  const int64_t t0 = (int64_t)(stride * ((int)blockIdx.x % per) + (int)blockIdx.x / per) * p.tokens_per_wg;
+  int64_t page = 0, off = 0;
+  bool head = false;
+  if (lane < p.tokens_per_wg && t0 + lane < p.n_rows) {
+    const int64_t t = t0 + lane;
+    int bad = 0;
     if constexpr (kDecode) {
       const int64_t slot = p.slot_ids[t];
       if (slot < 0 || slot >= p.n_slots) {
-        if (threadIdx.x == 0) set_err(p.err, CIE_ERRBIT_PAGE);
-        continue;
+        bad = CIE_ERRBIT_PAGE;
+      } else {
+        const int64_t pos = p.lens[slot];
+        if (pos < 0 || pos >= p.bt_width * p.page_size) {
+          bad = CIE_ERRBIT_LEN;
+        } else {
+          page = p.block_table[slot * p.bt_stride + pos / p.page_size];
+          off = pos % p.page_size;
+        }
       }
-      const int64_t pos = p.lens[slot];
-      if (pos < 0 || pos >= p.bt_width * p.page_size) {
-        if (threadIdx.x == 0) set_err(p.err, CIE_ERRBIT_LEN);
-        continue;
-      }
-      page = p.block_table[slot * p.bt_stride + pos / p.page_size];
-      off = pos % p.page_size;
+      head = true;
     } else {
       page = p.pages[t];
       off = p.offsets[t];
-      if (off < 0 || off >= p.page_size) {
-        if (threadIdx.x == 0) set_err(p.err, CIE_ERRBIT_OFFSET);
-        continue;
-      }
+      const int64_t page1 = t > 0 ? p.pages[t - 1] : -1, off1 = t > 0 ? p.offsets[t - 1] : -1;
+      if (off < 0 || off >= p.page_size) bad = CIE_ERRBIT_OFFSET;
+      head = page1 != page || off1 < 0 || off1 >= p.page_size || (int)off1 / kQ8Block != (int)off / kQ8Block;
     }
-    if (page < 0 || page >= p.n_pages) {
-      if (threadIdx.x == 0) set_err(p.err, CIE_ERRBIT_PAGE);
-      continue;
+    if (!bad && (page < 0 || page >= p.n_pages)) bad = CIE_ERRBIT_PAGE;
+    if (bad) {
+      head = false;
+      if (wave == 0) set_err(p.err, bad);
     }
-    const int block = (int)off / kQ8Block;
-    if (!kDecode && t > 0 && p.pages[t - 1] == page) {
-      const int64_t o = p.offsets[t - 1];
-      if (o >= 0 && o < p.page_size && (int)o / kQ8Block == block) continue;  // not its run's first token
-    }
+  }
+  for (uint64_t heads = __ballot(head); heads; heads &= heads - 1) {  // (uniform in the workgroup)
+    const int i = __builtin_ctzll(heads);
+    const int64_t t = t0 + i;
+    const int64_t pg = readlane64(page, i), o = readlane64(off, i);
+    const int block = (int)o / kQ8Block;
     __syncthreads();  // (the last token's block is done with `last`)
     if (threadIdx.x < kQ8Block) last[threadIdx.x] = -1;
     if (threadIdx.x == 0) earlier = 0;
@@ -191,23 +223,45 @@ __global__ __launch_bounds__(kAppendThreads) void q8_append_kernel(Q8Params p) {
       // a slot that comes again later in the batch writes the row
       const int64_t slot = p.slot_ids[t];
       bool again = false;
-      for (int64_t i = t + 1 + threadIdx.x; i < p.n_rows; i += kAppendThreads) again |= p.slot_ids[i] == slot;
+      for (int64_t k = t + 1 + threadIdx.x; k < p.n_rows; k += kAppendThreads) again |= p.slot_ids[k] == slot;
       if (again) earlier = 1;
-      if (threadIdx.x == 0) last[off % kQ8Block] = (int)t;
+      if (threadIdx.x == 0) last[o % kQ8Block] = (int)t;
     } else {
-      for (int64_t i = threadIdx.x; i < p.n_rows; i += kAppendThreads) {
-        if (p.pages[i] != page) continue;
-        const int64_t o = p.offsets[i];
-        if (o < 0 || o >= p.page_size || (int)o / kQ8Block != block) continue;
-        if (i < t) earlier = 1;
-        atomicMax(&last[o % kQ8Block], (int)i);
+      // the list's tokens of this block; kScan page ids a thread in flight
+      for (int64_t k0 = threadIdx.x; k0 < p.n_rows; k0 += kScan * kAppendThreads) {
+        int64_t q[kScan];
+#pragma unroll
+        for (int u = 0; u < kScan; ++u) q[u] = p.pages[min(k0 + u * kAppendThreads, p.n_rows - 1)];
+        bool any = false;
+#pragma unroll
+        for (int u = 0; u < kScan; ++u) any |= q[u] == pg;
+        if (any) {
+#pragma unroll
+          for (int u = 0; u < kScan; ++u) {
+            const int64_t k = k0 + u * kAppendThreads;
+            if (k < p.n_rows && q[u] == pg) {
+              const int64_t ko = p.offsets[k];
+              if (ko >= 0 && ko < p.page_size && (int)ko / kQ8Block == block) {
+                if (k < t) earlier = 1;
+                atomicMax(&last[ko % kQ8Block], (int)k);
+              }
+            }
+          }
+        }
       }
     }
     __syncthreads();
     if (earlier) continue;
-    const Q8Rows rows{page, block, last[0] >= 0, last};
-    for (int task = wave; task < 2 * p.H_kv; task += kAppendWaves)
-      append_block<D, kRope>(p, rows, task >> 1, task & 1, lane);
+    const Q8Rows rows{pg, block, last[0] >= 0, last};
+    const int n_tasks = 2 * p.H_kv;
+    BlockTask<D, kRope> task[2];
+    for (int k = wave; k < n_tasks; k += 2 * kAppendWaves) {
+      const bool two = k + kAppendWaves < n_tasks;
+      task[0].load(p, rows, k, lane);
+      if (two) task[1].load(p, rows, k + kAppendWaves, lane);
+      task[0].store(rows.fresh, lane);
+      if (two) task[1].store(rows.fresh, lane);
+    }
   }
 }
 
@@ -275,14 +329,16 @@ static int q8_check_pools(const void* k_pool, const void* v_pool, const void* sc
   return CIE_OK;
 }
 
-// Tokens a workgroup looks at: one, so that the rows of a decode batch, each a block of its own, run side
-// by side; four at more tokens than the chip holds workgroups at once (2,048), where most belong to a run
-// that another workgroup owns and only their number costs.
+// Tokens a workgroup looks at (a power of two, 16 at most): one up to the 2,048 workgroups that the chip holds at once,
+// so that the rows of a decode batch, each a block of its own, run side by side; more where it would take more rounds
+// of workgroups, most of whose tokens belong to a run that another owns.
 template <bool kDecode, bool kRope>
 static int q8_launch_append(Q8Params& p, int64_t D, hipStream_t stream) {
   if (p.n_rows > 0x7fffffff / 512) return CIE_EUNSUPPORTED;
-  p.tokens_per_wg = !kDecode && p.n_rows > 2048 ? 4 : 1;
-  p.n_append_wg = (int32_t)((p.n_rows + p.tokens_per_wg - 1) / p.tokens_per_wg);
+  p.tokens_per_wg = 1;
+  while (!kDecode && p.tokens_per_wg < kQ8Block && p.n_rows > 2048 * p.tokens_per_wg) p.tokens_per_wg *= 2;
+  const int32_t stride = kQ8Block / p.tokens_per_wg;
+  p.n_append_wg = (int32_t)((p.n_rows + kQ8Block - 1) / kQ8Block) * stride;
   int64_t blocks = p.n_append_wg;
   if (kRope) blocks += (p.n_rows * p.H_q * (D / 16) + kAppendThreads - 1) / kAppendThreads;
   if (blocks > 0x7fffffff) return CIE_EUNSUPPORTED;

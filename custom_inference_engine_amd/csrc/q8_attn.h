@@ -188,18 +188,17 @@ __device__ __forceinline__ void q8_step(SoftmaxAcc<D, NCT>& st, K k, V v, M mean
   }
 }
 
-// The same for one column tile from raw tiles.
-template <int D>
-__device__ __forceinline__ void q8_attend(SoftmaxAcc<D, 1>& st, const Q8Tile<D>& a, const Q8Tile<D>& b, float ksa,
-                                          float vsa, float ksb, float vsb, const f16x8 (&q)[1][Geo<D>::KS], int key0a,
-                                          int key0b, const int (&lim)[1], bool mask, float scale_log2, int grp) {
-  auto k = [&](int i, f16x8 (&ka)[Geo<D>::KS]) { q8_k_operand<D>(ka, i ? b : a, i ? ksb : ksa); };
-  auto v = [&](int, f16x8 (&va)[Geo<D>::NT]) {
-    q8_v_operand<D>(va, 0, a, vsa);
-    q8_v_operand<D>(va, 1, b, vsb);
+// The same for one column tile from raw tiles: NT2 = 2 NP of them with their K and V scales.
+template <int D, int NT2>
+__device__ __forceinline__ void q8_attend(SoftmaxAcc<D, 1>& st, const Q8Tile<D> (&t)[NT2], const f32x2 (&sc)[NT2],
+                                          const f16x8 (&q)[1][Geo<D>::KS], const int (&key0)[NT2], const int (&lim)[1],
+                                          bool mask, float scale_log2, int grp) {
+  auto k = [&](int i, f16x8 (&ka)[Geo<D>::KS]) { q8_k_operand<D>(ka, t[i], sc[i][0]); };
+  auto v = [&](int pr, f16x8 (&va)[Geo<D>::NT]) {
+    q8_v_operand<D>(va, 0, t[2 * pr], sc[2 * pr][1]);
+    q8_v_operand<D>(va, 1, t[2 * pr + 1], sc[2 * pr + 1][1]);
   };
-  const int key0[2] = {key0a, key0b};
-  q8_step<D, 1, 1, false>(st, k, v, [] {}, q, key0, lim, mask, scale_log2, grp);
+  q8_step<D, 1, NT2 / 2, false>(st, k, v, [] {}, q, key0, lim, mask, scale_log2, grp);
 }
 
 // Where a wave's tiles live: kv head g of the pools and of the scales.

@@ -12,9 +12,9 @@
 // its S * 4 waves, wave gw taking tiles gw, gw + 4 S, ... (the plan's deal).  A tile is
 // a block of the cache, so a wave's tile comes with one K and one V scale: lane k
 // holds the byte offset and the scales of the wave's k-th tile, gathered 64 at a
-// time, and a step reads two lanes.  A ring of kQ8Pf + 1 steps of raw bytes (a step is
-// 32 keys, 2 D bytes of K and V a key) keeps kQ8Pf steps of loads in flight; they are
-// converted when their step comes.
+// time, and a step of q8_tiles tiles reads as many lanes.  A ring of q8_pf + 1 steps of
+// raw bytes keeps q8_pf steps of loads in flight; they are converted when their step
+// comes.
 // The new row's tile belongs to the wave that it would be dealt to: that wave loads
 // the tile's bytes first of all, and after its other tiles rounds the new row under
 // the block's new scale, rewrites the block's rows if the scale grew, and attends the
@@ -32,10 +32,27 @@ constexpr int kQ8Waves = 4;
 constexpr int kQ8Threads = kQ8Waves * kWave;
 constexpr int kQ8MaxSplits = 64;
 constexpr int kQ8PlanDesc = 8;  // a plan's words per workgroup (paged_decode.hip)
-// 32-key steps of loads in flight
+// Tiles of a step, and steps of loads in flight ahead of the one at work.  A lone wave on its SIMD waits out each
+// step's chain (scores, maximum, exponentials, P.V), so at D = 64 a step takes four tiles.
+#ifndef T64
+#define T64 4
+#endif
+#ifndef PF64
+#define PF64 1
+#endif
+#ifndef T128
+#define T128 2
+#endif
+#ifndef PF128
+#define PF128 2
+#endif
+template <int D>
+constexpr int q8_tiles() {
+  return D == 64 ? T64 : T128;
+}
 template <int D>
 constexpr int q8_pf() {
-  return D == 64 ? 3 : 2;
+  return D == 64 ? PF64 : PF128;
 }
 
 struct Q8DecodeParams {
@@ -247,7 +264,7 @@ void q8_decode_kernel(const int64_t* __restrict__ a_slot_ids, const int32_t* __r
   constexpr int KS = Geo<D>::KS;
   constexpr int NT = Geo<D>::NT;
   constexpr int W = kQ8Waves;
-  constexpr int PF = q8_pf<D>();
+  constexpr int PF = q8_pf<D>(), NS = q8_tiles<D>();
   typedef typename HVec<NT>::type vhalf_t;
   __shared__ float sm_m[W][16];
   __shared__ float sm_l[W][16];
@@ -416,14 +433,14 @@ void q8_decode_kernel(const int64_t* __restrict__ a_slot_ids, const int32_t* __r
       lane_tiles(c0, (int)pg);
     }
     const int n_chunk = min(kWave, n_mine - c0);
-    const int n_steps = (n_chunk + 1) >> 1;
-    Q8Tile<D> ring[PF + 1][2];
-    // every iteration issues one step's loads (past the last: of no rows), so that the wait before a step
+    const int n_steps = (n_chunk + NS - 1) / NS;
+    Q8Tile<D> ring[PF + 1][NS];
+    // every iteration issues one step's loads (past the last tile: of no rows), so that the wait before a step
     // covers that step's loads only
     auto issue = [&](int i, int j) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int k = 2 * j + u;
+      for (int u = 0; u < NS; ++u) {
+        const int k = NS * j + u;
         const int kk = min(k, n_chunk - 1);
         const int rows = k < n_chunk ? min(16, L - (gw + (c0 + kk) * TW) * 16) : 0;
         const int64_t off = readlane64(toff, kk);
@@ -439,14 +456,17 @@ void q8_decode_kernel(const int64_t* __restrict__ a_slot_ids, const int32_t* __r
         const int j = j0 + u;
         issue((u + PF) % (PF + 1), j + PF);
         if (j < n_steps) {
-          const int ka = 2 * j, kb = min(ka + 1, n_chunk - 1);
-          const int key0a = (gw + (c0 + ka) * TW) * 16;
-          const int key0b = ka + 1 < n_chunk ? key0a + 16 * TW : kNoKey;
-          auto sc = [&](int i, int k) {
-            return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(tsc[i]), k));
-          };
-          q8_attend<D>(st, ring[u][0], ring[u][1], sc(0, ka), sc(1, ka), sc(0, kb), sc(1, kb), q, key0a, key0b, lim,
-                       max(key0a, key0b) + 16 > L, p.scale_log2, grp);
+          int key0[NS];
+          f32x2 sc[NS];
+#pragma unroll
+          for (int i = 0; i < NS; ++i) {
+            const int k = NS * j + i, kk = min(k, n_chunk - 1);
+            key0[i] = k < n_chunk ? (gw + (c0 + kk) * TW) * 16 : kNoKey;
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+              sc[i][w] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(tsc[w]), kk));
+          }
+          q8_attend<D, NS>(st, ring[u], sc, q, key0, lim, key0[NS - 1] + 16 > L, p.scale_log2, grp);
         }
       }
     }
@@ -456,7 +476,10 @@ void q8_decode_kernel(const int64_t* __restrict__ a_slot_ids, const int32_t* __r
       const int row = pos & 15;
       append_row<D>(nt, kn, vn, nk, nv, nscale, nsc, row, r16, grp, lo);
       q8_zero_rows<D>(nt, row + 1, grp);
-      q8_attend<D>(st, nt, nt, nsc[0], nsc[1], nsc[0], nsc[1], q, pos - row, kNoKey, lim, true, p.scale_log2, grp);
+      const Q8Tile<D> pair[2] = {nt, nt};  // (the second copy masked)
+      const f32x2 sc[2] = {nsc, nsc};
+      const int key0[2] = {pos - row, kNoKey};
+      q8_attend<D, 2>(st, pair, sc, q, key0, lim, true, p.scale_log2, grp);
     }
   }
 

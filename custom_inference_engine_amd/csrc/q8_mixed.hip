@@ -623,7 +623,7 @@ template <int D>
 __device__ __forceinline__ void narrow_item(const Q8MixedParams& p, const Q8Item& it, int cols, f32x4* lds, int wave,
                                             int lane) {
   constexpr int KS = Geo<D>::KS, NT = Geo<D>::NT, D4 = D / 4;
-  constexpr int PF = D == 64 ? 3 : 2;
+  constexpr int PF = D == 64 ? 1 : 2, NS = D == 64 ? 4 : 2;  // (as the decode kernel's)
   const int r16 = lane & 15, grp = lane >> 4;
   const Q8Lane<D> lo(r16, grp);
   const int key_end = it.pos0 - it.rows;  // (rows: negative here)
@@ -638,12 +638,12 @@ __device__ __forceinline__ void narrow_item(const Q8MixedParams& p, const Q8Item
   for (int c0 = 0; c0 < tiles.n; c0 += kWave) {
     if (c0 > 0) tiles.gather(c0);
     const int n_chunk = min(kWave, tiles.n - c0);
-    const int n_steps = (n_chunk + 1) >> 1;
-    Q8Tile<D> ring[PF + 1][2];
+    const int n_steps = (n_chunk + NS - 1) / NS;
+    Q8Tile<D> ring[PF + 1][NS];
     auto issue = [&](int i, int j) {  // (tiles past the last: no rows)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        tiles.template load<kBufNt>(ring[i][u], c0, 2 * j + u < n_chunk ? 2 * j + u : tiles.n, key_end, lo);
+      for (int u = 0; u < NS; ++u)
+        tiles.template load<kBufNt>(ring[i][u], c0, NS * j + u < n_chunk ? NS * j + u : tiles.n, key_end, lo);
     };
 #pragma unroll
     for (int j = 0; j < PF; ++j) issue(j, j);
@@ -653,11 +653,15 @@ __device__ __forceinline__ void narrow_item(const Q8MixedParams& p, const Q8Item
         const int j = j0 + u;
         issue((u + PF) % (PF + 1), j + PF);
         if (j < n_steps) {
-          const int ka = 2 * j, kb = min(ka + 1, n_chunk - 1);
-          const int key0a = 16 * (tiles.t0 + 4 * (c0 + ka));
-          const int key0b = ka + 1 < n_chunk ? key0a + 64 : kNoKey;
-          q8_attend<D>(st, ring[u][0], ring[u][1], tiles.scale(0, ka), tiles.scale(1, ka), tiles.scale(0, kb),
-                       tiles.scale(1, kb), q, key0a, key0b, lim, max(key0a, key0b) + 16 > mask_from, p.scale_log2, grp);
+          int key0[NS];
+          f32x2 sc[NS];
+#pragma unroll
+          for (int i = 0; i < NS; ++i) {
+            const int k = NS * j + i, kk = min(k, n_chunk - 1);
+            key0[i] = k < n_chunk ? 16 * (tiles.t0 + 4 * (c0 + kk)) : kNoKey;
+            sc[i] = f32x2{tiles.scale(0, kk), tiles.scale(1, kk)};
+          }
+          q8_attend<D, NS>(st, ring[u], sc, q, key0, lim, key0[NS - 1] + 16 > mask_from, p.scale_log2, grp);
         }
       }
     }

@@ -31,24 +31,44 @@ def _require(cond: bool, msg: str) -> None:
         raise AssertionError(msg)
 
 
-def check_cache_q8(k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor) -> None:
-    """What every operator on an 8-bit cache asks of its pools and scales."""
-    _require(k.dim() == 4 and k.shape == v.shape, "K/V pools must be (n_pages, H_kv, page_size, D)")
-    _require(k.dtype == torch.float8_e4m3fn and v.dtype == torch.float8_e4m3fn, "K/V pools must be float8_e4m3fn")
-    n_pages, h_kv, page_size, d = k.shape
-    st = k.stride()
-    _require(st == v.stride() and st[3] == 1 and st[2] == d,
-             "K/V pools need identical strides with dense (page_size, D) rows")
-    _require(page_size % BLOCK == 0, "page_size must be a multiple of 16")
-    _require(tuple(scales.shape) == (n_pages, h_kv, page_size // BLOCK, 2) and scales.dtype == torch.float32
-             and scales.is_contiguous(), "scales must be contiguous float32 (n_pages, H_kv, page_size // 16, 2)")
+def check_cache_q8(k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor):
+    """What every operator on an 8-bit cache asks of its pools and scales; the pools' shape and strides."""
+    shape, st = k.shape, k.stride()
+    if len(shape) != 4 or v.shape != shape:
+        raise AssertionError("K/V pools must be (n_pages, H_kv, page_size, D)")
+    if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn:
+        raise AssertionError("K/V pools must be float8_e4m3fn")
+    if v.stride() != st or st[3] != 1 or st[2] != shape[3]:
+        raise AssertionError("K/V pools need identical strides with dense (page_size, D) rows")
+    if shape[2] % BLOCK:
+        raise AssertionError("page_size must be a multiple of 16")
+    if (scales.shape != (shape[0], shape[1], shape[2] // BLOCK, 2) or scales.dtype != torch.float32
+            or not scales.is_contiguous()):
+        raise AssertionError("scales must be contiguous float32 (n_pages, H_kv, page_size // 16, 2)")
+    return shape, st
 
 
-def on_device(dev: torch.device):
-    """The tensors' device made current for a launch (no cost where it already is)."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+def one_device(*tensors: torch.Tensor) -> torch.device:
+    """The one HIP device of all tensors (there is no CPU path)."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != index or index < 0:
+            return _native.require_device(*tensors)  # (it says which)
+    return tensors[0].device
+
+
+def launch(dev: torch.device, name: str, *args, err=None) -> None:
+    """One call of the C entry ``name`` on the device's current stream, with that device current."""
+    fn = getattr(_native.load(), name)
+    index = dev.index
+    args += (None if err is None else err.data_ptr(), torch._C._cuda_getCurrentRawStream(index))
+    if index == torch.cuda.current_device():
+        status = fn(*args)
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args)
+    if status:
+        _native.check(status, name)
 
 
 def int64_index(t: torch.Tensor) -> torch.Tensor:
@@ -63,18 +83,24 @@ def int64_table(bt: torch.Tensor) -> torch.Tensor:
     return bt
 
 
-def new_rows(x: torch.Tensor, h_kv: int, d: int) -> torch.Tensor:
-    """New K or V as (rows, H_kv, D) that the kernels can read in 16-byte pieces."""
-    _require(x.dtype == torch.float16, "new K/V must be float16")
-    try:
-        rows = x.view(-1, h_kv, d)
-    except RuntimeError:
-        rows = x.reshape(-1, h_kv, d)
-    if rows.stride(2) != 1 or rows.stride(0) % 8 or rows.stride(1) % 8 or rows.data_ptr() % 16:
-        rows = rows.contiguous()
-    if rows.data_ptr() % 16:  # (contiguous already, at an odd address)
-        rows = rows.clone()
-    return rows
+def new_rows(x: torch.Tensor, n: int, h_kv: int, d: int):
+    """New K or V as n rows (H_kv, D) that the kernels can read in 16-byte pieces: the tensor that holds them
+    (the caller's, or a copy), and the strides of its rows and heads."""
+    if x.dtype != torch.float16:
+        raise AssertionError("new K/V must be float16")
+    shape, st = x.shape, x.stride()
+    if len(shape) < 3 or shape[-3:] != (n, h_kv, d) or any(m != 1 for m in shape[:-3]):
+        try:
+            x = x.view(-1, h_kv, d)
+        except RuntimeError:
+            x = x.reshape(-1, h_kv, d)
+        shape, st = x.shape, x.stride()
+        if shape[0] != n:
+            raise AssertionError(f"expected {n} new K/V rows, one a token, got {shape[0]}")
+    if st[-1] != 1 or st[-3] % 8 or st[-2] % 8 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        st = x.stride()
+    return x, st[-3], st[-2]
 
 
 def kv_append_decode_q8(k_cache, v_cache, scales, k, v, slot_ids, lens, block_table, err=None) -> None:
@@ -84,28 +110,17 @@ def kv_append_decode_q8(k_cache, v_cache, scales, k, v, slot_ids, lens, block_ta
     padding slot must not share the page they append to; of a slot that comes
     several times the last row is written.
     """
-    check_cache_q8(k_cache, v_cache, scales)
-    n_pages, h_kv, page_size, d = k_cache.shape
-    dev = _native.require_device(k_cache, v_cache, scales, k, v, slot_ids, lens, block_table)
-    kr, vr = new_rows(k, h_kv, d), new_rows(v, h_kv, d)
-    slot_ids, lens, block_table = int64_index(slot_ids), int64_index(lens), int64_table(block_table)
+    (n_pages, h_kv, page_size, d), (s_page, s_head, _, _) = check_cache_q8(k_cache, v_cache, scales)
+    dev = one_device(k_cache, v_cache, scales, k, v, slot_ids, lens, block_table)
     B = slot_ids.shape[0]
-    _require(kr.shape[0] == B and vr.shape[0] == B, f"expected {B} new rows, got {kr.shape[0]} / {vr.shape[0]}")
+    (k, k_row, k_head), (v, v_row, v_head) = new_rows(k, B, h_kv, d), new_rows(v, B, h_kv, d)
+    slot_ids, lens, block_table = int64_index(slot_ids), int64_index(lens), int64_table(block_table)
     if B == 0:
         return
-    lib = _native.load()
-    with on_device(dev):
-        _native.check(
-            lib.cie_q8_append_decode(
-                k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr(), kr.data_ptr(), vr.data_ptr(),
-                kr.stride(0), kr.stride(1), vr.stride(0), vr.stride(1),
-                slot_ids.data_ptr(), lens.data_ptr(), block_table.data_ptr(),
-                B, h_kv, page_size, d, n_pages, k_cache.stride(0), k_cache.stride(1),
-                block_table.stride(0), block_table.shape[1], min(lens.shape[0], block_table.shape[0]),
-                _native.ptr(err), _native.stream_handle(dev),
-            ),
-            "cie_q8_append_decode",
-        )
+    launch(dev, "cie_q8_append_decode", k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr(), k.data_ptr(),
+           v.data_ptr(), k_row, k_head, v_row, v_head, slot_ids.data_ptr(), lens.data_ptr(),
+           block_table.data_ptr(), B, h_kv, page_size, d, n_pages, s_page, s_head, block_table.stride(0),
+           block_table.shape[1], min(lens.shape[0], block_table.shape[0]), err=err)
 
 
 def kv_append_tokens_q8(k_cache, v_cache, scales, k, v, pages, offsets, err=None) -> None:
@@ -113,27 +128,18 @@ def kv_append_tokens_q8(k_cache, v_cache, scales, k, v, pages, offsets, err=None
 
     Rows in any order; of an index that comes several times the last row is written.
     """
-    check_cache_q8(k_cache, v_cache, scales)
-    n_pages, h_kv, page_size, d = k_cache.shape
-    dev = _native.require_device(k_cache, v_cache, scales, k, v, pages, offsets)
-    kr, vr = new_rows(k, h_kv, d), new_rows(v, h_kv, d)
-    pages, offsets = int64_index(pages), int64_index(offsets)
+    (n_pages, h_kv, page_size, d), (s_page, s_head, _, _) = check_cache_q8(k_cache, v_cache, scales)
+    dev = one_device(k_cache, v_cache, scales, k, v, pages, offsets)
     T = pages.shape[0]
-    _require(offsets.shape[0] == T and kr.shape[0] == T and vr.shape[0] == T,
-             "pages, offsets and new K/V must have one row per token")
+    if offsets.shape[0] != T:
+        raise AssertionError("pages and offsets must have one entry per token")
+    (k, k_row, k_head), (v, v_row, v_head) = new_rows(k, T, h_kv, d), new_rows(v, T, h_kv, d)
+    pages, offsets = int64_index(pages), int64_index(offsets)
     if T == 0:
         return
-    lib = _native.load()
-    with on_device(dev):
-        _native.check(
-            lib.cie_q8_append_tokens(
-                k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr(), kr.data_ptr(), vr.data_ptr(),
-                kr.stride(0), kr.stride(1), vr.stride(0), vr.stride(1),
-                pages.data_ptr(), offsets.data_ptr(), T, h_kv, page_size, d, n_pages,
-                k_cache.stride(0), k_cache.stride(1), _native.ptr(err), _native.stream_handle(dev),
-            ),
-            "cie_q8_append_tokens",
-        )
+    launch(dev, "cie_q8_append_tokens", k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr(), k.data_ptr(),
+           v.data_ptr(), k_row, k_head, v_row, v_head, pages.data_ptr(), offsets.data_ptr(), T, h_kv,
+           page_size, d, n_pages, s_page, s_head, err=err)
 
 
 def kv_read_tokens_q8(k_cache, v_cache, scales, pages, offsets, err=None):
@@ -142,9 +148,8 @@ def kv_read_tokens_q8(k_cache, v_cache, scales, pages, offsets, err=None):
     The values are the cache's own, exactly.  A bad index reads as zeros and is
     reported in ``err``.
     """
-    check_cache_q8(k_cache, v_cache, scales)
-    n_pages, h_kv, page_size, d = k_cache.shape
-    dev = _native.require_device(k_cache, v_cache, scales, pages, offsets)
+    (n_pages, h_kv, page_size, d), (s_page, s_head, _, _) = check_cache_q8(k_cache, v_cache, scales)
+    dev = one_device(k_cache, v_cache, scales, pages, offsets)
     pages, offsets = int64_index(pages), int64_index(offsets)
     T = pages.shape[0]
     _require(tuple(pages.shape) == (T,) and tuple(offsets.shape) == (T,), "pages / offsets must be (T,)")
@@ -152,16 +157,9 @@ def kv_read_tokens_q8(k_cache, v_cache, scales, pages, offsets, err=None):
     v = torch.empty_like(k)
     if T == 0:
         return k, v
-    lib = _native.load()
-    with on_device(dev):
-        _native.check(
-            lib.cie_q8_read_tokens(
-                k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr(),
-                pages.data_ptr(), offsets.data_ptr(), T, h_kv, page_size, d, n_pages,
-                k_cache.stride(0), k_cache.stride(1), _native.ptr(err), _native.stream_handle(dev),
-            ),
-            "cie_q8_read_tokens",
-        )
+    launch(dev, "cie_q8_read_tokens", k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+           scales.data_ptr(), pages.data_ptr(), offsets.data_ptr(), T, h_kv, page_size, d, n_pages, s_page, s_head,
+           err=err)
     return k, v
 
 
