@@ -24,6 +24,9 @@ namespace cie {
 constexpr int kAppendThreads = 256;
 constexpr int kAppendWaves = kAppendThreads / kWave;
 constexpr int kScan = 8;
+struct __attribute__((aligned(8))) PagePair {
+  int64_t a, b;
+};
 
 struct Q8Params {
   uint8_t* k_pool;
@@ -117,19 +120,32 @@ struct BlockTask {
     for (int u = 0; u < NU; ++u) {
       if (written[u]) {
         if (rope) rope8(x[u][0], x[u][1], cs[u][0], cs[u][1], cs[u][2], cs[u][3]);
-        mag = q8_mag8(x[u][0], q8_mag8(x[u][1], mag));
+        mag = q8_raw_max(x[u][0], q8_raw_max(x[u][1], mag));
       }
     }
+    mag = q8_wave_mag(mag);
+    if (mag > kQ8Limit) {  // uniform; rare
+      mag = 0;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        if (written[u]) {
+          mag = q8_mag8(x[u][0], q8_mag8(x[u][1], mag));
+          q8_limit8(x[u][0]);
+          q8_limit8(x[u][1]);
+        }
+      }
+      mag = q8_wave_mag(mag);
+    }
     const int e_old = fresh ? kQ8EMin : q8_scale_exponent(old_scale);
-    const int e = max(e_old, q8_exponent(q8_wave_mag(mag)));
-    const float inv = q8_pow2(-e), factor = q8_pow2(e_old - e);
+    const int e = max(e_old, q8_exponent(mag));
+    const float s = q8_pow2(e), factor = q8_pow2(e_old - e);
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int unit = lane + u * kWave;
       uint8_t* const dst = pool + (unit / kPer) * D + 8 * (unit % kPer);
       if (written[u]) {
-        *reinterpret_cast<u32x2*>(dst) = q8_round8(x[u][0], inv);
-        *reinterpret_cast<u32x2*>(dst + D / 2) = q8_round8(x[u][1], inv);
+        *reinterpret_cast<u32x2*>(dst) = q8_round8(x[u][0], s);
+        *reinterpret_cast<u32x2*>(dst + D / 2) = q8_round8(x[u][1], s);
       } else if (!fresh && e != e_old) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -137,7 +153,7 @@ struct BlockTask {
               u32x2{q8_rescale4(old[u][i][0], factor), q8_rescale4(old[u][i][1], factor)};
       }
     }
-    if (lane == 0) *scale = q8_pow2(e);
+    if (lane == 0) *scale = s;
   }
 };
 
@@ -227,26 +243,29 @@ __global__ __launch_bounds__(kAppendThreads) void q8_append_kernel(Q8Params p) {
       if (again) earlier = 1;
       if (threadIdx.x == 0) last[o % kQ8Block] = (int)t;
     } else {
-      // the list's tokens of this block; kScan page ids a thread in flight
-      for (int64_t k0 = threadIdx.x; k0 < p.n_rows; k0 += kScan * kAppendThreads) {
-        int64_t q[kScan];
+      // The list's tokens of this block: kScan loads of two page ids a thread in flight, what they hit as a bit each.
+      const int64_t last_pair = max((int64_t)0, p.n_rows - 2);
+      for (int64_t k0 = 2 * threadIdx.x; k0 < p.n_rows; k0 += 2 * kScan * kAppendThreads) {
+        uint32_t hits = 1;
+        if (p.n_rows >= 2) {
+          PagePair q[kScan];
 #pragma unroll
-        for (int u = 0; u < kScan; ++u) q[u] = p.pages[min(k0 + u * kAppendThreads, p.n_rows - 1)];
-        bool any = false;
-#pragma unroll
-        for (int u = 0; u < kScan; ++u) any |= q[u] == pg;
-        if (any) {
+          for (int u = 0; u < kScan; ++u)  // (past the list: its last two again)
+            q[u] = *reinterpret_cast<const PagePair*>(p.pages + min(k0 + 2 * u * kAppendThreads, last_pair));
+          hits = 0;
 #pragma unroll
           for (int u = 0; u < kScan; ++u) {
-            const int64_t k = k0 + u * kAppendThreads;
-            if (k < p.n_rows && q[u] == pg) {
-              const int64_t ko = p.offsets[k];
-              if (ko >= 0 && ko < p.page_size && (int)ko / kQ8Block == block) {
-                if (k < t) earlier = 1;
-                atomicMax(&last[ko % kQ8Block], (int)k);
-              }
-            }
+            const uint32_t h = (q[u].a == pg ? 1u : 0u) | (q[u].b == pg ? 2u : 0u);
+            hits |= k0 + 2 * u * kAppendThreads < p.n_rows ? h << (2 * u) : 0u;
           }
+        }
+        for (; hits; hits &= hits - 1) {
+          const int bit = __builtin_ctz(hits);
+          const int64_t k = min(k0 + (bit & ~1) * kAppendThreads, last_pair) + (bit & 1);
+          const int64_t ko = p.offsets[k];
+          if (ko < 0 || ko >= p.page_size || (int)ko / kQ8Block != block) continue;
+          if (k < t) earlier = 1;
+          atomicMax(&last[ko % kQ8Block], (int)k);
         }
       }
     }

@@ -34,14 +34,33 @@ constexpr uint32_t kQ8Limit = 0x7b80;  // fp16 bits of 61440
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
+// Fp16 magnitudes order as their bits.  q8_raw_max: the largest of eight (NaN the largest of all); where a wave's is
+// past the limit (rare) q8_limit8 first brings the values to it, and q8_mag8 leaves NaN out.  (Integer tests: the build
+// assumes no NaN in float ones.)
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t q8_raw_max(const f16x8& x, uint32_t m) {
+  const u32x4 w = __builtin_bit_cast(u32x4, x);
+  u16x2 t = __builtin_bit_cast(u16x2, w[0] & 0x7fff7fffu);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) t = __builtin_elementwise_max(t, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+  return max(m, (uint32_t)max(t[0], t[1]));
+}
 // (by value: a bit cast of a vector's element as an lvalue reads its first one)
 __device__ __forceinline__ uint32_t q8_bits(f16 x) { return __builtin_bit_cast(uint16_t, x); }
-
-// Magnitude bits of an fp16 value for amax (fp16 magnitudes order as their bits): infinities and values
-// past the limit count as the limit, NaN as 0.  (Integer tests: the build assumes no NaN in float ones.)
-__device__ __forceinline__ uint32_t q8_mag(uint32_t h) {
-  const uint32_t a = h & 0x7fff;
-  return a > 0x7c00 ? 0 : min(a, kQ8Limit);
+__device__ __forceinline__ uint32_t q8_mag8(const f16x8& x, uint32_t m) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t a = q8_bits(x[i]) & 0x7fff;
+    m = max(m, a > 0x7c00 ? 0 : min(a, kQ8Limit));
+  }
+  return m;
+}
+__device__ __forceinline__ void q8_limit8(f16x8& x) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t h = q8_bits(x[i]), a = h & 0x7fff;
+    x[i] = __builtin_bit_cast(f16, (uint16_t)((a > kQ8Limit && a <= 0x7c00 ? kQ8Limit : a) | (h & 0x8000)));
+  }
 }
 
 // Least e with amax <= 448 * 2^e (448 = 1.75 * 2^8), from amax's fp16 bits.
@@ -58,24 +77,17 @@ __device__ __forceinline__ int q8_scale_exponent(float s) {
   return max(kQ8EMin, min(kQ8EMax, e));
 }
 
-// An fp16 value limited to +-61440 (NaN stays).
-__device__ __forceinline__ uint16_t q8_limit(uint32_t h) {
-  const uint32_t a = h & 0x7fff;
-  return (uint16_t)((a > kQ8Limit && a <= 0x7c00 ? kQ8Limit : a) | (h & 0x8000));
-}
-
-// Eight fp16 values times inv = 2^-e, rounded to e4m3 (v_cvt_pk_fp8_f32: to nearest even).  The
-// product is exact in fp32, and at most 448 where e covers the values.
-__device__ __forceinline__ u32x2 q8_round8(const f16x8& x, float inv) {
+// Eight fp16 values over scale = 2^e, rounded to e4m3 (v_cvt_scalef32_pk_fp8_f16, two values: to nearest even, as one
+// rounding of the exact quotient; checked over every fp16 value and scale).  At most 448 where e covers the values.
+__device__ __forceinline__ u32x2 q8_round8(const f16x8& x, float scale) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
   u32x2 r;
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    float f[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      f[i] = (float)__builtin_bit_cast(f16, q8_limit(q8_bits(x[4 * w + i]))) * inv;
-    int b = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
-    r[w] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], b, true);
+    s16x2 b = {0, 0};
+    b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(b, f16x2{x[4 * w], x[4 * w + 1]}, scale, false);
+    b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(b, f16x2{x[4 * w + 2], x[4 * w + 3]}, scale, true);
+    r[w] = __builtin_bit_cast(uint32_t, b);
   }
   return r;
 }
@@ -99,13 +111,6 @@ __device__ __forceinline__ f16x8 q8_values8(uint32_t lo, uint32_t hi, float scal
   const f16x2 a = q8_pair<false>(lo, scale), b = q8_pair<true>(lo, scale);
   const f16x2 c = q8_pair<false>(hi, scale), d = q8_pair<true>(hi, scale);
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-
-// Largest magnitude of eight fp16 values (bits).
-__device__ __forceinline__ uint32_t q8_mag8(const f16x8& x, uint32_t m) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, q8_mag(q8_bits(x[i])));
-  return m;
 }
 
 // Over the wave's 64 lanes (every lane active).

@@ -126,22 +126,36 @@ __device__ __forceinline__ void rope_row(f16x8 (&x)[Geo<D>::KS], const f16x8 (&x
 // Put the new row (kn: the lane's K dims, vn: its V dims) into the tile at row `row` under the block's new
 // scales, and the bytes that changed into the pool.  sc: the scales of the block's rows, updated.
 template <int D>
-__device__ __forceinline__ void append_row(Q8Tile<D>& t, const f16x8 (&kn)[Geo<D>::KS],
+__device__ __forceinline__ void append_row(Q8Tile<D>& t, f16x8 (&kn)[Geo<D>::KS],
                                            const typename HVec<Geo<D>::NT>::type& vn, uint8_t* kt, uint8_t* vt,
                                            float* scale, f32x2& sc, int row, int r16, int grp,
                                            const Q8Lane<D>& lo) {
   constexpr int NJ = Q8Tile<D>::NJ;
   typedef typename Q8Tile<D>::vrow_t vrow_t;
-  uint32_t km = 0, vm = 0;
+  f16x8 v8 = {};
 #pragma unroll
-  for (int ks = 0; ks < Geo<D>::KS; ++ks) km = q8_mag8(kn[ks], km);
+  for (int i = 0; i < Geo<D>::NT; ++i) v8[i] = vn[i];
+  uint32_t km = 0, vm = q8_raw_max(v8, 0);
 #pragma unroll
-  for (int i = 0; i < Geo<D>::NT; ++i) vm = max(vm, q8_mag(q8_bits(vn[i])));
+  for (int ks = 0; ks < Geo<D>::KS; ++ks) km = q8_raw_max(kn[ks], km);
+  km = q8_wave_mag(km);
+  vm = q8_wave_mag(vm);
+  if (max(km, vm) > kQ8Limit) {  // uniform; rare
+    km = 0;
+#pragma unroll
+    for (int ks = 0; ks < Geo<D>::KS; ++ks) {
+      km = q8_mag8(kn[ks], km);
+      q8_limit8(kn[ks]);
+    }
+    km = q8_wave_mag(km);
+    vm = q8_wave_mag(q8_mag8(v8, 0));
+    q8_limit8(v8);
+  }
   const bool fresh = row == 0;
   const int k_old = fresh ? kQ8EMin : q8_scale_exponent(sc[0]);
   const int v_old = fresh ? kQ8EMin : q8_scale_exponent(sc[1]);
-  const int ke = uniform(max(k_old, q8_exponent(q8_wave_mag(km))));
-  const int ve = uniform(max(v_old, q8_exponent(q8_wave_mag(vm))));
+  const int ke = uniform(max(k_old, q8_exponent(km)));
+  const int ve = uniform(max(v_old, q8_exponent(vm)));
   const bool k_all = !fresh && ke != k_old, v_all = !fresh && ve != v_old;  // the block's rows change
   if (k_all) {
     const float f = q8_pow2(k_old - ke);
@@ -157,19 +171,16 @@ __device__ __forceinline__ void append_row(Q8Tile<D>& t, const f16x8 (&kn)[Geo<D
 #pragma unroll
       for (int i = 0; i < NJ; ++i) t.v[e][i] = q8_rescale4(t.v[e][i], f);
   }
-  const float ki = q8_pow2(-ke), vi = q8_pow2(-ve);
+  const float ks = q8_pow2(ke), vs = q8_pow2(ve);
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
-    const u32x2 a = q8_round8(kn[2 * j], ki), b = q8_round8(kn[2 * j + 1], ki);
+    const u32x2 a = q8_round8(kn[2 * j], ks), b = q8_round8(kn[2 * j + 1], ks);
     const u32x4 kq = {a[0], a[1], b[0], b[1]};
 #pragma unroll
     for (int i = 0; i < 4; ++i) t.k[j][i] = r16 == row ? kq[i] : t.k[j][i];
     if (k_all || r16 == row) *reinterpret_cast<u32x4*>(kt + lo.k + 64 * j) = t.k[j];
   }
-  f16x8 v8 = {};
-#pragma unroll
-  for (int i = 0; i < Geo<D>::NT; ++i) v8[i] = vn[i];
-  const u32x2 vq = q8_round8(v8, vi);
+  const u32x2 vq = q8_round8(v8, vs);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const bool mine = 4 * grp + e == row;
@@ -177,7 +188,7 @@ __device__ __forceinline__ void append_row(Q8Tile<D>& t, const f16x8 (&kn)[Geo<D
     for (int i = 0; i < NJ; ++i) t.v[e][i] = mine ? vq[i] : t.v[e][i];
     if (v_all || mine) *reinterpret_cast<vrow_t*>(vt + lo.v + e * D) = t.v[e];
   }
-  sc = f32x2{q8_pow2(ke), q8_pow2(ve)};
+  sc = f32x2{ks, vs};
   if (r16 == 0 && grp == 0) *reinterpret_cast<f32x2*>(scale) = sc;
 }
 
