@@ -12,8 +12,8 @@
 // its S * 4 waves, wave gw taking tiles gw, gw + 4 S, ... (the plan's deal).  A tile is
 // a block of the cache, so a wave's tile comes with one K and one V scale: lane k
 // holds the byte offset and the scales of the wave's k-th tile, gathered 64 at a
-// time, and a step of q8_tiles tiles reads as many lanes.  A ring of q8_pf + 1 steps of
-// raw bytes keeps q8_pf steps of loads in flight; they are converted when their step
+// time, and a step of q8_tiles tiles reads as many lanes.  A ring of kQ8Pf + 1 steps of
+// raw bytes keeps kQ8Pf steps of loads in flight; they are converted when their step
 // comes.
 // The new row's tile belongs to the wave that it would be dealt to: that wave loads
 // the tile's bytes first of all, and after its other tiles rounds the new row under
@@ -32,28 +32,14 @@ constexpr int kQ8Waves = 4;
 constexpr int kQ8Threads = kQ8Waves * kWave;
 constexpr int kQ8MaxSplits = 64;
 constexpr int kQ8PlanDesc = 8;  // a plan's words per workgroup (paged_decode.hip)
-// Tiles of a step, and steps of loads in flight ahead of the one at work.  A lone wave on its SIMD waits out each
-// step's chain (scores, maximum, exponentials, P.V), so at D = 64 a step takes four tiles.
-#ifndef T64
-#define T64 4
-#endif
-#ifndef PF64
-#define PF64 1
-#endif
-#ifndef T128
-#define T128 2
-#endif
-#ifndef PF128
-#define PF128 2
-#endif
+// Tiles of a step: its chain (scores, maximum, exponentials, P.V) is what a lone wave on its SIMD waits for, so four
+// at D = 64; one step's loads are in flight ahead of the one at work (two: no faster at either D, 3 % slower at 96
+// sequences of D = 128, whose second workgroup on a CU hides as much).
 template <int D>
 constexpr int q8_tiles() {
-  return D == 64 ? T64 : T128;
+  return D == 64 ? 4 : 2;
 }
-template <int D>
-constexpr int q8_pf() {
-  return D == 64 ? PF64 : PF128;
-}
+constexpr int kQ8Pf = 1;
 
 struct Q8DecodeParams {
   f16* o;
@@ -275,7 +261,7 @@ void q8_decode_kernel(const int64_t* __restrict__ a_slot_ids, const int32_t* __r
   constexpr int KS = Geo<D>::KS;
   constexpr int NT = Geo<D>::NT;
   constexpr int W = kQ8Waves;
-  constexpr int PF = q8_pf<D>(), NS = q8_tiles<D>();
+  constexpr int PF = kQ8Pf, NS = q8_tiles<D>();
   typedef typename HVec<NT>::type vhalf_t;
   __shared__ float sm_m[W][16];
   __shared__ float sm_l[W][16];

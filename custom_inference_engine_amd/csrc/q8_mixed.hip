@@ -623,7 +623,7 @@ template <int D>
 __device__ __forceinline__ void narrow_item(const Q8MixedParams& p, const Q8Item& it, int cols, f32x4* lds, int wave,
                                             int lane) {
   constexpr int KS = Geo<D>::KS, NT = Geo<D>::NT, D4 = D / 4;
-  constexpr int PF = D == 64 ? 1 : 2, NS = D == 64 ? 4 : 2;  // (as the decode kernel's)
+  constexpr int PF = 1, NS = D == 64 ? 4 : 2;  // (as the decode kernel's)
   const int r16 = lane & 15, grp = lane >> 4;
   const Q8Lane<D> lo(r16, grp);
   const int key_end = it.pos0 - it.rows;  // (rows: negative here)
