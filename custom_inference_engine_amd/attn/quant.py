@@ -16,8 +16,22 @@ import torch
 
 from .. import _native
 from ..kv_cache.quant import check_cache_q8, int64_index, int64_table, launch, new_rows, one_device
-from .core import (DECODE_MAX_SPLITS, GQA_DECODE_CONFIG, _plan_workgroups, _qkv_rows, _require, _rope_rows,
-                   default_decode_splits, split_counters)
+from .core import (DECODE_MAX_SPLITS, GQA_DECODE_CONFIG, _plan_workgroups, _require, default_decode_splits,
+                   split_counters)
+
+
+def _rows(t: torch.Tensor, n: int, width: int, what: str):
+    """(1, n, width) or (n, width) float16 rows that the kernels can read: the tensor that holds them and their stride."""
+    if t.dtype != torch.float16:
+        raise AssertionError(f"{what} must be float16")
+    shape = t.shape
+    if shape != (1, n, width) and shape != (n, width):
+        raise AssertionError(f"{what} must be (1, {n}, {width}), one row per token")
+    st = t.stride()
+    if st[-1] != 1 or st[-2] % 8 or (n > 1 and st[-2] < width) or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = t.stride()
+    return t, max(st[-2], width)
 
 
 def _decode(entry, o, q_args, cache, geometry, row_args, lens, slot_ids, block_table, H_q, append, num_programs, err,
@@ -118,15 +132,15 @@ def decode_qkv_rope_gqa_attention_q8(qkv, cos, sin, k_cache, v_cache, scales, le
     ``apply_rotary_pos_emb`` and ``decode_append_gqa_attention_q8``."""
     H_q, (_, H_kv, _, D), B = int(num_heads), k_cache.shape, slot_ids.shape[0]
     cache = (k_cache, v_cache, scales)
-    rows = _qkv_rows(qkv, (H_q + 2 * H_kv) * D)
-    geometry = _check_decode(H_q, cache, slot_ids, block_table, rows.shape[0])
-    dev = one_device(rows, cos, sin, k_cache, v_cache, scales, lens, slot_ids, block_table)
-    cr, sr = _rope_rows(cos, B, D), _rope_rows(sin, B, D)
-    _require(cr.stride(0) == sr.stride(0), "cos and sin need the same row stride")
-    o = rows.new_empty((1, B, H_q, D))
+    qkv, qkv_row = _rows(qkv, qkv.shape[-2], (H_q + 2 * H_kv) * D, "qkv")
+    geometry = _check_decode(H_q, cache, slot_ids, block_table, qkv.shape[-2])
+    dev = one_device(qkv, cos, sin, k_cache, v_cache, scales, lens, slot_ids, block_table)
+    (cos, cos_row), (sin, sin_row) = _rows(cos, B, D, "cos"), _rows(sin, B, D, "sin")
+    _require(cos_row == sin_row, "cos and sin need the same row stride")
+    o = torch.empty((1, B, H_q, D), dtype=torch.float16, device=dev)
     if B == 0:
         return o
-    q_args = (rows.data_ptr(), rows.stride(0), cr.data_ptr(), sr.data_ptr(), cr.stride(0))
+    q_args = (qkv.data_ptr(), qkv_row, cos.data_ptr(), sin.data_ptr(), cos_row)
     return _decode("cie_q8_decode_qkv_rope", o, q_args, cache, geometry, (), lens, slot_ids, block_table, H_q, True,
                    num_programs, err, counters, plan, dev)
 
@@ -135,18 +149,18 @@ def append_tokens_qkv_rope_q8(qkv, cos, sin, k_cache, v_cache, scales, pages, of
     """``append_tokens_qkv_rope`` into an 8-bit cache, one launch: returns the rotated q (1, T, H_q, D)."""
     (N_PAGES, H_kv, PAGE_SIZE, D), (s_page, s_head, _, _) = check_cache_q8(k_cache, v_cache, scales)
     H_q = int(num_heads)
-    rows = _qkv_rows(qkv, (H_q + 2 * H_kv) * D)
-    T = rows.shape[0]
-    _require(tuple(pages.shape) == (T,) and tuple(offsets.shape) == (T,), "pages / offsets must be (T,)")
-    dev = one_device(rows, cos, sin, k_cache, v_cache, scales, pages, offsets)
-    cr, sr = _rope_rows(cos, T, D), _rope_rows(sin, T, D)
-    _require(cr.stride(0) == sr.stride(0), "cos and sin need the same row stride")
+    T = qkv.shape[-2]
+    qkv, qkv_row = _rows(qkv, T, (H_q + 2 * H_kv) * D, "qkv")
+    _require(pages.shape == (T,) and offsets.shape == (T,), "pages / offsets must be (T,)")
+    dev = one_device(qkv, cos, sin, k_cache, v_cache, scales, pages, offsets)
+    (cos, cos_row), (sin, sin_row) = _rows(cos, T, D, "cos"), _rows(sin, T, D, "sin")
+    _require(cos_row == sin_row, "cos and sin need the same row stride")
     pages, offsets = int64_index(pages), int64_index(offsets)
-    q = rows.new_empty((1, T, H_q, D))
+    q = torch.empty((1, T, H_q, D), dtype=torch.float16, device=dev)
     if T == 0:
         return q
     launch(dev, "cie_q8_append_tokens_qkv_rope", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-           scales.data_ptr(), rows.data_ptr(), rows.stride(0), cr.data_ptr(), sr.data_ptr(), cr.stride(0),
+           scales.data_ptr(), qkv.data_ptr(), qkv_row, cos.data_ptr(), sin.data_ptr(), cos_row,
            pages.data_ptr(), offsets.data_ptr(), T, H_q, H_kv, PAGE_SIZE, D, N_PAGES, s_page, s_head, err=err)
     return q
 

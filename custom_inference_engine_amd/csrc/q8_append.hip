@@ -299,39 +299,34 @@ struct Q8ReadParams {
   int32_t* err;
 };
 
-// Row t of the outputs = the cache's row (pages[t], offsets[t]): a lane converts 16 values of K and of V.
-// Bound by memory.  A bad index reads as zeros and is reported.
+// Row t of the outputs = the cache's row (pages[t], offsets[t]): a lane converts 8 values of K and of V, so that a wave
+// writes whole lines, past the caches (the rows are read by other kernels, later).  Bound by memory.  A bad index reads
+// as zeros and is reported.
 template <int D>
 __global__ __launch_bounds__(256) void q8_read_kernel(Q8ReadParams p) {
-  constexpr int kPer = D / 16;
+  constexpr int kPer = D / 8;
   const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (gid >= p.T * p.H_kv * kPer) return;
-  const int d0 = 16 * (int)(gid % kPer);
+  const int d0 = 8 * (int)(gid % kPer);
   const int64_t row = gid / kPer;
   const int h = (int)(row % p.H_kv);
   const int64_t t = row / p.H_kv;
   const int64_t page = p.pages[t], off = p.offsets[t];
-  f16x8 k[2] = {}, v[2] = {};
+  f16x8 k = {}, v = {};
   const bool off_ok = off >= 0 && off < p.page_size, page_ok = page >= 0 && page < p.n_pages;
   if (off_ok && page_ok) {
     const int64_t at = page * p.pool_page_stride + h * p.pool_head_stride + off * D + d0;
-    const u32x4 kb = *reinterpret_cast<const u32x4*>(p.k_pool + at);
-    const u32x4 vb = *reinterpret_cast<const u32x4*>(p.v_pool + at);
-    const float* const s = p.scales + 2 * ((page * p.H_kv + h) * (p.page_size / kQ8Block) + off / kQ8Block);
-    const float ks = s[0], vs = s[1];
-    k[0] = q8_values8(kb[0], kb[1], ks);
-    k[1] = q8_values8(kb[2], kb[3], ks);
-    v[0] = q8_values8(vb[0], vb[1], vs);
-    v[1] = q8_values8(vb[2], vb[3], vs);
+    const u32x2 kb = stream_load(reinterpret_cast<const u32x2*>(p.k_pool + at));
+    const u32x2 vb = stream_load(reinterpret_cast<const u32x2*>(p.v_pool + at));
+    const f32x2 s = *reinterpret_cast<const f32x2*>(
+        p.scales + 2 * ((page * p.H_kv + h) * (p.page_size / kQ8Block) + off / kQ8Block));
+    k = q8_values8(kb[0], kb[1], s[0]);
+    v = q8_values8(vb[0], vb[1], s[1]);
   } else {
     set_err(p.err, off_ok ? CIE_ERRBIT_PAGE : CIE_ERRBIT_OFFSET);
   }
-  f16* const ko = p.k_out + row * D + d0;
-  f16* const vo = p.v_out + row * D + d0;
-  *reinterpret_cast<f16x8*>(ko) = k[0];
-  *reinterpret_cast<f16x8*>(ko + 8) = k[1];
-  *reinterpret_cast<f16x8*>(vo) = v[0];
-  *reinterpret_cast<f16x8*>(vo + 8) = v[1];
+  __builtin_nontemporal_store(k, reinterpret_cast<f16x8*>(p.k_out + row * D + d0));
+  __builtin_nontemporal_store(v, reinterpret_cast<f16x8*>(p.v_out + row * D + d0));
 }
 
 static bool q8_aligned(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
@@ -487,8 +482,8 @@ extern "C" int cie_q8_read_tokens(void* k_out, void* v_out, const void* k_pool, 
   Q8ReadParams p{static_cast<f16*>(k_out), static_cast<f16*>(v_out), static_cast<const uint8_t*>(k_pool),
                  static_cast<const uint8_t*>(v_pool), static_cast<const float*>(scales), pages, offsets, T, n_pages,
                  pool_page_stride, pool_head_stride, (int32_t)H_kv, (int32_t)page_size, err};
-  if (T > 0x7fffffffLL * 256 / (H_kv * (D / 16))) return CIE_EUNSUPPORTED;
-  const int64_t blocks = (T * H_kv * (D / 16) + 255) / 256;
+  if (T > 0x7fffffffLL * 256 / (H_kv * (D / 8))) return CIE_EUNSUPPORTED;
+  const int64_t blocks = (T * H_kv * (D / 8) + 255) / 256;
   if (D == 64)
     hipLaunchKernelGGL(q8_read_kernel<64>, dim3((unsigned)blocks), dim3(256), 0, static_cast<hipStream_t>(stream), p);
   else
