@@ -5,9 +5,10 @@
 // position kv_lens[b] + i and attends keys 0 .. kv_lens[b] + i of slot slot_ids[b].
 // Rows outside every sequence are left untouched.
 //
-// Work.  A query tile is up to R rows of a sequence and one kv head: R * G <= 64 CT
-// (row, head) columns.  An item is a tile and a range of its key tiles.
-//  * Wide items (more than 16 columns): every wave has up to CT column tiles of 16
+// Work.  A query tile is up to R rows of a sequence and one kv head: R * G <= kTileCols
+// (row, head) columns, or half of that in small launches.  An item is a tile and a
+// range of its key tiles.
+//  * Wide items (more than 16 columns): every wave has one or two column tiles of 16
 //    and all keys of the item.  Keys go by stages of 64: wave w loads the stage's
 //    16-key tile w as bytes (so its page and its two scales are scalars), converts it
 //    once and leaves it in LDS in MFMA operand order (K: slot [tile][k-step][lane];
@@ -27,7 +28,7 @@
 // its layers.
 //
 // What bounds it: prefill, the softmax's VALU work between the MFMAs (a step of 32
-// keys costs a wave 18 MFMAs and 16 exponentials at D = 64 and CT = 2); decode rows,
+// keys costs a wave 18 MFMAs and 16 exponentials at D = 64 and two column tiles); decode rows,
 // the K/V reads.
 #include "q8_attn.h"
 
@@ -36,7 +37,7 @@ namespace cie {
 constexpr int kMW = 4;  // waves a workgroup
 constexpr int kMThreads = kMW * kWave;
 constexpr int kQ8Slots = 256;        // items a launch's work is cut into, about
-constexpr int kMaxSplitItems = 2 * kQ8Slots;  // (see plan_share)
+constexpr int kMaxSplitItems = 2 * kQ8Slots;  // (see the plan)
 constexpr int kQ8MinShare = 32;  // key tiles (512 keys): below, an item's start costs more than its keys
 constexpr int kQ8MaxSeqs = 2048;
 constexpr int kItemWords = 12;
@@ -130,9 +131,9 @@ __device__ __forceinline__ Q8Seq q8_seq(const Q8PlanParams& p, int b, bool repor
 struct Q8Cut {
   bool narrow;
   int R, n_rt, share;
-  __device__ __forceinline__ Q8Cut(const Q8PlanParams& p, int L, int want) {
+  __device__ __forceinline__ Q8Cut(const Q8PlanParams& p, int L, int cols, int want) {
     narrow = (int64_t)L * p.G <= 16;
-    R = narrow ? max(1, L) : kTileCols / p.G;
+    R = narrow ? max(1, L) : cols / p.G;
     n_rt = (L + R - 1) / R;
     share = (max(kQ8MinShare, narrow ? 4 * want : want) + 3) & ~3;
   }
@@ -159,13 +160,21 @@ __device__ __forceinline__ int plan_block_scan(int v, int* red, int& all) {
 
 // One workgroup: a thread a sequence, then a thread a query tile.
 //
-// Key tiles an item holds at most: with W the launch's work in key tiles of wide items (a narrow item's key tile
-// counts a quarter), want = W / kQ8Slots, 4 want for narrow items, and kQ8MinShare at least.  A tile of kt > share
-// key tiles becomes ceil(kt / share) items, so the items beyond one a tile are at most kQ8Slots, split tiles at most
-// that many, and their items at most kMaxSplitItems.  (W is taken from closed forms that are no smaller.)
+// Columns of a wide tile: with W the launch's work in key tiles of wide items of kTileCols columns (a narrow item's
+// key tile counts a quarter), a launch of W <= kSmallWork * kQ8Slots takes tiles of half as many, one column tile a
+// wave: such a launch lasts as long as its items, whose stages are then shorter, and it has CUs for more of them (100
+// rows over 900 keys, 14 / 2 heads, D = 64: 17 -> 14 us; 32 / 8 heads, D = 128: 24 -> 18; 512 over 4,096: 34 -> 32).
+// Larger ones pay the K/V operands' conversion and LDS reads twice (4 x 8,192 rows: 568 us whole, 710 in halves).
+//
+// Key tiles an item holds at most: want = W / kQ8Slots (W in the tiles taken), 4 want for narrow items, and kQ8MinShare
+// at least.  A tile of kt > share key tiles becomes ceil(kt / share) items, so the items beyond one a tile are at most
+// kQ8Slots, split tiles at most that many, and their items at most kMaxSplitItems.  (W is taken from closed forms that
+// are no smaller.)  Splitting costs partial rows written and read, so no more than about an item a CU is split off
+// (4 x 2,048 rows: 49 us at 256 slots, 59 at 1,024).
 //
 // Items are listed the longest first, to kPlanLevels of length: the workgroups of a launch start in order, so what
 // starts last is short.
+constexpr int kSmallWork = 80;
 constexpr int kPlanLevels = 64;
 __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanParams p) {
   __shared__ int64_t sm_t0[kQ8MaxSeqs];
@@ -173,37 +182,45 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
   __shared__ int sm_first[kQ8MaxSeqs];  // a sequence's first tile
   __shared__ int sm_level[kPlanLevels];
   __shared__ int sm_red[kPlanWavesM];
-  __shared__ unsigned long long sm_work;
+  __shared__ unsigned long long sm_work[2];  // W of whole tiles, of half tiles
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
-  if (tid == 0) sm_work = 0;
+  if (tid < 2) sm_work[tid] = 0;
   if (tid < kPlanLevels) sm_level[tid] = 0;
   __syncthreads();
+  int64_t work[2] = {0, 0};
+  for (int b = tid; b < p.B; b += kPlanThreadsM) {
+    const Q8Seq s = q8_seq(p, b, true);
+    sm_t0[b] = s.t0;
+    sm_slot[b] = s.slot;
+    sm_L[b] = s.L;
+    sm_c[b] = s.c;
+    if (s.L == 0) continue;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const Q8Cut cut(p, s.L, kTileCols >> i, 0);
+      const int64_t n = cut.n_rt;
+      work[i] += cut.narrow ? (int64_t)((s.c + s.L) >> 6) + 1
+                            : n * ((s.c >> 4) + 2) + (int64_t)cut.R * n * (n + 1) / 32 + 1;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    for (int off = 1; off < kWave; off <<= 1) work[i] += __shfl_xor(work[i], off, kWave);
+    if (lane == 0 && work[i] > 0) atomicAdd(&sm_work[i], (unsigned long long)work[i]);
+  }
+  __syncthreads();
+  const bool small = (int64_t)sm_work[0] * p.H_kv <= (int64_t)kSmallWork * kQ8Slots;
+  const int cols = small ? kTileCols / 2 : kTileCols;
+  const int want = (int)min((int64_t)1 << 26, ((int64_t)sm_work[small] * p.H_kv + kQ8Slots - 1) / kQ8Slots);
   int n_tiles = 0;
-  int64_t work = 0;
   for (int b0 = 0; b0 < p.B; b0 += kPlanThreadsM) {
     const int b = b0 + tid;
-    int n = 0;
-    if (b < p.B) {
-      const Q8Seq s = q8_seq(p, b, true);
-      const Q8Cut cut(p, s.L, 0);
-      n = cut.n_rt;
-      sm_t0[b] = s.t0;
-      sm_slot[b] = s.slot;
-      sm_L[b] = s.L;
-      sm_c[b] = s.c;
-      if (s.L > 0)
-        work += cut.narrow ? (int64_t)((s.c + s.L) >> 6) + 1
-                           : (int64_t)n * ((s.c >> 4) + 2) + (int64_t)cut.R * n * (n + 1) / 32 + 1;
-    }
     int all;
-    const int first = plan_block_scan(n, sm_red, all);
+    const int first = plan_block_scan(b < p.B ? Q8Cut(p, sm_L[b], cols, 0).n_rt : 0, sm_red, all);
     if (b < p.B) sm_first[b] = n_tiles + first;
     n_tiles += all;
   }
-  for (int off = 1; off < kWave; off <<= 1) work += __shfl_xor(work, off, kWave);
-  if (lane == 0 && work > 0) atomicAdd(&sm_work, (unsigned long long)work);
   __syncthreads();
-  const int want = (int)min((int64_t)1 << 26, ((int64_t)sm_work * p.H_kv + kQ8Slots - 1) / kQ8Slots);
 
   // A thread's tile: sequence, rows, chunks, partial rows and arrival words before it.
   int b = 0, r = 0, n = 0, rows = 0, kt = 0, pbase = 0, ctr = 0, level = 0;
@@ -223,7 +240,7 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
           hi = mid - 1;
       }
       b = lo;
-      const Q8Cut cut(p, sm_L[b], want);
+      const Q8Cut cut(p, sm_L[b], cols, want);
       r = i - sm_first[b];
       R = cut.R;
       share = cut.share;
@@ -273,7 +290,7 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
     if (!once) tile(i0);
     if (n == 0) continue;
     const int abs_rows = rows < 0 ? -rows : rows;
-    const int R = rows < 0 ? 0 : kTileCols / p.G;  // (a narrow sequence has one tile)
+    const int R = rows < 0 ? 0 : cols / p.G;  // (a narrow sequence has one tile)
     int at = atomicAdd(&sm_level[level], n * p.H_kv);
     Q8Item it;
     it.tok0 = (int)sm_t0[b] + r * R;
@@ -374,13 +391,14 @@ __device__ __forceinline__ int part_piece(int d4) {
   return (d4 % Geo<D>::NT) * 4 + d4 / Geo<D>::NT;
 }
 
-// The chunks' pieces of a split tile, summed with their weights and stored: a thread owns UN pieces (4 dims of a
-// column; pieces tid + 256 i), kMergeLoads loads in flight.  Where the pieces are fewer than the threads, R threads
-// share one, each taking every R-th chunk, and are summed through LDS.
+// Merge a split tile's chunk states into o.  One workgroup does it, so memory round trips bound it.  A thread owns UN
+// pieces (4 dims of a column; pieces tid + 256 i), kMergeLoads loads in flight; where the pieces are fewer than the
+// threads, R threads share one, each taking every R-th chunk, and are summed through LDS.  The first loads go out
+// ahead of the chunks' weights 2^(m - M) / l, which `weights` leaves in sm_w.
 constexpr int kMergeLoads = 16;
-template <int D, int UN>
+template <int D, int UN, class Weights>
 __device__ __forceinline__ void merge_pieces(const Q8MixedParams& p, const Q8Item& it, int cols, const float* sm_w,
-                                             f32x4* sm_sum) {
+                                             f32x4* sm_sum, Weights weights) {
   constexpr int D4 = D / 4, CG = kMergeLoads / UN;
   const int n = it.n_chunks, n_units = cols * D4;
   const __amdgpu_buffer_rsrc_t racc =
@@ -391,8 +409,8 @@ __device__ __forceinline__ void merge_pieces(const Q8MixedParams& p, const Q8Ite
   f32x4 num[UN];
 #pragma unroll
   for (int i = 0; i < UN; ++i) num[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int c0 = r; c0 < n; c0 += R * CG) {
-    f32x4 x[CG][UN];
+  f32x4 x[CG][UN];
+  auto load = [&](int c0) {
 #pragma unroll
     for (int k = 0; k < CG; ++k)
 #pragma unroll
@@ -401,6 +419,10 @@ __device__ __forceinline__ void merge_pieces(const Q8MixedParams& p, const Q8Ite
         x[k][i] = agent_load4(racc, r < R && u < n_units && c < n ? (uint32_t)((c * n_units + u) * sizeof(f32x4))
                                                                   : 0x7ffffff0u);
       }
+  };
+  load(r);
+  weights();
+  for (int c0 = r; c0 < n;) {
 #pragma unroll
     for (int k = 0; k < CG; ++k)
 #pragma unroll
@@ -408,6 +430,8 @@ __device__ __forceinline__ void merge_pieces(const Q8MixedParams& p, const Q8Ite
         const int u = u0 + i * kMThreads, c = c0 + k * R;
         if (u < n_units && c < n) num[i] += sm_w[c * cols + u / D4] * x[k][i];
       }
+    c0 += R * CG;
+    if (c0 < n) load(c0);
   }
   if (R > 1) {
     sm_sum[threadIdx.x] = num[0];
@@ -429,15 +453,12 @@ __device__ __forceinline__ void merge_pieces(const Q8MixedParams& p, const Q8Ite
   }
 }
 
-// Merge a split tile's chunk states into o.  One workgroup does it, so memory round trips bound it: the chunks'
-// weights 2^(m - M) / l first (LDS), then the pieces.
-template <int D>
-__device__ __forceinline__ void q8_mixed_merge(const Q8MixedParams& p, const Q8Item& it, int cols, f32x4* lds) {
+// The chunks' weights of every column, in sm_w[chunk * cols + column]: tpc threads share a column's chunks.  sm_m:
+// [2][thread], their maxima and sums.
+__device__ __forceinline__ void merge_weights(const Q8MixedParams& p, const Q8Item& it, int cols, float* sm_w,
+                                              float* sm_m) {
   constexpr int kGroup = 8;
   const int n = it.n_chunks;
-  float* const sm_w = reinterpret_cast<float*>(lds);
-  float* const sm_m = sm_w + kTileCols * kQ8MaxChunks;  // [2][thread]: threads' maxima, sums
-  // threads share a column's chunks: tpc of them, chunk k * tpc + j
   const int tpc = kMThreads / cols;
   const int j = (int)threadIdx.x / cols, cc = threadIdx.x - j * cols;
   float M = kEmptyMax, den = 0.f;
@@ -479,18 +500,23 @@ __device__ __forceinline__ void q8_mixed_merge(const Q8MixedParams& p, const Q8I
     }
   }
   __syncthreads();
+}
+
+template <int D>
+__device__ __forceinline__ void q8_mixed_merge(const Q8MixedParams& p, const Q8Item& it, int cols, f32x4* lds) {
+  float* const sm_w = reinterpret_cast<float*>(lds);
+  float* const sm_m = sm_w + kTileCols * kQ8MaxChunks;
   f32x4* const sm_sum = lds + (kTileCols * kQ8MaxChunks + 2 * kMThreads) / 4;
+  auto weights = [&] { merge_weights(p, it, cols, sm_w, sm_m); };
   const int n_units = cols * (D / 4);
   if (n_units <= kMThreads)
-    merge_pieces<D, 1>(p, it, cols, sm_w, sm_sum);
+    merge_pieces<D, 1>(p, it, cols, sm_w, sm_sum, weights);
   else if (n_units <= 2 * kMThreads)
-    merge_pieces<D, 2>(p, it, cols, sm_w, sm_sum);
-  else if (n_units <= 4 * kMThreads)
-    merge_pieces<D, 4>(p, it, cols, sm_w, sm_sum);
-  else if (n_units <= 8 * kMThreads)
-    merge_pieces<D, 8>(p, it, cols, sm_w, sm_sum);
-  else
-    merge_pieces<D, 16>(p, it, cols, sm_w, sm_sum);
+    merge_pieces<D, 2>(p, it, cols, sm_w, sm_sum, weights);
+  else if (D == 64 || n_units <= 8 * kMThreads)
+    merge_pieces<D, 8>(p, it, cols, sm_w, sm_sum, weights);
+  else if constexpr (D == 128)
+    merge_pieces<D, 16>(p, it, cols, sm_w, sm_sum, weights);
 }
 
 template <int D>
@@ -749,10 +775,13 @@ void q8_mixed_kernel(Q8MixedParams p) {
   if (threadIdx.x == 0) counter_reset(arrival);
 }
 
-// Items a plan can hold: one a query tile and kv head, and kQ8Slots more from splitting.
+// Items a plan can hold: one a query tile and kv head, and kQ8Slots more from splitting.  A launch of half tiles has W <=
+// kSmallWork * kQ8Slots, a whole tile counts 2 at least in W, and a sequence has at most twice as many half ones.
 static int64_t q8_plan_items(int64_t B, int64_t total_T, int64_t H_q, int64_t H_kv) {
-  const int64_t R = kTileCols / (H_q / H_kv);
-  return H_kv * (total_T / R + B) + kQ8Slots;
+  const int64_t R = kTileCols / (H_q / H_kv), half = kTileCols / 2 / (H_q / H_kv);
+  const int64_t whole = H_kv * (total_T / R + B), small = H_kv * (total_T / half + B);
+  const int64_t most = kSmallWork * kQ8Slots + H_kv * B;
+  return kQ8Slots + (whole > most ? whole : small < most ? small : most);
 }
 
 // Partial rows a launch can need: its split items' columns, and no more than kQ8MaxChunks a query row and head.
