@@ -182,12 +182,11 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
   __shared__ int sm_first[kQ8MaxSeqs];  // a sequence's first tile
   __shared__ int sm_level[kPlanLevels];
   __shared__ int sm_red[kPlanWavesM];
-  __shared__ unsigned long long sm_work[2];  // W of whole tiles, of half tiles
+  __shared__ float sm_work[2][kPlanWavesM];  // a wave's part of W in whole tiles, in half tiles
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
-  if (tid < 2) sm_work[tid] = 0;
   if (tid < kPlanLevels) sm_level[tid] = 0;
   __syncthreads();
-  int64_t work[2] = {0, 0};
+  float work[2] = {0.f, 0.f};
   for (int b = tid; b < p.B; b += kPlanThreadsM) {
     const Q8Seq s = q8_seq(p, b, true);
     sm_t0[b] = s.t0;
@@ -198,20 +197,28 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const Q8Cut cut(p, s.L, kTileCols >> i, 0);
-      const int64_t n = cut.n_rt;
-      work[i] += cut.narrow ? (int64_t)((s.c + s.L) >> 6) + 1
-                            : n * ((s.c >> 4) + 2) + (int64_t)cut.R * n * (n + 1) / 32 + 1;
+      const float n = (float)cut.n_rt;
+      work[i] += cut.narrow ? (float)((s.c + s.L) >> 6) + 1.f
+                            : n * (float)((s.c >> 4) + 2) + (float)cut.R * n * (n + 1.f) * (1.f / 32) + 1.f;
     }
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    for (int off = 1; off < kWave; off <<= 1) work[i] += __shfl_xor(work[i], off, kWave);
-    if (lane == 0 && work[i] > 0) atomicAdd(&sm_work[i], (unsigned long long)work[i]);
+    const float w = wave_sum(work[i]);
+    if (lane == 0) sm_work[i][tid / kWave] = w;
   }
   __syncthreads();
-  const bool small = (int64_t)sm_work[0] * p.H_kv <= (int64_t)kSmallWork * kQ8Slots;
+  float total[2] = {0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < kPlanWavesM; ++w) {
+    total[0] += sm_work[0][w];
+    total[1] += sm_work[1][w];
+  }
+  // (fp32 sums of positive terms, each rounded by 2^-24 of itself a few times: 1e-3 more covers their errors)
+  const float per_slot = 1.001f * (float)p.H_kv / kQ8Slots;
+  const bool small = total[0] * per_slot <= (float)kSmallWork;
   const int cols = small ? kTileCols / 2 : kTileCols;
-  const int want = (int)min((int64_t)1 << 26, ((int64_t)sm_work[small] * p.H_kv + kQ8Slots - 1) / kQ8Slots);
+  const int want = (int)fminf(67108864.f, total[small] * per_slot + 1.f);
   int n_tiles = 0;
   for (int b0 = 0; b0 < p.B; b0 += kPlanThreadsM) {
     const int b = b0 + tid;
