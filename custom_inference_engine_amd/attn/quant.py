@@ -34,6 +34,11 @@ def _rows(t: torch.Tensor, n: int, width: int, what: str):
     return t, max(st[-2], width)
 
 
+def _check_counters(counters: torch.Tensor, n: int, dev: torch.device) -> None:
+    _require(counters.dtype == torch.int32 and counters.is_contiguous() and counters.numel() >= n, "counters too small")
+    _require(counters.get_device() == dev.index, "counters must be on the operator's device")
+
+
 def _decode(entry, o, q_args, cache, geometry, row_args, lens, slot_ids, block_table, H_q, append, num_programs, err,
             counters, plan, dev):
     """One decode launch of the C entry ``entry`` (cie_q8_decode*): its shared arguments and buffers."""
@@ -44,6 +49,7 @@ def _decode(entry, o, q_args, cache, geometry, row_args, lens, slot_ids, block_t
     n_groups = B * H_kv
     if plan is not None:  # a step's plan (decode_plan, same append mode)
         n_wg = P = _plan_workgroups(plan)
+        _require(plan.get_device() == dev.index, "plan must be on the operator's device")
     else:
         P = int(num_programs) if num_programs else default_decode_splits(B, H_kv, dev)
         _require(1 <= P <= DECODE_MAX_SPLITS, "num_programs outside [1, the kernel's split limit]")
@@ -55,7 +61,7 @@ def _decode(entry, o, q_args, cache, geometry, row_args, lens, slot_ids, block_t
         partials = buffer.data_ptr()
         if counters is None:
             counters = split_counters(dev, 2 * n_groups)
-        _require(counters.dtype == torch.int32 and counters.numel() >= 2 * n_groups, "counters too small")
+        _check_counters(counters, 2 * n_groups, dev)
     slots, width = block_table.shape
     launch(dev, entry, o.data_ptr(), *q_args, k.data_ptr(), v.data_ptr(), scales.data_ptr(), *row_args,
            lens.data_ptr(), slot_ids.data_ptr(), block_table.data_ptr(), None if plan is None else plan.data_ptr(),
@@ -215,7 +221,7 @@ def mixed_gqa_attention_q8(q, k, v, scales, max_seqlen: int, cu_seqlens, kv_lens
     if plan is None:
         plan = mixed_plan_q8(k, cu_seqlens, kv_lens, slot_ids, block_table, max_seqlen, total_T, H_q, err=err)
     else:
-        _require(plan.dtype == torch.int32 and plan.is_contiguous()
+        _require(plan.dtype == torch.int32 and plan.is_contiguous() and plan.get_device() == dev.index
                  and plan.numel() * 4 >= lib.cie_q8_mixed_plan_bytes(B, total_T, H_q, H_kv),
                  "plan must come from mixed_plan_q8 for this batch")
     n = lib.cie_q8_mixed_partials_bytes(total_T, H_q, D)
@@ -223,7 +229,7 @@ def mixed_gqa_attention_q8(q, k, v, scales, max_seqlen: int, cu_seqlens, kv_lens
     n_ctr = lib.cie_q8_mixed_counters()
     if counters is None:
         counters = split_counters(dev, n_ctr)
-    _require(counters.dtype == torch.int32 and counters.numel() >= n_ctr, "counters too small")
+    _check_counters(counters, n_ctr, dev)
     launch(dev, "cie_q8_mixed", o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), scales.data_ptr(),
            plan.data_ptr(), plan.numel() * 4, block_table.data_ptr(), partials.data_ptr(), n, counters.data_ptr(), B,
            total_T, H_q, H_kv, D, PAGE_SIZE, N_PAGES, s_page, s_head, block_table.stride(0), width, slots, err=err)

@@ -105,6 +105,10 @@ __device__ __forceinline__ void q8_v_operand(f16x8 (&va)[Geo<D>::NT], int half, 
   }
 }
 
+// A state that saw no key (its sum is +0; by its bits, since these files are built with -fno-honor-nans and a NaN among
+// the attended values has to stay one).
+__device__ __forceinline__ bool q8_no_key(float l) { return __float_as_uint(l) == 0; }
+
 // One step of NP 32-key pairs of tiles for NCT column tiles.  k(i, ka) gives the K operands of tile i (< 2 NP), whose
 // first key is key0[i] (kNoKey: absent, all masked), v(p, va) the V^T operands of pair p once the weights are known;
 // meanwhile() is work that needs nothing of the step, done while its S MFMAs run.

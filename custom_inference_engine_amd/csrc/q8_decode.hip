@@ -226,7 +226,7 @@ __device__ __forceinline__ void q8_merge(const Q8DecodeParams& p, int64_t row0, 
             const float M = wave_max(ms[i]);
             const float a = fast_exp2(ms[i] - M);
             const float den = wave_sum(a * ls[i]);
-            sm_w[hh * kQ8MaxSplits + lane] = den > 0.f ? a / den : 0.f;  // no key at all: o = 0
+            sm_w[hh * kQ8MaxSplits + lane] = q8_no_key(den) ? 0.f : a / den;  // no key at all: o = 0
           }
         }
         __syncthreads();
@@ -303,9 +303,21 @@ void q8_decode_kernel(const int64_t* __restrict__ a_slot_ids, const int32_t* __r
     S = d[3];
     slot = d[4];
     L = d[5];
-    pos = kAppend ? d[6] : -1;
+    pos = d[6];
     w_first = d[7];
+    // A plan of another batch or of the other append mode: nothing of it is followed.
+    const bool fits = b < p.B && (uint32_t)g < (uint32_t)p.H_kv && (uint32_t)split < (uint32_t)S && S <= kQ8MaxSplits &&
+                      w_first >= 0 && w_first <= a_n_wg - S && (uint32_t)d[4] < (uint32_t)p.n_slots && L >= 0 &&
+                      (L + 15) >> 4 <= row_tiles && pos == (kAppend ? L - 1 : -1);
+    if (!fits) {
+      set_err(p.err, CIE_ERRBIT_PLAN);
+      return;
+    }
     load_q();
+    if ((uint32_t)pages >= (uint32_t)p.n_pages) {
+      set_err(p.err, CIE_ERRBIT_PAGE);
+      pages = 0;
+    }
   } else {
     split = blockIdx.x;
     g = blockIdx.y;
@@ -513,7 +525,7 @@ void q8_decode_kernel(const int64_t* __restrict__ a_slot_ids, const int32_t* __r
     if (S == 1) {
       f16x4 o4;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o4[i] = (f16)(den == 0.f ? 0.f : num[i] / den);
+      for (int i = 0; i < 4; ++i) o4[i] = (f16)(q8_no_key(den) ? 0.f : num[i] / den);
       *reinterpret_cast<f16x4*>(p.o + ((int64_t)b * p.H_q + g * p.G + h) * D + 4 * d4) = o4;
     } else {
       const int row = split * p.G + h;
@@ -549,7 +561,7 @@ static int q8_decode_entry(Q8DecodeParams& p, void* partials, int32_t* counters,
                            int64_t pool_head_stride, int64_t bt_stride, int64_t bt_width, int64_t n_slots,
                            int64_t n_splits, int32_t* err, void* stream) {
   if (B < 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0 || n_pages <= 0 || bt_width <= 0 || bt_stride < bt_width ||
-      (!p.plan && n_slots <= 0) || n_splits <= 0 || page_size <= 0)
+      n_slots <= 0 || n_splits <= 0 || page_size <= 0)
     return CIE_EINVAL;
   if (B == 0) return CIE_OK;
   if (!p.o || !p.q || !p.k_pool || !p.v_pool || !p.scales || !p.block_table || (!p.plan && (!p.lens || !p.slot_ids)))

@@ -187,8 +187,10 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
   if (tid < kPlanLevels) sm_level[tid] = 0;
   __syncthreads();
   float work[2] = {0.f, 0.f};
+  bool falls = false;  // a range runs backwards, so others may overlap; the bounds below need disjoint ones
   for (int b = tid; b < p.B; b += kPlanThreadsM) {
     const Q8Seq s = q8_seq(p, b, true);
+    falls |= p.cu_seqlens[b + 1] < p.cu_seqlens[b];
     sm_t0[b] = s.t0;
     sm_slot[b] = s.slot;
     sm_L[b] = s.L;
@@ -207,7 +209,11 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
     const float w = wave_sum(work[i]);
     if (lane == 0) sm_work[i][tid / kWave] = w;
   }
-  __syncthreads();
+  if (__syncthreads_or(falls)) {
+    if (tid == 0) p.plan[0] = 0;
+    if (tid > 0 && tid < kHeadWords) p.plan[tid] = plan_word(p, tid - 1, p.D);
+    return;
+  }
   float total[2] = {0.f, 0.f};
 #pragma unroll
   for (int w = 0; w < kPlanWavesM; ++w) {
@@ -500,7 +506,7 @@ __device__ __forceinline__ void merge_weights(const Q8MixedParams& p, const Q8It
     float top = kEmptyMax, sum = 0.f;
     for (int i = 0; i < tpc; ++i) top = fmaxf(top, sm_m[i * cols + cc]);
     for (int i = 0; i < tpc; ++i) sum += fast_exp2(sm_m[i * cols + cc] - top) * sm_m[kMThreads + i * cols + cc];
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const float inv = q8_no_key(sum) ? 0.f : 1.f / sum;
     for (int c = j; c < n; c += tpc) {
       float* const w = &sm_w[c * cols + cc];
       *w = fast_exp2(*w - top) * inv;
@@ -625,7 +631,7 @@ __device__ __forceinline__ void wide_item(const Q8MixedParams& p, const Q8Item& 
       if (cc >= cols) continue;
       const float l = st.lsum[c][0];
       if (it.n_chunks == 1) {
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float inv = q8_no_key(l) ? 0.f : 1.f / l;
         f16* const o = p.o + out_row<D>(p, it, Q8Col(p, cc)) + NT * 4 * grp;
 #pragma unroll
         for (int i = 0; i < NT / 2; ++i) {  // the lane's 4 NT dims, 8 at a time
@@ -732,7 +738,7 @@ __device__ __forceinline__ void narrow_item(const Q8MixedParams& p, const Q8Item
     if (it.n_chunks == 1) {
       f16x4 o4;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o4[i] = (f16)(den > 0.f ? num[i] / den : 0.f);
+      for (int i = 0; i < 4; ++i) o4[i] = (f16)(q8_no_key(den) ? 0.f : num[i] / den);
       *reinterpret_cast<f16x4*>(p.o + out_row<D>(p, it, Q8Col(p, cc)) + 4 * d4) = o4;
     } else {
       const int row = it.chunk * cols + cc;

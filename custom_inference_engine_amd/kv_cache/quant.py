@@ -61,6 +61,8 @@ def launch(dev: torch.device, name: str, *args, err=None) -> None:
     """One call of the C entry ``name`` on the device's current stream, with that device current."""
     fn = getattr(_native.load(), name)
     index = dev.index
+    if err is not None and (err.dtype != torch.int32 or err.get_device() != index):
+        raise AssertionError("err must be an int32 tensor on the operator's device")
     args += (None if err is None else err.data_ptr(), torch._C._cuda_getCurrentRawStream(index))
     if index == torch.cuda.current_device():
         status = fn(*args)
@@ -131,7 +133,7 @@ def kv_append_tokens_q8(k_cache, v_cache, scales, k, v, pages, offsets, err=None
     (n_pages, h_kv, page_size, d), (s_page, s_head, _, _) = check_cache_q8(k_cache, v_cache, scales)
     dev = one_device(k_cache, v_cache, scales, k, v, pages, offsets)
     T = pages.shape[0]
-    if offsets.shape[0] != T:
+    if pages.dim() != 1 or offsets.shape != pages.shape:
         raise AssertionError("pages and offsets must have one entry per token")
     (k, k_row, k_head), (v, v_row, v_head) = new_rows(k, T, h_kv, d), new_rows(v, T, h_kv, d)
     pages, offsets = int64_index(pages), int64_index(offsets)
@@ -152,7 +154,7 @@ def kv_read_tokens_q8(k_cache, v_cache, scales, pages, offsets, err=None):
     dev = one_device(k_cache, v_cache, scales, pages, offsets)
     pages, offsets = int64_index(pages), int64_index(offsets)
     T = pages.shape[0]
-    _require(tuple(pages.shape) == (T,) and tuple(offsets.shape) == (T,), "pages / offsets must be (T,)")
+    _require(pages.dim() == 1 and offsets.shape == pages.shape, "pages / offsets must be (T,)")
     k = torch.empty((1, T, h_kv, d), dtype=torch.float16, device=dev)
     v = torch.empty_like(k)
     if T == 0:

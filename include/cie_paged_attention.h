@@ -473,8 +473,10 @@ int cie_q8_read_tokens(void* k_out, void* v_out, const void* k_pool, const void*
 /*
  * Decode over the 8-bit cache, as cie_paged_decode / _append / _qkv_rope, one launch.
  * plan: NULL, with n_splits splits per (sequence, kv head), or a step's
- * cie_paged_decode_plan (same append mode; lens / slot_ids / n_slots are then not
- * read), with n_splits its n_workgroups.  partials:
+ * cie_paged_decode_plan (same append mode; lens and slot_ids are then not read), with
+ * n_splits its n_workgroups; a plan that does not fit the call (made in the other
+ * append mode, or for more sequences, heads, slots or pages) is not followed and
+ * raises CIE_ERRBIT_PLAN, or CIE_ERRBIT_PAGE for its pages.  partials:
  * cie_paged_decode_planned_partials_bytes(workgroups, H_q, H_kv, D), workgroups =
  * B * H_kv * n_splits or the plan's; counters: 2 * B * H_kv words; both may be NULL
  * where workgroups == B * H_kv.  The appending forms leave the same bytes and scales
@@ -518,8 +520,8 @@ int cie_q8_decode_qkv_rope(void* o, const void* qkv, int64_t qkv_row_stride,
  *                       (not computed), are reported here.
  *   cie_q8_mixed        per layer.  A plan made for other sizes (B, total_T, heads,
  *                       D, page_size, block table) writes nothing and raises
- *                       CIE_ERRBIT_PLAN; so does a batch of overlapping sequences
- *                       whose items exceed the plan.
+ *                       CIE_ERRBIT_PLAN.  Where cu_seqlens decreases anywhere,
+ *                       nothing of the batch is computed (CIE_ERRBIT_PAGE).
  * partials: cie_q8_mixed_partials_bytes bytes, 16-byte aligned; counters:
  * cie_q8_mixed_counters() words, zero before the call and after it.
  * B <= 2048, H_q / H_kv <= 16, total_T <= 2^24.

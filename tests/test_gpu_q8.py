@@ -582,3 +582,138 @@ def test_unaligned_queries_are_refused(native_lib):
     with pytest.raises(AssertionError, match="num_programs"):
         cie.decode_gqa_attention_q8(c.q.to(DEV), c.k, c.v, c.scales, *c.dev("kv_lens", "slots", "table"),
                                     num_programs=65)
+
+
+# ---- larger calls, extremes, plans of other calls ----
+
+@pytest.mark.parametrize("shape", [
+    dict(prior=[0] * 3, new=[1500] * 3, h_q=16, h_kv=4),
+    dict(prior=[9000], new=[900]),
+    dict(prior=[6000], new=[700], h_q=16, h_kv=8, d=128),
+], ids=["prefill", "split64", "split128"])
+def test_mixed_whole_tiles(native_lib, shape):
+    """Launches large enough for tiles of 128 columns, unsplit and split over the keys."""
+    note(f"q8 mixed whole tiles {shape}")
+    test_mixed(native_lib, shape)
+
+
+def test_long_token_append_is_that_in_pieces(native_lib):
+    """17,700 tokens in one call (16 a workgroup) and in calls of 1,037 leave the same cache."""
+    note("q8 long append")
+    one, many = (Case(prior=[3, 0], new=[17000, 700], h_kv=1, h_q=1, seed=20).write_history() for _ in range(2))
+    append_tokens(one)
+    pages, offs = many.new_at()
+    for lo in range(0, many.T, 1037):
+        s = slice(lo, lo + 1037)
+        cie.kv_append_tokens_q8(many.k, many.v, many.scales, many.k_new[:, s].to(DEV), many.v_new[:, s].to(DEV),
+                                pages[s].to(DEV), offs[s].to(DEV))
+    for a, b in ((one.k, many.k), (one.v, many.v)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert torch.equal(one.scales.view(torch.int32), many.scales.view(torch.int32))
+
+
+@pytest.mark.parametrize("shape", [dict(h_q=14, h_kv=2), dict(h_q=8, h_kv=2, d=128)], ids=["d64", "d128"])
+def test_decode_append_of_extremes(native_lib, shape):
+    """A block's rows one decode at a time, from tiny to the largest fp16, infinities and a NaN: the cache of the
+    definition, and results that are NaN only in the heads that hold one."""
+    note(f"q8 decode extremes {shape}")
+    c = Case(prior=[14], new=[1], seed=21, **shape).write_history()
+    want = c.oracles()
+    c.table[1, 1] = 1 + c.table[1, 0] % 4  # (another of the four pages)
+    steps = [2.0 ** -24, -0.0, 2.0 ** -15, 0.3, 447.0, 65504.0, float("-inf"), float("inf"), -61441.0, float("nan")]
+    d = c.d
+    for i, x in enumerate(steps):
+        pos = 14 + i
+        k = torch.randn(1, 1, c.h_kv, d, generator=torch.Generator().manual_seed(i)).half() * 0.01
+        v = -k.flip(3)
+        k[0, 0, 0, i * d // len(steps)] = x
+        v[0, 0, 0, d - 1 - i] = -x
+        c.lens[1] = pos
+        o = cie.decode_append_gqa_attention_q8(c.q.to(DEV), c.k, c.v, c.scales, k.to(DEV), v.to(DEV),
+                                               *c.dev("lens", "slots", "table"), num_programs=1 + i % 3)
+        page, off = int(c.table[1, pos // 16]), pos % 16
+        for w, y in zip(want, (k, v)):
+            w.append(y[0], [page], [off])
+        same_cache(c, want)
+        group = c.h_q // c.h_kv
+        assert torch.isfinite(o[0, 0, group:]).all()
+        assert bool(o[0, 0, :group].isnan().all()) == (x != x) and bool(torch.isfinite(o[0, 0, :group]).all()) == (x == x)
+        first = 0 if abs(x) < 1 else group  # (scores of thousands are off by more than the tolerance counts)
+        seen = ref.attend(c.q[0], *want, [(0, 1, 1, pos + 1)], c.table)
+        check_attention(o[0, :, first:], tuple(y[:, first:] for y in seen), pos + 1, f"{x}")
+    # the NaN through the other forms: split decodes, and the last of mixed rows in narrow and wide items
+    args = (c.k, c.v, c.scales)
+    lens, table = torch.tensor([24], device=DEV), c.table.to(DEV)
+    outs = [cie.decode_gqa_attention_q8(c.q.to(DEV), *args, lens, c.slots.to(DEV), table, num_programs=P)
+            for P in (1, 2, 5)]
+    for n in (1, 2, 20):
+        q = c.q.to(DEV).expand(1, n, -1, -1).contiguous()
+        outs.append(cie.mixed_gqa_attention_q8(q, *args, n, torch.tensor([0, n], device=DEV), lens - n,
+                                               c.slots.to(DEV), table)[:, -1:])
+    for o in outs:
+        assert o[0, 0, :group].isnan().all()
+        check_attention(o[0, :, group:], tuple(y[:, group:] for y in seen), 24)
+
+
+def test_index_types_and_row_layouts(native_lib):
+    """int32 indices, and new rows as (B, H_kv, D), (B, 1, H_kv, D) or every other head of a wider tensor."""
+    note("q8 index types")
+    c = Case(prior=[20, 47, 5], new=[1, 1, 1], seed=22).write_history()
+    base = [t.clone() for t in (c.k.view(torch.uint8), c.v.view(torch.uint8), c.scales)]
+    want = decode_append(c)
+    after = [t.clone() for t in (c.k.view(torch.uint8), c.v.view(torch.uint8), c.scales)]
+    wide = torch.zeros(3, 4, 64, dtype=torch.float16, device=DEV)
+    wide[:, ::2] = c.k_new[0].to(DEV)
+    v = c.v_new.to(DEV)
+    for k, vv in ((c.k_new[0].to(DEV), v[0]), (c.k_new.transpose(0, 1).to(DEV), v.transpose(0, 1)), (wide[:, ::2], v)):
+        for t, b in zip((c.k.view(torch.uint8), c.v.view(torch.uint8), c.scales), base):
+            t.copy_(b)
+        o = cie.decode_append_gqa_attention_q8(c.q.to(DEV), c.k, c.v, c.scales, k, vv,
+                                               *(x.int() for x in c.dev("lens", "slots", "table")))
+        assert torch.equal(o, want)
+        for t, a in zip((c.k.view(torch.uint8), c.v.view(torch.uint8), c.scales.view(torch.int32)), after):
+            assert torch.equal(t, a.view(t.dtype))
+
+
+def test_plans_of_other_calls_are_not_followed(native_lib):
+    note("q8 other plans")
+    c = Case(prior=[20, 700, 5], new=[1, 1, 1], seed=23).write_history()
+    before = c.k.view(torch.uint8).clone()
+    err = err_word()
+    plain = cie.decode_plan(c.k, *c.dev("kv_lens", "slots", "table"), append=False)
+    app = cie.decode_plan(c.k, *c.dev("lens", "slots", "table"))
+    decode_append(c, plain, err=err)  # the other append mode, either way
+    torch.cuda.synchronize()
+    assert int(err) == PLAN and torch.equal(c.k.view(torch.uint8), before)
+    err.zero_()
+    cie.decode_gqa_attention_q8(c.q.to(DEV), c.k, c.v, c.scales, *c.dev("kv_lens", "slots", "table"), plan=app, err=err)
+    assert int(err) == PLAN
+    err.zero_()  # a plan of three sequences for two: those are right
+    o = cie.decode_gqa_attention_q8(c.q[:, :2].contiguous().to(DEV), c.k, c.v, c.scales, c.kv_lens[:2].to(DEV),
+                                    c.slots[:2].to(DEV), c.table.to(DEV), plan=plain, err=err)
+    assert int(err) == PLAN
+    want = ref.attend(c.q[0], *c.oracles(), decode_seqs(c, c.prior), c.table)
+    check_attention(o[0], tuple(x[:2] for x in want), 700)
+    # cu_seqlens that runs backwards: an empty plan
+    err.zero_()
+    plan = cie.mixed_plan_q8(c.k, torch.tensor([0, 2, 1, 3], device=DEV), *c.dev("kv_lens", "slots", "table"), 3, 3,
+                             14, err=err)
+    assert int(plan[0]) == 0 and int(err) == PAGE
+
+
+def test_operands_elsewhere_are_refused(native_lib):
+    """Counters, plans and error words that the device cannot use, before anything is launched."""
+    note("q8 operands elsewhere")
+    c = Case(prior=[20], new=[1]).write_history()
+    decode = (c.q.to(DEV), c.k, c.v, c.scales, *c.dev("kv_lens", "slots", "table"))
+    mixed = (c.q.to(DEV), c.k, c.v, c.scales, 1, *c.dev("cu", "kv_lens", "slots", "table"))
+    plan = cie.decode_plan(c.k, *c.dev("kv_lens", "slots", "table"), append=False)
+    host = torch.zeros(4096, dtype=torch.int32)
+    for call in (lambda: cie.decode_gqa_attention_q8(*decode, num_programs=2, counters=host),
+                 lambda: cie.decode_gqa_attention_q8(*decode, plan=plan.cpu()),
+                 lambda: cie.decode_gqa_attention_q8(*decode, err=host[:1]),
+                 lambda: cie.mixed_gqa_attention_q8(*mixed, counters=host),
+                 lambda: cie.mixed_gqa_attention_q8(*mixed, plan=plan.cpu()),
+                 lambda: cie.kv_read_tokens_q8(*decode[1:4], *[torch.zeros(1, 1, dtype=torch.int64, device=DEV)] * 2)):
+        with pytest.raises(AssertionError):
+            call()
