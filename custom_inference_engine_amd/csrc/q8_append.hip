@@ -21,8 +21,13 @@
 
 namespace cie {
 
-constexpr int kAppendThreads = 256;
-constexpr int kAppendWaves = kAppendThreads / kWave;
+// Waves a workgroup: 8 where a block has more than 4 (head, K or V) pairs to write, else 4; a wave holds one pair at a
+// time.  (Two in flight: 137 registers at D = 128, one 8-wave workgroup a CU instead of two, 19.4 us for 8,192 rows of 8
+// heads against 15.1; 4 waves 20.2.  464 rows of 2 heads with RoPE: 5.0 us, 5.4 with 8 waves.)  The rope form's 144
+// registers leave one 8-wave workgroup a CU: past kEachRow rows, whose blocks no longer have a CU each, it takes 4
+// (8,192 rows, 32 / 8 heads, D = 128: 38 us, 46 with 8; 300 rows: 9.5 with 4, 7.0 with 8).
+constexpr int kFewWaves = 4, kManyWaves = 8;
+constexpr int64_t kEachRow = 1024;  // rows up to which each has a workgroup of its own
 constexpr int kScan = 8;
 struct __attribute__((aligned(8))) PagePair {
   int64_t a, b;
@@ -65,7 +70,7 @@ struct Q8Rows {
   const int* last;  // [16] token of each row, -1: not written
 };
 
-// One wave's (block, head, K or V): loaded, then rounded and stored, so that a wave can load its next one between.
+// One wave's (block, head, K or V): loaded, then rounded and stored.
 template <int D, bool kRope>
 struct BlockTask {
   static constexpr int NU = D / 64;    // units of 16 values a lane
@@ -177,8 +182,10 @@ __device__ __forceinline__ void rotate_q(const Q8Params& p, int64_t gid) {
   *reinterpret_cast<f16x8*>(dst + D / 2) = hi;
 }
 
-template <int D, bool kDecode, bool kRope>
-__global__ __launch_bounds__(kAppendThreads) void q8_append_kernel(Q8Params p) {
+template <int D, int W, bool kDecode, bool kRope>
+__global__ __launch_bounds__(W * kWave)
+void q8_append_kernel(Q8Params p) {
+  constexpr int kAppendThreads = W * kWave;
   __shared__ int last[kQ8Block];
   __shared__ int earlier;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
@@ -191,7 +198,7 @@ __global__ __launch_bounds__(kAppendThreads) void q8_append_kernel(Q8Params p) {
   // The workgroup's tokens, a lane each (every wave the same): which of them start a run.
   // A prompt's run starts lie 16 tokens apart.  Workgroups go round the XCDs and their CUs in turn, so dealt in order
   // the ones with work would share a few CUs: the list is dealt with stride 16 tokens instead, which makes them
-  // neighbours (4 x 2,048 rows, D = 128: 29 us dealt in order).
+  // neighbours (4 x 2,048 rows of 8 heads, D = 128: 29 us dealt in order, 19 so, both before other steps).
   const int stride = kQ8Block / p.tokens_per_wg, per = p.n_append_wg / stride;
   const int64_t t0 = (int64_t)(stride * ((int)blockIdx.x % per) + (int)blockIdx.x / per) * p.tokens_per_wg;
   int64_t page = 0, off = 0;
@@ -273,13 +280,10 @@ __global__ __launch_bounds__(kAppendThreads) void q8_append_kernel(Q8Params p) {
     if (earlier) continue;
     const Q8Rows rows{pg, block, last[0] >= 0, last};
     const int n_tasks = 2 * p.H_kv;
-    BlockTask<D, kRope> task[2];
-    for (int k = wave; k < n_tasks; k += 2 * kAppendWaves) {
-      const bool two = k + kAppendWaves < n_tasks;
-      task[0].load(p, rows, k, lane);
-      if (two) task[1].load(p, rows, k + kAppendWaves, lane);
-      task[0].store(rows.fresh, lane);
-      if (two) task[1].store(rows.fresh, lane);
+    BlockTask<D, kRope> task;
+    for (int k = wave; k < n_tasks; k += W) {
+      task.load(p, rows, k, lane);
+      task.store(rows.fresh, lane);
     }
   }
 }
@@ -343,24 +347,32 @@ static int q8_check_pools(const void* k_pool, const void* v_pool, const void* sc
   return CIE_OK;
 }
 
-// Tokens a workgroup looks at (a power of two, 16 at most): one up to the 2,048 workgroups that the chip holds at once,
-// so that the rows of a decode batch, each a block of its own, run side by side; more where it would take more rounds
-// of workgroups, most of whose tokens belong to a run that another owns.
+template <int D, int W, bool kDecode, bool kRope>
+static int q8_launch(const Q8Params& p, hipStream_t stream) {
+  constexpr int n = W * kWave;
+  int64_t blocks = p.n_append_wg;
+  if (kRope) blocks += (p.n_rows * p.H_q * (D / 16) + n - 1) / n;
+  if (blocks > 0x7fffffff) return CIE_EUNSUPPORTED;
+  hipLaunchKernelGGL((q8_append_kernel<D, W, kDecode, kRope>), dim3((unsigned)blocks), dim3(n), 0, stream, p);
+  return (int)hipGetLastError();
+}
+
+// Tokens a workgroup looks at (a power of two, 16 at most): one up to kEachRow rows, about the workgroups that the chip
+// holds at once, so that the rows of a decode batch, each a block of its own, run side by side; more where it would
+// take more rounds of workgroups, most of whose tokens belong to a run that another owns (8,192 rows of 2 heads with
+// RoPE, D = 64: 9.8 us, 10.5 from 2,048; 1,500 rows, a block each: 7.6, and 10.8 from 512).
 template <bool kDecode, bool kRope>
 static int q8_launch_append(Q8Params& p, int64_t D, hipStream_t stream) {
   if (p.n_rows > 0x7fffffff / 512) return CIE_EUNSUPPORTED;
   p.tokens_per_wg = 1;
-  while (!kDecode && p.tokens_per_wg < kQ8Block && p.n_rows > 2048 * p.tokens_per_wg) p.tokens_per_wg *= 2;
+  while (!kDecode && p.tokens_per_wg < kQ8Block && p.n_rows > kEachRow * p.tokens_per_wg) p.tokens_per_wg *= 2;
   const int32_t stride = kQ8Block / p.tokens_per_wg;
   p.n_append_wg = (int32_t)((p.n_rows + kQ8Block - 1) / kQ8Block) * stride;
-  int64_t blocks = p.n_append_wg;
-  if (kRope) blocks += (p.n_rows * p.H_q * (D / 16) + kAppendThreads - 1) / kAppendThreads;
-  if (blocks > 0x7fffffff) return CIE_EUNSUPPORTED;
-  if (D == 64)
-    hipLaunchKernelGGL((q8_append_kernel<64, kDecode, kRope>), dim3((unsigned)blocks), dim3(kAppendThreads), 0, stream, p);
-  else
-    hipLaunchKernelGGL((q8_append_kernel<128, kDecode, kRope>), dim3((unsigned)blocks), dim3(kAppendThreads), 0, stream, p);
-  return (int)hipGetLastError();
+  const bool many = 2 * p.H_kv > kFewWaves && (!kRope || p.n_rows <= kEachRow);
+  return D == 64 ? (many ? q8_launch<64, kManyWaves, kDecode, kRope>(p, stream)
+                         : q8_launch<64, kFewWaves, kDecode, kRope>(p, stream))
+                 : (many ? q8_launch<128, kManyWaves, kDecode, kRope>(p, stream)
+                         : q8_launch<128, kFewWaves, kDecode, kRope>(p, stream));
 }
 
 static Q8Params q8_params(void* k_pool, void* v_pool, void* scales, int64_t n_rows, int64_t H_kv, int64_t page_size,

@@ -717,3 +717,7 @@ def test_operands_elsewhere_are_refused(native_lib):
                  lambda: cie.kv_read_tokens_q8(*decode[1:4], *[torch.zeros(1, 1, dtype=torch.int64, device=DEV)] * 2)):
         with pytest.raises(AssertionError):
             call()
+
+
+def test_rope_append_of_many_heads_and_rows(native_lib):
+    test_rope_append_is_rotate_then_append(native_lib, dict(prior=[20, 3], new=[1100, 1], h_q=4, h_kv=4, d=128))
