@@ -34,9 +34,13 @@ def _rows(t: torch.Tensor, n: int, width: int, what: str):
     return t, max(st[-2], width)
 
 
-def _check_counters(counters: torch.Tensor, n: int, dev: torch.device) -> None:
+def _counters(counters: Optional[torch.Tensor], n: int, dev: torch.device) -> torch.Tensor:
+    """The caller's arrival counters, or the device's own."""
+    if counters is None:
+        return split_counters(dev, n)
     _require(counters.dtype == torch.int32 and counters.is_contiguous() and counters.numel() >= n, "counters too small")
     _require(counters.get_device() == dev.index, "counters must be on the operator's device")
+    return counters
 
 
 def _decode(entry, o, q_args, cache, geometry, row_args, lens, slot_ids, block_table, H_q, append, num_programs, err,
@@ -59,9 +63,7 @@ def _decode(entry, o, q_args, cache, geometry, row_args, lens, slot_ids, block_t
         n = _native.load().cie_paged_decode_planned_partials_bytes(n_wg, H_q, H_kv, D)
         buffer = torch.empty(n, dtype=torch.uint8, device=dev)
         partials = buffer.data_ptr()
-        if counters is None:
-            counters = split_counters(dev, 2 * n_groups)
-        _check_counters(counters, 2 * n_groups, dev)
+        counters = _counters(counters, 2 * n_groups, dev)
     slots, width = block_table.shape
     launch(dev, entry, o.data_ptr(), *q_args, k.data_ptr(), v.data_ptr(), scales.data_ptr(), *row_args,
            lens.data_ptr(), slot_ids.data_ptr(), block_table.data_ptr(), None if plan is None else plan.data_ptr(),
@@ -227,9 +229,7 @@ def mixed_gqa_attention_q8(q, k, v, scales, max_seqlen: int, cu_seqlens, kv_lens
     n = lib.cie_q8_mixed_partials_bytes(total_T, H_q, D)
     partials = torch.empty(n, dtype=torch.uint8, device=dev)
     n_ctr = lib.cie_q8_mixed_counters()
-    if counters is None:
-        counters = split_counters(dev, n_ctr)
-    _check_counters(counters, n_ctr, dev)
+    counters = _counters(counters, n_ctr, dev)
     launch(dev, "cie_q8_mixed", o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), scales.data_ptr(),
            plan.data_ptr(), plan.numel() * 4, block_table.data_ptr(), partials.data_ptr(), n, counters.data_ptr(), B,
            total_T, H_q, H_kv, D, PAGE_SIZE, N_PAGES, s_page, s_head, block_table.stride(0), width, slots, err=err)

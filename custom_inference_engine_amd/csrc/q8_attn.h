@@ -121,6 +121,11 @@ __device__ __forceinline__ void q8_step(SoftmaxAcc<D, NCT>& st, K k, V v, M mean
   constexpr int KS = Geo<D>::KS;
   constexpr int NT = Geo<D>::NT;
   f32x4 s[NCT][2 * NP];
+  // Waves of two workgroups share a SIMD: at D = 64, where a step is mostly VALU work, the one that has MFMAs to issue
+  // goes first (4 x 2,048 rows, 14 / 2 heads: 49.4 -> 47.4 us, 300 rows over 8,192 keys 39.6 -> 36.3, 8,192 rows of 8 / 8
+  // heads 136 -> 141; at D = 128 ragged chunks 150 -> 160).
+  constexpr bool kFirst = LDS && D == 64;
+  if (kFirst) __builtin_amdgcn_s_setprio(1);
   f16x8 ka[2][KS];  // a tile's operands are fetched while the one before it is multiplied
   k(0, ka[0]);
 #pragma unroll
@@ -136,6 +141,7 @@ __device__ __forceinline__ void q8_step(SoftmaxAcc<D, NCT>& st, K k, V v, M mean
     if (LDS) __builtin_amdgcn_sched_barrier(0);
   }
   meanwhile();
+  if (kFirst) __builtin_amdgcn_s_setprio(0);
   if (mask) {
 #pragma unroll
     for (int c = 0; c < NCT; ++c)
