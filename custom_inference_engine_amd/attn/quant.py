@@ -10,6 +10,7 @@ float32, as in ``core.py``.  ``TritonQwen2Attention`` calls these where its
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -186,15 +187,34 @@ def mixed_plan_q8(k_cache, cu_seqlens, kv_lens, slot_ids, block_table, max_seqle
              "cu_seqlens must be (B+1,) and kv_lens (B,)")
     _require(N_PAGES == block_table.shape[1], "block_table width must equal n_pages")
     dev = one_device(k_cache, cu_seqlens, kv_lens, slot_ids, block_table)
-    cu_seqlens, kv_lens, slot_ids = int64_index(cu_seqlens), int64_index(kv_lens), int64_index(slot_ids)
-    lib = _native.load()
-    n = lib.cie_q8_mixed_plan_bytes(B, int(total_T), num_heads, H_kv)
-    _require(n > 0, "batch too large for a mixed plan")
+    n = _mixed_plan_bytes(B, int(total_T), num_heads, H_kv)
     plan = torch.empty(n // 4, dtype=torch.int32, device=dev)
-    launch(dev, "cie_q8_mixed_plan", plan.data_ptr(), n, cu_seqlens.data_ptr(), kv_lens.data_ptr(),
-           slot_ids.data_ptr(), B, int(total_T), int(max_seqlen), num_heads, H_kv, D, PAGE_SIZE, N_PAGES,
-           block_table.shape[0], err=err)
+    _make_plan(plan.data_ptr(), n, cu_seqlens, kv_lens, slot_ids, B, total_T, max_seqlen, num_heads, k_cache.shape,
+               block_table.shape[0], dev, err)
     return plan
+
+
+@functools.lru_cache(maxsize=1024)
+def _mixed_plan_bytes(B: int, total_T: int, H_q: int, H_kv: int) -> int:
+    n = _native.load().cie_q8_mixed_plan_bytes(B, total_T, H_q, H_kv)
+    _require(n > 0, "batch too large for a mixed plan")
+    return n
+
+
+@functools.lru_cache(maxsize=1024)
+def _mixed_buffers(total_T: int, H_q: int, D: int):
+    """Bytes of a call's partials, and words of its counters."""
+    lib = _native.load()
+    return lib.cie_q8_mixed_partials_bytes(total_T, H_q, D), lib.cie_q8_mixed_counters()
+
+
+def _make_plan(plan_ptr, n_bytes, cu_seqlens, kv_lens, slot_ids, B, total_T, max_seqlen, num_heads, pool_shape, n_slots,
+               dev, err):
+    N_PAGES, H_kv, PAGE_SIZE, D = pool_shape
+    cu_seqlens, kv_lens, slot_ids = int64_index(cu_seqlens), int64_index(kv_lens), int64_index(slot_ids)
+    launch(dev, "cie_q8_mixed_plan", plan_ptr, n_bytes, cu_seqlens.data_ptr(), kv_lens.data_ptr(),
+           slot_ids.data_ptr(), B, int(total_T), int(max_seqlen), num_heads, H_kv, D, PAGE_SIZE, N_PAGES,
+           n_slots, err=err)
 
 
 def mixed_gqa_attention_q8(q, k, v, scales, max_seqlen: int, cu_seqlens, kv_lens, slot_ids, block_table, err=None,
@@ -219,19 +239,21 @@ def mixed_gqa_attention_q8(q, k, v, scales, max_seqlen: int, cu_seqlens, kv_lens
     if B == 0 or total_T == 0 or int(max_seqlen) == 0:
         return o
     block_table = int64_table(block_table)
-    lib = _native.load()
-    if plan is None:
-        plan = mixed_plan_q8(k, cu_seqlens, kv_lens, slot_ids, block_table, max_seqlen, total_T, H_q, err=err)
+    plan_bytes = _mixed_plan_bytes(B, total_T, H_q, H_kv)
+    n, n_ctr = _mixed_buffers(total_T, H_q, D)
+    if plan is None:  # (the plan behind the partials, whose bytes are a multiple of 256)
+        partials = torch.empty(n + plan_bytes, dtype=torch.uint8, device=dev)
+        plan_ptr = partials.data_ptr() + n
+        _make_plan(plan_ptr, plan_bytes, cu_seqlens, kv_lens, slot_ids, B, total_T, max_seqlen, H_q, k.shape, slots,
+                   dev, err)
     else:
         _require(plan.dtype == torch.int32 and plan.is_contiguous() and plan.get_device() == dev.index
-                 and plan.numel() * 4 >= lib.cie_q8_mixed_plan_bytes(B, total_T, H_q, H_kv),
-                 "plan must come from mixed_plan_q8 for this batch")
-    n = lib.cie_q8_mixed_partials_bytes(total_T, H_q, D)
-    partials = torch.empty(n, dtype=torch.uint8, device=dev)
-    n_ctr = lib.cie_q8_mixed_counters()
+                 and plan.numel() * 4 >= plan_bytes, "plan must come from mixed_plan_q8 for this batch")
+        partials = torch.empty(n, dtype=torch.uint8, device=dev)
+        plan_ptr = plan.data_ptr()
     counters = _counters(counters, n_ctr, dev)
     launch(dev, "cie_q8_mixed", o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), scales.data_ptr(),
-           plan.data_ptr(), plan.numel() * 4, block_table.data_ptr(), partials.data_ptr(), n, counters.data_ptr(), B,
+           plan_ptr, plan_bytes, block_table.data_ptr(), partials.data_ptr(), n, counters.data_ptr(), B,
            total_T, H_q, H_kv, D, PAGE_SIZE, N_PAGES, s_page, s_head, block_table.stride(0), width, slots, err=err)
     return o
 
