@@ -141,24 +141,35 @@ struct Q8Cut {
 
 constexpr int kPlanWavesM = kPlanThreadsM / kWave;
 
-// Exclusive prefix sum of v over the workgroup's threads, and the sum; red: a word a wave.
-__device__ __forceinline__ int plan_block_scan(int v, int* red, int& all) {
+// Exclusive prefix sums of N values over the workgroup's threads, and their sums, with one barrier; red: not read by
+// anyone since the last.
+template <int N>
+__device__ __forceinline__ void plan_block_scan(const int (&v)[N], int (&before)[N], int (&all)[N],
+                                                int (&red)[N][kPlanWavesM]) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const int inc = wave_inclusive_sum(v);
-  __syncthreads();
-  if (lane == kWave - 1) red[wave] = inc;
-  __syncthreads();
-  int base = 0;
-  all = 0;
+  int inc[N];
 #pragma unroll
-  for (int w = 0; w < kPlanWavesM; ++w) {
-    if (w < wave) base += red[w];
-    all += red[w];
+  for (int i = 0; i < N; ++i) inc[i] = wave_inclusive_sum(v[i]);
+  if (lane == kWave - 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) red[i][wave] = inc[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    int base = 0;
+    all[i] = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWavesM; ++w) {
+      const int x = red[i][w];
+      base += w < wave ? x : 0;
+      all[i] += x;
+    }
+    before[i] = base + inc[i] - v[i];
   }
-  return base + inc - v;
 }
 
-// One workgroup: a thread a sequence, then a thread a query tile.
+// One workgroup: a thread up to kSeqsPer sequences in order, then a thread a query tile.  Barriers are most of its time
+// (five, where a batch has no more than kPlanThreadsM tiles).
 //
 // Columns of a wide tile: with W the launch's work in key tiles of wide items of kTileCols columns (a narrow item's
 // key tile counts a quarter), a launch of W <= kSmallWork * kQ8Slots takes tiles of half as many, one column tile a
@@ -181,16 +192,24 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
   __shared__ int sm_slot[kQ8MaxSeqs], sm_L[kQ8MaxSeqs], sm_c[kQ8MaxSeqs];
   __shared__ int sm_first[kQ8MaxSeqs];  // a sequence's first tile
   __shared__ int sm_level[kPlanLevels];
-  __shared__ int sm_red[kPlanWavesM];
+  __shared__ int sm_seq[3][kPlanWavesM], sm_tile[2][kPlanWavesM];
   __shared__ float sm_work[2][kPlanWavesM];  // a wave's part of W in whole tiles, in half tiles
+  __shared__ int sm_fits;
+  constexpr int kSeqsPer = kQ8MaxSeqs / kPlanThreadsM;
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   if (tid < kPlanLevels) sm_level[tid] = 0;
-  __syncthreads();
+  const int per_thread = (p.B + kPlanThreadsM - 1) / kPlanThreadsM, b_first = tid * per_thread;
   float work[2] = {0.f, 0.f};
-  bool falls = false;  // a range runs backwards, so others may overlap; the bounds below need disjoint ones
-  for (int b = tid; b < p.B; b += kPlanThreadsM) {
+  int n_seq[3] = {0, 0, 0};  // tiles if they are whole, if they are half ones; ranges that run backwards
+  int n_rt[2][kSeqsPer];
+#pragma unroll
+  for (int u = 0; u < kSeqsPer; ++u) {
+    n_rt[0][u] = n_rt[1][u] = 0;
+    const int b = b_first + u;
+    if (u >= per_thread || b >= p.B) continue;
     const Q8Seq s = q8_seq(p, b, true);
-    falls |= p.cu_seqlens[b + 1] < p.cu_seqlens[b];
+    // (others may overlap such a range; the bounds below need disjoint ones)
+    n_seq[2] |= p.cu_seqlens[b + 1] < p.cu_seqlens[b];
     sm_t0[b] = s.t0;
     sm_slot[b] = s.slot;
     sm_L[b] = s.L;
@@ -202,6 +221,8 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
       const float n = (float)cut.n_rt;
       work[i] += cut.narrow ? (float)((s.c + s.L) >> 6) + 1.f
                             : n * (float)((s.c >> 4) + 2) + (float)cut.R * n * (n + 1.f) * (1.f / 32) + 1.f;
+      n_rt[i][u] = cut.n_rt;
+      n_seq[i] += cut.n_rt;
     }
   }
 #pragma unroll
@@ -209,7 +230,9 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
     const float w = wave_sum(work[i]);
     if (lane == 0) sm_work[i][tid / kWave] = w;
   }
-  if (__syncthreads_or(falls)) {
+  int seq_before[3], seq_all[3];
+  plan_block_scan(n_seq, seq_before, seq_all, sm_seq);
+  if (seq_all[2]) {
     if (tid == 0) p.plan[0] = 0;
     if (tid > 0 && tid < kHeadWords) p.plan[tid] = plan_word(p, tid - 1, p.D);
     return;
@@ -224,14 +247,13 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
   const float per_slot = 1.001f * (float)p.H_kv / kQ8Slots;
   const bool small = total[0] * per_slot <= (float)kSmallWork;
   const int cols = small ? kTileCols / 2 : kTileCols;
-  const int want = (int)fminf(67108864.f, total[small] * per_slot + 1.f);
-  int n_tiles = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kPlanThreadsM) {
-    const int b = b0 + tid;
-    int all;
-    const int first = plan_block_scan(b < p.B ? Q8Cut(p, sm_L[b], cols, 0).n_rt : 0, sm_red, all);
-    if (b < p.B) sm_first[b] = n_tiles + first;
-    n_tiles += all;
+  const int want = (int)fminf(67108864.f, (small ? total[1] : total[0]) * per_slot + 1.f);
+  const int n_tiles = small ? seq_all[1] : seq_all[0];
+  int at_tile = small ? seq_before[1] : seq_before[0];
+#pragma unroll
+  for (int u = 0; u < kSeqsPer; ++u) {
+    if (u < per_thread && b_first + u < p.B) sm_first[b_first + u] = at_tile;
+    at_tile += small ? n_rt[1][u] : n_rt[0][u];
   }
   __syncthreads();
 
@@ -262,13 +284,14 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
       kt = (sm_c[b] + r * R + rows + 15) >> 4;
       n = min(kQ8MaxChunks, (kt + share - 1) / share);
     }
-    int all;
-    const int mine = n > 1 ? n * rows * p.G * p.H_kv : 0;
-    pbase = rows_at + plan_block_scan(mine, sm_red, all);
-    rows_at += all;
-    if ((int64_t)pbase + mine > p.part_cap) n = 1;  // its partial rows would end past the buffer: unsplit
-    ctr = ctr_at + plan_block_scan(n > 1 ? p.H_kv : 0, sm_red, all);
-    ctr_at += all;
+    const int mine[2] = {n > 1 ? n * rows * p.G * p.H_kv : 0, n > 1 ? p.H_kv : 0};
+    int before[2], all[2];
+    plan_block_scan(mine, before, all, sm_tile);
+    pbase = rows_at + before[0];
+    ctr = ctr_at + before[1];
+    rows_at += all[0];
+    ctr_at += all[1];
+    if ((int64_t)pbase + mine[0] > p.part_cap) n = 1;  // its partial rows would end past the buffer: unsplit
     if (n > 0) {
       const int len = (kt + n - 1) / n;  // an item's key tiles, in a wide item's
       level = kPlanLevels - 1 - min(kPlanLevels - 1, (int)((int64_t)len * kPlanLevels / (share + 1)));
@@ -277,6 +300,7 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
   };
   const bool once = n_tiles <= kPlanThreadsM;
   for (int i0 = 0; i0 < n_tiles; i0 += kPlanThreadsM) {
+    if (i0 > 0) __syncthreads();
     tile(i0);
     if (n > 0) atomicAdd(&sm_level[level], n * p.H_kv);
   }
@@ -288,19 +312,21 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
     if (tid == 0) {
       const bool fits = n_items <= p.plan_cap;
       if (!fits) set_err(p.err, CIE_ERRBIT_PLAN);
-      sm_red[0] = fits;
+      sm_fits = fits;
       p.plan[0] = fits ? n_items : 0;
 #pragma unroll
       for (int i = 1; i < kHeadWords; ++i) p.plan[i] = plan_word(p, i - 1, p.D);
     }
   }
   __syncthreads();
-  if (!sm_red[0]) return;
+  if (!sm_fits) return;
   Q8Item* const items = reinterpret_cast<Q8Item*>(p.plan + kHeadWords);
-  __syncthreads();
   rows_at = ctr_at = 0;
   for (int i0 = 0; i0 < n_tiles; i0 += kPlanThreadsM) {
-    if (!once) tile(i0);
+    if (!once) {
+      if (i0 > 0) __syncthreads();
+      tile(i0);
+    }
     if (n == 0) continue;
     const int abs_rows = rows < 0 ? -rows : rows;
     const int R = rows < 0 ? 0 : cols / p.G;  // (a narrow sequence has one tile)

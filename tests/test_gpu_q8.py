@@ -721,3 +721,14 @@ def test_operands_elsewhere_are_refused(native_lib):
 
 def test_rope_append_of_many_heads_and_rows(native_lib):
     test_rope_append_is_rotate_then_append(native_lib, dict(prior=[20, 3], new=[1100, 1], h_q=4, h_kv=4, d=128))
+
+
+def test_mixed_of_many_sequences(native_lib):
+    """More sequences, and more query tiles, than the plan's threads; split tiles among the last ones."""
+    prior = [i * 13 % 70 for i in range(600)]
+    new = [i % 4 for i in range(600)]
+    prior[7], prior[590], new[590], prior[595], new[595] = 3000, 5000, 1, 4000, 60
+    shape = dict(prior=prior, new=new, h_q=4, h_kv=2)
+    test_mixed(native_lib, shape)
+    # 2,100 rows in half tiles of 4: 525 beside one decode row over a long prefix
+    test_mixed(native_lib, dict(prior=[0] * 7 + [3000], new=[300] * 7 + [1], h_q=16, h_kv=1))
