@@ -13,7 +13,8 @@
 // whole list for the block: an earlier token with it makes that one's workgroup the
 // owner; otherwise the last token of each row is the one written.  So a list in any
 // order, or with the same index twice, gives one result, with no race on a block.
-// The search reads T page ids (L2 hits) and is shared by all heads of the block.
+// The search reads T page ids (L2 hits) and is shared by all heads of the block: T^2 / 16
+// ids in all, which shows from some 32,000 rows on.
 //
 // What bounds it: memory at many tokens, the start's chain (index, then rows) at
 // few.
