@@ -252,6 +252,55 @@ __device__ __forceinline__ void q8_merge(const Q8DecodeParams& p, int64_t row0, 
   }
 }
 
+// The same for few states: a thread owns 4 dims of a head and takes kFewLoads states a round, each with its m and l, so
+// that a round trip and no barrier serve kFewLoads splits (graph replays, 14 / 2 heads, D = 64: 32 sequences of 4,096
+// keys, 4 splits, 12.4 us through q8_merge, 11.2 so; 1 of 1,000, 16 splits, 8.6 and 7.0).
+constexpr int kFewLoads = 8, kFewStates = 16;
+template <int D>
+__device__ __forceinline__ void q8_merge_few(const Q8DecodeParams& p, int64_t row0, int b, int g, int S, int tid) {
+  constexpr int D4 = D / 4;
+  const __amdgpu_buffer_rsrc_t racc =
+      coherent_rsrc(p.part_acc + row0 * D, (uint32_t)(p.G * S * D * sizeof(float)));
+  for (int unit = tid; unit < p.G * D4; unit += kQ8Threads) {
+    const int h = unit / D4, d4 = unit - h * D4;
+    float M = kEmptyMax, den = 0.f;
+    f32x4 num = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < S; s0 += kFewLoads) {
+      float ms[kFewLoads], ls[kFewLoads];
+      f32x4 as[kFewLoads];
+#pragma unroll
+      for (int u = 0; u < kFewLoads; ++u) {
+        ms[u] = kEmptyMax;
+        ls[u] = 0.f;
+        as[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (s0 + u < S) {  // uniform
+          const int row = (s0 + u) * p.G + h;
+          ms[u] = agent_load(&p.part_m[row0 + row]);
+          ls[u] = agent_load(&p.part_l[row0 + row]);
+          as[u] = agent_load4(racc, (uint32_t)((row * D + 4 * d4) * sizeof(float)));
+        }
+      }
+      float Mn = M;
+#pragma unroll
+      for (int u = 0; u < kFewLoads; ++u) Mn = fmaxf(Mn, ms[u]);
+      const float c = fast_exp2(M - Mn);
+      num *= c;
+      den *= c;
+      M = Mn;
+#pragma unroll
+      for (int u = 0; u < kFewLoads; ++u) {
+        const float a = fast_exp2(ms[u] - M);
+        num += a * as[u];
+        den += a * ls[u];
+      }
+    }
+    f16x4 o4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o4[i] = (f16)(q8_no_key(den) ? 0.f : num[i] / den);
+    *reinterpret_cast<f16x4*>(p.o + ((int64_t)b * p.H_q + g * p.G + h) * D + 4 * d4) = o4;
+  }
+}
+
 // (leading arguments: preloaded into SGPRs, so the start's first loads need not wait for the argument load)
 template <int D, bool kAppend, bool kRope, bool kPlanned>
 __global__ __launch_bounds__(kQ8Threads) __attribute__((amdgpu_waves_per_eu(2)))
@@ -492,6 +541,11 @@ void q8_decode_kernel(const int64_t* __restrict__ a_slot_ids, const int32_t* __r
     }
   }
 
+  // Splits that hold a tile: dealt a tile a wave or less, those from this one on are empty (a plan has none).  They
+  // arrive, but leave no state.
+  const int S_used = kPlanned ? S : min(S, max(1, (n_tiles + W - 1) / W));
+  const int64_t row0 = (int64_t)w_first * p.G;
+  if (split < S_used) {  // (uniform)
   // Fold the workgroup's waves: a thread folds 4 dims of one head.
   if (grp == 0) {
     sm_m[wave][r16] = st.m[0];
@@ -505,7 +559,6 @@ void q8_decode_kernel(const int64_t* __restrict__ a_slot_ids, const int32_t* __r
                                                               st.acc[0][4 * n4 + 2][r], st.acc[0][4 * n4 + 3][r]};
   __syncthreads();
   constexpr int D4 = D / 4;
-  const int64_t row0 = (int64_t)w_first * p.G;
   const __amdgpu_buffer_rsrc_t racc =
       coherent_rsrc(p.part_acc + row0 * D, S > 1 ? (uint32_t)(p.G * S * D * sizeof(float)) : 0);
   for (int it = threadIdx.x; it < p.G * D4; it += kQ8Threads) {
@@ -536,10 +589,14 @@ void q8_decode_kernel(const int64_t* __restrict__ a_slot_ids, const int32_t* __r
       }
     }
   }
+  }
   if (S == 1) return;
   int32_t* const arrival = p.counters + b * p.H_kv + g;
   if (!arrive_last(arrival, (int64_t)p.B * p.H_kv, S, &sm_last, p.err)) return;
-  q8_merge<D>(p, row0, b, g, S, threadIdx.x, &sm_acc[0][0][0]);
+  if (S_used <= kFewStates)
+    q8_merge_few<D>(p, row0, b, g, S_used, threadIdx.x);
+  else
+    q8_merge<D>(p, row0, b, g, S_used, threadIdx.x, &sm_acc[0][0][0]);
   if (threadIdx.x == 0) counter_reset(arrival);
 }
 

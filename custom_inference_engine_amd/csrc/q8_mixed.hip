@@ -541,6 +541,72 @@ __device__ __forceinline__ void merge_weights(const Q8MixedParams& p, const Q8It
   __syncthreads();
 }
 
+// The same for few chunks: a thread owns UN pieces (tid + 256 i) and takes CH chunks a round, each with its m and l: a
+// round trip, no barrier (14 / 2 heads, D = 64, planned: 8 rows over 4,000 keys 12.2 us through merge_pieces, 9.2 so; 2 x
+// 64 rows over 2,000 15.3 and 14.1).  Past 4 pieces a thread it is the slower: 8 of them take 24 more registers (4 x
+// 8,192 rows 562 -> 620 us).
+template <int D, int UN, int CH>
+__device__ __forceinline__ void merge_few(const Q8MixedParams& p, const Q8Item& it, int cols) {
+  constexpr int D4 = D / 4;
+  const int n = it.n_chunks, n_units = cols * D4;
+  const __amdgpu_buffer_rsrc_t racc =
+      coherent_rsrc(p.part_acc + (int64_t)it.pbase * D, (uint32_t)(n_units * n * sizeof(f32x4)));
+  float M[UN], den[UN];
+  f32x4 num[UN];
+#pragma unroll
+  for (int i = 0; i < UN; ++i) {
+    M[i] = kEmptyMax;
+    den[i] = 0.f;
+    num[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  for (int c0 = 0; c0 < n; c0 += CH) {
+    float ms[CH][UN], ls[CH][UN];
+    f32x4 as[CH][UN];
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+#pragma unroll
+      for (int i = 0; i < UN; ++i) {
+        ms[u][i] = kEmptyMax;
+        ls[u][i] = 0.f;
+        as[u][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int unit = threadIdx.x + i * kMThreads;
+        if (c0 + u < n && unit < n_units) {
+          const int row = (c0 + u) * cols + unit / D4;
+          ms[u][i] = agent_load(&p.part_m[it.pbase + row]);
+          ls[u][i] = agent_load(&p.part_l[it.pbase + row]);
+          as[u][i] = agent_load4(racc, (uint32_t)((row * D + 4 * part_piece<D>(unit % D4)) * sizeof(float)));
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      float Mn = M[i];
+#pragma unroll
+      for (int u = 0; u < CH; ++u) Mn = fmaxf(Mn, ms[u][i]);
+      const float a0 = fast_exp2(M[i] - Mn);
+      num[i] *= a0;
+      den[i] *= a0;
+      M[i] = Mn;
+#pragma unroll
+      for (int u = 0; u < CH; ++u) {
+        const float a = fast_exp2(ms[u][i] - Mn);
+        num[i] += a * as[u][i];
+        den[i] += a * ls[u][i];
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < UN; ++i) {
+    const int unit = threadIdx.x + i * kMThreads;
+    if (unit >= n_units) continue;
+    const int cc = unit / D4, d4 = unit - cc * D4;
+    f16x4 o4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o4[j] = (f16)(q8_no_key(den[i]) ? 0.f : num[i][j] / den[i]);
+    *reinterpret_cast<f16x4*>(p.o + out_row<D>(p, it, Q8Col(p, cc)) + 4 * d4) = o4;
+  }
+}
+
 template <int D>
 __device__ __forceinline__ void q8_mixed_merge(const Q8MixedParams& p, const Q8Item& it, int cols, f32x4* lds) {
   float* const sm_w = reinterpret_cast<float*>(lds);
@@ -548,7 +614,11 @@ __device__ __forceinline__ void q8_mixed_merge(const Q8MixedParams& p, const Q8I
   f32x4* const sm_sum = lds + (kTileCols * kQ8MaxChunks + 2 * kMThreads) / 4;
   auto weights = [&] { merge_weights(p, it, cols, sm_w, sm_m); };
   const int n_units = cols * (D / 4);
-  if (n_units <= kMThreads)
+  if (it.n_chunks <= 16 && n_units <= kMThreads)
+    merge_few<D, 1, 8>(p, it, cols);
+  else if (it.n_chunks <= 8 && n_units <= 4 * kMThreads)
+    merge_few<D, 4, 4>(p, it, cols);
+  else if (n_units <= kMThreads)
     merge_pieces<D, 1>(p, it, cols, sm_w, sm_sum, weights);
   else if (n_units <= 2 * kMThreads)
     merge_pieces<D, 2>(p, it, cols, sm_w, sm_sum, weights);
