@@ -28,11 +28,11 @@ def _rows(t: torch.Tensor, n: int, width: int, what: str):
     shape = t.shape
     if shape != (1, n, width) and shape != (n, width):
         raise AssertionError(f"{what} must be (1, {n}, {width}), one row per token")
-    st = t.stride()
-    if st[-1] != 1 or st[-2] % 8 or (n > 1 and st[-2] < width) or t.data_ptr() % 16:
+    row, one = t.stride()[-2:]
+    if one != 1 or row & 7 or (n > 1 and row < width) or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
-        st = t.stride()
-    return t, max(st[-2], width)
+        row = width
+    return t, row if n > 1 else width
 
 
 def _counters(counters: Optional[torch.Tensor], n: int, dev: torch.device) -> torch.Tensor:
@@ -42,6 +42,11 @@ def _counters(counters: Optional[torch.Tensor], n: int, dev: torch.device) -> to
     _require(counters.dtype == torch.int32 and counters.is_contiguous() and counters.numel() >= n, "counters too small")
     _require(counters.get_device() == dev.index, "counters must be on the operator's device")
     return counters
+
+
+@functools.lru_cache(maxsize=1024)
+def _decode_partials_bytes(n_wg: int, H_q: int, H_kv: int, D: int) -> int:
+    return _native.load().cie_paged_decode_planned_partials_bytes(n_wg, H_q, H_kv, D)
 
 
 def _decode(entry, o, q_args, cache, geometry, row_args, lens, slot_ids, block_table, H_q, append, num_programs, err,
@@ -61,8 +66,7 @@ def _decode(entry, o, q_args, cache, geometry, row_args, lens, slot_ids, block_t
         n_wg = P * n_groups
     partials = 0
     if n_wg > n_groups:
-        n = _native.load().cie_paged_decode_planned_partials_bytes(n_wg, H_q, H_kv, D)
-        buffer = torch.empty(n, dtype=torch.uint8, device=dev)
+        buffer = torch.empty(_decode_partials_bytes(n_wg, H_q, H_kv, D), dtype=torch.uint8, device=dev)
         partials = buffer.data_ptr()
         counters = _counters(counters, 2 * n_groups, dev)
     slots, width = block_table.shape

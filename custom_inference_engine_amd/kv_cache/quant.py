@@ -24,6 +24,8 @@ import torch
 from .. import _native
 
 BLOCK = 16  # tokens that share a scale
+_F16, _F8, _F32, _I64 = torch.float16, torch.float8_e4m3fn, torch.float32, torch.int64
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _require(cond: bool, msg: str) -> None:
@@ -36,13 +38,14 @@ def check_cache_q8(k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor):
     shape, st = k.shape, k.stride()
     if len(shape) != 4 or v.shape != shape:
         raise AssertionError("K/V pools must be (n_pages, H_kv, page_size, D)")
-    if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn:
+    if k.dtype != _F8 or v.dtype != _F8:
         raise AssertionError("K/V pools must be float8_e4m3fn")
-    if v.stride() != st or st[3] != 1 or st[2] != shape[3]:
+    n_pages, h_kv, page_size, d = shape
+    if v.stride() != st or st[3] != 1 or st[2] != d:
         raise AssertionError("K/V pools need identical strides with dense (page_size, D) rows")
-    if shape[2] % BLOCK:
+    if page_size % BLOCK:
         raise AssertionError("page_size must be a multiple of 16")
-    if (scales.shape != (shape[0], shape[1], shape[2] // BLOCK, 2) or scales.dtype != torch.float32
+    if (scales.shape != (n_pages, h_kv, page_size // BLOCK, 2) or scales.dtype != _F32
             or not scales.is_contiguous()):
         raise AssertionError("scales must be contiguous float32 (n_pages, H_kv, page_size // 16, 2)")
     return shape, st
@@ -63,46 +66,46 @@ def launch(dev: torch.device, name: str, *args, err=None) -> None:
     index = dev.index
     if err is not None and (err.dtype != torch.int32 or err.get_device() != index):
         raise AssertionError("err must be an int32 tensor on the operator's device")
-    args += (None if err is None else err.data_ptr(), torch._C._cuda_getCurrentRawStream(index))
-    if index == torch.cuda.current_device():
-        status = fn(*args)
+    err = None if err is None else err.data_ptr()
+    if index == _current_device():
+        status = fn(*args, err, _current_stream(index))
     else:
         with torch.cuda.device(dev):
-            status = fn(*args)
+            status = fn(*args, err, _current_stream(index))
     if status:
         _native.check(status, name)
 
 
 def int64_index(t: torch.Tensor) -> torch.Tensor:
-    if t.dtype != torch.int64 or not t.is_contiguous():
-        t = t.to(torch.int64).contiguous()
+    if t.dtype != _I64 or not t.is_contiguous():
+        t = t.to(_I64).contiguous()
     return t
 
 
 def int64_table(bt: torch.Tensor) -> torch.Tensor:
-    if bt.dtype != torch.int64 or bt.stride(1) != 1:
-        bt = bt.to(torch.int64).contiguous()
+    if bt.dtype != _I64 or bt.stride(1) != 1:
+        bt = bt.to(_I64).contiguous()
     return bt
 
 
 def new_rows(x: torch.Tensor, n: int, h_kv: int, d: int):
     """New K or V as n rows (H_kv, D) that the kernels can read in 16-byte pieces: the tensor that holds them
     (the caller's, or a copy), and the strides of its rows and heads."""
-    if x.dtype != torch.float16:
+    if x.dtype != _F16:
         raise AssertionError("new K/V must be float16")
-    shape, st = x.shape, x.stride()
-    if len(shape) < 3 or shape[-3:] != (n, h_kv, d) or any(m != 1 for m in shape[:-3]):
+    shape = x.shape
+    if shape != (1, n, h_kv, d) and shape != (n, h_kv, d):
         try:
             x = x.view(-1, h_kv, d)
         except RuntimeError:
             x = x.reshape(-1, h_kv, d)
-        shape, st = x.shape, x.stride()
-        if shape[0] != n:
-            raise AssertionError(f"expected {n} new K/V rows, one a token, got {shape[0]}")
-    if st[-1] != 1 or st[-3] % 8 or st[-2] % 8 or x.data_ptr() % 16:
+        if x.shape[0] != n:
+            raise AssertionError(f"expected {n} new K/V rows, one a token, got {x.shape[0]}")
+    row, head, one = x.stride()[-3:]
+    if one != 1 or (row | head) & 7 or x.data_ptr() & 15:
         x = x.clone(memory_format=torch.contiguous_format)
-        st = x.stride()
-    return x, st[-3], st[-2]
+        row, head, one = x.stride()[-3:]
+    return x, row, head
 
 
 def kv_append_decode_q8(k_cache, v_cache, scales, k, v, slot_ids, lens, block_table, err=None) -> None:
