@@ -357,9 +357,10 @@ void q8_decode_kernel(const int64_t* __restrict__ a_slot_ids, const int32_t* __r
     pos = d[6];
     w_first = d[7];
     // A plan of another batch or of the other append mode: nothing of it is followed.
-    const bool fits = b < p.B && (uint32_t)g < (uint32_t)p.H_kv && (uint32_t)split < (uint32_t)S && S <= kQ8MaxSplits &&
-                      w_first >= 0 && w_first <= a_n_wg - S && (uint32_t)d[4] < (uint32_t)p.n_slots && L >= 0 &&
-                      (L + 15) >> 4 <= row_tiles && pos == (kAppend ? L - 1 : -1);
+    const bool fits = b < p.B && (uint32_t)g < (uint32_t)p.H_kv && (uint32_t)S <= (uint32_t)kQ8MaxSplits &&
+                      (uint32_t)split < (uint32_t)S && w_first >= 0 && w_first <= a_n_wg - S &&
+                      (uint32_t)d[4] < (uint32_t)p.n_slots && L >= 0 && L <= 16 * row_tiles &&
+                      pos == (kAppend ? L - 1 : -1);
     if (!fits) {
       set_err(p.err, CIE_ERRBIT_PLAN);
       return;
