@@ -256,7 +256,8 @@ __device__ __forceinline__ void q8_merge(const Q8DecodeParams& p, int64_t row0, 
 
 // The same for few states: a thread owns 4 dims of a head and takes kFewLoads states a round, each with its m and l, so
 // that a round trip and no barrier serve kFewLoads splits (graph replays, 14 / 2 heads, D = 64: 32 sequences of 4,096
-// keys, 4 splits, 12.4 us through q8_merge, 11.2 so; 1 of 1,000, 16 splits, 8.6 and 7.0).
+// keys, 4 splits, 12.4 us through q8_merge, 11.2 so; 1 of 1,000, 16 splits, 8.6 and 7.0; 4 of 8,000, 32 splits, 10.6 and
+// 11.3).
 constexpr int kFewLoads = 8, kFewStates = 16;
 template <int D>
 __device__ __forceinline__ void q8_merge_few(const Q8DecodeParams& p, int64_t row0, int b, int g, int S, int tid) {
