@@ -357,15 +357,19 @@ void q8_decode_kernel(const int64_t* __restrict__ a_slot_ids, const int32_t* __r
     L = d[5];
     pos = d[6];
     w_first = d[7];
-    // A plan of another batch or of the other append mode: nothing of it is followed.
+    // A plan of another batch or of the other append mode: nothing of it is followed.  (Without partials, which the host
+    // allows where the workgroups are as many as the call's (sequence, kv head) pairs, no pair is split; a plan of fewer
+    // sequences may be as long and split them.)
     const bool fits = b < p.B && (uint32_t)g < (uint32_t)p.H_kv && (uint32_t)S <= (uint32_t)kQ8MaxSplits &&
                       (uint32_t)split < (uint32_t)S && w_first >= 0 && w_first <= a_n_wg - S &&
                       (uint32_t)d[4] < (uint32_t)p.n_slots && L >= 0 && L <= 16 * row_tiles &&
-                      pos == (kAppend ? L - 1 : -1);
-    if (!fits) {
-      set_err(p.err, CIE_ERRBIT_PLAN);
-      return;
-    }
+                      pos == (kAppend ? L - 1 : -1) && (S == 1 || a_n_wg > p.B * p.H_kv);
+    // Descriptors come in order: the last live one has to be the call's last pair's, else the plan lacks sequences or
+    // heads (theirs stay as they are).  (Past the last descriptor lie page ids, so the word may be read.)
+    const int next_b = d[kQ8PlanDesc];
+    const bool whole = (w + 1 < a_n_wg && next_b >= 0) || (b == p.B - 1 && g == p.H_kv - 1);
+    if (!fits || !whole) set_err(p.err, CIE_ERRBIT_PLAN);
+    if (!fits) return;
     load_q();
     if ((uint32_t)pages >= (uint32_t)p.n_pages) {
       set_err(p.err, CIE_ERRBIT_PAGE);

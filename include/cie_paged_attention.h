@@ -475,8 +475,11 @@ int cie_q8_read_tokens(void* k_out, void* v_out, const void* k_pool, const void*
  * plan: NULL, with n_splits splits per (sequence, kv head), or a step's
  * cie_paged_decode_plan (same append mode; lens and slot_ids are then not read), with
  * n_splits its n_workgroups; a plan that does not fit the call (made in the other
- * append mode, or for more sequences, heads, slots or pages) is not followed and
- * raises CIE_ERRBIT_PLAN, or CIE_ERRBIT_PAGE for its pages.  partials:
+ * append mode, for more sequences, heads, slots or pages, or split where the call has
+ * no partials) is not followed and raises CIE_ERRBIT_PLAN, or CIE_ERRBIT_PAGE for its
+ * pages; of a plan for fewer sequences or heads the others are left as they are, and
+ * CIE_ERRBIT_PLAN raised.  (Its lengths, page size and block table are the caller's to
+ * keep the same.)  partials:
  * cie_paged_decode_planned_partials_bytes(workgroups, H_q, H_kv, D), workgroups =
  * B * H_kv * n_splits or the plan's; counters: 2 * B * H_kv words; both may be NULL
  * where workgroups == B * H_kv.  The appending forms leave the same bytes and scales
