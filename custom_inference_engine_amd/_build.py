@@ -43,8 +43,8 @@ HIPCC_FLAGS = [
     "-Wall",
     "-Wno-unused-function",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-    # no kernel produces NaN (masked scores are -inf and the running max is
-    # always finite): lets max trees use v_max3 without canonicalizing moves
+    # no kernel of the 16-bit cache produces NaN (masked scores are -inf and the running
+    # max is always finite): lets max trees use v_max3 without canonicalizing moves
     "-fno-honor-nans",
     "-munsafe-fp-atomics",
     # kernel-argument preloading: a kernel's first 3 scalar arguments arrive
@@ -53,6 +53,12 @@ HIPCC_FLAGS = [
     # first loads need there, so they do not wait for the argument load.
     "-mllvm", "-amdgpu-kernarg-preload-count=3",
 ]
+
+
+def source_flags(src: str) -> list:
+    """The flags that ``src`` is compiled with: the 8-bit cache keeps NaNs, so its kernels honour them."""
+    honour = os.path.basename(src).startswith("q8_")
+    return [f for f in HIPCC_FLAGS if not (honour and f == "-fno-honor-nans")]
 
 
 def hipcc() -> str:
@@ -64,7 +70,7 @@ def hipcc() -> str:
 
 def _compile(src: str, verbose: bool, obj_dir: str = BUILD_DIR, defines: tuple = ()) -> str:
     obj = os.path.join(obj_dir, os.path.splitext(src)[0].replace("/", "_") + ".o")
-    cmd = [hipcc(), *HIPCC_FLAGS, *(f"-D{d}" for d in defines), "-I", INCLUDE, "-I", CSRC, "-c",
+    cmd = [hipcc(), *source_flags(src), *(f"-D{d}" for d in defines), "-I", INCLUDE, "-I", CSRC, "-c",
            os.path.join(CSRC, src), "-o", obj, "-Rpass-analysis=kernel-resource-usage"]
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -105,9 +105,26 @@ __device__ __forceinline__ void q8_v_operand(f16x8 (&va)[Geo<D>::NT], int half, 
   }
 }
 
-// A state that saw no key (its sum is +0; by its bits, since these files are built with -fno-honor-nans and a NaN among
-// the attended values has to stay one).
-__device__ __forceinline__ bool q8_no_key(float l) { return __float_as_uint(l) == 0; }
+// A state that saw no key (its sum is 0; a NaN among the attended values leaves a NaN, which is not).
+__device__ __forceinline__ bool q8_no_key(float l) { return l == 0.f; }
+
+// The larger of two, NaN if either is (v_maximum3_f32 takes operands as they are, where fmaxf's v_max_f32 needs each
+// made canonical first).  A NaN score is its column's whole result, so no maximum has to look past it.
+__device__ __forceinline__ float q8_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+// As col_max4 and wave_max, so.
+__device__ __forceinline__ float q8_col_max4(float x) {
+  float a, b;
+  swap16(x, a, b);
+  swap32(q8_max(a, b), a, b);
+  return q8_max(a, b);
+}
+__device__ __forceinline__ float q8_wave_max(float x) {
+  x = q8_max(x, row_ror<8>(x));
+  x = q8_max(x, row_ror<4>(x));
+  x = q8_max(x, row_ror<2>(x));
+  x = q8_max(x, row_ror<1>(x));
+  return q8_col_max4(x);
+}
 
 // One step of NP 32-key pairs of tiles for NCT column tiles.  k(i, ka) gives the K operands of tile i (< 2 NP), whose
 // first key is key0[i] (kNoKey: absent, all masked), v(p, va) the V^T operands of pair p once the weights are known;
@@ -159,13 +176,13 @@ __device__ __forceinline__ void q8_step(SoftmaxAcc<D, NCT>& st, K k, V v, M mean
   for (int c = 0; c < NCT; ++c) {
     xb[c] = s[c][0][0];
 #pragma unroll
-    for (int i = 0; i < 8 * NP; ++i) xb[c] = fmaxf(xb[c], s[c][i / 4][i % 4]);
+    for (int i = 1; i < 8 * NP; ++i) xb[c] = q8_max(xb[c], s[c][i / 4][i % 4]);
     need |= xb[c] > st.thr[c];
   }
   if (__any(need)) {  // rare: move the reference max
 #pragma unroll
     for (int c = 0; c < NCT; ++c) {
-      const float m_new = fmaxf(st.m[c], col_max4(xb[c]) * scale_log2);
+      const float m_new = q8_max(st.m[c], q8_col_max4(xb[c]) * scale_log2);
       const float alpha = fast_exp2(st.m[c] - m_new);
       st.m[c] = m_new;
       st.thr[c] = (m_new + kRescaleSlack) / scale_log2;

@@ -23,6 +23,8 @@
 // does not enter amax.
 #pragma once
 
+#include <type_traits>
+
 #include "cie_common.h"
 
 namespace cie {
@@ -35,8 +37,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // Fp16 magnitudes order as their bits.  q8_raw_max: the largest of eight (NaN the largest of all); where a wave's is
-// past the limit (rare) q8_limit8 first brings the values to it, and q8_mag8 leaves NaN out.  (Integer tests: the build
-// assumes no NaN in float ones.)
+// past the limit (rare) q8_limit8 first brings the values to it, and q8_mag8 leaves NaN out.
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t q8_raw_max(const f16x8& x, uint32_t m) {
   const u32x4 w = __builtin_bit_cast(u32x4, x);
@@ -113,7 +114,19 @@ __device__ __forceinline__ f16x8 q8_values8(uint32_t lo, uint32_t hi, float scal
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Over the wave's 64 lanes (every lane active).
-__device__ __forceinline__ uint32_t q8_wave_mag(uint32_t m) { return (uint32_t)wave_max((float)m); }
+// Over the wave's 64 lanes (every lane active): wave_max's steps on integers.
+__device__ __forceinline__ uint32_t q8_wave_mag(uint32_t m) {
+  auto ror = [](uint32_t x, auto n) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + decltype(n)::value, 0xf, 0xf, false);
+  };
+  m = max(m, ror(m, std::integral_constant<int, 8>{}));
+  m = max(m, ror(m, std::integral_constant<int, 4>{}));
+  m = max(m, ror(m, std::integral_constant<int, 2>{}));
+  m = max(m, ror(m, std::integral_constant<int, 1>{}));
+  const auto a = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  m = max((uint32_t)a[0], (uint32_t)a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+  return max((uint32_t)b[0], (uint32_t)b[1]);
+}
 
 }  // namespace cie

@@ -225,7 +225,7 @@ __device__ __forceinline__ void q8_merge(const Q8DecodeParams& p, int64_t row0, 
         for (int i = 0; i < kHeads; ++i) {
           const int hh = wave + i * kQ8Waves;
           if (hh < p.G) {  // uniform in the wave
-            const float M = wave_max(ms[i]);
+            const float M = q8_wave_max(ms[i]);
             const float a = fast_exp2(ms[i] - M);
             const float den = wave_sum(a * ls[i]);
             sm_w[hh * kQ8MaxSplits + lane] = q8_no_key(den) ? 0.f : a / den;  // no key at all: o = 0
@@ -285,7 +285,7 @@ __device__ __forceinline__ void q8_merge_few(const Q8DecodeParams& p, int64_t ro
       }
       float Mn = M;
 #pragma unroll
-      for (int u = 0; u < kFewLoads; ++u) Mn = fmaxf(Mn, ms[u]);
+      for (int u = 0; u < kFewLoads; ++u) Mn = q8_max(Mn, ms[u]);
       const float c = fast_exp2(M - Mn);
       num *= c;
       den *= c;
@@ -574,7 +574,7 @@ void q8_decode_kernel(const int64_t* __restrict__ a_slot_ids, const int32_t* __r
     const int d4 = it - h * D4;
     float M = kEmptyMax;
 #pragma unroll
-    for (int w = 0; w < W; ++w) M = fmaxf(M, sm_m[w][h]);
+    for (int w = 0; w < W; ++w) M = q8_max(M, sm_m[w][h]);
     f32x4 num = {0.f, 0.f, 0.f, 0.f};
     float den = 0.f;
 #pragma unroll

@@ -514,7 +514,7 @@ __device__ __forceinline__ void merge_weights(const Q8MixedParams& p, const Q8It
       }
       float Mn = M;
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) Mn = fmaxf(Mn, ms[i]);  // (the last chunk again past the end: no matter)
+      for (int i = 0; i < kGroup; ++i) Mn = q8_max(Mn, ms[i]);  // (the last chunk again past the end: no matter)
       den *= fast_exp2(M - Mn);
       M = Mn;
 #pragma unroll
@@ -532,7 +532,7 @@ __device__ __forceinline__ void merge_weights(const Q8MixedParams& p, const Q8It
   __syncthreads();
   if (j < tpc) {
     float top = kEmptyMax, sum = 0.f;
-    for (int i = 0; i < tpc; ++i) top = fmaxf(top, sm_m[i * cols + cc]);
+    for (int i = 0; i < tpc; ++i) top = q8_max(top, sm_m[i * cols + cc]);
     for (int i = 0; i < tpc; ++i) sum += fast_exp2(sm_m[i * cols + cc] - top) * sm_m[kMThreads + i * cols + cc];
     const float inv = q8_no_key(sum) ? 0.f : 1.f / sum;
     for (int c = j; c < n; c += tpc) {
@@ -584,7 +584,7 @@ __device__ __forceinline__ void merge_few(const Q8MixedParams& p, const Q8Item& 
     for (int i = 0; i < UN; ++i) {
       float Mn = M[i];
 #pragma unroll
-      for (int u = 0; u < CH; ++u) Mn = fmaxf(Mn, ms[u][i]);
+      for (int u = 0; u < CH; ++u) Mn = q8_max(Mn, ms[u][i]);
       const float a0 = fast_exp2(M[i] - Mn);
       num[i] *= a0;
       den[i] *= a0;
@@ -825,7 +825,7 @@ __device__ __forceinline__ void narrow_item(const Q8MixedParams& p, const Q8Item
     const int cc = u / D4, d4 = u - cc * D4;
     float M = kEmptyMax, den = 0.f;
 #pragma unroll
-    for (int w = 0; w < kMW; ++w) M = fmaxf(M, sm_m[w][cc]);
+    for (int w = 0; w < kMW; ++w) M = q8_max(M, sm_m[w][cc]);
     f32x4 num = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < kMW; ++w) {
