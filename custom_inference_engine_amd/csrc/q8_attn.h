@@ -84,6 +84,63 @@ __device__ __forceinline__ void q8_zero_rows(Q8Tile<D>& t, int n_rows, int grp) 
     if (4 * grp + e >= n_rows) t.v[e] = vrow_t{};
 }
 
+// NaN among V where keys are masked.  A masked key's weight is 0, but 0 times NaN is NaN, in every column of the tile.
+// So a tile that holds one takes part with zeros in its place, and leaves a map in LDS, [key][r16] a byte with a bit for
+// each of dims NT r16 + 0 .. NT - 1; q8_nan_fix then makes NaN what the columns that attend such a key hold.  (Rare.)
+constexpr int kQ8NanMap = kQ8Block * 16;  // bytes a tile
+
+// The NaNs of a tile's V words, as the top bits of their bytes.
+__device__ __forceinline__ uint32_t q8_nan_bytes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// Whether a V byte of the wave's tile is a NaN (uniform).
+template <int D>
+__device__ __forceinline__ bool q8_has_nan(const Q8Tile<D>& t) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+#pragma unroll
+    for (int w = 0; w < Q8Tile<D>::NJ; ++w) m |= q8_nan_bytes(t.v[e][w]);
+  return __any(m != 0);
+}
+
+template <int D>
+__device__ __forceinline__ void q8_nan_map(Q8Tile<D>& t, uint8_t* map, int r16, int grp) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int w = 0; w < Q8Tile<D>::NJ; ++w) {
+      const uint32_t m = q8_nan_bytes(t.v[e][w]) >> 7;
+      bits |= (m * 0x10204080u >> 28) << (4 * w);
+      t.v[e][w] &= ~(m * 0xffu);
+    }
+    map[(4 * grp + e) * 16 + r16] = (uint8_t)bits;
+  }
+}
+
+// hit[c]: byte r the bits of dims NT (4 grp + r) + nt that hold a NaN among the keys that column c attends, of the tile
+// of `map`, whose first key is key0.
+template <int NCT>
+__device__ __forceinline__ void q8_nan_hits(uint32_t (&hit)[NCT], const uint8_t* map, int key0, const int (&lim)[NCT],
+                                            int grp) {
+  for (int key = 0; key < kQ8Block; ++key) {
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(map + key * 16 + 4 * grp);
+#pragma unroll
+    for (int c = 0; c < NCT; ++c) hit[c] |= key0 + key < lim[c] ? word : 0u;
+  }
+}
+
+template <int D, int NCT>
+__device__ __forceinline__ void q8_nan_fix(SoftmaxAcc<D, NCT>& st, const uint32_t (&hit)[NCT]) {
+#pragma unroll
+  for (int c = 0; c < NCT; ++c)
+#pragma unroll
+    for (int nt = 0; nt < Geo<D>::NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        st.acc[c][nt][r] = hit[c] >> (8 * r + nt) & 1 ? __builtin_nanf("") : st.acc[c][nt][r];
+}
+
 // Keys 4 grp + 0 .. 3 of a tile as elements 4 half .. 4 half + 3 of the V^T operands (dim NT r16 + nt).
 template <int D>
 __device__ __forceinline__ void q8_v_operand(f16x8 (&va)[Geo<D>::NT], int half, const Q8Tile<D>& t, float scale) {
@@ -226,6 +283,27 @@ __device__ __forceinline__ void q8_attend(SoftmaxAcc<D, 1>& st, const Q8Tile<D> 
     q8_v_operand<D>(va, 1, t[2 * pr + 1], sc[2 * pr + 1][1]);
   };
   q8_step<D, 1, NT2 / 2, false>(st, k, v, [] {}, q, key0, lim, mask, scale_log2, grp);
+}
+
+// The same where several rows share the column tile, so that a key that one masks may be another's.  map: the wave's,
+// kQ8NanMap bytes a tile.
+template <int D, int NT2>
+__device__ __forceinline__ void q8_attend_rows(SoftmaxAcc<D, 1>& st, Q8Tile<D> (&t)[NT2], const f32x2 (&sc)[NT2],
+                                               const f16x8 (&q)[1][Geo<D>::KS], const int (&key0)[NT2],
+                                               const int (&lim)[1], bool mask, float scale_log2, uint8_t* map, int r16,
+                                               int grp) {
+  uint32_t hit[1] = {0};
+  if (mask) {
+#pragma unroll
+    for (int i = 0; i < NT2; ++i) {
+      if (!q8_has_nan<D>(t[i])) continue;
+      q8_nan_map<D>(t[i], map + i * kQ8NanMap, r16, grp);
+      __builtin_amdgcn_wave_barrier();
+      q8_nan_hits<1>(hit, map + i * kQ8NanMap, key0[i], lim, grp);
+    }
+  }
+  q8_attend<D, NT2>(st, t, sc, q, key0, lim, mask, scale_log2, grp);
+  if (__any(hit[0] != 0)) q8_nan_fix<D, 1>(st, hit);
 }
 
 // Where a wave's tiles live: kv head g of the pools and of the scales.

@@ -364,8 +364,10 @@ struct Q8Lds {
   static constexpr int kStage = kK + kV;
   static constexpr int kFold = kMW * 16 * (D / 4 + 1) + 2 * kMW * 16 / 4;
   static constexpr int kMerge = (kTileCols * kQ8MaxChunks + 2 * kMThreads) / 4 + kMThreads;
-  static constexpr int kSlots = 2 * kStage > kFold ? 2 * kStage : kFold;
+  static constexpr int kNans = 4 * kQ8NanMap / 16;  // NaN maps of a stage
+  static constexpr int kSlots = 2 * kStage + 2 * kNans;
   static_assert(kSlots >= kMerge, "the merge's scratch");
+  static_assert(kSlots >= kFold + kMW * kNans, "the fold, and NaN maps for the waves' steps of narrow items");
   static_assert(kMThreads >= kTileCols && kTileCols * (D / 4) <= 16 * kMThreads, "the merge's threads");
 };
 
@@ -646,8 +648,8 @@ __device__ __forceinline__ void load_col_q(f16x8 (&q)[Geo<D>::KS], int& lim, con
 
 // Wide item, NA column tiles in this wave (0: it only loads).
 template <int D, int NA>
-__device__ __forceinline__ void wide_item(const Q8MixedParams& p, const Q8Item& it, int cols, f32x4* lds, int wave,
-                                          int lane) {
+__device__ __forceinline__ void wide_item(const Q8MixedParams& p, const Q8Item& it, int cols, f32x4* lds,
+                                          uint32_t (*sm_nan)[kMW], int wave, int lane) {
   constexpr int KS = Geo<D>::KS, NT = Geo<D>::NT;
   constexpr int NC = NA > 0 ? NA : 1;
   const int r16 = lane & 15, grp = lane >> 4;
@@ -673,11 +675,21 @@ __device__ __forceinline__ void wide_item(const Q8MixedParams& p, const Q8Item& 
   const int n_stages = uniform((it.t1 - it.t0 + 3) >> 2);
   Q8Tile<D> raw;
   f16x8* const buf = reinterpret_cast<f16x8*>(lds);
+  // Stages of which some row masks a key; their tiles' NaN maps.
+  auto masked = [&](int sg) { return 16 * (it.t0 + 4 * (sg + 1)) > it.pos0 + 1; };
+  auto nan_map = [&](int sg, int i) {
+    return reinterpret_cast<uint8_t*>(lds + 2 * Q8Lds<D>::kStage + (sg & 1) * Q8Lds<D>::kNans) + i * kQ8NanMap;
+  };
   // this wave's tile of stage sg (its bytes in raw), converted into operand slots; then stage sg + 1's loads
-  auto stage = [&](int sg) {
+  auto stage = [&](int sg, bool look) {
     f16x8* const kbuf = buf + (sg & 1) * Q8Lds<D>::kStage;
     f16x8* const vbuf = kbuf + Q8Lds<D>::kK;
     const int k = sg & (kWave - 1);
+    if (look && masked(sg)) {
+      const bool nan = q8_has_nan<D>(raw);
+      if (nan) q8_nan_map<D>(raw, nan_map(sg, wave), r16, grp);
+      if (lane == 0) sm_nan[sg & 1][wave] = nan;
+    }
     const float ks = tiles.scale(0, k), vs = tiles.scale(1, k);
     f16x8 ko[KS];
     q8_k_operand<D>(ko, raw, ks);
@@ -693,9 +705,10 @@ __device__ __forceinline__ void wide_item(const Q8MixedParams& p, const Q8Item& 
     if (next == 0) tiles.gather(sg + 1);
     tiles.template load<0>(raw, sg + 1 - next, next, key_end, lo);  // (past the last: no rows)
   };
-  tiles.template load<0>(raw, 0, 0, key_end, lo);
-  stage(0);
-  for (int sg = 0; sg < n_stages; ++sg) {
+  // stage sg; kLook: it, or the next one, holds masked keys (else no code for them: 4 x 2,048 rows, 14 / 2 heads, D =
+  // 64, 48.0 us, 48.3 with it in every stage; 47.1 without a look at NaNs)
+  auto step = [&](int sg, auto look) {
+    constexpr bool kLook = decltype(look)::value;
     // stage sg is written, and stage sg - 1's buffer free: the next one is converted while sg's S MFMAs run
     __syncthreads();
     const f16x8* const kbuf = buf + (sg & 1) * Q8Lds<D>::kStage;
@@ -712,12 +725,26 @@ __device__ __forceinline__ void wide_item(const Q8MixedParams& p, const Q8Item& 
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) va[nt] = vbuf[(pr * NT + nt) * kWave + lane];
       };
-      q8_step<D, NC, 2, true>(st, k, v, [&] { stage(sg + 1); }, q, key0, lim, key0[3] + 16 > mask_from, p.scale_log2,
-                              grp);
+      q8_step<D, NC, 2, true>(st, k, v, [&] { stage(sg + 1, kLook); }, q, key0, lim,
+                              kLook && key0[3] + 16 > mask_from, p.scale_log2, grp);
+      if (kLook && masked(sg)) {
+        uint32_t hit[NC] = {};
+        for (int i = 0; i < 4; ++i)
+          if (uniform((int)sm_nan[sg & 1][i])) q8_nan_hits<NC>(hit, nan_map(sg, i), key0[0] + 16 * i, lim, grp);
+        bool any = false;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) any |= hit[c] != 0;
+        if (__any(any)) q8_nan_fix<D, NC>(st, hit);
+      }
     } else {
-      stage(sg + 1);
+      stage(sg + 1, kLook);
     }
-  }
+  };
+  tiles.template load<0>(raw, 0, 0, key_end, lo);
+  stage(0, true);
+  int sg = 0;
+  for (; sg < n_stages && !masked(sg + 1); ++sg) step(sg, std::false_type{});
+  for (; sg < n_stages; ++sg) step(sg, std::true_type{});
   __syncthreads();  // (the merge takes the buffers)
   if constexpr (NA > 0) {
     const __amdgpu_buffer_rsrc_t racc =
@@ -769,6 +796,7 @@ __device__ __forceinline__ void narrow_item(const Q8MixedParams& p, const Q8Item
   f16x8 q[1][KS];
   int lim[1];
   load_col_q<D>(q[0], lim[0], p, it, cols, r16, grp);
+  uint8_t* const map = reinterpret_cast<uint8_t*>(lds + Q8Lds<D>::kFold) + wave * NS * kQ8NanMap;
   const int mask_from = it.pos0 + 1;  // the first row's keys
   SoftmaxAcc<D, 1> st;
   st.init();
@@ -798,7 +826,8 @@ __device__ __forceinline__ void narrow_item(const Q8MixedParams& p, const Q8Item
             key0[i] = k < n_chunk ? 16 * (tiles.t0 + 4 * (c0 + kk)) : kNoKey;
             sc[i] = f32x2{tiles.scale(0, kk), tiles.scale(1, kk)};
           }
-          q8_attend<D, NS>(st, ring[u], sc, q, key0, lim, key0[NS - 1] + 16 > mask_from, p.scale_log2, grp);
+          q8_attend_rows<D, NS>(st, ring[u], sc, q, key0, lim, key0[NS - 1] + 16 > mask_from, p.scale_log2, map, r16,
+                               grp);
         }
       }
     }
@@ -853,6 +882,7 @@ template <int D>
 __global__ __launch_bounds__(kMThreads) __attribute__((amdgpu_waves_per_eu(2)))
 void q8_mixed_kernel(Q8MixedParams p) {
   __shared__ f32x4 lds[Q8Lds<D>::kSlots];
+  __shared__ uint32_t sm_nan[2][kMW];  // whether a stage's V tile holds a NaN (stages of masked keys)
   __shared__ int sm_last;
   const int32_t* const head = p.plan;
   const Q8Item it = reinterpret_cast<const Q8Item*>(head + kHeadWords)[blockIdx.x];  // (read with the head)
@@ -873,11 +903,11 @@ void q8_mixed_kernel(Q8MixedParams p) {
     const int n_ct = (cols + 15) >> 4;
     const int na = n_ct > wave ? (n_ct - wave + kMW - 1) / kMW : 0;  // column tiles wave, wave + 4, ..
     if (na == 2)
-      wide_item<D, 2>(p, it, cols, lds, wave, lane);
+      wide_item<D, 2>(p, it, cols, lds, sm_nan, wave, lane);
     else if (na == 1)
-      wide_item<D, 1>(p, it, cols, lds, wave, lane);
+      wide_item<D, 1>(p, it, cols, lds, sm_nan, wave, lane);
     else
-      wide_item<D, 0>(p, it, cols, lds, wave, lane);
+      wide_item<D, 0>(p, it, cols, lds, sm_nan, wave, lane);
   }
   if (it.n_chunks == 1) return;
   int32_t* const arrival = p.counters + it.ctr;

@@ -525,6 +525,7 @@ int cie_q8_decode_qkv_rope(void* o, const void* qkv, int64_t qkv_row_stride,
  *                       D, page_size, block table) writes nothing and raises
  *                       CIE_ERRBIT_PLAN.  Where cu_seqlens decreases anywhere,
  *                       nothing of the batch is computed (CIE_ERRBIT_PAGE).
+ * A NaN in a key's K or V row reaches the rows that attend the key, and no others.
  * partials: cie_q8_mixed_partials_bytes bytes, 16-byte aligned; counters:
  * cie_q8_mixed_counters() words, zero before the call and after it.
  * B <= 2048, H_q / H_kv <= 16, total_T <= 2^24.

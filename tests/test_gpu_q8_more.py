@@ -6,7 +6,7 @@ import custom_inference_engine_amd as cie
 from oracle import q8_cache as ref
 from tests.gpu_helpers import DEV, err_word, note
 from tests.q8_helpers import Case
-from tests.test_gpu_q8 import PLAN, check_attention, decode_seqs
+from tests.test_gpu_q8 import PLAN, append_tokens, check_attention, decode_seqs, mixed_seqs
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,58 @@ def test_decode_plan_of_fewer_sequences(native_lib, append, d, h_q, h_kv):
     with pytest.raises(RuntimeError, match="invalid argument"):  # fewer workgroups than pairs
         call(8, plan(2, 1))
     assert not cie.attn.core.split_counters(torch.device(DEV), 1).any()
+
+
+NANS = [  # (shape, positions of the last sequence that hold a NaN in V, and in K)
+    (dict(prior=[0], new=[128], h_q=4, h_kv=4), [100], []),             # one head a group: 128 rows a tile
+    (dict(prior=[0], new=[70], h_q=4, h_kv=4, d=128), [0, 3, 69], [68]),
+    (dict(prior=[37], new=[100]), [40, 41, 57, 136], [129]),            # 18 rows a tile
+    (dict(prior=[0, 30], new=[60, 90], d=128, h_q=32, h_kv=8, page=32), [33, 118, 119], []),
+    (dict(prior=[5], new=[14], h_q=2, h_kv=2), [12, 18], [9]),          # narrow items of several rows
+    (dict(prior=[21], new=[2]), [22], []),
+    (dict(prior=[300], new=[4], d=128, h_q=32, h_kv=8), [301, 303], [302]),
+    (dict(prior=[6000], new=[64]), [5, 6031], [6050]),                  # split over the keys
+    (dict(prior=[9000], new=[2], h_q=4, h_kv=1), [9001], []),
+    (dict(prior=[0] * 3, new=[1500] * 3, h_q=16, h_kv=4), [700, 1499], []),  # whole tiles
+    (dict(prior=[6000], new=[700], h_q=16, h_kv=8, d=128), [6350, 6351], []),
+]
+
+
+@pytest.mark.parametrize("shape,in_v,in_k", NANS, ids=lambda x: f"{x['prior']}+{x['new']}d{x.get('d', 64)}" if isinstance(x, dict) else str(x))
+def test_mixed_nan_reaches_the_rows_that_attend_it(native_lib, shape, in_v, in_k):
+    """A NaN in V is NaN in that dim of its head's rows from its own on, one in K in every dim; earlier rows, which mask
+    the key, are as if it were any number."""
+    note(f"q8 mixed nan {shape} {in_v} {in_k}")
+    c = Case(**shape, seed=31).write_history()
+    last, g = c.B - 1, torch.Generator().manual_seed(32)
+    t0, prior = int(c.cu[last]), c.prior[last]
+    held = {p: (int(torch.randint(c.h_kv, (1,), generator=g)), int(torch.randint(c.d, (1,), generator=g)))
+            for p in in_v + in_k}
+    nan = torch.tensor([float("nan"), -float("nan")]).half()
+    nan[1] = torch.tensor([-512], dtype=torch.int16).view(torch.float16)[0]  # 0xfe00: negative
+    for x, where in ((c.v_new, in_v), (c.k_new, in_k)):
+        for i, p in enumerate(where):
+            h, dim = held[p]
+            if p >= prior:
+                x[0, t0 + p - prior, h, dim] = nan[i % 2]
+            else:  # (in the rows held before)
+                pages, offs = c.at(last, p, 1)
+                (c.v if x is c.v_new else c.k).view(torch.uint8)[int(pages), h, int(offs), dim] = 0x7f + 0x80 * (i % 2)
+    append_tokens(c)
+    want = torch.zeros(c.T, c.h_q, c.d, dtype=torch.bool)  # NaN
+    group = c.h_q // c.h_kv
+    for where, whole in ((in_v, False), (in_k, True)):
+        for p in where:
+            h, dim = held[p]
+            rows = slice(max(t0, t0 + p - prior), c.T)
+            want[rows, h * group:(h + 1) * group, slice(None) if whole else dim] = True
+    kc, vc = c.oracles()
+    for x in (kc, vc):
+        x.vals.nan_to_num_(0.0)
+    seen = ref.attend(c.q[0], kc, vc, mixed_seqs(c), c.table)
+    args = (c.q.to(DEV), c.k, c.v, c.scales, max(c.new), *c.dev("cu", "kv_lens", "slots", "table"))
+    for _ in range(2):
+        o = cie.mixed_gqa_attention_q8(*args)[0].cpu()
+        assert torch.equal(o.isnan(), want)
+        check_attention(o.masked_fill(want, 0.0), tuple(x.masked_fill(want, 0.0) if x.shape == want.shape else x for x in seen),
+                        max(p + n for p, n in zip(c.prior, c.new)))
