@@ -149,8 +149,10 @@ class ModuleExecutor:
         self.mixed_modules = {}
         piecewise = [t for t in self.token_counts if piecewise_above is not None and t > piecewise_above]
         if graph_mixed and piecewise:
+            # (attention over an 8-bit cache answers in the type of its queries, float16)
+            dtype = kv_cache.dtype if getattr(kv_cache, "scales", None) is None else torch.float16
             self.buffer = torch.zeros((1, max(piecewise), kv_cache.num_q_heads, kv_cache.head_dim),
-                                      dtype=model.dtype, device=kv_cache.device)
+                                      dtype=dtype, device=kv_cache.device)
         if graph_mixed:
             for t in sorted(self.token_counts, reverse=True):
                 if t in piecewise:

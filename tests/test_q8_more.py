@@ -7,6 +7,8 @@ from transformers import Qwen2Config
 
 import custom_inference_engine_amd as cie
 from custom_inference_engine_amd import _build
+from custom_inference_engine_amd.scheduler import decode_module, mixed_module
+from custom_inference_engine_amd.scheduler.scheduler import ModuleExecutor
 
 
 @pytest.mark.parametrize("src", _build.SOURCES)
@@ -22,3 +24,23 @@ def test_kernels_that_keep_nans_are_built_to(src, tmp_path, monkeypatch):
     _build._compile(src, False, str(tmp_path))
     assert ("-fno-honor-nans" in seen[0]) != src.startswith("q8_")
     assert "-ffast-math" not in seen[0] and "-packed-fp32-ops" in seen[0]
+
+
+def config():
+    return Qwen2Config(hidden_size=896, num_attention_heads=14, num_key_value_heads=2, intermediate_size=256,
+                       num_hidden_layers=2, vocab_size=128, max_position_embeddings=512)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float8_e4m3fn], ids=str)
+def test_piecewise_buffer_needs_no_dtype_of_the_model(dtype, monkeypatch):
+    """The attention outputs' buffer has the cache's type, float16 beside an 8-bit one; the model's object, which need
+    not have one, is not asked."""
+    for module, name in ((decode_module, "DecodeModule"), (mixed_module, "FullMixedModule"),
+                         (mixed_module, "PiecewiseMixedModule")):
+        monkeypatch.setattr(module, name, lambda *args, **kw: types.SimpleNamespace(**kw))
+    kv = cie.KVStorage(config(), max_cache_len=64, page_size=16, n_slots=3, device="cpu", dtype=dtype)
+    model = object()
+    executor = ModuleExecutor(model, kv, [1, 2], [16, 128, 160], pool=object(), piecewise_above=128)
+    assert executor.buffer.dtype == (torch.float16 if dtype == torch.float8_e4m3fn else dtype)
+    assert executor.buffer.shape == (1, 160, 14, 64) and executor.mixed_modules[160].buffer is executor.buffer
+    assert not hasattr(executor.mixed_modules[128], "buffer")
