@@ -202,11 +202,15 @@ class KVStorage:
 
     def read_tokens(self, layer_num: int, pages: torch.Tensor, offsets: torch.Tensor):
         """The held rows ``(pages[t], :, offsets[t])``: K and V, each (1, T, H_kv, D), as
-        ``mixed_update`` takes them (what an 8-bit cache holds comes back as float16)."""
+        ``mixed_update`` takes them (what an 8-bit cache holds comes back as float16).
+        A row outside the pool reads as zeros."""
         if self.scales is not None:
             return quant.kv_read_tokens_q8(self.keys[layer_num], self.values[layer_num], self.scales[layer_num],
                                            pages, offsets)
-        return tuple(pool[layer_num][pages, :, offsets][None] for pool in (self.keys, self.values))
+        held = (pages >= 0) & (pages < self.n_pages) & (offsets >= 0) & (offsets < self.page_size)
+        pages, offsets = torch.where(held, pages, 0), torch.where(held, offsets, 0)
+        return tuple(torch.where(held[:, None, None], pool[layer_num][pages, :, offsets], 0)[None]
+                     for pool in (self.keys, self.values))
 
     # lens[unused_idx] = 0 as a device kernel (a 1-element multiply), not a
     # host scalar copy, so a decode step that contains it can be graph-captured

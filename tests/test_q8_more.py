@@ -44,3 +44,25 @@ def test_piecewise_buffer_needs_no_dtype_of_the_model(dtype, monkeypatch):
     assert executor.buffer.dtype == (torch.float16 if dtype == torch.float8_e4m3fn else dtype)
     assert executor.buffer.shape == (1, 160, 14, 64) and executor.mixed_modules[160].buffer is executor.buffer
     assert not hasattr(executor.mixed_modules[128], "buffer")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("index", [torch.int64, torch.int32], ids=str)
+def test_read_tokens_of_a_16_bit_cache(dtype, index):
+    """Rows in any order, as mixed_update takes them; what lies outside the pool reads as zeros, as from an 8-bit cache."""
+    kv = cie.KVStorage(config(), max_cache_len=64, page_size=16, n_slots=3, device="cpu", dtype=dtype)
+    g = torch.Generator().manual_seed(0)
+    for pool in (kv.keys[1], kv.values[1]):
+        pool.copy_(torch.randn(pool.shape, generator=g))
+    kv.keys[1][0, :, 0] = float("nan")  # (what a clamped index would read)
+    n = kv.n_pages
+    pages = torch.tensor([3, 0, n, -1, 2, 1, 1, 10 ** 6], dtype=index)
+    offs = torch.tensor([15, 7, 0, 0, 0, 16, -1, 3], dtype=index)
+    held = [True, True, False, False, True, False, False, False]
+    for got, pool in zip(kv.read_tokens(1, pages, offs), (kv.keys[1], kv.values[1])):
+        assert got.shape == (1, 8, 2, 64) and got.dtype == dtype
+        for t, ok in enumerate(held):
+            want = pool[int(pages[t]), :, int(offs[t])] if ok else torch.zeros(2, 64, dtype=dtype)
+            assert torch.equal(got[0, t], want)
+    none = kv.read_tokens(0, pages[:0], offs[:0])
+    assert [x.shape for x in none] == [(1, 0, 2, 64)] * 2
