@@ -14,7 +14,8 @@
 // included) and lose nothing after the cache's own rounding.  A block whose scale
 // grows by 2^n has its rows rounded again; their bytes change exactly (the
 // exponent moves) unless they fall under e4m3's smallest normal, 2^-6: then by at
-// most half of 2^-9.
+// most half of 2^-9, in the new scale, each time.  Over all growths that is less than
+// 2^-9 of the last scale (the halves of steps that double at least: 1/2 + 1/4 + ..).
 //
 // e of a block is the least with amax <= 448 * 2^e, over the rows written since
 // its first row was: writing a block's row 0 starts it anew (its page may have

@@ -9,10 +9,13 @@ V's, and a held value is ``pool.float() * scale``.
 A scale is a power of two, 2^e with -15 <= e <= 8: the least with amax <= 448 * 2^e
 over the rows written since the block's first row was.  Writing a block's row 0
 starts it anew; writing another row keeps the others, which are rounded again where
-the scale grows.  Rows are rounded to nearest even from their float16 inputs (the
-error is at most 2^-4 of a value, or half of 2^-9 * scale under 2^-6 * scale);
-values beyond +-61440, infinities among them, are held as that, NaN as NaN.  So a
-held value is always a float16 value, and ``kv_read_tokens_q8`` and the attention of
+the scale grows.  Rows are rounded to nearest even from their float16 inputs: off by
+2^-4 of the value, or by half a step of 2^-9 * scale under 2^-6 * scale, at most.  Each
+growth may round what lies under 2^-6 of the new scale once more, by half of its step,
+and as the steps double at least these add up to less than a step of the last scale:
+after any growths a value x is held to 2^-4 |x| + 2^-9 * scale, and values far under
+the block's largest may be held as 0.  Values beyond +-61440, infinities among them,
+are held as that, NaN as NaN.  So a held value is always a float16 value, and ``kv_read_tokens_q8`` and the attention of
 ``attn/quant.py`` use it exactly.
 """
 from __future__ import annotations

@@ -9,6 +9,7 @@ import custom_inference_engine_amd as cie
 from custom_inference_engine_amd import _build
 from custom_inference_engine_amd.scheduler import decode_module, mixed_module
 from custom_inference_engine_amd.scheduler.scheduler import ModuleExecutor
+from oracle import q8_cache as ref
 
 
 @pytest.mark.parametrize("src", _build.SOURCES)
@@ -66,3 +67,34 @@ def test_read_tokens_of_a_16_bit_cache(dtype, index):
             assert torch.equal(got[0, t], want)
     none = kv.read_tokens(0, pages[:0], offs[:0])
     assert [x.shape for x in none] == [(1, 0, 2, 64)] * 2
+
+
+def test_held_values_stay_within_the_stated_error():
+    """Rows that come one at a time, each of which may make the block grow: 2^-4 |x| + 2^-9 * scale, and half of the
+    second where a row has seen no growth.  Half of it alone does not hold after growths."""
+    g = torch.Generator().manual_seed(4)
+    past_half = 0
+    for case in range(200):
+        c = ref.Q8Cache(torch.zeros(1, 1, 16, 64).double(), torch.zeros(1, 1, 1).double())
+        grow = torch.cumsum(torch.randint(0, 3, (16,), generator=g), 0)
+        x = (torch.randn(16, 1, 64, generator=g) * 2.0 ** (grow - 12.0 - 2 * torch.rand(16, generator=g))[:, None, None])
+        x = (x * 2.0 ** (-9.0 * torch.rand(16, 1, 64, generator=g))).half()
+        for t in range(16):
+            before = float(c.exps[0, 0, 0])
+            c.append(x[t:t + 1], [0], [t])
+            scale = 2.0 ** float(c.exps[0, 0, 0])
+            want = x[:t + 1, 0].double()
+            off = (c.values()[0, 0, :t + 1] - want).abs()
+            assert (off <= want.abs() * 2.0 ** -4 + scale * 2.0 ** -9).all()
+            assert (off[t] <= torch.maximum(want[t].abs() * 2.0 ** -4, torch.tensor(scale * 2.0 ** -10))).all()
+            assert t == 0 or c.exps[0, 0, 0] >= before
+            past_half += int((off > torch.maximum(want.abs() * 2.0 ** -4, torch.tensor(scale * 2.0 ** -10))).sum())
+    assert past_half > 0
+    # 2.51 steps are held as 3; in steps twice as large, 1.5, as 2: off by 0.745 of such a step
+    c = ref.Q8Cache(torch.zeros(1, 1, 16, 1).double(), torch.zeros(1, 1, 1).double())
+    x = 2.51 * 2.0 ** -9
+    c.append(torch.tensor([448.0, x]).view(2, 1, 1), [0, 0], [0, 1])
+    assert c.values()[0, 0, 1, 0] == 3 * 2.0 ** -9
+    c.append(torch.tensor([800.0]).view(1, 1, 1), [0], [2])
+    assert c.exps[0, 0, 0] == 1 and c.values()[0, 0, 1, 0] == 2 * 2.0 ** -8
+    assert abs(2 * 2.0 ** -8 - x) > 0.74 * 2.0 ** -8
