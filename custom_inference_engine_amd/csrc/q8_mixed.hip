@@ -293,7 +293,7 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
     ctr = ctr_at + before[1];
     rows_at += all[0];
     ctr_at += all[1];
-    if ((int64_t)pbase + mine[0] > p.part_cap) n = 1;  // its partial rows would end past the buffer: unsplit
+    if ((int64_t)pbase + mine[0] > p.part_cap) n = 1;  // (a guard: partial rows past the buffer; q8_part_rows holds all)
     if (n > 0) {
       const int len = (kt + n - 1) / n;  // an item's key tiles, in a wide item's
       level = kPlanLevels - 1 - min(kPlanLevels - 1, (int)((int64_t)len * kPlanLevels / (share + 1)));
@@ -312,7 +312,7 @@ __global__ __launch_bounds__(kPlanThreadsM) void q8_mixed_plan_kernel(Q8PlanPara
     sm_level[tid] = inc - v;
     const int n_items = __builtin_amdgcn_readlane(inc, kWave - 1);
     if (tid == 0) {
-      const bool fits = n_items <= p.plan_cap;
+      const bool fits = n_items <= p.plan_cap;  // (a guard: q8_plan_items holds all)
       if (!fits) set_err(p.err, CIE_ERRBIT_PLAN);
       sm_fits = fits;
       p.plan[0] = fits ? n_items : 0;
@@ -917,7 +917,9 @@ void q8_mixed_kernel(Q8MixedParams p) {
 }
 
 // Items a plan can hold: one a query tile and kv head, and kQ8Slots more from splitting.  A launch of half tiles has W <=
-// kSmallWork * kQ8Slots, a whole tile counts 2 at least in W, and a sequence has at most twice as many half ones.
+// kSmallWork * kQ8Slots, and a sequence no more half tiles than its part of W: with n whole ones of R rows that part is
+// 2 n + R n (n + 1) / 32 + 1 at least, 2.5 n + 1 as R >= 8, and its half ones are 2.25 n + 1 at most (13 and 14 heads a
+// group: 9 rows a whole tile, 4 a half one).
 static int64_t q8_plan_items(int64_t B, int64_t total_T, int64_t H_q, int64_t H_kv) {
   const int64_t R = kTileCols / (H_q / H_kv), half = kTileCols / 2 / (H_q / H_kv);
   const int64_t whole = H_kv * (total_T / R + B), small = H_kv * (total_T / half + B);

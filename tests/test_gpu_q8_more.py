@@ -112,3 +112,70 @@ def test_mixed_nan_reaches_the_rows_that_attend_it(native_lib, shape, in_v, in_k
         assert torch.equal(o.isnan(), want)
         check_attention(o.masked_fill(want, 0.0), tuple(x.masked_fill(want, 0.0) if x.shape == want.shape else x for x in seen),
                         max(p + n for p, n in zip(c.prior, c.new)))
+
+
+def plan_items(c, plan):
+    """A mixed plan's items: (row, rows, g, slot, pos, first and last key tile, chunk, chunks) each."""
+    words = plan.cpu()
+    return [tuple(words[12 + 12 * i:21 + 12 * i].tolist()) for i in range(int(words[0]))]
+
+
+MERGES = [  # (shape, columns times D / 4 of the split tile, its chunks): every form of the merge, and the cap on chunks
+    (dict(prior=[9000], new=[3]), (257, 512), (9, 48)),                                # two pieces a thread, D = 64
+    (dict(prior=[9000], new=[2], d=128, h_q=8, h_kv=1), (257, 512), (9, 48)),          # the same at D = 128
+    (dict(prior=[9000], new=[2], d=128, h_q=14, h_kv=2), (257, 512), (9, 48)),
+    (dict(prior=[3000], new=[3], d=128, h_q=8, h_kv=1), (257, 1024), (2, 8)),          # four, chunks a few
+    (dict(prior=[3000], new=[5], d=64), (257, 1024), (2, 8)),
+    (dict(prior=[2300], new=[1], d=128, h_q=32, h_kv=8), (1, 256), (2, 16)),           # one
+    (dict(prior=[12000], new=[1], d=128, h_q=16, h_kv=2), (1, 256), (17, 48)),
+    (dict(prior=[9000], new=[40], d=128, h_q=4, h_kv=1), (513, 2048), (9, 48)),        # eight
+    (dict(prior=[65500], new=[1], h_q=4, h_kv=1), (1, 256), (48, 48)),                 # the cap, a narrow item's
+    (dict(prior=[40000], new=[20], h_q=4, h_kv=1), (513, 2048), (48, 48)),             # and a wide one's
+    (dict(prior=[30001], new=[11], h_q=7, h_kv=1, d=128), (513, 2048), (48, 48)),      # (9 rows a half tile: 63 x 32)
+    (dict(prior=[20000], new=[360], h_q=7, h_kv=1, d=128), (2049, 4096), (9, 48)),     # sixteen: 18 rows a whole one
+    (dict(prior=[20000], new=[360], h_q=7, h_kv=1), (1025, 2048), (9, 48)),
+]
+
+
+@pytest.mark.parametrize("shape,units,chunks", MERGES, ids=lambda x: f"{x['prior']}+{x['new']}d{x.get('d', 64)}" if isinstance(x, dict) else str(x))
+def test_mixed_merge_forms(native_lib, shape, units, chunks):
+    note(f"q8 mixed merge {shape}")
+    c = Case(**shape, seed=33).write_history()
+    append_tokens(c)
+    want = ref.attend(c.q[0], *c.oracles(), mixed_seqs(c), c.table)
+    args = (c.q.to(DEV), c.k, c.v, c.scales, max(c.new), *c.dev("cu", "kv_lens", "slots", "table"))
+    err = err_word()
+    plan = cie.mixed_plan_q8(c.k, *c.dev("cu", "kv_lens", "slots", "table"), max(c.new), c.T, c.h_q, err=err)
+    items = plan_items(c, plan)
+    kt = -(-(c.prior[0] + c.new[0]) // 16)
+    split = [i for i in items if i[8] > 1]
+    assert split and max(abs(i[1]) for i in split) * (c.h_q // c.h_kv) * c.d // 4 in range(units[0], units[1] + 1)
+    assert chunks[0] <= max(i[8] for i in items) <= chunks[1]
+    for g in range(c.h_kv):  # the chunks of every tile cover its keys once
+        for row in {i[0] for i in items}:
+            tile = sorted(i for i in items if i[2] == g and i[0] == row)
+            at = 0
+            for i in sorted(tile, key=lambda i: i[7]):
+                assert i[5] == at and i[6] >= at
+                at = i[6]
+            assert at == -(-(tile[0][4] + abs(tile[0][1])) // 16) <= kt and len(tile) == tile[0][8]
+    o = cie.mixed_gqa_attention_q8(*args, plan=plan, err=err)
+    check_attention(o[0], want, c.prior[0] + c.new[0])
+    assert int(err) == 0 and torch.equal(cie.mixed_gqa_attention_q8(*args, plan=plan), o)
+    assert not cie.attn.core.split_counters(torch.device(DEV), 1).any()
+
+
+def test_mixed_ranges_that_run_backwards_leave_the_plan_empty(native_lib):
+    """cu_seqlens that falls anywhere: no item, the page bit alone, and no row of the outputs computed."""
+    note("q8 mixed backwards")
+    c = Case(prior=[20, 30], new=[9, 4], seed=17).write_history()
+    append_tokens(c)
+    many = torch.tensor([0, c.T] * 200 + [0], device=DEV)
+    B = many.shape[0] - 1
+    lens, slots = torch.zeros(B, dtype=torch.int64, device=DEV), torch.ones(B, dtype=torch.int64, device=DEV)
+    err = err_word()
+    plan = cie.mixed_plan_q8(c.k, many, lens, slots, c.table.to(DEV), c.T, c.T, c.h_q, err=err)
+    assert int(err) == 1 and int(plan[0]) == 0
+    cie.mixed_gqa_attention_q8(c.q.to(DEV), c.k, c.v, c.scales, c.T, many, lens, slots, c.table.to(DEV), plan=plan, err=err)
+    torch.cuda.synchronize()
+    assert int(err) == 1

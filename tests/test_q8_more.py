@@ -1,5 +1,8 @@
 """The 8-bit cache without a GPU, further cases: how it is built, and what its paths refuse and accept."""
+import os
+import re
 import types
+from collections import Counter
 
 import pytest
 import torch
@@ -10,6 +13,7 @@ from custom_inference_engine_amd import _build
 from custom_inference_engine_amd.scheduler import decode_module, mixed_module
 from custom_inference_engine_amd.scheduler.scheduler import ModuleExecutor
 from oracle import q8_cache as ref
+from tests import test_asm_order as asm
 
 
 @pytest.mark.parametrize("src", _build.SOURCES)
@@ -98,3 +102,103 @@ def test_held_values_stay_within_the_stated_error():
     c.append(torch.tensor([800.0]).view(1, 1, 1), [0], [2])
     assert c.exps[0, 0, 0] == 1 and c.values()[0, 0, 1, 0] == 2 * 2.0 ** -8
     assert abs(2 * 2.0 ** -8 - x) > 0.74 * 2.0 ** -8
+
+
+# ---- a mixed plan's capacity: the plan kernel's arithmetic, over every group size ----
+
+SLOTS, COLS, MIN_SHARE, MAX_CHUNKS, SMALL = 256, 128, 32, 48, 80
+
+
+def plan_of(lens, kv_lens, G, h_kv):
+    """(items, partial rows, arrival words, columns of a wide tile) of the plan kernel for these sequences."""
+    def cut(L, cols):
+        narrow = L * G <= 16
+        R = L if narrow else cols // G
+        return narrow, R, -(-L // R)
+
+    seqs = [(L, c, times) for (L, c), times in Counter(zip(lens, kv_lens)).items() if L]
+    total = []
+    for cols in (COLS, COLS // 2):
+        w = 0.0
+        for L, c, times in seqs:
+            narrow, R, n = cut(L, cols)
+            w += times * (((c + L) >> 6) + 1.0 if narrow else n * ((c >> 4) + 2) + R * n * (n + 1) / 32 + 1)
+        total.append(w)
+    per = 1.001 * h_kv / SLOTS
+    small = total[0] * per <= SMALL
+    cols, want = (COLS // 2, total[1]) if small else (COLS, total[0])
+    want = int(min(2.0 ** 26, want * per + 1))
+    items = rows_out = words = 0
+    for L, c, times in seqs:
+        narrow, R, n_rt = cut(L, cols)
+        share = (max(MIN_SHARE, 4 * want if narrow else want) + 3) & ~3
+        for r in range(n_rt):
+            rows = min(R, L - r * R)
+            n = min(MAX_CHUNKS, -(-((c + r * R + rows + 15) >> 4) // share))
+            items += times * n * h_kv
+            if n > 1:
+                rows_out += times * n * rows * G * h_kv
+                words += times * h_kv
+    return items, rows_out, words, cols
+
+
+def test_mixed_plans_fit_what_the_sizes_promise(native_lib):
+    """Items, partial rows and arrival words of batches chosen to need many: one row more than a whole or a half tile
+    holds (5 heads a group: 25 rows, one whole tile and three half ones), many short sequences, long prefixes."""
+    g = torch.Generator().manual_seed(9)
+
+    def rand(lo, hi):
+        return int(torch.randint(lo, hi + 1, (1,), generator=g))
+
+    seen = set()
+    for G in range(1, 17):
+        half, whole = COLS // 2 // G, COLS // G
+        edges = [1, half, half + 1, 2 * half + 1, whole, whole + 1, 2 * whole, 2 * whole + 1, 3 * half + 1]
+        batches = []
+        for h_kv in (1, 2, 3, 8, 32):
+            for L in edges:
+                for B in (1, 7, 64, 500, 2048):
+                    batches += [([L] * B, [0] * B, h_kv), ([L] * B, [rand(0, 3000)] * B, h_kv)]
+            for L in (1, 2, 16 // G + 1, whole, 700, 9000):
+                batches += [([L], [c], h_kv) for c in (0, 511, 512, 4000, 65536, 2 ** 20)]
+            for _ in range(40):
+                B = rand(1, 60)
+                batches.append(([rand(0, 1) * rand(0, 2 ** rand(0, 9)) for _ in range(B)],
+                                [rand(0, 2 ** rand(0, 16)) for _ in range(B)], h_kv))
+            # the largest launches of half tiles: batches of edge lengths up to the limit of W
+            for L in edges:
+                for B in range(1, 2048, 97):
+                    batches.append(([L] * B, [0] * B, h_kv))
+        for lens, kv_lens, h_kv in batches:
+            T, B, h_q = sum(lens), len(lens), G * h_kv
+            if T == 0:
+                continue
+            items, rows, words, cols = plan_of(lens, kv_lens, G, h_kv)
+            assert 48 + 48 * items <= native_lib.cie_q8_mixed_plan_bytes(B, T, h_q, h_kv), (G, h_kv, lens[0], B)
+            assert rows * (64 + 2) * 4 <= native_lib.cie_q8_mixed_partials_bytes(T, h_q, 64), (G, h_kv, lens[0], B)
+            assert 2 * words <= native_lib.cie_q8_mixed_counters(), (G, h_kv, lens[0], B)
+            seen.add((cols, rows > 0))
+    assert seen == {(COLS, True), (COLS, False), (COLS // 2, True), (COLS // 2, False)}
+    assert plan_of([25], [0], 5, 1)[0] == 3  # one whole tile would have held them
+
+
+# ---- the kernels' assembly ----
+
+@pytest.mark.skipif(not os.path.exists(asm.HIPCC), reason="hipcc not available")
+@pytest.mark.parametrize("src,kernel", [("q8_decode.hip", "q8_decode_kernel"), ("q8_mixed.hip", "q8_mixed_kernel"),
+                                        ("q8_append.hip", "q8_append_kernel")])
+def test_assembly_of_the_8_bit_kernels(src, kernel, tmp_path, monkeypatch):
+    """Partial states are stored before their arrival is counted, rotations round to fp32 first, and nothing takes
+    the packed fp32 forms; as the 16-bit kernels, with the files' own flags."""
+    monkeypatch.setattr(_build, "HIPCC_FLAGS", _build.source_flags(src))
+    text = asm._assembly(src, tmp_path)
+    assert "buffer_wbl2" not in text and "buffer_inv" not in text
+    assert not re.search(r"\bv_pk_(add|mul|fma)_f32\b", text)
+    kernels = {n: b for n, b in asm._kernels(text).items() if kernel in n}
+    assert kernels
+    for name, body in kernels.items():
+        assert not any(asm.FMA_MIX_F16.match(l) for l in body), name
+        if src != "q8_append.hip":
+            asm._check_arrival(name, body)
+            parts = [l for l in body if asm.STORE.match(l) and "dwordx4" in l and "buffer_store" in l]
+            assert parts and all("sc1" in l for l in parts), name
