@@ -307,7 +307,7 @@ def gqa_decode_qkv_rope_attention_q8_op(
 
 @gqa_decode_qkv_rope_attention_q8_op.register_fake
 def _(qkv, cos, sin, k_cache, v_cache, scales, lens, slot_ids, block_table, num_heads, plan=None):
-    return qkv.new_empty((1, qkv.shape[1], num_heads, k_cache.shape[-1]))
+    return qkv.new_empty((1, qkv.shape[-2], num_heads, k_cache.shape[-1]))
 
 
 @torch.library.custom_op("inference::kv_append_tokens_qkv_rope_q8", mutates_args=("k_cache", "v_cache", "scales"))
@@ -320,7 +320,7 @@ def kv_append_tokens_qkv_rope_q8_op(
 
 @kv_append_tokens_qkv_rope_q8_op.register_fake
 def _(qkv, cos, sin, k_cache, v_cache, scales, pages, offsets, num_heads):
-    return qkv.new_empty((1, qkv.shape[1], num_heads, k_cache.shape[-1]))
+    return qkv.new_empty((1, qkv.shape[-2], num_heads, k_cache.shape[-1]))
 
 
 @torch.library.custom_op("inference::gqa_mixed_attention_q8", mutates_args=())

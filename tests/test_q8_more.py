@@ -104,6 +104,19 @@ def test_held_values_stay_within_the_stated_error():
     assert abs(2 * 2.0 ** -8 - x) > 0.74 * 2.0 ** -8
 
 
+@pytest.mark.parametrize("lead", [(1,), ()], ids=["3d", "2d"])
+def test_fake_impls_of_the_projection_forms_take_both_layouts(lead):
+    """(1, n, width) and (n, width) rows, which the calls accept, have outputs of n rows in a traced graph too."""
+    n, width = 5, 18 * 64
+    qkv, cs = (torch.empty(*lead, n, w, dtype=torch.float16, device="meta") for w in (width, 64))
+    k = torch.empty(6, 2, 16, 64, dtype=torch.float8_e4m3fn, device="meta")
+    scales = torch.empty(6, 2, 1, 2, device="meta")
+    i, table = torch.empty(n, dtype=torch.int64, device="meta"), torch.empty(9, 6, dtype=torch.int64, device="meta")
+    ops = torch.ops.inference
+    assert ops.kv_append_tokens_qkv_rope_q8(qkv, cs, cs, k, k.clone(), scales, i, i, 14).shape == (1, n, 14, 64)
+    assert ops.gqa_decode_qkv_rope_attention_q8(qkv, cs, cs, k, k.clone(), scales, i, i, table, 14).shape == (1, n, 14, 64)
+
+
 # ---- a mixed plan's capacity: the plan kernel's arithmetic, over every group size ----
 
 SLOTS, COLS, MIN_SHARE, MAX_CHUNKS, SMALL = 256, 128, 32, 48, 80
