@@ -179,3 +179,22 @@ def test_mixed_ranges_that_run_backwards_leave_the_plan_empty(native_lib):
     cie.mixed_gqa_attention_q8(c.q.to(DEV), c.k, c.v, c.scales, c.T, many, lens, slots, c.table.to(DEV), plan=plan, err=err)
     torch.cuda.synchronize()
     assert int(err) == 1
+
+
+@pytest.mark.parametrize("shape", [dict(prior=[0], new=[8192], h_q=8, h_kv=8), dict(prior=[700], new=[6000], h_q=32, h_kv=8, d=128)],
+                         ids=["d64", "d128"])
+def test_mixed_items_of_many_stages(native_lib, shape):
+    """Unsplit wide items of more than 64 stages: a wave gathers its page ids and scales more than once."""
+    note(f"q8 mixed many stages {shape}")
+    c = Case(**shape, seed=34).write_history()
+    append_tokens(c)
+    index = c.dev("cu", "kv_lens", "slots", "table")
+    plan = cie.mixed_plan_q8(c.k, *index, c.T, c.T, c.h_q)
+    assert max(i[6] - i[5] for i in plan_items(c, plan) if i[8] == 1) > 4 * 64
+    o = cie.mixed_gqa_attention_q8(c.q.to(DEV), c.k, c.v, c.scales, c.T, *index, plan=plan)[0]
+    oracles = c.oracles()
+    for first in (0, c.T // 2 - 7, c.T - 40):  # (some rows: the rest differ by their keys only)
+        want = ref.attend(c.q[0], *oracles, [(first, 40, 1, c.prior[0] + first + 1)], c.table)
+        rows = slice(first, first + 40)
+        check_attention(o[rows], tuple(x[rows] for x in want), c.prior[0] + c.T)
+    assert torch.isfinite(o).all()
