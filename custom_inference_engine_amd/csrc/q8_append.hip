@@ -16,8 +16,12 @@
 // The search reads T page ids (L2 hits) and is shared by all heads of the block: T^2 / 16
 // ids in all, which shows from some 32,000 rows on.
 //
-// What bounds it: memory at many tokens (8,192 rows of 8 heads, D = 128: 50 MB in 15.1
-// us, 3.3 TB/s), the start's chain (index, search, rows) at few (3 rows 3.8 us).
+// What bounds it: memory at many tokens (8,192 rows of 8 heads, D = 128: 50 MB in 14.8
+// us, 3.4 TB/s; from the projection, 32 / 8 heads, 189 MB in 42 us, 4.5 TB/s), the
+// start's chain (index, search, rows) at few (3 rows of 2 heads, D = 64: 3.7 us).  Decode
+// rows: 32 of 2 heads, D = 64, 3.7 us, 256 3.9, of 8 heads, D = 128, 5.1 and 6.3: slot,
+// length, page and rows, one after the other (the fp16 append's 2.4 to 2.7, which needs
+// no block's other rows), and with 8 heads two (head, K or V) pairs a wave in turn.
 #include "q8_cache.h"
 
 namespace cie {
@@ -26,7 +30,7 @@ namespace cie {
 // time.  (Two in flight: 137 registers at D = 128, one 8-wave workgroup a CU instead of two, 19.4 us for 8,192 rows of 8
 // heads against 15.1; 4 waves 20.2.  464 rows of 2 heads with RoPE: 5.0 us, 5.4 with 8 waves.)  The rope form's 144
 // registers leave one 8-wave workgroup a CU: past kEachRow rows, whose blocks no longer have a CU each, it takes 4
-// (8,192 rows, 32 / 8 heads, D = 128: 38 us, 46 with 8; 300 rows: 9.5 with 4, 7.0 with 8).
+// (8,192 rows, 32 / 8 heads, D = 128: 42 us, 46 with 8; 300 rows: 9.5 with 4, 7.0 with 8).
 constexpr int kFewWaves = 4, kManyWaves = 8;
 constexpr int64_t kEachRow = 1024;  // rows up to which each has a workgroup of its own
 constexpr int kScan = 8;
@@ -306,7 +310,7 @@ struct Q8ReadParams {
 
 // Row t of the outputs = the cache's row (pages[t], offsets[t]): a lane converts 8 values of K and of V, so that a wave
 // writes whole lines, past the caches (the rows are read by other kernels, later).  Bound by memory: 105,537 rows of 8
-// heads, D = 128, 648 MB in 117 us, 5.5 TB/s.  A bad index reads as zeros and is reported.
+// heads, D = 128, 648 MB in 120 us, 5.4 TB/s.  A bad index reads as zeros and is reported.
 template <int D>
 __global__ __launch_bounds__(256) void q8_read_kernel(Q8ReadParams p) {
   constexpr int kPer = D / 8;

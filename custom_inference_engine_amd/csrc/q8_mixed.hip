@@ -27,11 +27,13 @@
 // first.  It depends on the step's sequences only, so a step makes it once for all
 // its layers.
 //
-// What bounds it: prefill, the softmax's VALU work between the MFMAs (a step of 32
-// keys costs a wave 18 MFMAs and 16 exponentials at D = 64 and two column tiles): 4 x
-// 8,192 rows, 14 / 2 heads, D = 64, 556 us, 865 TFLOP/s; 8,192 rows, 32 / 8 heads,
-// D = 128, 571 us, 963 TFLOP/s (a large fp16 product reaches 1,135).  Decode rows, the
-// K/V reads and the chain around them (32 rows over 8,000 keys 16 us).
+// What bounds it: prefill of several rounds of items, the softmax's VALU work between
+// the MFMAs (a step of 32 keys costs a wave 18 MFMAs and 16 exponentials at D = 64 and two
+// column tiles): 4 x 8,192 rows, 14 / 2 heads, D = 64, 506 us, 950 TFLOP/s; 8,192 rows, 32 /
+// 8 heads, D = 128, 505 us, 1,088 TFLOP/s (a large fp16 product reaches 1,135).  Launches
+// whose items all start at once last as long as the longest: 8,192 rows, 8 / 8 heads, D =
+// 64, 512 items of up to 128 stages, 65 on average, 131 us, 526 TFLOP/s.  Decode rows, the
+// K/V reads and the chain around them (32 rows over 8,000 keys 15.8 us).
 #include "q8_attn.h"
 
 namespace cie {

@@ -135,9 +135,9 @@ def kv_append_tokens_q8(k_cache, v_cache, scales, k, v, pages, offsets, err=None
     """``kv_append_tokens`` into an 8-bit cache: row t goes to ``(pages[t], :, offsets[t])``.
 
     Rows in any order; of an index that comes several times the last row is written.
-    Every block's rows are looked for in the whole list, so past some 32,000 rows (54 us
-    at 8 heads of 128, 1.3 times their bytes' time) that search outgrows the writing
-    (262,144 rows: 1.3 ms, 3.8 times) and several calls, cut between sequences, take less.
+    Every block's rows are looked for in the whole list, so past some 32,000 rows (63 us
+    at 8 heads of 128, 1.5 times their bytes' time) that search outgrows the writing
+    (262,144 rows: 1.3 ms, 4 times) and several calls, cut between sequences, take less.
     """
     (n_pages, h_kv, page_size, d), (s_page, s_head, _, _) = check_cache_q8(k_cache, v_cache, scales)
     dev = one_device(k_cache, v_cache, scales, k, v, pages, offsets)
