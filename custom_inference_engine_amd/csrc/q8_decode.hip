@@ -24,7 +24,7 @@
 // merges the splits' states by log-sum-exp (arrive_last).
 //
 // What bounds it: the HBM reads of K and V, half the fp16 pools' (96 sequences of 2,048 to 16,384 keys, 32 / 8 heads, D
-// = 128: 1.82 GB in 322 us, 5.6 TB/s; fp16 571 us); where those are few, the chain of launch, index, page, tile, fold,
+// = 128: 1.82 GB in 322 us, 5.7 TB/s; fp16 571 us); where those are few, the chain of launch, index, page, tile, fold,
 // arrival and merge, about 7 us (32 sequences of 4,096 keys, 14 / 2 heads, D = 64: 12.0 us, 34 MB; 11.5 with a plan).
 #include "q8_attn.h"
 
