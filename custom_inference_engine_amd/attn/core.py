@@ -173,9 +173,13 @@ def _planned_buffers(lib, dev, B, H_q, H_kv, D, n_wg, counters):
 
 
 @functools.lru_cache(maxsize=None)
+def _device_cus(index: int) -> int:
+    return torch.cuda.get_device_properties(index).multi_processor_count
+
+
 def _cu_count(dev: torch.device | None) -> int:
     if dev is not None and dev.type == "cuda":
-        return torch.cuda.get_device_properties(dev).multi_processor_count
+        return _device_cus(dev.index if dev.index is not None else torch.cuda.current_device())
     return DECODE_DEFAULT_CUS
 
 

@@ -117,6 +117,27 @@ def test_fake_impls_of_the_projection_forms_take_both_layouts(lead):
     assert ops.gqa_decode_qkv_rope_attention_q8(qkv, cs, cs, k, k.clone(), scales, i, i, table, 14).shape == (1, n, 14, 64)
 
 
+def test_default_splits_are_the_current_devices(monkeypatch):
+    """A device without an index is the current one, each time it is asked."""
+    from custom_inference_engine_amd.attn import core
+
+    cus, current = {0: 256, 1: 64}, [0]
+    monkeypatch.setattr(core.torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(core.torch.cuda, "get_device_properties", lambda d: types.SimpleNamespace(
+        multi_processor_count=cus[getattr(d, "index", d) if getattr(d, "index", d) is not None else current[0]]))
+    for cached in (core._cu_count, getattr(core, "_device_cus", core._cu_count)):
+        getattr(cached, "cache_clear", lambda: None)()
+    try:
+        any_device = torch.device("cuda")
+        assert core.default_decode_splits(4, 2, any_device) == 32
+        current[0] = 1
+        assert core.default_decode_splits(4, 2, any_device) == 8
+        assert core.default_decode_splits(4, 2, torch.device("cuda", 0)) == 32
+        assert core.default_decode_splits(4, 2) == 32  # (no device: 256 CUs)
+    finally:
+        core._device_cus.cache_clear()
+
+
 # ---- a mixed plan's capacity: the plan kernel's arithmetic, over every group size ----
 
 SLOTS, COLS, MIN_SHARE, MAX_CHUNKS, SMALL = 256, 128, 32, 48, 80
