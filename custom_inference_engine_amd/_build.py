@@ -28,7 +28,7 @@ BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_NAME = "libcie_paged.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = ("capi.hip", "kv_append.hip", "paged_decode.hip", "mixed_attention.hip", "q8_append.hip", "q8_decode.hip",
-           "q8_mixed.hip")
+           "q8_mixed.hip", "step_maps.hip", "rotary.hip", "adapters.hip")
 # bench.py's measurement helpers: a library of their own, never linked into the product
 BENCH_SOURCES = ("bench/gather_probe.hip",)
 BENCH_LIB_PATH = os.path.join(PKG_DIR, "libcie_bench.so")
@@ -56,9 +56,12 @@ HIPCC_FLAGS = [
 
 
 def source_flags(src: str) -> list:
-    """The flags that ``src`` is compiled with: the 8-bit cache keeps NaNs, so its kernels honour them."""
-    honour = os.path.basename(src).startswith("q8_")
-    return [f for f in HIPCC_FLAGS if not (honour and f == "-fno-honor-nans")]
+    """The flags that ``src`` is compiled with: the 8-bit cache keeps NaNs, so its kernels honour them; a NaN in
+    a row that is rotated or adapted comes out of it, so those kernels do too (the last such flag counts)."""
+    name = os.path.basename(src)
+    honour = name.startswith("q8_")
+    flags = [f for f in HIPCC_FLAGS if not (honour and f == "-fno-honor-nans")]
+    return flags + ["-fhonor-nans"] if name in ("rotary.hip", "adapters.hip") else flags
 
 
 def hipcc() -> str:

@@ -170,9 +170,37 @@ _SIGNATURES = {
          _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
          _c_i64, _c_i64, _c_ptr, _c_ptr],
     ),
+    "cie_step_maps": (ctypes.c_int, [_c_i64p] * 10 + [_c_i64] * 7 + [_c_ptr, _c_ptr]),
+    "cie_release_pages": (ctypes.c_int, [_c_i64p] * 6 + [_c_i64] * 6 + [_c_ptr, _c_ptr]),
+    "cie_rotary": (
+        ctypes.c_int,
+        [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64p, _c_ptr,
+         ctypes.c_float, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int, _c_ptr],
+    ),
+    "cie_kv_append_tokens_qkv_rotary": (
+        ctypes.c_int,
+        [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64p, _c_ptr, ctypes.c_float, _c_i64p, _c_i64p,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int,
+         ctypes.c_int, _c_ptr, _c_ptr],
+    ),
+    "cie_rotary_tables": (
+        ctypes.c_int,
+        [_c_ptr, _c_ptr, _c_i64p, _c_ptr, ctypes.c_float, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int,
+         _c_ptr],
+    ),
+    "cie_adapter_plan_bytes": (_c_i64, [_c_i64, _c_i64]),
+    "cie_adapter_plan": (
+        ctypes.c_int,
+        [_c_ptr, _c_i64, _c_i64p, _c_i64p, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr],
+    ),
+    "cie_adapter_add": (
+        ctypes.c_int,
+        [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64,
+         _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, ctypes.c_int, _c_ptr, _c_ptr],
+    ),
 }
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
@@ -232,6 +260,18 @@ def require_device(*tensors: torch.Tensor) -> torch.device:
 
 def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def call(device: torch.device, name: str, *args) -> None:
+    """The C entry ``name`` on the device's current stream, with that device current."""
+    fn = getattr(load(), name)
+    if device.index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if status:
+        check(status, name)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

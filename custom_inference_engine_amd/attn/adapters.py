@@ -1,0 +1,220 @@
+"""Low-rank adapters of many requests at once, beside a shared projection.
+
+``y[t, s] += scales[i] * B[i, s] (A[i, s] x[t])`` in place, for the slices s of y's columns
+(a fused QKV projection has three) and the adapter i of row t's request; rows without one
+are left as they are.  ``adapter_plan`` works out once per step which rows share an adapter
+(like ``decode_plan`` / ``mixed_plan``: every layer and projection of the step reads it),
+``adapter_add_`` is one launch per projection.  ``AdapterBank`` holds the weights of one
+projection's adapters, ``use_adapters`` puts banks beside the projections of a model's
+attention layers.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+from typing import Optional
+
+import torch
+
+from .. import _native
+from ..kv_cache.quant import int64_index, launch, one_device
+
+RANK_UNIT = 16  # a bank's ranks come in 16s
+MAX_RANK = 128
+_TYPES = {torch.float16: 0, torch.bfloat16: 1}  # CIE_F16, CIE_BF16
+
+
+@functools.lru_cache(maxsize=4096)
+def _plan_words(T: int, n_adapters: int) -> int:
+    n = _native.load().cie_adapter_plan_bytes(T, n_adapters)
+    if n <= 0:
+        raise AssertionError("a plan takes 1 to 1,024 adapters and at most 2^24 rows")
+    return n // 4
+
+
+@functools.lru_cache(maxsize=256)
+def _widths(slices: tuple):
+    return (ctypes.c_int64 * len(slices))(*slices), sum(slices), len(slices)
+
+
+def new_adapter_plan(n_rows: int, n_adapters: int, device) -> torch.Tensor:
+    """Room for the plans of a module whose steps have ``n_rows`` rows, where they need one address (a captured piece)."""
+    return torch.zeros(_plan_words(n_rows, n_adapters), dtype=torch.int32, device=device)
+
+
+def adapter_plan(row_slots: Optional[torch.Tensor], slot_adapters: torch.Tensor, n_adapters: int,
+                 out: Optional[torch.Tensor] = None, err=None) -> torch.Tensor:
+    """One step's plan: row t has adapter ``slot_adapters[row_slots[t]]``, none where that is negative.
+
+    ``row_slots`` (T,): a mixed step's ``StepMaps.slots``, a decode step's slot ids; None:
+    ``slot_adapters`` has an entry for each row.  Pass the int32 tensor as ``plan`` to the
+    step's ``adapter_add_`` calls, on banks of ``n_adapters``.  ``out``: a
+    ``new_adapter_plan`` of as many rows and adapters, to write to.
+    """
+    if slot_adapters.dim() != 1 or (row_slots is not None and row_slots.dim() != 1):
+        raise AssertionError("row_slots must be (T,) and slot_adapters (n_slots,)")
+    dev = one_device(slot_adapters) if row_slots is None else one_device(slot_adapters, row_slots)
+    slot_adapters = int64_index(slot_adapters)
+    rows, T = None, slot_adapters.shape[0]
+    if row_slots is not None:
+        row_slots = int64_index(row_slots)
+        rows, T = row_slots.data_ptr(), row_slots.shape[0]
+    words = _plan_words(T, n_adapters)
+    if out is None:
+        plan = torch.empty(words, dtype=torch.int32, device=dev)
+    else:
+        plan = out
+        one_device(slot_adapters, plan)
+        if plan.dtype != torch.int32 or plan.shape != (words,) or not plan.is_contiguous():
+            raise AssertionError("out must come from new_adapter_plan for these rows and adapters")
+    if T:
+        launch(dev, "cie_adapter_plan", plan.data_ptr(), 4 * words, rows, slot_adapters.data_ptr(), T,
+               slot_adapters.shape[0], n_adapters, err=err)
+    return plan
+
+
+def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    """(T, width), or (1, T, width): the rows, dense within each."""
+    if t.dim() == 3 and t.shape[0] == 1:
+        t = t[0]
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise AssertionError(f"{name} must be (T, width) or (1, T, width), its rows dense")
+    return t
+
+
+def adapter_add_(y, x, a, b, scales, ranks, plan, slices, err=None):
+    """``y`` with its rows' adapters added, in place.
+
+    y (T, d_out) and x (T, d_in), or with a leading 1; a (n, len(slices), R, d_in), b (n,
+    d_out, R), of y's type (float16 or bfloat16), R a multiple of 16 up to 128;
+    ``slices``: the widths of y's parts, d_out together; scales (n,) float32; ranks (n,)
+    int32: an adapter's rows of rank, those behind them being zeros in a and b.  ``plan``:
+    the step's ``adapter_plan``.  A plan of other rows or adapters is reported in ``err``
+    (CIE_ERRBIT_PLAN), and y left as it is.
+    """
+    yr, xr = _rows(y, "y"), _rows(x, "x")
+    T, d_in = xr.shape
+    widths, d_out, n_slices = _widths(tuple(slices))
+    kind = _TYPES.get(y.dtype)
+    if kind is None or x.dtype != y.dtype or a.dtype != y.dtype or b.dtype != y.dtype:
+        raise AssertionError("y, x, a and b must share float16 or bfloat16")
+    if yr.shape[0] != T or yr.shape[1] != d_out:
+        raise AssertionError(f"y must be ({T}, {d_out}): x's rows, the slices' widths")
+    n, S, R, w = a.shape if a.dim() == 4 else (0,) * 4
+    if S != n_slices or w != d_in or R % RANK_UNIT or not 0 < R <= MAX_RANK or not a.is_contiguous():
+        raise AssertionError(f"a must be contiguous (n, {n_slices}, R, {d_in}), R a multiple of 16 up to 128")
+    if b.shape != (n, d_out, R) or not b.is_contiguous():
+        raise AssertionError(f"b must be contiguous ({n}, {d_out}, {R})")
+    if scales.shape != (n,) or scales.dtype != torch.float32 or not scales.is_contiguous():
+        raise AssertionError(f"scales must be contiguous float32 ({n},)")
+    if ranks.shape != (n,) or ranks.dtype != torch.int32 or not ranks.is_contiguous():
+        raise AssertionError(f"ranks must be contiguous int32 ({n},)")
+    words = _plan_words(T, n)
+    if plan.dtype != torch.int32 or plan.dim() != 1 or not plan.is_contiguous() or plan.shape[0] < words:
+        raise AssertionError("plan must come from adapter_plan for these rows and adapters")
+    y_row = yr.stride(0)
+    if T > 1 and y_row < d_out:
+        raise AssertionError("y's rows must not share memory")
+    dev = one_device(y, x, a, b, scales, ranks, plan)
+    if T:
+        x_row = xr.stride(0)
+        if T > 1 and x_row < d_in:
+            xr = xr.contiguous()
+            x_row = d_in
+        launch(dev, "cie_adapter_add", yr.data_ptr(), y_row, xr.data_ptr(), x_row, a.data_ptr(), b.data_ptr(),
+               scales.data_ptr(), ranks.data_ptr(), plan.data_ptr(), 4 * plan.shape[0], T, n, R, d_in, widths,
+               n_slices, kind, err=err)
+    return y
+
+
+@torch.library.custom_op("inference::adapter_add_", mutates_args=("y",))
+def adapter_add_op(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor,
+                   ranks: torch.Tensor, plan: torch.Tensor, slices: list[int]) -> None:
+    adapter_add_(y, x, a, b, scales, ranks, plan, slices)
+
+
+@adapter_add_op.register_fake
+def _(y, x, a, b, scales, ranks, plan, slices) -> None:
+    return None
+
+
+class AdapterBank(torch.nn.Module):
+    """The adapters of one projection: ``n_adapters`` places for A and B of up to ``rank``, empty until ``load``.
+
+    ``out_features``: the projection's width, or the widths of a fused projection's parts.
+    """
+
+    def __init__(self, n_adapters: int, rank: int, in_features: int, out_features, dtype=torch.float16, device=None):
+        super().__init__()
+        self.slices = tuple(out_features) if isinstance(out_features, (tuple, list)) else (out_features,)
+        if not 1 <= rank <= MAX_RANK or not 1 <= n_adapters <= 1024 or not 1 <= len(self.slices) <= 4:
+            raise AssertionError("a bank has 1 to 1,024 adapters of rank 1 to 128, beside 1 to 4 slices")
+        if dtype not in _TYPES:
+            raise AssertionError("adapters are float16 or bfloat16")
+        self.n_adapters, self.rank = n_adapters, rank
+        R = -(-rank // RANK_UNIT) * RANK_UNIT
+        make = functools.partial(torch.zeros, device=device)
+        self.register_buffer("a", make((n_adapters, len(self.slices), R, in_features), dtype=dtype), persistent=False)
+        self.register_buffer("b", make((n_adapters, sum(self.slices), R), dtype=dtype), persistent=False)
+        self.register_buffer("scales", make((n_adapters,), dtype=torch.float32), persistent=False)
+        self.register_buffer("ranks", make((n_adapters,), dtype=torch.int32), persistent=False)
+
+    @torch.no_grad()
+    def load(self, i: int, a, b, scale: float = 1.0) -> None:
+        """Adapter i: for each slice A (r, in_features) and B (width, r), or None for a slice without one."""
+        if not 0 <= i < self.n_adapters:
+            raise IndexError(f"adapter {i} of {self.n_adapters}")
+        a, b = ((x,) if isinstance(x, torch.Tensor) else tuple(x) for x in (a, b))
+        if len(a) != len(self.slices) or len(b) != len(self.slices):
+            raise AssertionError(f"one A and one B for each of the {len(self.slices)} slices")
+        r = 0
+        for x, z, width in zip(a, b, self.slices):
+            if (x is None) != (z is None):
+                raise AssertionError("A and B of a slice come together")
+            if x is not None:
+                if (x.dim() != 2 or x.shape[1] != self.a.shape[3] or not 1 <= x.shape[0] <= self.rank
+                        or z.shape != (width, x.shape[0])):
+                    raise AssertionError(f"A must be (r, {self.a.shape[3]}) and B ({width}, r), r <= {self.rank}")
+                r = max(r, x.shape[0])
+        self.clear(i)
+        col = 0
+        for s, (x, z, width) in enumerate(zip(a, b, self.slices)):
+            if x is not None:
+                self.a[i, s, :x.shape[0]] = x.to(self.a)
+                self.b[i, col:col + width, :x.shape[0]] = z.to(self.b)
+            col += width
+        self.scales[i] = float(scale)
+        self.ranks[i] = r
+
+    @torch.no_grad()
+    def clear(self, i: int) -> None:
+        """Empties place i: rows with this adapter are left as they are."""
+        if not 0 <= i < self.n_adapters:
+            raise IndexError(f"adapter {i} of {self.n_adapters}")
+        for t in (self.a, self.b, self.scales, self.ranks):
+            t[i] = 0
+
+    def add_(self, y, x, plan) -> None:
+        adapter_add_op(y, x, self.a, self.b, self.scales, self.ranks, plan, self.slices)
+
+
+def use_adapters(model, kv_cache, n_adapters: int, rank: int) -> list:
+    """Places for ``n_adapters`` low-rank adapters beside every attention layer's QKV and output projections.
+
+    ``use_triton_attention`` comes first, step modules and schedulers (whose graphs record
+    the adapters' launches) after.  Returns the layers: ``layer.qkv_adapters.load(i, (A_q,
+    A_k, A_v), (B_q, B_k, B_v), scale)`` and ``layer.o_adapters.load(i, A, B, scale)``
+    fill place i.  A request's adapter is its slot's, ``kv_cache.slot_adapters[slot]`` (-1:
+    none), which ``Scheduler.call(prompt, adapter=i)`` sets.
+    """
+    from .core import TritonQwen2Attention
+
+    layers = [m for m in model.modules() if isinstance(m, TritonQwen2Attention)]
+    if not layers:
+        raise AssertionError("use_triton_attention(model) first")
+    for layer in layers:
+        w, o = layer.qkv_weight, layer.original.o_proj
+        layer.qkv_adapters = AdapterBank(n_adapters, rank, w.shape[1], layer.qkv_sizes, w.dtype, w.device)
+        layer.o_adapters = AdapterBank(n_adapters, rank, o.in_features, o.out_features, w.dtype, w.device)
+    kv_cache.use_adapters(n_adapters)
+    return layers

@@ -669,6 +669,7 @@ def _(k_cache, cu_seqlens, kv_lens, slot_ids, block_table, max_seqlen, total_T, 
 
 
 from . import quant as _q8  # noqa: E402  (it takes this module's helpers, above)
+from .rotary import apply_rotary_op, kv_append_tokens_qkv_rotary_op  # noqa: E402
 
 
 class TritonQwen2Attention(torch.nn.Module):
@@ -708,10 +709,16 @@ class TritonQwen2Attention(torch.nn.Module):
         # instead of views, apply_rotary_pos_emb's elementwise kernels and the
         # plain append.
         self.fuse_rope = True
+        # low-rank adapters beside the two projections (adapters.use_adapters)
+        self.qkv_adapters = self.o_adapters = None
+        # rows turned here rather than by cos / sin rows: (interleaved, scale) (rotary.use_rotary)
+        self.rotary = None
 
     def forward(self, hidden_states, position_embeddings, attention_mask=None,
                 past_key_values=None, kv_manager=None, **kwargs):
         if kv_manager is None:
+            if self.rotary is not None:
+                raise AssertionError("the wrapped module's own path has no rotary positions of this layout")
             return self.original(hidden_states, position_embeddings, attention_mask,
                                  past_key_values=past_key_values, **kwargs)
         metadata = kwargs.get("metadata")
@@ -723,8 +730,15 @@ class TritonQwen2Attention(torch.nn.Module):
         hidden_shape = (1, total_T, -1, self.head_dim)
         keys, values = kv_manager.keys[self.layer_idx], kv_manager.values[self.layer_idx]
         scales = kv_manager.scales[self.layer_idx] if getattr(kv_manager, "scales", None) is not None else None
+        if self.qkv_adapters is not None or self.rotary is not None:
+            if not self.fuse_qkv:
+                raise AssertionError("adapters and use_rotary need the fused QKV projection")
+        if self.rotary is not None:
+            qkv = self._project_qkv(hidden_states, metadata)
+            o = self._attend_rotary(qkv, *position_embeddings, kv_manager, metadata, scales)
+            return self._project_o(o.reshape(1, total_T, self.num_heads * self.head_dim), metadata), None
         if self.fuse_qkv and self.fuse_rope and (self.fuse_append or not metadata.full_decode):
-            qkv = torch.nn.functional.linear(hidden_states, self.qkv_weight, self.qkv_bias)
+            qkv = self._project_qkv(hidden_states, metadata)
             cos, sin = position_embeddings
             if metadata.full_decode and scales is not None:
                 o = _q8.gqa_decode_qkv_rope_attention_q8_op(
@@ -746,12 +760,10 @@ class TritonQwen2Attention(torch.nn.Module):
                         qkv, cos, sin, keys, values, metadata.pages, metadata.offsets, self.num_heads,
                     )
                 o = self._mixed(query_states, kv_manager, metadata, scales)
-            attn_output = attn.o_proj(o.reshape(1, total_T, self.num_heads * self.head_dim))
-            return attn_output, None
+            return self._project_o(o.reshape(1, total_T, self.num_heads * self.head_dim), metadata), None
 
         if self.fuse_qkv:
-            q, k, v = torch.nn.functional.linear(hidden_states, self.qkv_weight, self.qkv_bias).split(
-                self.qkv_sizes, dim=-1)
+            q, k, v = self._project_qkv(hidden_states, metadata).split(self.qkv_sizes, dim=-1)
         else:
             q, k, v = attn.q_proj(hidden_states), attn.k_proj(hidden_states), attn.v_proj(hidden_states)
         query_states = q.view(hidden_shape)
@@ -789,8 +801,42 @@ class TritonQwen2Attention(torch.nn.Module):
             kv_manager.mixed_update(self.layer_idx, metadata.pages, metadata.offsets,
                                     key_states, value_states)
             o = self._mixed(query_states, kv_manager, metadata, scales)
-        attn_output = attn.o_proj(o.reshape(1, total_T, self.num_heads * self.head_dim))
-        return attn_output, None
+        return self._project_o(o.reshape(1, total_T, self.num_heads * self.head_dim), metadata), None
+
+    def _project_qkv(self, hidden_states, metadata):
+        """The fused projection, with the adapters of the step's rows."""
+        qkv = torch.nn.functional.linear(hidden_states, self.qkv_weight, self.qkv_bias)
+        plan = getattr(metadata, "adapter_plan", None)
+        if self.qkv_adapters is not None and plan is not None:
+            self.qkv_adapters.add_(qkv, hidden_states, plan)
+        return qkv
+
+    def _project_o(self, o, metadata):
+        out = self.original.o_proj(o)
+        plan = getattr(metadata, "adapter_plan", None)
+        if self.o_adapters is not None and plan is not None:
+            self.o_adapters.add_(out, o, plan)
+        return out
+
+    def _attend_rotary(self, qkv, positions, frequencies, kv_manager, metadata, scales):
+        """Append and attention of rows that are turned here (``rotary.use_rotary``)."""
+        keys, values = kv_manager.keys[self.layer_idx], kv_manager.values[self.layer_idx]
+        if not metadata.full_decode and scales is None:
+            q = kv_append_tokens_qkv_rotary_op(qkv, positions, frequencies, keys, values, metadata.pages,
+                                               metadata.offsets, self.num_heads, *self.rotary)
+            return self._mixed(q, kv_manager, metadata, scales)
+        n_kv = self.qkv_sizes[1] // self.head_dim
+        q, k, v = qkv.view(1, qkv.shape[1], -1, self.head_dim).split((self.num_heads, n_kv, n_kv), dim=2)
+        q, k = apply_rotary_op(q, k, positions, frequencies, *self.rotary)
+        if not metadata.full_decode:
+            kv_manager.mixed_update(self.layer_idx, metadata.pages, metadata.offsets, k, v)
+            return self._mixed(q, kv_manager, metadata, scales)
+        plan = getattr(metadata, "decode_plan", None)
+        if scales is not None:
+            return _q8.gqa_decode_append_attention_q8_op(q, keys, values, scales, k, v, kv_manager.lens,
+                                                         metadata.slot_ids, kv_manager.block_table, plan=plan)
+        return gqa_decode_append_attention_op(q, keys, values, k, v, kv_manager.lens, metadata.slot_ids,
+                                              kv_manager.block_table, plan=plan)
 
     def _mixed(self, query_states, kv_manager, metadata, scales):
         """The step's varlen attention on this layer's pools (16-bit, or 8-bit with ``scales``)."""

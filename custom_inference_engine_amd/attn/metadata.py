@@ -26,6 +26,8 @@ class AttentionMetadata:
         self.decode_plan = None
         # a mixed step's plan (inference::gqa_mixed_plan), likewise
         self.mixed_plan = None
+        # which of the step's rows share a low-rank adapter (adapters.adapter_plan)
+        self.adapter_plan = None
 
     def prepare_full_graph(self, batch_size: int) -> None:
         self.slot_ids = torch.zeros((batch_size,), dtype=torch.long, device=self.device)

@@ -1,0 +1,576 @@
+// Low-rank adapters of many requests beside a shared projection:
+//   y[t, s] += scale_i * B_is (A_is x_t),   i = the adapter of row t's request,
+// for the slices s of y's columns (a fused projection has one a part).
+//
+// cie_adapter_plan sorts a step's rows by adapter into tiles of up to M rows of
+// one adapter (M = 16 or 32), once for all of the step's projections.
+// cie_adapter_add is one launch: a workgroup takes a tile and a range of y's
+// columns.  Its eight waves share the sum over d_in (64 values of x at a time each,
+// MFMA 16x16x32, ranks as rows and tokens as columns), their partial sums meet in
+// LDS, and then each wave takes 64 columns of y at a time.  So x is read once and y
+// read and written once, and nothing goes through memory between the two products.
+//
+// u = A x is fp32.  It enters the second product as two values of the element
+// type, u = hi + lo, side by side in the MFMA's K: 16 ranks fill K = 32, and B's
+// values serve both halves.  In fp16 each row of u is first scaled by a power of two
+// to below 2^15, so that no u overflows or loses bits to fp16's range.  What is
+// left of the rounding of u is 2^-22 (bf16: 2^-16) of it; the sum with y rounds
+// once, as the plain form does.
+//
+// Bound by memory: r <= 128 ranks are 2 r flops for each value of x and y, far from
+// what the matrix cores could do.
+#include "cie_common.h"
+
+namespace cie {
+
+typedef __bf16 bf16;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+template <class E>
+struct Lane8;
+template <>
+struct Lane8<f16> {
+  typedef f16x8 type;
+};
+template <>
+struct Lane8<bf16> {
+  typedef bf16x8 type;
+};
+__device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// ---- the plan ----
+
+constexpr int kAdMaxAdapters = 1024;
+constexpr int64_t kAdMaxRows = 1 << 24;
+constexpr int kAdMaxSlices = 4;
+constexpr int kAdMagic = 0x61647031;
+// Header words: tiles, T, N, M, kAdMagic; then tiles of kAdTileHead + M words:
+// adapter, rows, two unused, the rows' indexes.
+constexpr int kAdHead = 8, kAdTileHead = 4;
+constexpr int kPlanWaves = 8;
+constexpr int kPlanBatch = 8;  // rows of a lane whose loads are in flight
+
+// Rows of a tile: more share A's and B's reads, fewer fill the chip.
+__host__ __device__ static inline int tile_rows(int64_t T) { return T <= 2048 ? 16 : 32; }
+static inline int64_t max_tiles(int64_t T, int64_t N, int M) {
+  const int64_t groups = T < N ? T : N;  // (a group of c rows has ceil(c / M) <= (c - 1) / M + 1 tiles)
+  return groups + (T - groups) / M;
+}
+
+struct PlanParams {
+  int32_t* plan;
+  const int64_t* row_slots;
+  const int64_t* slot_adapters;
+  int64_t T, n_slots;
+  int32_t N, M;
+  int32_t* err;
+};
+
+// A lane's next rows' adapters (-1: none): rows first, first + 64, ...
+__device__ __forceinline__ void load_ids(const PlanParams& p, int64_t first, int64_t end, int* id, int& mistakes) {
+  int64_t slot[kPlanBatch];
+#pragma unroll
+  for (int i = 0; i < kPlanBatch; ++i) {
+    const int64_t row = first + i * kWave;
+    slot[i] = row < end ? (p.row_slots ? p.row_slots[row] : row) : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < kPlanBatch; ++i) {
+    const bool ok = slot[i] >= 0 && slot[i] < p.n_slots;
+    const int64_t a = p.slot_adapters[ok ? slot[i] : 0];
+    id[i] = -1;
+    if (first + i * kWave >= end) continue;
+    if (!ok)
+      mistakes |= CIE_ERRBIT_PAGE;
+    else if (a >= p.N)
+      mistakes |= CIE_ERRBIT_ADAPTER;
+    else if (a >= 0)
+      id[i] = (int)a;
+  }
+}
+
+// Rows are dealt to the waves in order, 64 adjacent rows at a time, and each wave
+// counts its own, so that a group's rows keep their order and the plan is the same
+// every time.  Two dependent loads, the count, a scan over adapters, the rows.
+__global__ __launch_bounds__(kPlanWaves* kWave) void adapter_plan_kernel(PlanParams p) {
+  extern __shared__ int lds[];
+  __shared__ int sums[kPlanWaves];
+  int* const count = lds;                    // [kPlanWaves][N]: rows of a wave, then the next one's place
+  int* const tile0 = lds + kPlanWaves * p.N;  // [N] first tile of an adapter
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int64_t share = (p.T + kPlanWaves * kWave - 1) / (kPlanWaves * kWave) * kWave;
+  const int64_t first = wave * share, end = min(first + share, p.T);
+  for (int i = tid; i < kPlanWaves * p.N; i += kPlanWaves * kWave) count[i] = 0;
+  __syncthreads();
+
+  int mistakes = 0;
+  int id[kPlanBatch];
+  for (int64_t at = first; at < end; at += kPlanBatch * kWave) {
+    load_ids(p, at + lane, end, id, mistakes);
+#pragma unroll
+    for (int i = 0; i < kPlanBatch; ++i) {
+      uint64_t todo = __ballot(id[i] >= 0);
+      while (todo) {
+        const int a = __builtin_amdgcn_readlane(id[i], __builtin_ctzll(todo));
+        const uint64_t same = __ballot(id[i] == a);
+        if (lane == 0) atomicAdd(&count[wave * p.N + a], __popcll(same));
+        todo &= ~same;
+      }
+    }
+  }
+  __syncthreads();
+
+  // Adapter a's rows before each wave's, and its tiles.  A thread has up to two adapters.
+  const int per = (p.N + kPlanWaves * kWave - 1) / (kPlanWaves * kWave);
+  int tiles = 0;
+  for (int a = tid * per; a < min(tid * per + per, p.N); ++a) {
+    int n = 0;
+    for (int w = 0; w < kPlanWaves; ++w) {
+      const int c = count[w * p.N + a];
+      count[w * p.N + a] = n;
+      n += c;
+    }
+    tile0[a] = tiles;
+    tiles += (n + p.M - 1) / p.M;
+  }
+  const int incl = wave_inclusive_sum(tiles);
+  if (lane == kWave - 1) sums[wave] = incl;
+  __syncthreads();
+  int before = incl - tiles, total = 0;
+  for (int w = 0; w < kPlanWaves; ++w) {
+    if (w < wave) before += sums[w];
+    total += sums[w];
+  }
+  for (int a = tid * per; a < min(tid * per + per, p.N); ++a) tile0[a] += before;
+  __syncthreads();
+
+  int* const out = p.plan + kAdHead;
+  const int words = kAdTileHead + p.M;
+  for (int64_t at = first; at < end; at += kPlanBatch * kWave) {
+    if (share > kPlanBatch * kWave) load_ids(p, at + lane, end, id, mistakes);  // (else they are still there)
+#pragma unroll
+    for (int i = 0; i < kPlanBatch; ++i) {
+      uint64_t todo = __ballot(id[i] >= 0);
+      while (todo) {
+        const int a = __builtin_amdgcn_readlane(id[i], __builtin_ctzll(todo));
+        const uint64_t same = __ballot(id[i] == a);
+        int base = 0;
+        if (lane == 0) base = atomicAdd(&count[wave * p.N + a], __popcll(same));
+        base = __builtin_amdgcn_readlane(base, 0);
+        if (id[i] == a) {
+          const int k = base + __popcll(same & ((1ull << lane) - 1));
+          int* const tile = out + (int64_t)(tile0[a] + k / p.M) * words;
+          tile[kAdTileHead + k % p.M] = (int)(at + i * kWave + lane);
+        }
+        todo &= ~same;
+      }
+    }
+  }
+  __syncthreads();
+  // (the last wave's next place is now each adapter's row count)
+  for (int a = tid; a < p.N; a += kPlanWaves * kWave) {
+    const int n = count[(kPlanWaves - 1) * p.N + a];
+    for (int k = 0; k * p.M < n; ++k) {
+      int* const tile = out + (int64_t)(tile0[a] + k) * words;
+      tile[0] = a;
+      tile[1] = min(n - k * p.M, p.M);
+    }
+  }
+  if (tid == 0) {
+    p.plan[0] = total;
+    p.plan[1] = (int)p.T;
+    p.plan[2] = p.N;
+    p.plan[3] = p.M;
+    p.plan[4] = kAdMagic;
+  }
+  if (mistakes) set_err(p.err, mistakes);
+}
+
+// ---- the products ----
+
+constexpr int kAdWaves = 8;
+constexpr int kAdThreads = kAdWaves * kWave;
+constexpr int kAdBlock = 64;   // values of x a wave takes at a time: two MFMAs
+constexpr int kAdUnits = 8;    // 16-rank units of u held at once: one slice of 128 ranks, or several of fewer
+
+struct AddParams {
+  void* y;
+  const void* x;
+  const void* a;
+  const void* b;
+  const float* scales;
+  const int32_t* ranks;
+  const int32_t* plan;
+  int64_t y_stride, x_stride;
+  int32_t T, N, M, R, d_in, d_out, n_slices, chunks, col_tiles;
+  int32_t slice_col[kAdMaxSlices + 1];   // a slice's first column
+  int32_t slice_tile[kAdMaxSlices + 1];  // and its first 64-column tile
+  int32_t* err;
+};
+
+// Eight values from k on, zeros at and past n.
+template <class E, bool kAligned>
+__device__ __forceinline__ typename Lane8<E>::type load8(const E* row, int k, int n) {
+  typedef typename Lane8<E>::type vec;
+  vec v = {};
+  if constexpr (kAligned) {
+    if (k < n) v = *reinterpret_cast<const vec*>(row + k);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (k + e < n) v[e] = row[k + e];
+  }
+  return v;
+}
+
+// 2^e that takes m (fp16: the largest |u| of a row) to [2^14, 2^15); 1 where there is no such.
+template <class E>
+__device__ __forceinline__ int row_shift(float m) {
+  if constexpr (sizeof(E) == 2 && __is_same(E, f16)) {
+    if (!(m > 0.f)) return 0;
+    return min(15 - __builtin_amdgcn_frexp_expf(m), 100);
+  }
+  return 0;
+}
+
+template <class E, int MR, int NT, bool kAligned>
+__global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
+  typedef typename Lane8<E>::type vec;
+  constexpr int M = 16 * MR;
+  constexpr int kRow = NT * 16 + 4;  // floats of a row of partial sums (padded: rows start in other banks)
+  constexpr int kLanes = NT * 4;     // threads that hold a row of u, four ranks each
+  constexpr int kPasses = (kAdUnits + NT - 1) / NT;
+  constexpr int kDepth = MR * NT >= 6 ? 2 : 4;  // blocks of x whose loads are in flight
+  static_assert(M * kLanes <= kAdThreads, "a thread has four values of u at most");
+  __shared__ float part[kAdWaves][M][kRow];
+  __shared__ __align__(16) E u_hl[kAdUnits][M][32];  // of 16 ranks, hi then lo
+  __shared__ float factor[M];
+
+  const int32_t* const head = p.plan;
+  const int n_tiles = head[0];
+  if (head[1] != p.T || head[2] != p.N || head[3] != M || head[4] != kAdMagic) {
+    if (threadIdx.x == 0 && blockIdx.x == 0) set_err(p.err, CIE_ERRBIT_PLAN);
+    return;
+  }
+  // An XCD (workgroups go to the eight in turn) takes adjacent tiles, mostly of one
+  // adapter, with all their column ranges: A and B come from its L2 after the first.
+  const int items = n_tiles * p.chunks, share = (items + 7) / 8;
+  const int item = (int)(blockIdx.x % 8) * share + (int)(blockIdx.x / 8);
+  if ((int)(blockIdx.x / 8) >= share || item >= items) return;
+  const int tile = item / p.chunks, chunk = item - tile * p.chunks;
+  const int32_t* const desc = p.plan + kAdHead + (int64_t)tile * (kAdTileHead + M);
+  const int adapter = uniform(desc[0]), rows = uniform(desc[1]);
+  const int units = uniform((p.ranks[adapter] + 15) / 16);
+  if (units <= 0 || units * 16 > p.R) return;
+  const float scale = p.scales[adapter];
+
+  const int tid = threadIdx.x, lane = tid % kWave, wave = uniform(tid / kWave), m = lane % 16, g = lane / 16;
+  int64_t row[MR];
+#pragma unroll
+  for (int r = 0; r < MR; ++r) row[r] = desc[kAdTileHead + min(16 * r + m, rows - 1)];
+
+  const int per_chunk = (p.col_tiles + p.chunks - 1) / p.chunks;
+  const int ct0 = chunk * per_chunk, ct1 = min(ct0 + per_chunk, p.col_tiles);
+  if (ct0 >= ct1) return;
+  int s0 = 0;
+  while (s0 + 1 < p.n_slices && p.slice_tile[s0 + 1] <= ct0) ++s0;
+  const int at_once = max(1, kAdUnits / units);
+
+  const E* x_row[MR];
+#pragma unroll
+  for (int r = 0; r < MR; ++r) x_row[r] = static_cast<const E*>(p.x) + row[r] * p.x_stride;
+  const int blocks = p.d_in / kAdBlock;
+
+  for (; s0 < p.n_slices && p.slice_tile[s0] < ct1; s0 += at_once) {
+    int s1 = s0 + 1;  // slices [s0, s1) of this workgroup's columns
+    while (s1 < p.n_slices && s1 < s0 + at_once && p.slice_tile[s1] < ct1) ++s1;
+    const int n_units = (s1 - s0) * units;
+
+    // u = A x, NT units at a time.
+    f32x4 kept[kPasses];
+#pragma unroll
+    for (int pass = 0; pass < kPasses; ++pass) {
+      kept[pass] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (pass * NT >= n_units) continue;
+      const E* a_row[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int i = min(pass * NT + n, n_units - 1), s = s0 + i / units;
+        a_row[n] = static_cast<const E*>(p.a) +
+                   (((int64_t)adapter * p.n_slices + s) * p.R + 16 * (i % units) + m) * p.d_in;
+      }
+      f32x4 acc[MR][NT] = {};
+      if constexpr (kAligned) {
+        for (int b = wave; b < blocks; b += kAdWaves * kDepth) {
+          vec xv[kDepth][MR][2], av[kDepth][NT][2];
+#pragma unroll
+          for (int d = 0; d < kDepth; ++d) {
+            // (past the end: the last block again, not used)
+            const int k = min(b + d * kAdWaves, blocks - 1) * kAdBlock + 16 * g;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+              for (int r = 0; r < MR; ++r) xv[d][r][j] = *reinterpret_cast<const vec*>(x_row[r] + k + 8 * j);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) av[d][n][j] = *reinterpret_cast<const vec*>(a_row[n] + k + 8 * j);
+            }
+          }
+#pragma unroll
+          for (int d = 0; d < kDepth; ++d) {
+            if (b + d * kAdWaves >= blocks) break;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int r = 0; r < MR; ++r)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[r][n] = mma(av[d][n][j], xv[d][r][j], acc[r][n]);
+          }
+        }
+      }
+      // The last values of a row, fewer than a block; unaligned rows: all of them.
+      for (int b = kAligned ? blocks + (wave - blocks % kAdWaves + kAdWaves) % kAdWaves : wave;
+           b * kAdBlock < p.d_in; b += kAdWaves) {
+        const int k = b * kAdBlock + 16 * g;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          vec xv[MR];
+#pragma unroll
+          for (int r = 0; r < MR; ++r) xv[r] = load8<E, kAligned>(x_row[r], k + 8 * j, p.d_in);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const vec av = load8<E, kAligned>(a_row[n], k + 8 * j, p.d_in);
+#pragma unroll
+            for (int r = 0; r < MR; ++r) acc[r][n] = mma(av, xv[r], acc[r][n]);
+          }
+        }
+      }
+      // A lane has ranks 4g .. 4g + 3 of token m.
+#pragma unroll
+      for (int r = 0; r < MR; ++r)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          *reinterpret_cast<f32x4*>(&part[wave][16 * r + m][16 * n + 4 * g]) = acc[r][n];
+      __syncthreads();
+      if (tid < M * kLanes) {
+        const int t = tid / kLanes, q = tid % kLanes;
+        if (pass * NT + q / 4 < n_units) {
+#pragma unroll
+          for (int w = 0; w < kAdWaves; ++w) kept[pass] += *reinterpret_cast<const f32x4*>(&part[w][t][4 * q]);
+        }
+      }
+      __syncthreads();
+    }
+
+    if (tid < M * kLanes) {
+      const int t = tid / kLanes, q = tid % kLanes;
+      // The row's largest finite |u| decides its scale: an infinity stays one.
+      int shift = 0;
+      if constexpr (__is_same(E, f16)) {
+        float top = 0.f;
+#pragma unroll
+        for (int pass = 0; pass < kPasses; ++pass)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v = __builtin_fabsf(kept[pass][e]);
+            if (v < __builtin_huge_valf() && v > top) top = v;
+          }
+#pragma unroll
+        for (int o = 1; o < kLanes; o *= 2) top = fmaxf(top, __shfl_xor(top, o, kWave));
+        shift = row_shift<E>(top);
+      }
+#pragma unroll
+      for (int pass = 0; pass < kPasses; ++pass) {
+        if (pass * NT + q / 4 >= n_units) continue;
+        E* const to = &u_hl[pass * NT + q / 4][t][4 * (q % 4)];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = __builtin_ldexpf(kept[pass][e], shift);
+          const E hi = (E)v;
+          const float left = v - (float)hi;
+          to[e] = hi;
+          to[16 + e] = (E)(__builtin_isfinite(left) ? left : 0.f);  // (of an infinity or a NaN: hi says it all)
+        }
+      }
+      if (q == 0) factor[t] = __builtin_ldexpf(scale, -shift);
+    }
+    __syncthreads();
+
+    // y += scale B u: 64 columns at a time.  B's rows are dealt so that a lane ends
+    // with 16 adjacent columns of its token: row m of part j is column
+    // 16 (m / 4) + 4 j + m % 4.
+    const int first = max(ct0, p.slice_tile[s0]), last = min(ct1, p.slice_tile[s1]);
+    for (int ct = first + wave; ct < last; ct += kAdWaves) {
+      int s = s0;
+      while (s + 1 < s1 && p.slice_tile[s + 1] <= ct) ++s;
+      const int col = p.slice_col[s] + (ct - p.slice_tile[s]) * 64, end = p.slice_col[s + 1];
+      const E* b_row[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int d = min(col + 16 * (m / 4) + 4 * j + m % 4, end - 1);
+        b_row[j] = static_cast<const E*>(p.b) + ((int64_t)adapter * p.d_out + d) * p.R + 8 * (g & 1);
+      }
+      vec yv[MR][2];
+#pragma unroll
+      for (int r = 0; r < MR; ++r)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const E* const from = static_cast<const E*>(p.y) + row[r] * p.y_stride;
+          yv[r][h] = load8<E, kAligned>(from, col + 16 * g + 8 * h, end);
+        }
+      f32x4 acc[MR][4] = {};
+      for (int i = 0; i < units; ++i) {
+        vec bv[4], uv[MR];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bv[j] = *reinterpret_cast<const vec*>(b_row[j] + 16 * i);
+#pragma unroll
+        for (int r = 0; r < MR; ++r)
+          uv[r] = *reinterpret_cast<const vec*>(&u_hl[(s - s0) * units + i][16 * r + m][8 * g]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int r = 0; r < MR; ++r) acc[r][j] = mma(bv[j], uv[r], acc[r][j]);
+      }
+#pragma unroll
+      for (int r = 0; r < MR; ++r) {
+        if (16 * r + m >= rows) continue;
+        const float f = factor[16 * r + m];
+        E* const to = static_cast<E*>(p.y) + row[r] * p.y_stride;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int c = col + 16 * g + 8 * h;
+          vec out;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            out[e] = (E)__builtin_fmaf(acc[r][2 * h + e / 4][e % 4], f, (float)yv[r][h][e]);
+          if constexpr (kAligned) {
+            if (c < end) *reinterpret_cast<vec*>(to + c) = out;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (c + e < end) to[c + e] = out[e];
+          }
+        }
+      }
+    }
+  }
+}
+
+static bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
+
+template <class E, int MR, bool kAligned>
+static void launch_add(const AddParams& p, int units, dim3 grid, hipStream_t stream) {
+  // Few units in all: no registers or partial sums for more.
+  if (kAligned && units == 1)
+    hipLaunchKernelGGL((adapter_add_kernel<E, MR, kAligned ? 1 : 4, kAligned>), grid, dim3(kAdThreads), 0, stream, p);
+  else if (kAligned && units == 2)
+    hipLaunchKernelGGL((adapter_add_kernel<E, MR, kAligned ? 2 : 4, kAligned>), grid, dim3(kAdThreads), 0, stream, p);
+  else
+    hipLaunchKernelGGL((adapter_add_kernel<E, MR, 4, kAligned>), grid, dim3(kAdThreads), 0, stream, p);
+}
+
+template <class E>
+static int dispatch_add(const AddParams& p, int units, bool aligned, dim3 grid, hipStream_t stream) {
+  if (p.M == 16)
+    aligned ? launch_add<E, 1, true>(p, units, grid, stream) : launch_add<E, 1, false>(p, units, grid, stream);
+  else
+    aligned ? launch_add<E, 2, true>(p, units, grid, stream) : launch_add<E, 2, false>(p, units, grid, stream);
+  return (int)hipGetLastError();
+}
+
+}  // namespace cie
+
+using namespace cie;
+
+extern "C" int64_t cie_adapter_plan_bytes(int64_t T, int64_t N) {
+  if (T < 0 || N <= 0 || T > kAdMaxRows || N > kAdMaxAdapters) return -1;
+  const int M = tile_rows(T);
+  return 4 * (kAdHead + max_tiles(T, N, M) * (kAdTileHead + M));
+}
+
+extern "C" int cie_adapter_plan(int32_t* plan, int64_t plan_bytes, const int64_t* row_slots,
+                                const int64_t* slot_adapters, int64_t T, int64_t n_slots, int64_t N, int32_t* err,
+                                void* stream) {
+  if (T < 0 || N <= 0 || n_slots <= 0) return CIE_EINVAL;
+  if (T > kAdMaxRows || N > kAdMaxAdapters) return CIE_EUNSUPPORTED;
+  if (!plan || !aligned16(plan) || plan_bytes < cie_adapter_plan_bytes(T, N) || !slot_adapters ||
+      (!row_slots && n_slots < T))
+    return CIE_EINVAL;
+  PlanParams p{};
+  p.plan = plan;
+  p.row_slots = row_slots;
+  p.slot_adapters = slot_adapters;
+  p.T = T;
+  p.n_slots = n_slots;
+  p.N = (int32_t)N;
+  p.M = tile_rows(T);
+  p.err = err;
+  hipLaunchKernelGGL(adapter_plan_kernel, dim3(1), dim3(kPlanWaves * kWave), (kPlanWaves + 1) * N * 4,
+                     static_cast<hipStream_t>(stream), p);
+  return (int)hipGetLastError();
+}
+
+extern "C" int cie_adapter_add(void* y, int64_t y_row_stride, const void* x, int64_t x_row_stride, const void* a,
+                               const void* b, const float* scales, const int32_t* ranks, const int32_t* plan,
+                               int64_t plan_bytes, int64_t T, int64_t N, int64_t R, int64_t d_in,
+                               const int64_t* slice_widths, int64_t n_slices, int dtype, int32_t* err, void* stream) {
+  if (T < 0 || N <= 0 || R <= 0 || d_in <= 0 || n_slices <= 0 || !slice_widths) return CIE_EINVAL;
+  if (T > kAdMaxRows || N > kAdMaxAdapters || R % 16 || R > 16 * kAdUnits || d_in > 1 << 24 ||
+      n_slices > kAdMaxSlices || (dtype != CIE_F16 && dtype != CIE_BF16))
+    return CIE_EUNSUPPORTED;
+  AddParams p{};
+  bool aligned = d_in % 8 == 0 && x_row_stride % 8 == 0 && y_row_stride % 8 == 0 && aligned16(x) && aligned16(y) &&
+                 aligned16(a);
+  int64_t d_out = 0, tiles = 0;
+  for (int s = 0; s < n_slices; ++s) {
+    if (slice_widths[s] <= 0) return CIE_EINVAL;
+    if (slice_widths[s] > 1 << 24) return CIE_EUNSUPPORTED;
+    p.slice_col[s] = (int32_t)d_out;
+    p.slice_tile[s] = (int32_t)tiles;
+    d_out += slice_widths[s];
+    tiles += (slice_widths[s] + 63) / 64;
+    aligned = aligned && slice_widths[s] % 8 == 0;
+  }
+  for (int s = (int)n_slices; s <= kAdMaxSlices; ++s) {
+    p.slice_col[s] = (int32_t)d_out;
+    p.slice_tile[s] = (int32_t)tiles;
+  }
+  if (T == 0) return CIE_OK;
+  if (!y || !x || !a || !b || !scales || !ranks || !plan || !aligned16(b) || !aligned16(plan) ||
+      (T > 1 && (x_row_stride < d_in || y_row_stride < d_out)) || plan_bytes < cie_adapter_plan_bytes(T, N))
+    return CIE_EINVAL;
+  p.y = y;
+  p.x = x;
+  p.a = a;
+  p.b = b;
+  p.scales = scales;
+  p.ranks = ranks;
+  p.plan = plan;
+  p.y_stride = y_row_stride;
+  p.x_stride = x_row_stride;
+  p.T = (int32_t)T;
+  p.N = (int32_t)N;
+  p.M = tile_rows(T);
+  p.R = (int32_t)R;
+  p.d_in = (int32_t)d_in;
+  p.d_out = (int32_t)d_out;
+  p.n_slices = (int32_t)n_slices;
+  p.col_tiles = (int32_t)tiles;
+  p.err = err;
+  // Few tiles: several workgroups share one's columns (each computes u again), down to a
+  // column tile a wave.
+  const int64_t bound = max_tiles(T, N, p.M);
+  int64_t chunks = 512 / bound;
+  if (chunks > (tiles + kAdWaves - 1) / kAdWaves) chunks = (tiles + kAdWaves - 1) / kAdWaves;
+  p.chunks = (int32_t)(chunks < 1 ? 1 : chunks);
+  const int64_t blocks = (bound * p.chunks + 7) / 8 * 8;
+  if (blocks > 0x7fffffff) return CIE_EUNSUPPORTED;
+  const dim3 grid((unsigned)blocks);
+  const int units = (int)(n_slices * (R / 16) < 5 ? n_slices * (R / 16) : 4);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return dtype == CIE_F16 ? dispatch_add<f16>(p, units, aligned, grid, st) : dispatch_add<bf16>(p, units, aligned, grid, st);
+}

@@ -20,6 +20,7 @@ import math
 import torch
 
 from .. import _native
+from . import pages as _pages
 from . import quant
 
 
@@ -176,6 +177,36 @@ class KVStorage:
         self.block_table = torch.zeros((n_slots, self.n_pages), dtype=torch.long, device=self.device)
         self.last_generated = torch.zeros((n_slots,), dtype=torch.long, device=self.device)
 
+        self.free_list = None      # block tables kept on the device (manage_pages)
+        self.slot_adapters = None  # each slot's low-rank adapter, -1: none (use_adapters)
+        self.n_adapters = 0
+
+    def manage_pages(self) -> None:
+        """Block tables are kept on the device from here on: the step modules' steps take the pages that their new
+        tokens need from ``free_list`` (``pages.step_maps``), ``release`` gives them back.  Comes before the step
+        modules and the scheduler, with every slot empty."""
+        if bool(self.lens.any()) or bool(self.block_table.any()):
+            raise AssertionError("manage_pages needs every slot empty")
+        self.free_list = _pages.new_free_list(self.n_pages, self.device)
+
+    def step_maps(self, slot_ids: torch.Tensor, new_tokens: torch.Tensor, total_T: int, out=None) -> _pages.StepMaps:
+        """A packed step's maps (``pages.step_maps``), with pages for its new tokens if the pool manages them."""
+        return _pages.step_maps(slot_ids, new_tokens, self.lens, self.block_table, self.page_size, total_T,
+                                free_list=self.free_list, out=out)
+
+    def release(self, slot_ids: list[int]) -> None:
+        """``reset`` of a pool that manages its pages: the slots are emptied and their pages free."""
+        if slot_ids:
+            slots = torch.tensor(slot_ids, dtype=torch.long).to(self.lens.device)
+            _pages.release_pages(self.free_list, slots, self.lens, self.block_table, self.page_size)
+            if self.slot_adapters is not None:
+                self.slot_adapters[slots] = -1
+
+    def use_adapters(self, n_adapters: int) -> None:
+        """Slots may have one of ``n_adapters`` low-rank adapters (``attn.adapters``)."""
+        self.slot_adapters = torch.full((self.n_slots,), -1, dtype=torch.long, device=self.device)
+        self.n_adapters = n_adapters
+
     def mixed_update(self, layer_num: int, pages: torch.Tensor, offsets: torch.Tensor,
                      k_proj: torch.Tensor, v_proj: torch.Tensor) -> None:
         if self.scales is not None:
@@ -226,3 +257,5 @@ class KVStorage:
     def reset(self, slot_ids: list[int]) -> None:
         self.lens[slot_ids] = 0
         self.block_table[slot_ids] = 0
+        if self.slot_adapters is not None:
+            self.slot_adapters[slot_ids] = -1

@@ -28,6 +28,7 @@ from __future__ import annotations
 
 import torch
 
+from ..attn.adapters import adapter_plan
 from ..attn.core import gqa_decode_plan_op
 from ..attn.metadata import AttentionMetadata
 from ..graphs import StepGraph, StepInputs
@@ -49,12 +50,17 @@ class DecodeModule:
         self.metadata.slot_ids = self.slots
         self.tokens = torch.zeros((batch_size,), dtype=torch.long, device=dev)
         self.positions = torch.zeros((batch_size,), dtype=torch.long, device=dev)
+        self.ones = torch.ones((batch_size,), dtype=torch.long, device=dev)
         with torch.inference_mode():
             self.step = StepGraph(self._step, pool=pool, warmup=warmup_iters, device=dev)
         self.logits = self.step.output  # (batch_size, vocab), rewritten by every replay
 
     def _step(self) -> torch.Tensor:
         kv = self.kv_cache
+        if kv.free_list is not None:  # pages for the new tokens, before the plan reads the block tables
+            kv.step_maps(self.slots, self.ones, self.batch_size)
+        if kv.slot_adapters is not None:
+            self.metadata.adapter_plan = adapter_plan(self.slots, kv.slot_adapters, kv.n_adapters)
         # one plan for every layer's decode launch (their slots, lengths and
         # block-table rows are the step's): splits balanced by length, page
         # ids resolved once

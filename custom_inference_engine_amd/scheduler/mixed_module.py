@@ -19,7 +19,9 @@ by a cumulative sum of the lengths; the sequence of each packed row by a
 binary search in ``cu_seqlens``; its position ``lens[slot] + offset in its
 chunk``, page ``block_table[slot, pos // page_size]`` and in-page offset; rows
 past the batch's tokens get slot 0, position 0, page 0, offset 0 (the
-reserved padding targets).  Padded sequences have zero query rows, which the
+reserved padding targets).  One launch does all of this
+(``kv_cache.pages.step_maps``); where the pool manages its pages, the same
+launch gives the step's new tokens theirs.  Padded sequences have zero query rows, which the
 varlen kernel skips at no cost (it plans its work on the device), so one
 token bucket serves every batch size.  After the decoder stack, ``_advance``
 moves each slot's length on by its chunk and ``_logits`` applies the LM head
@@ -44,10 +46,12 @@ import contextlib
 
 import torch
 
+from ..attn.adapters import adapter_plan, new_adapter_plan
 from ..attn.core import gqa_mixed_plan_op
 from ..attn.quant import gqa_mixed_plan_q8_op
 from ..attn.metadata import AttentionMetadata
 from ..graphs import StepGraph, StepInputs
+from ..kv_cache.pages import StepMaps
 from ..piecewise import get_piecewise_backend
 
 
@@ -73,6 +77,11 @@ class MixedModule:
         self.metadata.slot_ids = self.slots
         self.metadata.cu_seqlens = self.cu_seqlens
         self.metadata.max_seqlen = T
+        self.row_slots = torch.zeros((T,), dtype=torch.long, device=dev)
+        self.maps = StepMaps(self.cu_seqlens, self.row_slots, self.positions, self.metadata.pages,
+                             self.metadata.offsets)
+        if kv_cache.slot_adapters is not None:  # (read by captured pieces: one address for every step)
+            self.metadata.adapter_plan = new_adapter_plan(T, kv_cache.n_adapters, dev)
         self.last_logits = None  # (n, vocab) of the last forward
 
     # -- the step, in pieces
@@ -80,15 +89,10 @@ class MixedModule:
     def _prepare(self) -> None:
         """cu_seqlens, positions, pages and offsets from (slots, chunk_lens)."""
         kv, B = self.kv_cache, self.batch_size
-        torch.cumsum(self.chunk_lens, 0, out=self.cu_seqlens[1:])
-        seq = torch.searchsorted(self.cu_seqlens[1:], self.rows, right=True)
-        live = seq < B
-        seq.clamp_(max=B - 1)
-        slot = torch.where(live, self.slots[seq], kv.unused_idx)
-        pos = torch.where(live, kv.lens[slot] + (self.rows - self.cu_seqlens[seq]), 0)
-        self.positions.copy_(pos)
-        self.metadata.pages.copy_(torch.where(live, kv.block_table[slot, pos // kv.page_size], 0))
-        self.metadata.offsets.copy_(pos % kv.page_size)
+        if kv.keys[0].is_cuda:
+            kv.step_maps(self.slots, self.chunk_lens, self.token_count, out=self.maps)
+        else:
+            self._prepare_host(kv, B)
         # one plan for every layer's mixed attention: the step's sequences are
         # the same for all of them (the lengths advance after the step).  (A
         # step prepared on the CPU — traced, never run — has none.)
@@ -98,6 +102,20 @@ class MixedModule:
             self.metadata.mixed_plan = make_plan(
                 kv.keys[0], self.cu_seqlens, kv.lens[self.slots], self.slots, kv.block_table, T, T,
                 self.model.config.num_attention_heads)
+            if kv.slot_adapters is not None:
+                adapter_plan(self.row_slots, kv.slot_adapters, kv.n_adapters, out=self.metadata.adapter_plan)
+
+    def _prepare_host(self, kv, B: int) -> None:
+        """The maps of a step prepared on the CPU (``step_maps`` in torch)."""
+        torch.cumsum(self.chunk_lens, 0, out=self.cu_seqlens[1:])
+        seq = torch.searchsorted(self.cu_seqlens[1:], self.rows, right=True)
+        live = seq < B
+        seq.clamp_(max=B - 1)
+        slot = torch.where(live, self.slots[seq], kv.unused_idx)
+        pos = torch.where(live, kv.lens[slot] + (self.rows - self.cu_seqlens[seq]), 0)
+        self.positions.copy_(pos)
+        self.metadata.pages.copy_(torch.where(live, kv.block_table[slot, pos // kv.page_size], 0))
+        self.metadata.offsets.copy_(pos % kv.page_size)
 
     def _forward(self) -> torch.Tensor:
         return self.model.model(input_ids=self.tokens[None], position_ids=self.positions[None],

@@ -53,6 +53,7 @@ class Request:
     new_tokens: list[int] = field(default_factory=list)
     pages: list[int] = field(default_factory=list)
     prefilled: bool = False
+    adapter: int = -1        # the low-rank adapter it is served with; -1: none
 
     def requires_page(self, page_size: int) -> bool:
         return len(self.pages) * page_size == self.kv_len
@@ -221,6 +222,8 @@ class Scheduler:
 
         self.model = model
         self.kv_cache = kv_cache
+        # the pool keeps its block tables itself (KVStorage.manage_pages): pages are only counted here
+        self.device_pages = kv_cache.free_list is not None
         self.n_slots = n_slots
         self.page_size = kv_cache.page_size
         self.n_pages = kv_cache.n_pages
@@ -273,7 +276,8 @@ class Scheduler:
             req = self.slots[s]
             start = len(req.pages)
             new = [self._free_pages.pop() for _ in range(count)]
-            self.kv_cache.block_table[s, start:start + count] = self._device_ids(new)
+            if not self.device_pages:
+                self.kv_cache.block_table[s, start:start + count] = self._device_ids(new)
             req.pages.extend(new)
 
     def _device_ids(self, ids: list[int]):
@@ -291,7 +295,9 @@ class Scheduler:
             self._free_slots.add(s)
             if s in self.order:
                 self.order.remove(s)
-        if slot_ids:
+        if slot_ids and self.device_pages:
+            self.kv_cache.release(slot_ids)
+        elif slot_ids:
             self.kv_cache.reset(slot_ids)
 
     # ------------------------------------------------------------------ one step
@@ -379,6 +385,9 @@ class Scheduler:
         for s, n in zip(slot_ids, budgets):
             self.slots[s].budget = n
         self._palloc(slot_ids, page_counts)
+        if slot_ids and self.kv_cache.slot_adapters is not None:
+            self.kv_cache.slot_adapters[self._device_ids(slot_ids)] = self._device_ids(
+                [self.slots[s].adapter for s in slot_ids])
 
     def _run_step(self) -> None:
         served = [s for s in self.order if self.slots[s].budget > 0]
@@ -424,16 +433,19 @@ class Scheduler:
 
     # ------------------------------------------------------------------ public surface
 
-    def call(self, prompt: list[int]) -> Future:
+    def call(self, prompt: list[int], adapter: int = -1) -> Future:
+        """A request of ``prompt``, served with low-rank adapter ``adapter`` (``use_adapters``; -1: none)."""
         fut: Future = Future()
         if not self.open:
             fut.set_exception(RuntimeError("Loop is not open."))
+        elif adapter != -1 and not 0 <= adapter < self.kv_cache.n_adapters:
+            fut.set_exception(ValueError(f"No adapter {adapter} of {self.kv_cache.n_adapters}."))
         elif len(prompt) == 0:
             fut.set_exception(ValueError("Empty prompts are not allowed."))
         elif self._required_pages(len(prompt), total=True) > self.n_pages - 1:
             fut.set_exception(ValueError("Possible amount of tokens exceeds available pages."))
         else:
-            self.requests.put(Request(future=fut, prompt=list(prompt), t_arrival=time.perf_counter()))
+            self.requests.put(Request(future=fut, prompt=list(prompt), t_arrival=time.perf_counter(), adapter=adapter))
         return fut
 
     def stop(self) -> None:
@@ -463,9 +475,13 @@ class Scheduler:
             self._end(exc)
             raise
 
-    def generate(self, prompts: list[list[int]]) -> list[RequestResult]:
-        """Serve ``prompts`` to completion in this thread; results in prompt order."""
-        futures = [self.call(p) for p in prompts]
+    def generate(self, prompts: list[list[int]], adapters: list[int] | None = None) -> list[RequestResult]:
+        """Serve ``prompts`` (prompt i with ``adapters[i]``) to completion in this thread; results in prompt order."""
+        if adapters is None:
+            adapters = [-1] * len(prompts)
+        if len(adapters) != len(prompts):
+            raise ValueError("one adapter per prompt")
+        futures = [self.call(p, adapter=i) for p, i in zip(prompts, adapters)]
         self.stop()
         self.loop()
         return [f.result() for f in futures]

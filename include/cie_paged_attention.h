@@ -47,6 +47,14 @@ extern "C" {
                                  batch shape or partials budget (the call wrote
                                  nothing), or a batch with more work items than
                                  its plan holds (cie_mixed_plan)                  */
+#define CIE_ERRBIT_FREE 32    /* a free list with too few pages (or too many given
+                                 back), or a slot that comes twice in the call    */
+#define CIE_ERRBIT_ADAPTER 64 /* adapter id at or past the number of adapters     */
+
+/* Element types of the entry points that take one. */
+#define CIE_F16 0
+#define CIE_BF16 1
+#define CIE_F32 2
 
 /* Version of this ABI (bumped on any signature change). */
 int cie_abi_version(void);
@@ -546,6 +554,123 @@ int cie_q8_mixed(void* o, const void* q, const void* k_pool, const void* v_pool,
                  int64_t pool_page_stride, int64_t pool_head_stride,
                  int64_t bt_stride, int64_t bt_width, int64_t n_slots,
                  int32_t* err, void* stream);
+
+/*
+ * Block tables and slot maps from request lengths.  Sequence b is slot
+ * slot_ids[b], holds lens[slot] tokens (lens (n_slots,)) and has new_tokens[b] new
+ * ones, packed one sequence after another:
+ *   cu_seqlens[b + 1] = cu_seqlens[b] + new_tokens[b]              (B + 1 words)
+ *   row t of sequence b: slots[t] = slot, positions[t] = lens[slot] + t - cu[b],
+ *     pages[t] = block_table[slot, position / page_size],
+ *     offsets[t] = position % page_size                            (T words each)
+ * Rows behind the last sequence get zeros (slot 0 and page 0: the padding rows').
+ * Beside the reference's AttentionMetadata and its mixed step's index recipe
+ * (attn/metadata.py:3-55, scheduler/mixed_module.py:99-132).
+ *
+ * free_list (nullable): n_pages + 2 words: the count of free pages, a word of the
+ * kernels' own (0), and the free pages, the next one last.  With it, each sequence
+ * of a slot other than 0 first gets the pages that its new tokens need, in the
+ * order of the sequences and of their positions: into block_table, and out of the
+ * list.  If the list has too few, or a slot comes twice among sequences with new
+ * tokens, no sequence gets any (CIE_ERRBIT_FREE).  Rows whose page the sequence has
+ * not got are mapped to page 0.
+ * A bad slot id: its rows are padding rows (CIE_ERRBIT_PAGE).  A position past the
+ * table's row: page 0, offset 0, and no new pages for its sequence; rows past T are
+ * dropped, negative counts are 0 (CIE_ERRBIT_LEN).  Page ids are not checked, but
+ * for those of the list (CIE_ERRBIT_PAGE, page 0 in their place).
+ * lens is not advanced.  B <= 2048, T <= 2^24, n_pages and bt_width <= 2^24.
+ */
+int cie_step_maps(int64_t* cu_seqlens, int64_t* slots, int64_t* positions, int64_t* pages,
+                  int64_t* offsets, const int64_t* slot_ids, const int64_t* new_tokens,
+                  const int64_t* lens, int64_t* block_table, int64_t* free_list,
+                  int64_t B, int64_t T, int64_t page_size, int64_t n_pages,
+                  int64_t bt_stride, int64_t bt_width, int64_t n_slots,
+                  int32_t* err, void* stream);
+
+/*
+ * Gives pages back: sequence b keeps keep[b] tokens (NULL: none) of the held[b]
+ * whose pages it has (NULL: lens[slot]; held >= lens[slot], as after cie_step_maps
+ * and before lens is advanced).  Its pages past the kept tokens go back to the list, in the reverse
+ * of the order in which cie_step_maps hands pages out, their table entries become
+ * 0, and lens[slot] = keep[b].  Slot 0 is left as it is.
+ * A slot that comes twice, or a list that has no room for the pages: nothing is
+ * done (CIE_ERRBIT_FREE).  A bad slot id (CIE_ERRBIT_PAGE) or lengths that are not
+ * 0 <= keep <= held <= the table's row, lens[slot] <= held (CIE_ERRBIT_LEN): that
+ * sequence is left as it is.  A bad page id goes into the list as page 0
+ * (CIE_ERRBIT_PAGE).  Sizes as cie_step_maps.
+ */
+int cie_release_pages(int64_t* free_list, const int64_t* slot_ids, int64_t* lens,
+                      int64_t* block_table, const int64_t* keep, const int64_t* held,
+                      int64_t B, int64_t page_size, int64_t n_pages,
+                      int64_t bt_stride, int64_t bt_width, int64_t n_slots,
+                      int32_t* err, void* stream);
+
+/*
+ * Rotary positions.  Pair i of a head's first rot dims, (x, y), becomes
+ *   scale * (x cos a - y sin a, y cos a + x sin a),  a = positions[t] * freqs[i]
+ * with freqs[i] in radians a position (rot / 2 doubles).  Pairs are dims
+ * (i, i + rot / 2), or (2i, 2i + 1) where interleaved; dims from rot on are copied.
+ * Angles are computed in fp64, products and sums in fp32, outputs rounded once.
+ * Beside apply_rotary_pos_emb of the reference's layer (attn/core.py:193-198).
+ *   cie_rotary         q (T, H_q, D) and k (T, H_kv, D) views, their own token and
+ *                      head strides (elements), dims dense; either may have no
+ *                      heads.  Outputs dense, and not in the inputs' memory.
+ *   cie_kv_append_tokens_qkv_rotary
+ *                      from rows of the fused QKV projection, as
+ *                      cie_kv_append_tokens_qkv_rope: q into q_out, k and v into
+ *                      the pools (16-bit types).
+ *   cie_rotary_tables  scale * cos a and scale * sin a for each of rot dims,
+ *                      (T, rot) each.
+ * dtype: CIE_F16, CIE_BF16 or CIE_F32, of inputs and outputs.  rot, D even.
+ */
+int cie_rotary(void* q_out, void* k_out, const void* q, const void* k,
+               int64_t q_tok_stride, int64_t q_head_stride,
+               int64_t k_tok_stride, int64_t k_head_stride,
+               const int64_t* positions, const double* freqs, float scale,
+               int64_t T, int64_t H_q, int64_t H_kv, int64_t D, int64_t rot,
+               int interleaved, int dtype, void* stream);
+int cie_kv_append_tokens_qkv_rotary(void* q_out, void* k_pool, void* v_pool, const void* qkv,
+                                    int64_t qkv_row_stride, const int64_t* positions,
+                                    const double* freqs, float scale,
+                                    const int64_t* pages, const int64_t* offsets,
+                                    int64_t T, int64_t H_q, int64_t H_kv, int64_t page_size,
+                                    int64_t D, int64_t n_pages, int64_t pool_page_stride,
+                                    int64_t pool_head_stride, int64_t rot, int interleaved,
+                                    int dtype, int32_t* err, void* stream);
+int cie_rotary_tables(void* cos, void* sin, const int64_t* positions, const double* freqs,
+                      float scale, int64_t T, int64_t rot, int interleaved, int dtype,
+                      void* stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection:
+ *   y[t, s] += scales[i] * B[i, s] (A[i, s] x[t]),   i = the adapter of row t,
+ * for each slice s of y's columns, in place.  a (N, n_slices, R, d_in) and b
+ * (N, d_out, R) dense, d_out the slices' widths together; scales (N) float;
+ * ranks (N) int32: adapter i has ranks[i] <= R rows of rank, and zeros behind them
+ * in a and b.  Rows without an adapter, and rows behind T, are left as they are.
+ * A x is summed in fp32 and enters the second product as two values of the
+ * element type (22 bits, bf16: 16), that one summed in fp32 and added to y in fp32:
+ * one rounding to the element type at the end.
+ *   cie_adapter_plan   once per step: which rows share an adapter, into `plan`
+ *                      (cie_adapter_plan_bytes(T, N) bytes, 16-byte aligned, any
+ *                      contents).  Row t has adapter slot_adapters[row_slots[t]]
+ *                      (row_slots NULL: slot_adapters[t]); a negative one is none, as
+ *                      is a bad slot (CIE_ERRBIT_PAGE) or one >= N (CIE_ERRBIT_ADAPTER).
+ *   cie_adapter_add    per projection.  A plan made for other T or N: nothing is
+ *                      written, CIE_ERRBIT_PLAN.
+ * slice_widths: n_slices (<= 4) host values.  R a multiple of 16, R <= 128;
+ * N <= 1024, T <= 2^24; dtype CIE_F16 or CIE_BF16; x and y rows are dense, with
+ * their own row strides (elements), x not in y's memory.
+ */
+int64_t cie_adapter_plan_bytes(int64_t T, int64_t N);
+int cie_adapter_plan(int32_t* plan, int64_t plan_bytes, const int64_t* row_slots,
+                     const int64_t* slot_adapters, int64_t T, int64_t n_slots, int64_t N,
+                     int32_t* err, void* stream);
+int cie_adapter_add(void* y, int64_t y_row_stride, const void* x, int64_t x_row_stride,
+                    const void* a, const void* b, const float* scales, const int32_t* ranks,
+                    const int32_t* plan, int64_t plan_bytes, int64_t T, int64_t N, int64_t R,
+                    int64_t d_in, const int64_t* slice_widths, int64_t n_slices,
+                    int dtype, int32_t* err, void* stream);
 
 #ifdef __cplusplus
 }
