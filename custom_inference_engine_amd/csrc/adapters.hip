@@ -193,10 +193,11 @@ __global__ __launch_bounds__(kPlanWaves* kWave) void adapter_plan_kernel(PlanPar
 
 // ---- the products ----
 
-constexpr int kAdWaves = 8;
-constexpr int kAdThreads = kAdWaves * kWave;
 constexpr int kAdBlock = 64;   // values of x a wave takes at a time: two MFMAs
 constexpr int kAdUnits = 8;    // 16-rank units of u held at once: one slice of 128 ranks, or several of fewer
+
+constexpr int kAdWaves = 8;
+constexpr int kAdThreads = kAdWaves * kWave;
 
 struct AddParams {
   void* y;
@@ -207,7 +208,7 @@ struct AddParams {
   const int32_t* ranks;
   const int32_t* plan;
   int64_t y_stride, x_stride;
-  int32_t T, N, M, R, d_in, d_out, n_slices, chunks, col_tiles;
+  int32_t T, N, R, d_in, d_out, n_slices, chunks, col_tiles, max_tiles;
   int32_t slice_col[kAdMaxSlices + 1];   // a slice's first column
   int32_t slice_tile[kAdMaxSlices + 1];  // and its first 64-column tile
   int32_t* err;
@@ -238,53 +239,105 @@ __device__ __forceinline__ int row_shift(float m) {
   return 0;
 }
 
+// Copies 16 bytes a lane from p to the wave's KiB at dst (LDS, lane order), without
+// passing through registers.  Assembly, as the compiler would make every later LDS
+// read wait for all copies in flight; wait_copies publishes them to the wave.
+__device__ __forceinline__ void copy16(void* dst, const void* p) {
+  typedef __attribute__((address_space(3))) char lds_char;
+  const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_char*)dst);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(p) : "memory", "m0");
+}
+__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+// Every LDS read of this wave has returned: what it read may be overwritten.
+__device__ __forceinline__ void wait_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
+
+// Lanes of a wave read what others of it wrote: LDS accesses run in order, and the compiler keeps theirs here.
+__device__ __forceinline__ void lds_order() { asm volatile("" : : : "memory"); }
+
+// LDS of an instance.  A wave has a region of its own: kDepth blocks of x and A on
+// their way to the matrix cores, then its partial sums of u, then B's values for 64
+// columns and the products for 16 rows of them.
+template <int MR, int NT>
+struct AddLds {
+  static constexpr int M = 16 * MR;
+  static constexpr int kDepth = MR == 1 ? (NT == 1 ? 4 : NT < 4 ? 2 : 1) : (NT == 1 ? 2 : 1);
+  static constexpr int kSlab = 2048;                       // 16 rows of 64 values
+  static constexpr int kBlock = (MR + NT) * kSlab;         // a block: x's rows, then A's
+  static constexpr int kSumRow = NT * 16 + 4;              // floats (padded: rows start in other banks)
+  static constexpr int kOutRow = 64 + 4;
+  static constexpr int kB = NT == 1 ? 2048 : NT == 2 ? 4096 : 8192;  // up to 16 * NT (64) ranks of 64 columns
+  static constexpr int kSecond = kB + 16 * kOutRow * 4;
+  static constexpr int kRegion = kDepth * kBlock > kSecond ? kDepth * kBlock : kSecond;
+  static_assert(M * kSumRow * 4 <= kRegion, "partial sums fit a region");
+  static constexpr int kU = kAdUnits * M * 64;             // 16 ranks of u a unit: hi then lo
+  static constexpr int kBytes = kAdWaves * kRegion + kU + M * 4;
+  static_assert(kBytes <= 160 * 1024, "a workgroup's LDS");
+};
+
 template <class E, int MR, int NT, bool kAligned>
 __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
   typedef typename Lane8<E>::type vec;
-  constexpr int M = 16 * MR;
-  constexpr int kRow = NT * 16 + 4;  // floats of a row of partial sums (padded: rows start in other banks)
-  constexpr int kLanes = NT * 4;     // threads that hold a row of u, four ranks each
-  constexpr int kPasses = (kAdUnits + NT - 1) / NT;
-  constexpr int kDepth = MR * NT >= 6 ? 2 : 4;  // blocks of x whose loads are in flight
+  typedef AddLds<MR, NT> L;
+  constexpr int M = L::M, NW = kAdWaves, kDepth = L::kDepth;
+  constexpr int kLanes = NT == 3 ? 16 : NT * 4;  // threads that hold a row of u, four ranks each
+  constexpr int kPasses = NT < 4 ? 1 : kAdUnits / NT;  // (fewer units than four in all: the host's choice)
   static_assert(M * kLanes <= kAdThreads, "a thread has four values of u at most");
-  __shared__ float part[kAdWaves][M][kRow];
-  __shared__ __align__(16) E u_hl[kAdUnits][M][32];  // of 16 ranks, hi then lo
-  __shared__ float factor[M];
+  __shared__ __align__(16) char lds[L::kBytes];
+  E* const u_hl = reinterpret_cast<E*>(lds + NW * L::kRegion);
+  float* const factor = reinterpret_cast<float*>(lds + NW * L::kRegion + L::kU);
 
+  // Which tile, and its rows.  Small launches deal tiles to the XCDs (workgroups go
+  // to the eight in turn) one by one and read the tile's words along with the
+  // header; large ones give an XCD adjacent tiles, mostly of one adapter, whose A
+  // and B then come from its L2.
   const int32_t* const head = p.plan;
-  const int n_tiles = head[0];
+  const int xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
+  int tile, chunk;
+  if constexpr (MR == 1) {
+    chunk = nth % p.chunks;
+    tile = nth / p.chunks * 8 + xcd;
+  } else {
+    const int items = head[0] * p.chunks, share = (items + 7) / 8;
+    const int item = nth < share ? xcd * share + nth : items;
+    tile = item / p.chunks;
+    chunk = item - tile * p.chunks;
+  }
+  const int32_t* const desc = p.plan + kAdHead + (int64_t)min(tile, p.max_tiles - 1) * (kAdTileHead + M);
+  const int tid = threadIdx.x, lane = tid % kWave, wave = uniform(tid / kWave), m = lane % 16, g = lane / 16;
+  const int r8 = lane / 8, c8 = lane % 8;  // memory order: eight rows of eight 16-byte pieces
+  const int adapter = uniform(desc[0]), rows = uniform(desc[1]);
+  int row_of[2 * MR];  // rows r8, 8 + r8, ... of the tile
+#pragma unroll
+  for (int r = 0; r < 2 * MR; ++r) row_of[r] = desc[kAdTileHead + 8 * r + r8];
   if (head[1] != p.T || head[2] != p.N || head[3] != M || head[4] != kAdMagic) {
-    if (threadIdx.x == 0 && blockIdx.x == 0) set_err(p.err, CIE_ERRBIT_PLAN);
+    if (tid == 0 && blockIdx.x == 0) set_err(p.err, CIE_ERRBIT_PLAN);
     return;
   }
-  // An XCD (workgroups go to the eight in turn) takes adjacent tiles, mostly of one
-  // adapter, with all their column ranges: A and B come from its L2 after the first.
-  const int items = n_tiles * p.chunks, share = (items + 7) / 8;
-  const int item = (int)(blockIdx.x % 8) * share + (int)(blockIdx.x / 8);
-  if ((int)(blockIdx.x / 8) >= share || item >= items) return;
-  const int tile = item / p.chunks, chunk = item - tile * p.chunks;
-  const int32_t* const desc = p.plan + kAdHead + (int64_t)tile * (kAdTileHead + M);
-  const int adapter = uniform(desc[0]), rows = uniform(desc[1]);
-  const int units = uniform((p.ranks[adapter] + 15) / 16);
-  if (units <= 0 || units * 16 > p.R) return;
-  const float scale = p.scales[adapter];
-
-  const int tid = threadIdx.x, lane = tid % kWave, wave = uniform(tid / kWave), m = lane % 16, g = lane / 16;
-  int64_t row[MR];
-#pragma unroll
-  for (int r = 0; r < MR; ++r) row[r] = desc[kAdTileHead + min(16 * r + m, rows - 1)];
-
+  if (tile >= head[0]) return;
   const int per_chunk = (p.col_tiles + p.chunks - 1) / p.chunks;
   const int ct0 = chunk * per_chunk, ct1 = min(ct0 + per_chunk, p.col_tiles);
   if (ct0 >= ct1) return;
+  // (a tile's last rows: its first again, not written)
+  const int row0 = uniform(row_of[0]);
+#pragma unroll
+  for (int r = 0; r < 2 * MR; ++r)
+    if (8 * r + r8 >= rows) row_of[r] = row0;
+  const int rank = p.ranks[adapter];
+  const float scale = p.scales[adapter];
+  // With one unit a slice the loads need not wait for the rank: an empty place is left at the end.
+  const int units = p.R == 16 ? 1 : min(uniform((rank + 15) / 16), p.R / 16);
+  if (units <= 0) return;
   int s0 = 0;
   while (s0 + 1 < p.n_slices && p.slice_tile[s0 + 1] <= ct0) ++s0;
   const int at_once = max(1, kAdUnits / units);
 
-  const E* x_row[MR];
+  char* const mine = lds + wave * L::kRegion;
+  const E* x_row[2 * MR];
 #pragma unroll
-  for (int r = 0; r < MR; ++r) x_row[r] = static_cast<const E*>(p.x) + row[r] * p.x_stride;
-  const int blocks = p.d_in / kAdBlock;
+  for (int r = 0; r < 2 * MR; ++r) x_row[r] = static_cast<const E*>(p.x) + row_of[r] * p.x_stride;
+  const int blocks = (p.d_in + kAdBlock - 1) / kAdBlock, whole = kAligned ? p.d_in / kAdBlock : 0;
+  // Slabs hold piece c of row r in place c ^ (r % 8): the lanes that read a piece of 16 rows meet no bank twice.
+  const int k8 = 8 * (c8 ^ r8);
 
   for (; s0 < p.n_slices && p.slice_tile[s0] < ct1; s0 += at_once) {
     int s1 = s0 + 1;  // slices [s0, s1) of this workgroup's columns
@@ -297,73 +350,97 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
     for (int pass = 0; pass < kPasses; ++pass) {
       kept[pass] = f32x4{0.f, 0.f, 0.f, 0.f};
       if (pass * NT >= n_units) continue;
-      const E* a_row[NT];
+      const E* a_row[NT];  // row r8 of a unit; its row 8 + r8 is 8 d_in further
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int i = min(pass * NT + n, n_units - 1), s = s0 + i / units;
         a_row[n] = static_cast<const E*>(p.a) +
-                   (((int64_t)adapter * p.n_slices + s) * p.R + 16 * (i % units) + m) * p.d_in;
+                   (((int64_t)adapter * p.n_slices + s) * p.R + 16 * (i % units) + r8) * p.d_in;
       }
       f32x4 acc[MR][NT] = {};
-      if constexpr (kAligned) {
-        for (int b = wave; b < blocks; b += kAdWaves * kDepth) {
-          vec xv[kDepth][MR][2], av[kDepth][NT][2];
+
+      // Block b's rows into place d of the wave's region.
+      const auto fetch = [&](int b, int d) {
+        char* const to = mine + d * L::kBlock;
+        const int k = b * kAdBlock + k8;
+        if (b < whole) {
 #pragma unroll
-          for (int d = 0; d < kDepth; ++d) {
-            // (past the end: the last block again, not used)
-            const int k = min(b + d * kAdWaves, blocks - 1) * kAdBlock + 16 * g;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-#pragma unroll
-              for (int r = 0; r < MR; ++r) xv[d][r][j] = *reinterpret_cast<const vec*>(x_row[r] + k + 8 * j);
-#pragma unroll
-              for (int n = 0; n < NT; ++n) av[d][n][j] = *reinterpret_cast<const vec*>(a_row[n] + k + 8 * j);
-            }
-          }
-#pragma unroll
-          for (int d = 0; d < kDepth; ++d) {
-            if (b + d * kAdWaves >= blocks) break;
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-              for (int r = 0; r < MR; ++r)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) acc[r][n] = mma(av[d][n][j], xv[d][r][j], acc[r][n]);
-          }
-        }
-      }
-      // The last values of a row, fewer than a block; unaligned rows: all of them.
-      for (int b = kAligned ? blocks + (wave - blocks % kAdWaves + kAdWaves) % kAdWaves : wave;
-           b * kAdBlock < p.d_in; b += kAdWaves) {
-        const int k = b * kAdBlock + 16 * g;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          vec xv[MR];
-#pragma unroll
-          for (int r = 0; r < MR; ++r) xv[r] = load8<E, kAligned>(x_row[r], k + 8 * j, p.d_in);
+          for (int r = 0; r < 2 * MR; ++r) copy16(to + 1024 * r, x_row[r] + k);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const vec av = load8<E, kAligned>(a_row[n], k + 8 * j, p.d_in);
-#pragma unroll
-            for (int r = 0; r < MR; ++r) acc[r][n] = mma(av, xv[r], acc[r][n]);
+            if (pass * NT + n >= n_units) continue;
+            copy16(to + (MR + n) * L::kSlab, a_row[n] + k);
+            copy16(to + (MR + n) * L::kSlab + 1024, a_row[n] + k + (int64_t)8 * p.d_in);
           }
+        } else {  // a row's last values, fewer than a block; unaligned rows: all of them
+#pragma unroll
+          for (int r = 0; r < 2 * MR; ++r)
+            reinterpret_cast<vec*>(to + 1024 * r)[lane] = load8<E, kAligned>(x_row[r], k, p.d_in);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            if (pass * NT + n >= n_units) continue;
+            vec* const at = reinterpret_cast<vec*>(to + (MR + n) * L::kSlab) + lane;
+            at[0] = load8<E, kAligned>(a_row[n], k, p.d_in);
+            at[64] = load8<E, kAligned>(a_row[n] + (int64_t)8 * p.d_in, k, p.d_in);
+          }
+        }
+      };
+      int b = wave;
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d)
+        if (b + d * NW < blocks) fetch(b + d * NW, d);
+      for (; b < blocks; b += NW * kDepth) {
+        vec xv[kDepth][MR][2], av[kDepth][NT][2];
+        wait_copies();
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) {
+          if (b + d * NW >= blocks) break;
+          const char* const from = mine + d * L::kBlock + m * 128;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int at = 16 * ((4 * j + g) ^ (m % 8));
+#pragma unroll
+            for (int r = 0; r < MR; ++r) xv[d][r][j] = *reinterpret_cast<const vec*>(from + r * L::kSlab + at);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              if (pass * NT + n < n_units)
+                av[d][n][j] = *reinterpret_cast<const vec*>(from + (MR + n) * L::kSlab + at);
+          }
+        }
+        wait_lds_reads();
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d)
+          if (b + (d + kDepth) * NW < blocks) fetch(b + (d + kDepth) * NW, d);
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) {
+          if (b + d * NW >= blocks) break;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              if (pass * NT + n < n_units) {
+#pragma unroll
+                for (int r = 0; r < MR; ++r) acc[r][n] = mma(av[d][n][j], xv[d][r][j], acc[r][n]);
+              }
         }
       }
       // A lane has ranks 4g .. 4g + 3 of token m.
+      float* const sums = reinterpret_cast<float*>(mine) + m * L::kSumRow + 4 * g;
 #pragma unroll
       for (int r = 0; r < MR; ++r)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
-          *reinterpret_cast<f32x4*>(&part[wave][16 * r + m][16 * n + 4 * g]) = acc[r][n];
+          *reinterpret_cast<f32x4*>(sums + 16 * r * L::kSumRow + 16 * n) = acc[r][n];
       __syncthreads();
       if (tid < M * kLanes) {
         const int t = tid / kLanes, q = tid % kLanes;
-        if (pass * NT + q / 4 < n_units) {
+        if (q / 4 < NT && pass * NT + q / 4 < n_units) {
 #pragma unroll
-          for (int w = 0; w < kAdWaves; ++w) kept[pass] += *reinterpret_cast<const f32x4*>(&part[w][t][4 * q]);
+          for (int w = 0; w < NW; ++w)
+            kept[pass] += reinterpret_cast<const f32x4*>(lds + w * L::kRegion)[t * (L::kSumRow / 4) + q];
         }
       }
-      __syncthreads();
+      if (kPasses > 1) __syncthreads();
     }
 
     if (tid < M * kLanes) {
@@ -385,78 +462,121 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
       }
 #pragma unroll
       for (int pass = 0; pass < kPasses; ++pass) {
-        if (pass * NT + q / 4 >= n_units) continue;
-        E* const to = &u_hl[pass * NT + q / 4][t][4 * (q % 4)];
+        const int i = pass * NT + q / 4;
+        if (q / 4 >= NT || i >= n_units) continue;
+        // Of two units side by side the first has both his, the second both los; a last
+        // one has its hi, then its lo.
+        const int of = i % units, s = i - of, r = 4 * (q % 4);
+        const bool pair = (of | 1) < units;
+        E* const hi = u_hl + ((s + (pair ? of & ~1 : of)) * M + t) * 32 + (pair ? 16 * (of & 1) : 0) + r;
+        E* const lo = u_hl + ((s + (pair ? of | 1 : of)) * M + t) * 32 + (pair ? 16 * (of & 1) : 16) + r;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float v = __builtin_ldexpf(kept[pass][e], shift);
-          const E hi = (E)v;
-          const float left = v - (float)hi;
-          to[e] = hi;
-          to[16 + e] = (E)(__builtin_isfinite(left) ? left : 0.f);  // (of an infinity or a NaN: hi says it all)
+          hi[e] = (E)v;
+          const float left = v - (float)(E)v;
+          lo[e] = (E)(__builtin_isfinite(left) ? left : 0.f);  // (of an infinity or a NaN: hi says it all)
         }
       }
       if (q == 0) factor[t] = __builtin_ldexpf(scale, -shift);
     }
     __syncthreads();
+    if (rank <= 0) return;
 
-    // y += scale B u: 64 columns at a time.  B's rows are dealt so that a lane ends
-    // with 16 adjacent columns of its token: row m of part j is column
-    // 16 (m / 4) + 4 j + m % 4.
+    // y += scale B u: 64 columns at a time, B's rows as rows and tokens as columns of
+    // the product, which goes through LDS to the memory's order.
     const int first = max(ct0, p.slice_tile[s0]), last = min(ct1, p.slice_tile[s1]);
-    for (int ct = first + wave; ct < last; ct += kAdWaves) {
+    float* const out = reinterpret_cast<float*>(mine + L::kB);
+    constexpr int kGroup = NT < 4 ? NT : 4;  // units whose B values are in LDS at once
+    for (int ct = first + wave; ct < last; ct += NW) {
       int s = s0;
       while (s + 1 < s1 && p.slice_tile[s + 1] <= ct) ++s;
       const int col = p.slice_col[s] + (ct - p.slice_tile[s]) * 64, end = p.slice_col[s + 1];
-      const E* b_row[4];
+      vec yv[2 * MR];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int d = min(col + 16 * (m / 4) + 4 * j + m % 4, end - 1);
-        b_row[j] = static_cast<const E*>(p.b) + ((int64_t)adapter * p.d_out + d) * p.R + 8 * (g & 1);
-      }
-      vec yv[MR][2];
-#pragma unroll
-      for (int r = 0; r < MR; ++r)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const E* const from = static_cast<const E*>(p.y) + row[r] * p.y_stride;
-          yv[r][h] = load8<E, kAligned>(from, col + 16 * g + 8 * h, end);
-        }
+      for (int r = 0; r < 2 * MR; ++r)
+        yv[r] = load8<E, kAligned>(static_cast<const E*>(p.y) + row_of[r] * p.y_stride, col + 8 * c8, end);
       f32x4 acc[MR][4] = {};
-      for (int i = 0; i < units; ++i) {
-        vec bv[4], uv[MR];
+      for (int i0 = 0; i0 < units; i0 += kGroup) {
+        const int n = min(units - i0, kGroup);
+        // Columns of 2, 4 or 8 pieces, piece c of column d in place c ^ (d / (8 / pieces) % pieces).
+        const int shift = n == 1 ? 1 : n == 2 ? 2 : 3, pieces = 1 << shift;
+        const E* const from = static_cast<const E*>(p.b) + ((int64_t)adapter * p.d_out + col) * p.R + 16 * i0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) bv[j] = *reinterpret_cast<const vec*>(b_row[j] + 16 * i);
+        for (int k = 0; k < 2 * (kGroup == 3 ? 4 : kGroup); ++k) {
+          if (k >= pieces) break;
+          const int d = (64 * k + lane) >> shift, c = lane % pieces ^ (d >> (3 - shift)) % pieces;
+          if (c < 2 * n) copy16(mine + 1024 * k, from + (int64_t)min(d, end - 1 - col) * p.R + 8 * c);
+        }
+        wait_copies();
+        const auto b_at = [&](int j, int c) {  // piece c of column 16 j + m
+          const int d = 16 * j + m;
+          return *reinterpret_cast<const vec*>(mine + ((d << shift) + (c ^ (d >> (3 - shift)) % pieces)) * 16);
+        };
+        const auto u_at = [&](int i, int r) {
+          return *reinterpret_cast<const vec*>(u_hl + (((s - s0) * units + i0 + i) * M + 16 * r + m) * 32 + 8 * g);
+        };
+        int i = 0;
+        for (; i + 1 < n; i += 2) {  // 32 ranks: their his, then their los
+          vec bv[4], uv[2][MR];
 #pragma unroll
-        for (int r = 0; r < MR; ++r)
-          uv[r] = *reinterpret_cast<const vec*>(&u_hl[(s - s0) * units + i][16 * r + m][8 * g]);
+          for (int j = 0; j < 4; ++j) bv[j] = b_at(j, 2 * i + g);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+          for (int l = 0; l < 2; ++l)
 #pragma unroll
-          for (int r = 0; r < MR; ++r) acc[r][j] = mma(bv[j], uv[r], acc[r][j]);
+            for (int r = 0; r < MR; ++r) uv[l][r] = u_at(i + l, r);
+#pragma unroll
+          for (int l = 0; l < 2; ++l)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int r = 0; r < MR; ++r) acc[r][j] = mma(bv[j], uv[l][r], acc[r][j]);
+        }
+        if (i < n) {  // 16 ranks: hi and lo in one K of 32, B's values twice
+          vec bv[4], uv[MR];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) bv[j] = b_at(j, 2 * i + g % 2);
+#pragma unroll
+          for (int r = 0; r < MR; ++r) uv[r] = u_at(i, r);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < MR; ++r) acc[r][j] = mma(bv[j], uv[r], acc[r][j]);
+        }
+        wait_lds_reads();
       }
 #pragma unroll
       for (int r = 0; r < MR; ++r) {
-        if (16 * r + m >= rows) continue;
-        const float f = factor[16 * r + m];
-        E* const to = static_cast<E*>(p.y) + row[r] * p.y_stride;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(out + m * L::kOutRow + 16 * j + 4 * g) = acc[r][j];
+        lds_order();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int c = col + 16 * g + 8 * h;
-          vec out;
+          const int t = 8 * h + r8, c = col + 8 * c8;
+          const f32x4* const got = reinterpret_cast<const f32x4*>(out + t * L::kOutRow + 8 * c8);
+          const f32x4 lo = got[0], hi = got[1];
+          if (16 * r + t >= rows) continue;
+          const float f = factor[16 * r + t];
+          E* const to = static_cast<E*>(p.y) + row_of[2 * r + h] * p.y_stride;
+          vec v;
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            out[e] = (E)__builtin_fmaf(acc[r][2 * h + e / 4][e % 4], f, (float)yv[r][h][e]);
+          for (int e = 0; e < 8; ++e) {
+            float sum = __builtin_fmaf(e < 4 ? lo[e % 4] : hi[e % 4], f, (float)yv[2 * r + h][e]);
+            asm volatile("" : "+v"(sum));  // (to fp32 first, in every variant: no v_fma_mixlo_f16)
+            v[e] = (E)sum;
+          }
           if constexpr (kAligned) {
-            if (c < end) *reinterpret_cast<vec*>(to + c) = out;
+            if (c < end) *reinterpret_cast<vec*>(to + c) = v;
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              if (c + e < end) to[c + e] = out[e];
+              if (c + e < end) to[c + e] = v[e];
           }
         }
+        lds_order();
       }
     }
+    if (s0 + at_once < p.n_slices) __syncthreads();  // (the regions and u are used again)
   }
 }
 
@@ -465,17 +585,20 @@ static bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr
 template <class E, int MR, bool kAligned>
 static void launch_add(const AddParams& p, int units, dim3 grid, hipStream_t stream) {
   // Few units in all: no registers or partial sums for more.
+  const dim3 block(kAdThreads);
   if (kAligned && units == 1)
-    hipLaunchKernelGGL((adapter_add_kernel<E, MR, kAligned ? 1 : 4, kAligned>), grid, dim3(kAdThreads), 0, stream, p);
+    hipLaunchKernelGGL((adapter_add_kernel<E, MR, kAligned ? 1 : 4, kAligned>), grid, block, 0, stream, p);
   else if (kAligned && units == 2)
-    hipLaunchKernelGGL((adapter_add_kernel<E, MR, kAligned ? 2 : 4, kAligned>), grid, dim3(kAdThreads), 0, stream, p);
+    hipLaunchKernelGGL((adapter_add_kernel<E, MR, kAligned ? 2 : 4, kAligned>), grid, block, 0, stream, p);
+  else if (kAligned && units == 3)
+    hipLaunchKernelGGL((adapter_add_kernel<E, MR, kAligned ? 3 : 4, kAligned>), grid, block, 0, stream, p);
   else
-    hipLaunchKernelGGL((adapter_add_kernel<E, MR, 4, kAligned>), grid, dim3(kAdThreads), 0, stream, p);
+    hipLaunchKernelGGL((adapter_add_kernel<E, MR, 4, kAligned>), grid, block, 0, stream, p);
 }
 
 template <class E>
 static int dispatch_add(const AddParams& p, int units, bool aligned, dim3 grid, hipStream_t stream) {
-  if (p.M == 16)
+  if (tile_rows(p.T) == 16)
     aligned ? launch_add<E, 1, true>(p, units, grid, stream) : launch_add<E, 1, false>(p, units, grid, stream);
   else
     aligned ? launch_add<E, 2, true>(p, units, grid, stream) : launch_add<E, 2, false>(p, units, grid, stream);
@@ -554,7 +677,7 @@ extern "C" int cie_adapter_add(void* y, int64_t y_row_stride, const void* x, int
   p.x_stride = x_row_stride;
   p.T = (int32_t)T;
   p.N = (int32_t)N;
-  p.M = tile_rows(T);
+  p.max_tiles = (int32_t)max_tiles(T, N, tile_rows(T));
   p.R = (int32_t)R;
   p.d_in = (int32_t)d_in;
   p.d_out = (int32_t)d_out;
@@ -563,11 +686,11 @@ extern "C" int cie_adapter_add(void* y, int64_t y_row_stride, const void* x, int
   p.err = err;
   // Few tiles: several workgroups share one's columns (each computes u again), down to a
   // column tile a wave.
-  const int64_t bound = max_tiles(T, N, p.M);
-  int64_t chunks = 512 / bound;
-  if (chunks > (tiles + kAdWaves - 1) / kAdWaves) chunks = (tiles + kAdWaves - 1) / kAdWaves;
-  p.chunks = (int32_t)(chunks < 1 ? 1 : chunks);
-  const int64_t blocks = (bound * p.chunks + 7) / 8 * 8;
+  const int64_t per_tile = (tiles + kAdWaves - 1) / kAdWaves;
+  int64_t chunks = 512 / p.max_tiles;
+  chunks = chunks < 1 ? 1 : chunks > per_tile ? per_tile : chunks;
+  p.chunks = (int32_t)chunks;
+  const int64_t blocks = (int64_t)(p.max_tiles + 7) / 8 * 8 * chunks;
   if (blocks > 0x7fffffff) return CIE_EUNSUPPORTED;
   const dim3 grid((unsigned)blocks);
   const int units = (int)(n_slices * (R / 16) < 5 ? n_slices * (R / 16) : 4);

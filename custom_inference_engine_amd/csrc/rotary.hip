@@ -89,6 +89,7 @@ __device__ __forceinline__ void turn(Pack<E, V>& lo, Pack<E, V>& hi, const float
     const float a = x[i0], b = x[i1];
     x[i0] = __builtin_fmaf(a, c[j], -(b * s[j]));
     x[i1] = __builtin_fmaf(b, c[j], a * s[j]);
+    asm volatile("" : "+v"(x[i0]), "+v"(x[i1]));  // (to fp32 first, in every variant: no v_fma_mixlo_f16)
   }
 #pragma unroll
   for (int j = 0; j < V; ++j) {
