@@ -52,7 +52,8 @@ constexpr int kAdMagic = 0x61647031;
 // Header words: tiles, T, N, M, kAdMagic; then tiles of kAdTileHead + M words:
 // adapter, rows, two unused, the rows' indexes.
 constexpr int kAdHead = 8, kAdTileHead = 4;
-constexpr int kPlanWaves = 8;
+constexpr int kPlanWaves = 16;
+constexpr int kPlanThreads = kPlanWaves * kWave;
 constexpr int kPlanBatch = 8;  // rows of a lane whose loads are in flight
 
 // Rows of a tile: more share A's and B's reads, fewer fill the chip.
@@ -67,117 +68,110 @@ struct PlanParams {
   const int64_t* row_slots;
   const int64_t* slot_adapters;
   int64_t T, n_slots;
-  int32_t N, M;
+  int32_t N, M, log_m;
   int32_t* err;
 };
 
-// A lane's next rows' adapters (-1: none): rows first, first + 64, ...
-__device__ __forceinline__ void load_ids(const PlanParams& p, int64_t first, int64_t end, int* id, int& mistakes) {
-  int64_t slot[kPlanBatch];
-#pragma unroll
-  for (int i = 0; i < kPlanBatch; ++i) {
-    const int64_t row = first + i * kWave;
-    slot[i] = row < end ? (p.row_slots ? p.row_slots[row] : row) : 0;
-  }
-#pragma unroll
-  for (int i = 0; i < kPlanBatch; ++i) {
-    const bool ok = slot[i] >= 0 && slot[i] < p.n_slots;
-    const int64_t a = p.slot_adapters[ok ? slot[i] : 0];
-    id[i] = -1;
-    if (first + i * kWave >= end) continue;
-    if (!ok)
-      mistakes |= CIE_ERRBIT_PAGE;
-    else if (a >= p.N)
-      mistakes |= CIE_ERRBIT_ADAPTER;
-    else if (a >= 0)
-      id[i] = (int)a;
-  }
-}
-
 // Rows are dealt to the waves in order, 64 adjacent rows at a time, and each wave
 // counts its own, so that a group's rows keep their order and the plan is the same
-// every time.  Two dependent loads, the count, a scan over adapters, the rows.
-__global__ __launch_bounds__(kPlanWaves* kWave) void adapter_plan_kernel(PlanParams p) {
-  extern __shared__ int lds[];
-  __shared__ int sums[kPlanWaves];
-  int* const count = lds;                    // [kPlanWaves][N]: rows of a wave, then the next one's place
-  int* const tile0 = lds + kPlanWaves * p.N;  // [N] first tile of an adapter
+// every time.  Lanes of one adapter find each other by a ballot a bit of its number,
+// and the first of them takes as many places as they are.  Two dependent loads, the
+// count, a scan over adapters, the rows.  The code is kept short (loops are not
+// unrolled but for the loads'): it runs once, from a cold instruction cache.
+__global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p) {
+  __shared__ int count[kPlanWaves * kAdMaxAdapters];  // [wave][N]: rows of a wave, then their first place
+  __shared__ int tile0[kAdMaxAdapters], sums[kPlanWaves];
+  __shared__ int seen[kPlanWaves][kPlanBatch][kWave];  // a batch's adapters and places (kPlaceBits), -1: none
+  constexpr int kPlaceBits = 21;                       // (a wave has 2^20 rows at most)
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int64_t share = (p.T + kPlanWaves * kWave - 1) / (kPlanWaves * kWave) * kWave;
+  const int64_t share = (p.T + kPlanThreads - 1) / kPlanThreads * kWave;
   const int64_t first = wave * share, end = min(first + share, p.T);
-  for (int i = tid; i < kPlanWaves * p.N; i += kPlanWaves * kWave) count[i] = 0;
-  __syncthreads();
+  const int waves = (int)min((p.T + share - 1) / share, (int64_t)kPlanWaves);  // that have rows
+  const int bits = 32 - __builtin_clz(p.N);
+  const uint64_t below = (1ull << lane) - 1;
+  int* const mine = count + wave * p.N;
 
-  int mistakes = 0;
-  int id[kPlanBatch];
-  for (int64_t at = first; at < end; at += kPlanBatch * kWave) {
-    load_ids(p, at + lane, end, id, mistakes);
-#pragma unroll
-    for (int i = 0; i < kPlanBatch; ++i) {
-      uint64_t todo = __ballot(id[i] >= 0);
-      while (todo) {
-        const int a = __builtin_amdgcn_readlane(id[i], __builtin_ctzll(todo));
-        const uint64_t same = __ballot(id[i] == a);
-        if (lane == 0) atomicAdd(&count[wave * p.N + a], __popcll(same));
-        todo &= ~same;
-      }
-    }
-  }
-  __syncthreads();
-
-  // Adapter a's rows before each wave's, and its tiles.  A thread has up to two adapters.
-  const int per = (p.N + kPlanWaves * kWave - 1) / (kPlanWaves * kWave);
-  int tiles = 0;
-  for (int a = tid * per; a < min(tid * per + per, p.N); ++a) {
-    int n = 0;
-    for (int w = 0; w < kPlanWaves; ++w) {
-      const int c = count[w * p.N + a];
-      count[w * p.N + a] = n;
-      n += c;
-    }
-    tile0[a] = tiles;
-    tiles += (n + p.M - 1) / p.M;
-  }
-  const int incl = wave_inclusive_sum(tiles);
-  if (lane == kWave - 1) sums[wave] = incl;
-  __syncthreads();
-  int before = incl - tiles, total = 0;
-  for (int w = 0; w < kPlanWaves; ++w) {
-    if (w < wave) before += sums[w];
-    total += sums[w];
-  }
-  for (int a = tid * per; a < min(tid * per + per, p.N); ++a) tile0[a] += before;
-  __syncthreads();
-
+  int mistakes = 0, before = 0, total = 0, n = 0, tiles = 0;
   int* const out = p.plan + kAdHead;
   const int words = kAdTileHead + p.M;
-  for (int64_t at = first; at < end; at += kPlanBatch * kWave) {
-    if (share > kPlanBatch * kWave) load_ids(p, at + lane, end, id, mistakes);  // (else they are still there)
+  const bool again = share > kPlanBatch * kWave;  // (else a wave's places are still there the second time)
+  for (int i = tid; i < waves * p.N; i += kPlanThreads) count[i] = 0;
+  __syncthreads();
+  for (int pass = 0; pass < 2; ++pass) {  // counted, then written
+    for (int64_t at = first; at < end; at += kPlanBatch * kWave) {
+      const int batch = (int)min((end - at + kWave - 1) / kWave, (int64_t)kPlanBatch);
+      if (pass == 0 || again) {
+        int64_t slot[kPlanBatch];
 #pragma unroll
-    for (int i = 0; i < kPlanBatch; ++i) {
-      uint64_t todo = __ballot(id[i] >= 0);
-      while (todo) {
-        const int a = __builtin_amdgcn_readlane(id[i], __builtin_ctzll(todo));
-        const uint64_t same = __ballot(id[i] == a);
-        int base = 0;
-        if (lane == 0) base = atomicAdd(&count[wave * p.N + a], __popcll(same));
-        base = __builtin_amdgcn_readlane(base, 0);
-        if (id[i] == a) {
-          const int k = base + __popcll(same & ((1ull << lane) - 1));
-          int* const tile = out + (int64_t)(tile0[a] + k / p.M) * words;
-          tile[kAdTileHead + k % p.M] = (int)(at + i * kWave + lane);
+        for (int i = 0; i < kPlanBatch; ++i) {
+          const int64_t row = at + lane + i * kWave;
+          slot[i] = row < end ? (p.row_slots ? p.row_slots[row] : row) : -1;
+          if (row < end && (slot[i] < 0 || slot[i] >= p.n_slots)) {
+            mistakes |= CIE_ERRBIT_PAGE;
+            slot[i] = -1;
+          }
         }
-        todo &= ~same;
+#pragma unroll
+        for (int i = 0; i < kPlanBatch; ++i) {
+          const int64_t a = p.slot_adapters[max(slot[i], (int64_t)0)];
+          const bool none = slot[i] < 0 || a < 0 || a >= p.N;
+          if (slot[i] >= 0 && a >= p.N) mistakes |= CIE_ERRBIT_ADAPTER;
+          seen[wave][i][lane] = none ? -1 : (int)a << kPlaceBits;
+        }
+      }
+#pragma unroll 1
+      for (int i = 0; i < batch; ++i) {
+        const int was = seen[wave][i][lane], id = was >> kPlaceBits;
+        const bool live = was >= 0;
+        int place = was & ((1 << kPlaceBits) - 1);
+        if (pass == 0 || again) {
+          uint64_t same = __ballot(live);
+#pragma unroll 1
+          for (int k = 0; k < bits; ++k) {
+            const uint64_t ones = __ballot(id >> k & 1);
+            same &= id >> k & 1 ? ones : ~ones;
+          }
+          int from = 0;
+          if (live && (same & below) == 0) from = atomicAdd(&mine[id], __popcll(same));
+          place = __shfl(from, live ? __builtin_ctzll(same) : 0, kWave) + __popcll(same & below);
+          if (pass == 0 && !again && live) seen[wave][i][lane] = id << kPlaceBits | place;
+        }
+        if (pass == 1 && live) {
+          const int k = place + (again ? 0 : mine[id]);
+          out[(int64_t)(tile0[id] + (k >> p.log_m)) * words + kAdTileHead + (k & (p.M - 1))] =
+              (int)(at + i * kWave + lane);
+        }
       }
     }
+    if (pass == 1) break;
+    __syncthreads();
+    // Adapter a's rows before each wave's, and its tiles.
+    if (tid < p.N) {
+#pragma unroll 1
+      for (int w = 0; w < waves; ++w) {
+        const int c = count[w * p.N + tid];
+        count[w * p.N + tid] = n;
+        n += c;
+      }
+    }
+    tiles = (n + p.M - 1) >> p.log_m;
+    const int incl = wave_inclusive_sum(tiles);
+    if (lane == kWave - 1) sums[wave] = incl;
+    __syncthreads();
+    before = incl - tiles;
+#pragma unroll 1
+    for (int w = 0; w < kPlanWaves; ++w) {
+      if (w < wave) before += sums[w];
+      total += sums[w];
+    }
+    if (tid < p.N) tile0[tid] = before;
+    __syncthreads();
   }
-  __syncthreads();
-  // (the last wave's next place is now each adapter's row count)
-  for (int a = tid; a < p.N; a += kPlanWaves * kWave) {
-    const int n = count[(kPlanWaves - 1) * p.N + a];
-    for (int k = 0; k * p.M < n; ++k) {
-      int* const tile = out + (int64_t)(tile0[a] + k) * words;
-      tile[0] = a;
+  if (tid < p.N) {
+#pragma unroll 1
+    for (int k = 0; k < tiles; ++k) {
+      int* const tile = out + (int64_t)(before + k) * words;
+      tile[0] = tid;
       tile[1] = min(n - k * p.M, p.M);
     }
   }
@@ -208,7 +202,7 @@ struct AddParams {
   const int32_t* ranks;
   const int32_t* plan;
   int64_t y_stride, x_stride;
-  int32_t T, N, R, d_in, d_out, n_slices, chunks, col_tiles, max_tiles;
+  int32_t T, N, R, d_in, d_out, n_slices, chunks, per_chunk, col_tiles, max_tiles;
   int32_t slice_col[kAdMaxSlices + 1];   // a slice's first column
   int32_t slice_tile[kAdMaxSlices + 1];  // and its first 64-column tile
   int32_t* err;
@@ -254,37 +248,45 @@ __device__ __forceinline__ void wait_lds_reads() { asm volatile("s_waitcnt lgkmc
 // Lanes of a wave read what others of it wrote: LDS accesses run in order, and the compiler keeps theirs here.
 __device__ __forceinline__ void lds_order() { asm volatile("" : : : "memory"); }
 
-// LDS of an instance.  A wave has a region of its own: kDepth blocks of x and A on
-// their way to the matrix cores, then its partial sums of u, then B's values for 64
-// columns and the products for 16 rows of them.
+// LDS of an instance.  A wave has a region of its own: a stage, which holds kDepth
+// blocks of x and A on their way to the matrix cores, then the wave's partial sums of
+// u, then the products for 16 rows of 64 columns; and room for B's values.
 template <int MR, int NT>
 struct AddLds {
   static constexpr int M = 16 * MR;
   static constexpr int kDepth = MR == 1 ? (NT == 1 ? 4 : NT < 4 ? 2 : 1) : (NT == 1 ? 2 : 1);
-  static constexpr int kSlab = 2048;                       // 16 rows of 64 values
-  static constexpr int kBlock = (MR + NT) * kSlab;         // a block: x's rows, then A's
-  static constexpr int kSumRow = NT * 16 + 4;              // floats (padded: rows start in other banks)
+  static constexpr int kSlab = 2048;                // 16 rows of 64 values
+  static constexpr int kBlock = (MR + NT) * kSlab;  // a block: x's rows, then A's
+  static constexpr int kStage = kDepth * kBlock;
+  static constexpr int kSumRow = NT * 16 + 4;       // floats (padded: rows start in other banks)
   static constexpr int kOutRow = 64 + 4;
-  static constexpr int kB = NT == 1 ? 2048 : NT == 2 ? 4096 : 8192;  // up to 16 * NT (64) ranks of 64 columns
-  static constexpr int kSecond = kB + 16 * kOutRow * 4;
-  static constexpr int kRegion = kDepth * kBlock > kSecond ? kDepth * kBlock : kSecond;
-  static_assert(M * kSumRow * 4 <= kRegion, "partial sums fit a region");
-  static constexpr int kU = kAdUnits * M * 64;             // 16 ranks of u a unit: hi then lo
+  static constexpr int kOut = 16 * kOutRow * 4;
+  // B's values for 64 columns: 2 KiB a unit.  One or two units have room beside the
+  // stage, and come in while it is in use; more (up to 8 KiB) lie behind the products.
+  static constexpr int kB = NT == 1 || (NT == 3 && MR == 1) ? 2048 : 4096;
+  static constexpr int kGroup = NT < 4 ? NT : 4;    // units whose B values are in LDS at once
+  static constexpr int kRegion = kStage + kB;
+  static_assert(M * kSumRow * 4 <= kStage && kOut <= kStage, "sums and products fit the stage");
+  static_assert((kGroup < 3 ? kGroup * 2048 : 8192) <= (kGroup < 3 ? kB : kRegion - kOut), "B's values fit");
+  static constexpr int kU = kAdUnits * M * 64;      // 16 ranks of u a unit: in fp32, then hi and lo
   static constexpr int kBytes = kAdWaves * kRegion + kU + M * 4;
   static_assert(kBytes <= 160 * 1024, "a workgroup's LDS");
 };
 
+// The code of small launches is kept short: each runs once, and a workgroup waits
+// some 0.25 us for each further KiB of instructions (7.3 us with loops unrolled,
+// 16 KB, for one row into three slices).
 template <class E, int MR, int NT, bool kAligned>
 __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
   typedef typename Lane8<E>::type vec;
   typedef AddLds<MR, NT> L;
   constexpr int M = L::M, NW = kAdWaves, kDepth = L::kDepth;
-  constexpr int kLanes = NT == 3 ? 16 : NT * 4;  // threads that hold a row of u, four ranks each
-  constexpr int kPasses = NT < 4 ? 1 : kAdUnits / NT;  // (fewer units than four in all: the host's choice)
-  static_assert(M * kLanes <= kAdThreads, "a thread has four values of u at most");
+  constexpr int kLanes = NT == 3 ? 16 : NT * 4;  // threads that sum a row of u, four ranks each
+  constexpr int kHeld = NT < 4 ? NT : kAdUnits;  // units of u (fewer than four in all: the host's choice)
+  static_assert(M * 16 <= kAdThreads, "a thread sums four values of u at most, and splits one a unit");
   __shared__ __align__(16) char lds[L::kBytes];
-  E* const u_hl = reinterpret_cast<E*>(lds + NW * L::kRegion);
-  float* const factor = reinterpret_cast<float*>(lds + NW * L::kRegion + L::kU);
+  char* const u_lds = lds + NW * L::kRegion;  // [unit][token]: 16 floats, or 16 his and 16 los
+  float* const factor = reinterpret_cast<float*>(u_lds + L::kU);
 
   // Which tile, and its rows.  Small launches deal tiles to the XCDs (workgroups go
   // to the eight in turn) one by one and read the tile's words along with the
@@ -314,9 +316,14 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
     return;
   }
   if (tile >= head[0]) return;
-  const int per_chunk = (p.col_tiles + p.chunks - 1) / p.chunks;
-  const int ct0 = chunk * per_chunk, ct1 = min(ct0 + per_chunk, p.col_tiles);
-  if (ct0 >= ct1) return;
+  const int ct0 = chunk * p.per_chunk, ct1 = min(ct0 + p.per_chunk, p.col_tiles);
+  // The slices' first columns and column tiles, by index: not by a load each time.
+  const auto slice_of = [&](int ct) {
+    return (int)(ct >= p.slice_tile[1]) + (int)(ct >= p.slice_tile[2]) + (int)(ct >= p.slice_tile[3]);
+  };
+  const auto pick = [](const int32_t* v, int i) {
+    return i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : i == 3 ? v[3] : v[4];
+  };
   // (a tile's last rows: its first again, not written)
   const int row0 = uniform(row_of[0]);
 #pragma unroll
@@ -327,101 +334,124 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
   // With one unit a slice the loads need not wait for the rank: an empty place is left at the end.
   const int units = p.R == 16 ? 1 : min(uniform((rank + 15) / 16), p.R / 16);
   if (units <= 0) return;
-  int s0 = 0;
-  while (s0 + 1 < p.n_slices && p.slice_tile[s0 + 1] <= ct0) ++s0;
-  const int at_once = max(1, kAdUnits / units);
+  const int at_once = units > kAdUnits / 2 ? 1 : units > 2 ? 2 : 4;  // slices whose u is held
+  const int s_end = slice_of(ct1 - 1) + 1;
 
   char* const mine = lds + wave * L::kRegion;
   const E* x_row[2 * MR];
 #pragma unroll
   for (int r = 0; r < 2 * MR; ++r) x_row[r] = static_cast<const E*>(p.x) + row_of[r] * p.x_stride;
-  const int blocks = (p.d_in + kAdBlock - 1) / kAdBlock, whole = kAligned ? p.d_in / kAdBlock : 0;
+  const int blocks = (p.d_in + kAdBlock - 1) / kAdBlock;
   // Slabs hold piece c of row r in place c ^ (r % 8): the lanes that read a piece of 16 rows meet no bank twice.
   const int k8 = 8 * (c8 ^ r8);
+  const int64_t unit_step = (int64_t)16 * p.d_in, slice_step = (int64_t)p.R * p.d_in;
 
-  for (; s0 < p.n_slices && p.slice_tile[s0] < ct1; s0 += at_once) {
-    int s1 = s0 + 1;  // slices [s0, s1) of this workgroup's columns
-    while (s1 < p.n_slices && s1 < s0 + at_once && p.slice_tile[s1] < ct1) ++s1;
+#pragma unroll 1
+  for (int s0 = slice_of(ct0); s0 < s_end; s0 += at_once) {
+    const int s1 = min(s0 + at_once, s_end);  // slices [s0, s1) of this workgroup's columns
     const int n_units = (s1 - s0) * units;
 
-    // u = A x, NT units at a time.
-    f32x4 kept[kPasses];
-#pragma unroll
-    for (int pass = 0; pass < kPasses; ++pass) {
-      kept[pass] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (pass * NT >= n_units) continue;
-      const E* a_row[NT];  // row r8 of a unit; its row 8 + r8 is 8 d_in further
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int i = min(pass * NT + n, n_units - 1), s = s0 + i / units;
-        a_row[n] = static_cast<const E*>(p.a) +
-                   (((int64_t)adapter * p.n_slices + s) * p.R + 16 * (i % units) + r8) * p.d_in;
+    // The 64 columns that come next: their slice, first and last column, y's values (in
+    // memory order) and B's first units.
+    const int first = max(ct0, pick(p.slice_tile, s0)), last = min(ct1, pick(p.slice_tile, s1));
+    const int b_first = min(units, L::kGroup);
+    const bool beside = (b_first == 1 ? 2048 : b_first == 2 ? 4096 : 8192) <= L::kB;
+    char* const b_room = mine + (beside ? L::kStage : L::kOut);
+    float* const out = reinterpret_cast<float*>(mine);
+    int cs = 0, c0 = 0, c1 = 0;
+    vec y_in[2 * MR];
+    // Columns of 2, 4 or 8 pieces, piece c of column d in place c ^ (d / (8 / pieces) % pieces).
+    const auto fetch_b = [&](int i0) {
+      const int n = min(units - i0, L::kGroup);
+      const int shift = n == 1 ? 1 : n == 2 ? 2 : 3, pieces = 1 << shift;
+      const E* const from = static_cast<const E*>(p.b) + ((int64_t)adapter * p.d_out + c0) * p.R + 16 * i0;
+#pragma unroll 1
+      for (int k = 0; k < pieces; ++k) {
+        const int d = (64 * k + lane) >> shift, c = lane % pieces ^ (d >> (3 - shift)) % pieces;
+        if (c < 2 * n) copy16(b_room + 1024 * k, from + (int64_t)min(d, c1 - 1 - c0) * p.R + 8 * c);
       }
-      f32x4 acc[MR][NT] = {};
+    };
+    const auto open = [&](int ct) {
+      cs = slice_of(ct);
+      c0 = pick(p.slice_col, cs) + (ct - pick(p.slice_tile, cs)) * 64;
+      c1 = pick(p.slice_col, cs + 1);
+#pragma unroll
+      for (int r = 0; r < 2 * MR; ++r)
+        y_in[r] = load8<E, kAligned>(static_cast<const E*>(p.y) + row_of[r] * p.y_stride, c0 + 8 * c8, c1);
+      fetch_b(0);
+    };
 
-      // Block b's rows into place d of the wave's region.
+    // u = A x, NT units at a time.
+    int in_slice = 0;
+    const E* a_unit = static_cast<const E*>(p.a) + ((int64_t)adapter * p.n_slices + s0) * slice_step + (int64_t)r8 * p.d_in;
+#pragma unroll 1
+    for (int u0 = 0; u0 < n_units; u0 += NT) {
+      const int now = min(n_units - u0, NT);
+      f32x4 acc[MR][NT] = {};
+      // Block b's rows into place d of the wave's stage.
       const auto fetch = [&](int b, int d) {
-        char* const to = mine + d * L::kBlock;
+        char* to = mine + d * L::kBlock;
         const int k = b * kAdBlock + k8;
-        if (b < whole) {
+        // (a row's last block: zeros past its end)
+        const bool in = k < p.d_in;
 #pragma unroll
-          for (int r = 0; r < 2 * MR; ++r) copy16(to + 1024 * r, x_row[r] + k);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if (pass * NT + n >= n_units) continue;
-            copy16(to + (MR + n) * L::kSlab, a_row[n] + k);
-            copy16(to + (MR + n) * L::kSlab + 1024, a_row[n] + k + (int64_t)8 * p.d_in);
-          }
-        } else {  // a row's last values, fewer than a block; unaligned rows: all of them
-#pragma unroll
-          for (int r = 0; r < 2 * MR; ++r)
-            reinterpret_cast<vec*>(to + 1024 * r)[lane] = load8<E, kAligned>(x_row[r], k, p.d_in);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if (pass * NT + n >= n_units) continue;
-            vec* const at = reinterpret_cast<vec*>(to + (MR + n) * L::kSlab) + lane;
-            at[0] = load8<E, kAligned>(a_row[n], k, p.d_in);
-            at[64] = load8<E, kAligned>(a_row[n] + (int64_t)8 * p.d_in, k, p.d_in);
+        for (int r = 0; r < 2 * MR; ++r, to += 1024) {
+          if (!kAligned)
+            reinterpret_cast<vec*>(to)[lane] = load8<E, false>(x_row[r], k, p.d_in);
+          else if (in)
+            copy16(to, x_row[r] + k);
+          else
+            reinterpret_cast<vec*>(to)[lane] = vec{};
+        }
+        const E* row = a_unit;
+        int i = in_slice;
+#pragma unroll 1
+        for (int n = 0; n < 2 * now; ++n, to += 1024) {
+          if (!kAligned)
+            reinterpret_cast<vec*>(to)[lane] = load8<E, false>(row, k, p.d_in);
+          else if (in)
+            copy16(to, row + k);
+          else
+            reinterpret_cast<vec*>(to)[lane] = vec{};
+          row += unit_step / 2;
+          if (n % 2 && ++i == units) {
+            i = 0;
+            row += slice_step - units * unit_step;
           }
         }
       };
-      int b = wave;
-#pragma unroll
+      // Each place's next block is on its way while the matrix cores have the others.
+#pragma unroll 1
       for (int d = 0; d < kDepth; ++d)
-        if (b + d * NW < blocks) fetch(b + d * NW, d);
-      for (; b < blocks; b += NW * kDepth) {
-        vec xv[kDepth][MR][2], av[kDepth][NT][2];
-        wait_copies();
+        if (wave + d * NW < blocks) fetch(wave + d * NW, d);
+      if (MR == 1 && u0 == 0 && beside && first + wave < last) open(first + wave);
+#pragma unroll 1
+      for (int b = wave, d = 0; b < blocks; b += NW, d = d + 1 == kDepth ? 0 : d + 1) {
+        vec xv[MR][2], av[NT][2];
+        if (kDepth == 1 || d == 0) wait_copies();
+        const char* const from = mine + d * L::kBlock + m * 128;
 #pragma unroll
-        for (int d = 0; d < kDepth; ++d) {
-          if (b + d * NW >= blocks) break;
-          const char* const from = mine + d * L::kBlock + m * 128;
+        for (int j = 0; j < 2; ++j) {
+          const int at = 16 * ((4 * j + g) ^ (m % 8));
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int at = 16 * ((4 * j + g) ^ (m % 8));
+          for (int r = 0; r < MR; ++r) xv[r][j] = *reinterpret_cast<const vec*>(from + r * L::kSlab + at);
 #pragma unroll
-            for (int r = 0; r < MR; ++r) xv[d][r][j] = *reinterpret_cast<const vec*>(from + r * L::kSlab + at);
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-              if (pass * NT + n < n_units)
-                av[d][n][j] = *reinterpret_cast<const vec*>(from + (MR + n) * L::kSlab + at);
-          }
+          for (int n = 0; n < NT; ++n) av[n][j] = *reinterpret_cast<const vec*>(from + (MR + n) * L::kSlab + at);
         }
         wait_lds_reads();
+        if (b + NW * kDepth < blocks) fetch(b + NW * kDepth, d);
 #pragma unroll
-        for (int d = 0; d < kDepth; ++d)
-          if (b + (d + kDepth) * NW < blocks) fetch(b + (d + kDepth) * NW, d);
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int d = 0; d < kDepth; ++d) {
-          if (b + d * NW >= blocks) break;
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-              if (pass * NT + n < n_units) {
-#pragma unroll
-                for (int r = 0; r < MR; ++r) acc[r][n] = mma(av[d][n][j], xv[d][r][j], acc[r][n]);
-              }
+            for (int r = 0; r < MR; ++r) acc[r][n] = mma(av[n][j], xv[r][j], acc[r][n]);  // (n >= now: not used)
+      }
+      for (int n = 0; n < now; ++n) {
+        a_unit += unit_step;
+        if (++in_slice == units) {
+          in_slice = 0;
+          a_unit += slice_step - units * unit_step;
         }
       }
       // A lane has ranks 4g .. 4g + 3 of token m.
@@ -432,51 +462,43 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
         for (int n = 0; n < NT; ++n)
           *reinterpret_cast<f32x4*>(sums + 16 * r * L::kSumRow + 16 * n) = acc[r][n];
       __syncthreads();
-      if (tid < M * kLanes) {
+      if (tid < M * kLanes && tid % kLanes < 4 * now) {
         const int t = tid / kLanes, q = tid % kLanes;
-        if (q / 4 < NT && pass * NT + q / 4 < n_units) {
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int w = 0; w < NW; ++w)
-            kept[pass] += reinterpret_cast<const f32x4*>(lds + w * L::kRegion)[t * (L::kSumRow / 4) + q];
-        }
+        for (int w = 0; w < NW; ++w)
+          sum += reinterpret_cast<const f32x4*>(lds + w * L::kRegion)[t * (L::kSumRow / 4) + q];
+        reinterpret_cast<f32x4*>(u_lds + ((u0 + q / 4) * M + t) * 64)[q % 4] = sum;
       }
-      if (kPasses > 1) __syncthreads();
+      __syncthreads();
     }
 
-    if (tid < M * kLanes) {
-      const int t = tid / kLanes, q = tid % kLanes;
-      // The row's largest finite |u| decides its scale: an infinity stays one.
+    // u = hi + lo: sixteen lanes a row, one rank of each unit.
+    if (tid < M * 16) {
+      const int t = tid / 16, q = tid % 16;
+      float v[kHeld];
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i)
+        v[i] = i < n_units ? reinterpret_cast<const float*>(u_lds + (i * M + t) * 64)[q] : 0.f;
       int shift = 0;
       if constexpr (__is_same(E, f16)) {
+        // The row's largest finite |u| decides its scale: an infinity stays one.
         float top = 0.f;
 #pragma unroll
-        for (int pass = 0; pass < kPasses; ++pass)
+        for (int i = 0; i < kHeld; ++i)
+          if (__builtin_fabsf(v[i]) < __builtin_huge_valf()) top = fmaxf(top, __builtin_fabsf(v[i]));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float v = __builtin_fabsf(kept[pass][e]);
-            if (v < __builtin_huge_valf() && v > top) top = v;
-          }
-#pragma unroll
-        for (int o = 1; o < kLanes; o *= 2) top = fmaxf(top, __shfl_xor(top, o, kWave));
+        for (int o = 1; o < 16; o *= 2) top = fmaxf(top, __shfl_xor(top, o, kWave));
         shift = row_shift<E>(top);
       }
+      lds_order();  // (the row's lanes are one wave's: all have read)
 #pragma unroll
-      for (int pass = 0; pass < kPasses; ++pass) {
-        const int i = pass * NT + q / 4;
-        if (q / 4 >= NT || i >= n_units) continue;
-        // Of two units side by side the first has both his, the second both los; a last
-        // one has its hi, then its lo.
-        const int of = i % units, s = i - of, r = 4 * (q % 4);
-        const bool pair = (of | 1) < units;
-        E* const hi = u_hl + ((s + (pair ? of & ~1 : of)) * M + t) * 32 + (pair ? 16 * (of & 1) : 0) + r;
-        E* const lo = u_hl + ((s + (pair ? of | 1 : of)) * M + t) * 32 + (pair ? 16 * (of & 1) : 16) + r;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = __builtin_ldexpf(kept[pass][e], shift);
-          hi[e] = (E)v;
-          const float left = v - (float)(E)v;
-          lo[e] = (E)(__builtin_isfinite(left) ? left : 0.f);  // (of an infinity or a NaN: hi says it all)
-        }
+      for (int i = 0; i < kHeld; ++i) {
+        if (i >= n_units) break;
+        E* const at = reinterpret_cast<E*>(u_lds + (i * M + t) * 64);
+        const float u = __builtin_ldexpf(v[i], shift), left = u - (float)(E)u;
+        at[q] = (E)u;
+        at[16 + q] = (E)(__builtin_isfinite(left) ? left : 0.f);  // (of an infinity, a NaN: hi says it)
       }
       if (q == 0) factor[t] = __builtin_ldexpf(scale, -shift);
     }
@@ -485,59 +507,32 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
 
     // y += scale B u: 64 columns at a time, B's rows as rows and tokens as columns of
     // the product, which goes through LDS to the memory's order.
-    const int first = max(ct0, p.slice_tile[s0]), last = min(ct1, p.slice_tile[s1]);
-    float* const out = reinterpret_cast<float*>(mine + L::kB);
-    constexpr int kGroup = NT < 4 ? NT : 4;  // units whose B values are in LDS at once
+    if (!(MR == 1 && beside) && first + wave < last) open(first + wave);
+#pragma unroll 1
     for (int ct = first + wave; ct < last; ct += NW) {
-      int s = s0;
-      while (s + 1 < s1 && p.slice_tile[s + 1] <= ct) ++s;
-      const int col = p.slice_col[s] + (ct - p.slice_tile[s]) * 64, end = p.slice_col[s + 1];
+      const int s = cs, col = c0, end = c1;
       vec yv[2 * MR];
 #pragma unroll
-      for (int r = 0; r < 2 * MR; ++r)
-        yv[r] = load8<E, kAligned>(static_cast<const E*>(p.y) + row_of[r] * p.y_stride, col + 8 * c8, end);
+      for (int r = 0; r < 2 * MR; ++r) yv[r] = y_in[r];
       f32x4 acc[MR][4] = {};
-      for (int i0 = 0; i0 < units; i0 += kGroup) {
-        const int n = min(units - i0, kGroup);
-        // Columns of 2, 4 or 8 pieces, piece c of column d in place c ^ (d / (8 / pieces) % pieces).
+#pragma unroll 1
+      for (int i0 = 0; i0 < units; i0 += L::kGroup) {
+        const int n = min(units - i0, L::kGroup);
         const int shift = n == 1 ? 1 : n == 2 ? 2 : 3, pieces = 1 << shift;
-        const E* const from = static_cast<const E*>(p.b) + ((int64_t)adapter * p.d_out + col) * p.R + 16 * i0;
-#pragma unroll
-        for (int k = 0; k < 2 * (kGroup == 3 ? 4 : kGroup); ++k) {
-          if (k >= pieces) break;
-          const int d = (64 * k + lane) >> shift, c = lane % pieces ^ (d >> (3 - shift)) % pieces;
-          if (c < 2 * n) copy16(mine + 1024 * k, from + (int64_t)min(d, end - 1 - col) * p.R + 8 * c);
-        }
+        if (i0 > 0) fetch_b(i0);
         wait_copies();
-        const auto b_at = [&](int j, int c) {  // piece c of column 16 j + m
-          const int d = 16 * j + m;
-          return *reinterpret_cast<const vec*>(mine + ((d << shift) + (c ^ (d >> (3 - shift)) % pieces)) * 16);
-        };
-        const auto u_at = [&](int i, int r) {
-          return *reinterpret_cast<const vec*>(u_hl + (((s - s0) * units + i0 + i) * M + 16 * r + m) * 32 + 8 * g);
-        };
-        int i = 0;
-        for (; i + 1 < n; i += 2) {  // 32 ranks: their his, then their los
-          vec bv[4], uv[2][MR];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) bv[j] = b_at(j, 2 * i + g);
-#pragma unroll
-          for (int l = 0; l < 2; ++l)
-#pragma unroll
-            for (int r = 0; r < MR; ++r) uv[l][r] = u_at(i + l, r);
-#pragma unroll
-          for (int l = 0; l < 2; ++l)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int r = 0; r < MR; ++r) acc[r][j] = mma(bv[j], uv[l][r], acc[r][j]);
-        }
-        if (i < n) {  // 16 ranks: hi and lo in one K of 32, B's values twice
+        // 16 ranks at a time: hi and lo in one K of 32, B's values twice
+#pragma unroll 2
+        for (int i = 0; i < n; ++i) {
           vec bv[4], uv[MR];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) bv[j] = b_at(j, 2 * i + g % 2);
+          for (int j = 0; j < 4; ++j) {
+            const int d = 16 * j + m, c = 2 * i + g % 2;
+            bv[j] = *reinterpret_cast<const vec*>(b_room + ((d << shift) + (c ^ (d >> (3 - shift)) % pieces)) * 16);
+          }
 #pragma unroll
-          for (int r = 0; r < MR; ++r) uv[r] = u_at(i, r);
+          for (int r = 0; r < MR; ++r)
+            uv[r] = *reinterpret_cast<const vec*>(u_lds + (((s - s0) * units + i0 + i) * M + 16 * r + m) * 64 + 16 * g);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -545,6 +540,7 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
         }
         wait_lds_reads();
       }
+      if (ct + NW < last) open(ct + NW);
 #pragma unroll
       for (int r = 0; r < MR; ++r) {
 #pragma unroll
@@ -576,7 +572,7 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
         lds_order();
       }
     }
-    if (s0 + at_once < p.n_slices) __syncthreads();  // (the regions and u are used again)
+    if (s1 < s_end) __syncthreads();  // (the regions and u are used again)
   }
 }
 
@@ -631,9 +627,9 @@ extern "C" int cie_adapter_plan(int32_t* plan, int64_t plan_bytes, const int64_t
   p.n_slots = n_slots;
   p.N = (int32_t)N;
   p.M = tile_rows(T);
+  p.log_m = p.M == 16 ? 4 : 5;
   p.err = err;
-  hipLaunchKernelGGL(adapter_plan_kernel, dim3(1), dim3(kPlanWaves * kWave), (kPlanWaves + 1) * N * 4,
-                     static_cast<hipStream_t>(stream), p);
+  hipLaunchKernelGGL(adapter_plan_kernel, dim3(1), dim3(kPlanThreads), 0, static_cast<hipStream_t>(stream), p);
   return (int)hipGetLastError();
 }
 
@@ -687,10 +683,11 @@ extern "C" int cie_adapter_add(void* y, int64_t y_row_stride, const void* x, int
   // Few tiles: several workgroups share one's columns (each computes u again), down to a
   // column tile a wave.
   const int64_t per_tile = (tiles + kAdWaves - 1) / kAdWaves;
-  int64_t chunks = 512 / p.max_tiles;
+  int64_t chunks = 256 / p.max_tiles;
   chunks = chunks < 1 ? 1 : chunks > per_tile ? per_tile : chunks;
-  p.chunks = (int32_t)chunks;
-  const int64_t blocks = (int64_t)(p.max_tiles + 7) / 8 * 8 * chunks;
+  p.per_chunk = (int32_t)((tiles + chunks - 1) / chunks);
+  p.chunks = (int32_t)((tiles + p.per_chunk - 1) / p.per_chunk);
+  const int64_t blocks = (int64_t)(p.max_tiles + 7) / 8 * 8 * p.chunks;
   if (blocks > 0x7fffffff) return CIE_EUNSUPPORTED;
   const dim3 grid((unsigned)blocks);
   const int units = (int)(n_slices * (R / 16) < 5 ? n_slices * (R / 16) : 4);
