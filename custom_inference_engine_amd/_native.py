@@ -202,6 +202,8 @@ _SIGNATURES = {
 
 ABI_VERSION = 12
 
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -265,11 +267,12 @@ def stream_handle(device: torch.device) -> int:
 def call(device: torch.device, name: str, *args) -> None:
     """The C entry ``name`` on the device's current stream, with that device current."""
     fn = getattr(load(), name)
-    if device.index == torch._C._cuda_getDevice():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    index = device.index
+    if index == _current_device():
+        status = fn(*args, _current_stream(index))
     else:
         with torch.cuda.device(device):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+            status = fn(*args, _current_stream(index))
     if status:
         check(status, name)
 

@@ -22,6 +22,7 @@ from ..kv_cache.quant import int64_index, launch, one_device
 RANK_UNIT = 16  # a bank's ranks come in 16s
 MAX_RANK = 128
 _TYPES = {torch.float16: 0, torch.bfloat16: 1}  # CIE_F16, CIE_BF16
+_F32, _I32 = torch.float32, torch.int32
 
 
 @functools.lru_cache(maxsize=4096)
@@ -94,23 +95,25 @@ def adapter_add_(y, x, a, b, scales, ranks, plan, slices, err=None):
     """
     yr, xr = _rows(y, "y"), _rows(x, "x")
     T, d_in = xr.shape
-    widths, d_out, n_slices = _widths(tuple(slices))
-    kind = _TYPES.get(y.dtype)
-    if kind is None or x.dtype != y.dtype or a.dtype != y.dtype or b.dtype != y.dtype:
+    widths, d_out, n_slices = _widths(slices if type(slices) is tuple else tuple(slices))
+    dtype = y.dtype
+    kind = _TYPES.get(dtype)
+    if kind is None or x.dtype != dtype or a.dtype != dtype or b.dtype != dtype:
         raise AssertionError("y, x, a and b must share float16 or bfloat16")
-    if yr.shape[0] != T or yr.shape[1] != d_out:
+    if yr.shape != (T, d_out):
         raise AssertionError(f"y must be ({T}, {d_out}): x's rows, the slices' widths")
     n, S, R, w = a.shape if a.dim() == 4 else (0,) * 4
     if S != n_slices or w != d_in or R % RANK_UNIT or not 0 < R <= MAX_RANK or not a.is_contiguous():
         raise AssertionError(f"a must be contiguous (n, {n_slices}, R, {d_in}), R a multiple of 16 up to 128")
     if b.shape != (n, d_out, R) or not b.is_contiguous():
         raise AssertionError(f"b must be contiguous ({n}, {d_out}, {R})")
-    if scales.shape != (n,) or scales.dtype != torch.float32 or not scales.is_contiguous():
+    if scales.shape != (n,) or scales.dtype != _F32 or not scales.is_contiguous():
         raise AssertionError(f"scales must be contiguous float32 ({n},)")
-    if ranks.shape != (n,) or ranks.dtype != torch.int32 or not ranks.is_contiguous():
+    if ranks.shape != (n,) or ranks.dtype != _I32 or not ranks.is_contiguous():
         raise AssertionError(f"ranks must be contiguous int32 ({n},)")
     words = _plan_words(T, n)
-    if plan.dtype != torch.int32 or plan.dim() != 1 or not plan.is_contiguous() or plan.shape[0] < words:
+    held = plan.numel()
+    if plan.dtype != _I32 or held < words or not plan.is_contiguous():
         raise AssertionError("plan must come from adapter_plan for these rows and adapters")
     y_row = yr.stride(0)
     if T > 1 and y_row < d_out:
@@ -122,7 +125,7 @@ def adapter_add_(y, x, a, b, scales, ranks, plan, slices, err=None):
             xr = xr.contiguous()
             x_row = d_in
         launch(dev, "cie_adapter_add", yr.data_ptr(), y_row, xr.data_ptr(), x_row, a.data_ptr(), b.data_ptr(),
-               scales.data_ptr(), ranks.data_ptr(), plan.data_ptr(), 4 * plan.shape[0], T, n, R, d_in, widths,
+               scales.data_ptr(), ranks.data_ptr(), plan.data_ptr(), 4 * held, T, n, R, d_in, widths,
                n_slices, kind, err=err)
     return y
 

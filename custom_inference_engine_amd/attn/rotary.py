@@ -83,15 +83,9 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
     return torch.tensor(freqs, dtype=torch.float64, device=device), float(scale)
 
 
-def _type_of(t: torch.Tensor) -> int:
-    kind = _TYPES.get(t.dtype)
-    if kind is None:
-        raise AssertionError("rows must be float16, bfloat16 or float32")
-    return kind
-
-
 def _positions(positions: torch.Tensor, T: int) -> torch.Tensor:
-    if positions.numel() != T or positions.dim() > 2:
+    shape = positions.shape
+    if shape != (T,) and shape != (1, T):
         raise AssertionError("positions must have one entry per row")
     return int64_index(positions)
 
@@ -109,7 +103,7 @@ def _frequencies(frequencies: torch.Tensor, d: int) -> int:
 def rotary_tables(positions, frequencies, dtype=torch.float16, interleaved: bool = False, scale: float = 1.0):
     """cos and sin of the positions, (1, T, 2 * pairs) each, times ``scale``: a value for each dim of a head, as the
     fused append and decode calls take them (half layout, the whole head turned)."""
-    T = positions.numel()
+    T = positions.shape[-1] if positions.dim() else 0
     rot = _frequencies(frequencies, 2 * frequencies.numel())
     if dtype not in _TYPES:
         raise AssertionError("tables are float16, bfloat16 or float32")
@@ -123,18 +117,6 @@ def rotary_tables(positions, frequencies, dtype=torch.float16, interleaved: bool
     return cos, sin
 
 
-def _heads(x: torch.Tensor, name: str):
-    """(1, T, heads, D) or (T, heads, D): a view with dense heads, T, heads, D and the strides of rows and heads."""
-    if x.dim() not in (3, 4) or (x.dim() == 4 and x.shape[0] != 1):
-        raise AssertionError(f"{name} must be (1, T, heads, D) or (T, heads, D)")
-    T, h, d = x.shape[-3:]
-    row, head, one = x.stride()[-3:]
-    if one != 1 and d > 1:
-        x = x.contiguous()
-        row, head, one = x.stride()[-3:]
-    return x, T, h, d, row, head
-
-
 def apply_rotary(q, k, positions, frequencies, interleaved: bool = False, scale: float = 1.0):
     """q and k turned by their rows' positions, into new dense tensors of their shapes.
 
@@ -142,25 +124,44 @@ def apply_rotary(q, k, positions, frequencies, interleaved: bool = False, scale:
     float32: views into the fused QKV projection's output need no copy.  positions (T,)
     or (1, T).  ``k`` may be None.
     """
-    q, T, h_q, d, q_row, q_head = _heads(q, "q")
-    rot, kind = _frequencies(frequencies, d), _type_of(q)
+    shape, dtype = q.shape, q.dtype
+    kind = _TYPES.get(dtype)
+    if kind is None:
+        raise AssertionError("rows must be float16, bfloat16 or float32")
+    if len(shape) not in (3, 4) or (len(shape) == 4 and shape[0] != 1):
+        raise AssertionError("q and k must be (1, T, heads, D) or (T, heads, D)")
+    T, h_q, d = shape[-3:]
+    rot = _frequencies(frequencies, d)
     if k is None:
         dev = one_device(q, positions, frequencies)
     else:
-        if k.dtype != q.dtype or k.dim() < 3 or k.shape[-3] != T or k.shape[-1] != d:
+        k_shape = k.shape
+        h_kv = k_shape[-2] if len(k_shape) == len(shape) else -1
+        if k.dtype != dtype or k_shape != (*shape[:-2], h_kv, d):
             raise AssertionError("q and k must have the same rows, head_dim and type")
         dev = one_device(q, k, positions, frequencies)
     positions = _positions(positions, T)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    k_out, h_kv, k_row, k_head = None, 0, 0, 0
-    if k is not None:
-        k, _, h_kv, _, k_row, k_head = _heads(k, "k")
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=dev)
+    q, q_row, q_head = _dense_heads(q, d)
+    q_out = q.new_empty(shape)
+    if k is None:
+        k_out, k_ptr, to_k, h_kv, k_row, k_head = None, None, None, 0, 0, 0
+    else:
+        k, k_row, k_head = _dense_heads(k, d)
+        k_out = k.new_empty(k_shape)
+        k_ptr, to_k = k.data_ptr(), k_out.data_ptr()
     if T and h_q + h_kv:
-        _native.call(dev, "cie_rotary", q_out.data_ptr(), _native.ptr(k_out), q.data_ptr(), _native.ptr(k), q_row,
-                     q_head, k_row, k_head, positions.data_ptr(), frequencies.data_ptr(), scale, T, h_q, h_kv, d, rot,
-                     interleaved, kind)
+        _native.call(dev, "cie_rotary", q_out.data_ptr(), to_k, q.data_ptr(), k_ptr, q_row, q_head, k_row, k_head,
+                     positions.data_ptr(), frequencies.data_ptr(), scale, T, h_q, h_kv, d, rot, interleaved, kind)
     return q_out, k_out
+
+
+def _dense_heads(x: torch.Tensor, d: int):
+    """x with the dims of a head side by side (itself, or a copy), and its strides of rows and heads."""
+    st = x.stride()
+    if st[-1] != 1 and d > 1:
+        x = x.contiguous()
+        st = x.stride()
+    return x, st[-3], st[-2]
 
 
 def append_tokens_qkv_rotary(qkv, positions, frequencies, k_cache, v_cache, pages, offsets, num_heads: int,

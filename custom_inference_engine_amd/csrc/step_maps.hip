@@ -27,10 +27,10 @@
 
 namespace cie {
 
-constexpr int kMapThreads = 256;
-constexpr int kMapMaxSeqs = 2048;          // (scans and hash table of a batch: 56 KB of LDS)
+constexpr int kMapMaxSeqs = 2048;          // (scans and hash table of a batch: 64 KB of LDS)
 constexpr int64_t kMapMaxRows = 1 << 24;   // sums over a batch stay below 2^31
 constexpr int64_t kMapMaxPages = 1 << 24;
+constexpr int64_t kMapMaxPage = 1 << 30;   // tokens a page: a page and a step's rows stay below 2^32
 
 struct MapParams {
   int64_t* cu;         // (B + 1) or null
@@ -45,21 +45,40 @@ struct MapParams {
   int64_t* block_table;
   int64_t* free_list;
   int64_t bt_stride, bt_width, n_slots, n_pages, T;
+  double per_page;        // 1 / page_size
   int32_t B, page_size, hash_size;
   int32_t* err;
 };
 
-// a / d for 0 <= a, 0 < d < 2^31.
-__device__ __forceinline__ int64_t div_by(int64_t a, int32_t d) {
-  return (uint64_t)a >> 32 ? a / d : (int64_t)((uint32_t)a / (uint32_t)d);
+// Whole pages of n tokens, and the rest: 0 <= n <= 2^24 pages.  (The product is off by
+// far less than one, so the quotient by one at most.)
+__device__ __forceinline__ int whole_pages(int64_t n, const MapParams& p, uint32_t& rest) {
+  int q = (int)((double)n * p.per_page);
+  int64_t r = n - (int64_t)q * p.page_size;
+  if (r < 0) {
+    --q;
+    r += p.page_size;
+  } else if (r >= p.page_size) {
+    ++q;
+    r -= p.page_size;
+  }
+  rest = (uint32_t)r;
+  return q;
+}
+__device__ __forceinline__ int pages_of(int64_t n, const MapParams& p) {
+  uint32_t rest;
+  const int q = whole_pages(n, p, rest);
+  return q + (rest > 0);
 }
 
 // A batch's scans, in LDS.
 struct Batch {
+  int64_t* len;    // [B] held tokens
   int32_t* cu;     // [B + 1] rows before sequence b
   int32_t* rank;   // [B + 1] pages handed out (or given back) before sequence b
   int32_t* slot;   // [B] -1: not a slot
-  int64_t* len;    // [B] held tokens; release: the first page given back
+  int32_t* page;   // [B] whole pages held (release: pages kept)
+  uint32_t* rest;  // [B] tokens held past them
   int32_t* hash;   // [hash_size] the slots that get (or give back) pages
 };
 
@@ -69,30 +88,43 @@ __device__ __forceinline__ Batch batch_in(char* lds, int B) {
   s.cu = reinterpret_cast<int32_t*>(s.len + B);
   s.rank = s.cu + B + 1;
   s.slot = s.rank + B + 1;
-  s.hash = s.slot + B;
+  s.page = s.slot + B;
+  s.rest = reinterpret_cast<uint32_t*>(s.page + B);
+  s.hash = reinterpret_cast<int32_t*>(s.rest + B);
   return s;
 }
 static inline size_t batch_bytes(int B, int hash_size) {
-  return (size_t)B * 8 + (size_t)(B + 1) * 8 + (size_t)B * 4 + (size_t)hash_size * 4;
+  return (size_t)B * 8 + (size_t)(B + 1) * 8 + (size_t)B * 12 + (size_t)hash_size * 4;
 }
 
-// Exclusive prefix sum over the workgroup's threads, saturated at cap (< 2^25:
-// a wave's sum fits 31 bits), and the total.  sm: a word a wave.
-__device__ __forceinline__ int block_exclusive(int v, int cap, int* sm, int& total) {
-  v = min(v, cap);
-  const int incl = wave_inclusive_sum(v);
+// Exclusive prefix sums of two values over the workgroup's threads, and their totals,
+// saturated at the caps (< 2^25: a wave's sum fits 31 bits).
+template <int kThreads>
+__device__ __forceinline__ void block_exclusive(int& a, int& b, int cap_a, int cap_b, int (*sm)[2], int& total_a,
+                                                int& total_b) {
+  a = min(a, cap_a);
+  b = min(b, cap_b);
+  const int in_a = wave_inclusive_sum(a), in_b = wave_inclusive_sum(b);
   const int wave = threadIdx.x / kWave;
   __syncthreads();  // (a former call's words are read)
-  if (threadIdx.x % kWave == kWave - 1) sm[wave] = min(incl, cap);
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kMapThreads / kWave; ++w) {
-    if (w == wave) before = total;
-    total = min(total + sm[w], cap);
+  if (threadIdx.x % kWave == kWave - 1) {
+    sm[wave][0] = min(in_a, cap_a);
+    sm[wave][1] = min(in_b, cap_b);
   }
-  return min(before + min(incl - v, cap), cap);
+  __syncthreads();
+  int before_a = 0, before_b = 0;
+  total_a = total_b = 0;
+#pragma unroll 4
+  for (int w = 0; w < kThreads / kWave; ++w) {
+    if (w == wave) {
+      before_a = total_a;
+      before_b = total_b;
+    }
+    total_a = min(total_a + sm[w][0], cap_a);
+    total_b = min(total_b + sm[w][1], cap_b);
+  }
+  a = min(before_a + min(in_a - a, cap_a), cap_a);
+  b = min(before_b + min(in_b - b, cap_b), cap_b);
 }
 
 // Adds slot to the set; false if it was there.  At most half of the set is filled.
@@ -130,23 +162,31 @@ __device__ __forceinline__ bool last_of_grid(int64_t* word, int* flag) {
   return *flag != 0;
 }
 
-template <bool kReserve>
-__global__ __launch_bounds__(kMapThreads) void step_maps_kernel(MapParams p) {
+template <bool kReserve, int kThreads>
+__global__ __launch_bounds__(kThreads) void step_maps_kernel(MapParams p) {
   extern __shared__ __align__(8) char lds[];
-  __shared__ int sm[kMapThreads / kWave], flag, bad;
+  __shared__ int sm[kThreads / kWave][2], flag, bad;
   const Batch s = batch_in(lds, p.B);
-  const int tid = threadIdx.x, B = p.B, P = p.page_size;
-  const int each = (B + kMapThreads - 1) / kMapThreads, b0 = min(tid * each, B), b1 = min(b0 + each, B);
+  const int tid = threadIdx.x, B = p.B, T = (int)p.T;
+  const uint32_t P = (uint32_t)p.page_size;
+  const int each = (B + kThreads - 1) / kThreads, b0 = min(tid * each, B), b1 = min(b0 + each, B);
   const int64_t capacity = p.bt_width * P;
-  const int T = (int)p.T;
 
   int64_t avail = 0;
   if constexpr (kReserve) {
     avail = p.free_list[0];
-    for (int i = tid; i < p.hash_size; i += kMapThreads) s.hash[i] = -1;
+    for (int i = tid; i < p.hash_size; i += kThreads) s.hash[i] = -1;
     if (tid == 0) bad = 0;
   }
-  int rows = 0, mistakes = 0;
+  // New pages of a sequence whose n tokens are all mapped; 0 for the padding rows' slot and where they do not fit.
+  const auto more_pages = [&](int b, int n) {
+    const int64_t len = s.len[b];
+    if (s.slot[b] <= 0 || n == 0 || len < 0 || len + n > capacity) return 0;
+    const uint32_t rest = s.rest[b];
+    return (int)((rest + (uint32_t)n + P - 1) / P) - (rest > 0);
+  };
+  int rows = 0, need = 0, mistakes = 0;
+#pragma unroll 1
   for (int b = b0; b < b1; ++b) {
     const int64_t slot = p.slot_ids[b], n = p.counts[b];
     const bool ok = slot >= 0 && slot < p.n_slots;
@@ -155,54 +195,72 @@ __global__ __launch_bounds__(kMapThreads) void step_maps_kernel(MapParams p) {
     if (n < 0 || len < 0) mistakes |= CIE_ERRBIT_LEN;
     s.slot[b] = ok ? (int)slot : -1;
     s.len[b] = len;
+    uint32_t rest;
+    s.page[b] = whole_pages(min(max(len, (int64_t)0), capacity), p, rest);
+    s.rest[b] = rest;
     s.cu[b] = rows;  // (within the thread, completed below)
-    rows = min(rows + (int)min(max(n, (int64_t)0), p.T), T + 1);
+    s.rank[b] = need;
+    const int take = (int)min(max(n, (int64_t)0), p.T);
+    rows = min(rows + take, T + 1);
+    if constexpr (kReserve) need += more_pages(b, take);
   }
-  int total;
-  const int before = block_exclusive(rows, T + 1, sm, total);
-  for (int b = b0; b < b1; ++b) s.cu[b] = min(s.cu[b] + before, T);
-  if (total > T) mistakes |= CIE_ERRBIT_LEN;
+  int total, need_total;
+  int first_row = rows, first_page = need;
+  block_exclusive<kThreads>(first_row, first_page, T + 1, 1 << 25, sm, total, need_total);
+  for (int b = b0; b < b1; ++b) {
+    s.cu[b] = min(s.cu[b] + first_row, T);
+    s.rank[b] += first_page;
+  }
+  const bool cut = total > T;
+  if (cut) mistakes |= CIE_ERRBIT_LEN;
   total = min(total, T);
-  if (tid == 0) s.cu[B] = total;
+  if (tid == 0) {
+    s.cu[B] = total;
+    s.rank[B] = need_total;
+  }
   __syncthreads();
 
-  int need_total = 0;
   bool granted = false;
   if constexpr (kReserve) {
-    int need = 0;
-    for (int b = b0; b < b1; ++b) {
-      const int n = s.cu[b + 1] - s.cu[b], slot = s.slot[b];
-      const int64_t len = s.len[b];
-      s.rank[b] = need;
-      if (slot <= 0 || n == 0 || len < 0) continue;  // (slot 0 is the padding rows')
-      if (len + n > capacity) {
-        mistakes |= CIE_ERRBIT_LEN;
-        continue;
+    if (cut) {  // pages for the rows that are mapped only
+      need = 0;
+      for (int b = b0; b < b1; ++b) {
+        s.rank[b] = need;
+        need += more_pages(b, s.cu[b + 1] - s.cu[b]);
       }
-      const int more = (int)(div_by(len + n + P - 1, P) - div_by(len + P - 1, P));
-      if (!add_slot(s.hash, p.hash_size, slot)) bad = 1;
-      need += more;
+      int none = 0, no_total;
+      block_exclusive<kThreads>(need, none, 1 << 25, 1, sm, need_total, no_total);
+      for (int b = b0; b < b1; ++b) s.rank[b] += need;
+      if (tid == 0) s.rank[B] = need_total;
     }
-    const int first = block_exclusive(need, 1 << 25, sm, need_total);
-    for (int b = b0; b < b1; ++b) s.rank[b] += first;
-    if (tid == 0) s.rank[B] = need_total;
+    for (int b = b0; b < b1; ++b) {
+      const int n = s.cu[b + 1] - s.cu[b];
+      const int64_t len = s.len[b];
+      if (s.slot[b] <= 0 || n == 0 || len < 0) continue;
+      if (len + n > capacity)
+        mistakes |= CIE_ERRBIT_LEN;
+      else if (!add_slot(s.hash, p.hash_size, s.slot[b]))
+        bad = 1;
+    }
     __syncthreads();
     granted = !bad && need_total <= avail && avail <= p.n_pages;
     if (!granted) mistakes |= CIE_ERRBIT_FREE;
     if (granted) {
-      for (int j = blockIdx.x * kMapThreads + tid; j < need_total; j += gridDim.x * kMapThreads) {
+#pragma unroll 1
+      for (int j = blockIdx.x * kThreads + tid; j < need_total; j += gridDim.x * kThreads) {
         const int b = find(s.rank, B, j);
         int64_t id = p.free_list[2 + avail - 1 - j];
         if (id <= 0 || id >= p.n_pages) {
           mistakes |= CIE_ERRBIT_PAGE;
           id = 0;
         }
-        p.block_table[(int64_t)s.slot[b] * p.bt_stride + div_by(s.len[b] + P - 1, P) + (j - s.rank[b])] = id;
+        p.block_table[(int64_t)s.slot[b] * p.bt_stride + s.page[b] + (s.rest[b] > 0) + (j - s.rank[b])] = id;
       }
     }
   }
 
-  for (int t = blockIdx.x * kMapThreads + tid; t < T; t += gridDim.x * kMapThreads) {
+#pragma unroll 1
+  for (int t = blockIdx.x * kThreads + tid; t < T; t += gridDim.x * kThreads) {
     int64_t slot = 0, pos = 0, page = 0, off = 0;
     if (t < total) {
       const int b = find(s.cu, B, t);
@@ -213,11 +271,13 @@ __global__ __launch_bounds__(kMapThreads) void step_maps_kernel(MapParams p) {
         if (pos < 0 || pos >= capacity) {
           mistakes |= CIE_ERRBIT_LEN;
         } else {
-          const int64_t at = div_by(pos, P);
-          off = pos - at * P;
+          // (past the whole pages held, or from a negative length on: below 2^32)
+          const uint32_t past = len < 0 ? (uint32_t)pos : s.rest[b] + (uint32_t)(t - s.cu[b]), more = past / P;
+          const int64_t at = s.page[b] + (int64_t)more;
+          off = past - more * P;
           bool fresh = false;
           if constexpr (kReserve) {
-            const int64_t have = div_by(max(len, (int64_t)0) + P - 1, P);
+            const int have = s.page[b] + (s.rest[b] > 0);
             fresh = slot > 0 && at >= have;
             if (fresh && granted && s.rank[b + 1] > s.rank[b]) {
               page = p.free_list[2 + avail - 1 - (s.rank[b] + (at - have))];
@@ -234,7 +294,7 @@ __global__ __launch_bounds__(kMapThreads) void step_maps_kernel(MapParams p) {
     p.offsets[t] = off;
   }
   if (blockIdx.x == 0)
-    for (int b = tid; b <= B; b += kMapThreads) p.cu[b] = s.cu[b];
+    for (int b = tid; b <= B; b += kThreads) p.cu[b] = s.cu[b];
   if (mistakes) set_err(p.err, mistakes);
   if constexpr (kReserve) {
     if (last_of_grid(p.free_list + 1, &flag) && tid == 0) {
@@ -244,20 +304,24 @@ __global__ __launch_bounds__(kMapThreads) void step_maps_kernel(MapParams p) {
   }
 }
 
-__global__ __launch_bounds__(kMapThreads) void release_pages_kernel(MapParams p) {
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void release_pages_kernel(MapParams p) {
   extern __shared__ __align__(8) char lds[];
-  __shared__ int sm[kMapThreads / kWave], flag, bad;
+  __shared__ int sm[kThreads / kWave][2], flag, bad;
   const Batch s = batch_in(lds, p.B);
-  const int tid = threadIdx.x, B = p.B, P = p.page_size;
-  const int each = (B + kMapThreads - 1) / kMapThreads, b0 = min(tid * each, B), b1 = min(b0 + each, B);
-  const int64_t capacity = p.bt_width * P, avail = p.free_list[0];
+  const int tid = threadIdx.x, B = p.B;
+  const int each = (B + kThreads - 1) / kThreads, b0 = min(tid * each, B), b1 = min(b0 + each, B);
+  const int64_t capacity = p.bt_width * p.page_size, avail = p.free_list[0];
 
-  for (int i = tid; i < p.hash_size; i += kMapThreads) s.hash[i] = -1;
+  for (int i = tid; i < p.hash_size; i += kThreads) s.hash[i] = -1;
   if (tid == 0) bad = 0;
   __syncthreads();
   int gone = 0, mistakes = 0;
+#pragma unroll 1
   for (int b = b0; b < b1; ++b) {
     const int64_t slot = p.slot_ids[b];
+    const int64_t keep = p.counts ? p.counts[b] : 0;
+    int64_t held = p.held ? p.held[b] : 0;
     s.rank[b] = gone;
     s.slot[b] = -1;
     if (slot == 0) continue;  // the padding rows' slot holds no pages
@@ -266,19 +330,20 @@ __global__ __launch_bounds__(kMapThreads) void release_pages_kernel(MapParams p)
       continue;
     }
     const int64_t len = p.lens[slot];
-    const int64_t held = p.held ? p.held[b] : len;
-    const int64_t keep = p.counts ? p.counts[b] : 0;
+    if (!p.held) held = len;
     if (held < len || held < 0 || held > capacity || keep < 0 || keep > held) {
       mistakes |= CIE_ERRBIT_LEN;
       continue;
     }
     if (!add_slot(s.hash, p.hash_size, (int)slot)) bad = 1;
     s.slot[b] = (int)slot;
-    s.len[b] = div_by(keep + P - 1, P);
-    gone = (int)min(gone + div_by(held + P - 1, P) - s.len[b], kMapMaxPages + 1);
+    s.len[b] = keep;
+    s.page[b] = pages_of(keep, p);
+    gone = (int)min((int64_t)gone + pages_of(held, p) - s.page[b], kMapMaxPages + 1);
   }
-  int total;
-  const int before = block_exclusive(gone, (int)kMapMaxPages + 1, sm, total);
+  int total, none = 0, no_total;
+  int before = gone;
+  block_exclusive<kThreads>(before, none, (int)kMapMaxPages + 1, 1, sm, total, no_total);
   for (int b = b0; b < b1; ++b) s.rank[b] = min(s.rank[b] + before, (int)kMapMaxPages + 1);
   if (tid == 0) s.rank[B] = total;
   __syncthreads();
@@ -286,9 +351,10 @@ __global__ __launch_bounds__(kMapThreads) void release_pages_kernel(MapParams p)
   const bool taken = !bad && avail >= 0 && avail + total < p.n_pages;
   if (!taken) mistakes |= CIE_ERRBIT_FREE;
   if (taken) {
-    for (int j = blockIdx.x * kMapThreads + tid; j < total; j += gridDim.x * kMapThreads) {
+#pragma unroll 1
+    for (int j = blockIdx.x * kThreads + tid; j < total; j += gridDim.x * kThreads) {
       const int b = find(s.rank, B, j);
-      int64_t* const entry = p.block_table + (int64_t)s.slot[b] * p.bt_stride + s.len[b] + (j - s.rank[b]);
+      int64_t* const entry = p.block_table + (int64_t)s.slot[b] * p.bt_stride + s.page[b] + (j - s.rank[b]);
       int64_t id = *entry;
       if (id <= 0 || id >= p.n_pages) {
         mistakes |= CIE_ERRBIT_PAGE;
@@ -301,8 +367,8 @@ __global__ __launch_bounds__(kMapThreads) void release_pages_kernel(MapParams p)
   if (mistakes) set_err(p.err, mistakes);
   if (last_of_grid(p.free_list + 1, &flag)) {
     if (taken) {
-      for (int b = tid; b < B; b += kMapThreads)
-        if (s.slot[b] > 0) p.lens[s.slot[b]] = p.counts ? p.counts[b] : 0;
+      for (int b = tid; b < B; b += kThreads)
+        if (s.slot[b] > 0) p.lens[s.slot[b]] = s.len[b];
       if (tid == 0) p.free_list[0] = avail + total;
     }
     if (tid == 0) p.free_list[1] = 0;
@@ -327,7 +393,7 @@ extern "C" int cie_step_maps(int64_t* cu_seqlens, int64_t* slots, int64_t* posit
   if (B < 0 || T < 0 || page_size <= 0 || bt_width <= 0 || bt_stride < bt_width || n_slots <= 0 ||
       (free_list && n_pages <= 0))
     return CIE_EINVAL;
-  if (B > kMapMaxSeqs || T > kMapMaxRows || page_size > 0x7fffffff || bt_width > kMapMaxPages ||
+  if (B > kMapMaxSeqs || T > kMapMaxRows || page_size > kMapMaxPage || bt_width > kMapMaxPages ||
       n_slots > 0x7fffffff || (free_list && n_pages > kMapMaxPages))
     return CIE_EUNSUPPORTED;
   if (!cu_seqlens || (T > 0 && (!slots || !positions || !pages || !offsets)) ||
@@ -353,14 +419,23 @@ extern "C" int cie_step_maps(int64_t* cu_seqlens, int64_t* slots, int64_t* posit
   p.page_size = (int32_t)page_size;
   p.hash_size = free_list ? hash_size_of(B) : 0;
   p.err = err;
-  // A row a thread, to one workgroup a CU: further rows are a loop.
-  const int64_t blocks = (T + kMapThreads - 1) / kMapThreads;
-  const dim3 grid((unsigned)(blocks < 1 ? 1 : blocks < 256 ? blocks : 256));
+  p.per_page = 1.0 / (double)page_size;
   const size_t lds = batch_bytes((int)B, p.hash_size);
-  if (free_list)
-    hipLaunchKernelGGL(step_maps_kernel<true>, grid, dim3(kMapThreads), lds, static_cast<hipStream_t>(stream), p);
+  const auto grid = [&](int64_t rows) {  // of a workgroup's rows; to one workgroup a CU, further rows are a loop
+    const int64_t blocks = (T + rows - 1) / rows;
+    return dim3((unsigned)(blocks < 1 ? 1 : blocks < 256 ? blocks : 256));
+  };
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  // Scans want a sequence a thread; four times the threads start 0.5 us later.  Where pages are handed out, further workgroups
+  // cost an arrival (1 us): two rows a thread, so that most steps are one workgroup.
+  if (free_list && B <= 256 && T <= 256)
+    hipLaunchKernelGGL((step_maps_kernel<true, 256>), dim3(1), dim3(256), lds, st, p);
+  else if (free_list)
+    hipLaunchKernelGGL((step_maps_kernel<true, 1024>), grid(2048), dim3(1024), lds, st, p);
+  else if (B > 256)
+    hipLaunchKernelGGL((step_maps_kernel<false, 1024>), grid(1024), dim3(1024), lds, st, p);
   else
-    hipLaunchKernelGGL(step_maps_kernel<false>, grid, dim3(kMapThreads), lds, static_cast<hipStream_t>(stream), p);
+    hipLaunchKernelGGL((step_maps_kernel<false, 256>), grid(256), dim3(256), lds, st, p);
   return (int)hipGetLastError();
 }
 
@@ -370,7 +445,7 @@ extern "C" int cie_release_pages(int64_t* free_list, const int64_t* slot_ids, in
                                  int32_t* err, void* stream) {
   if (B < 0 || page_size <= 0 || n_pages <= 0 || bt_width <= 0 || bt_stride < bt_width || n_slots <= 0)
     return CIE_EINVAL;
-  if (B > kMapMaxSeqs || page_size > 0x7fffffff || bt_width > kMapMaxPages || n_slots > 0x7fffffff ||
+  if (B > kMapMaxSeqs || page_size > kMapMaxPage || bt_width > kMapMaxPages || n_slots > 0x7fffffff ||
       n_pages > kMapMaxPages)
     return CIE_EUNSUPPORTED;
   if (B == 0) return CIE_OK;
@@ -390,9 +465,16 @@ extern "C" int cie_release_pages(int64_t* free_list, const int64_t* slot_ids, in
   p.page_size = (int32_t)page_size;
   p.hash_size = hash_size_of(B);
   p.err = err;
-  // Four sequences' pages a wave or so; the page counts are known on the device only.
-  const int64_t blocks = (B + 15) / 16;
-  hipLaunchKernelGGL(release_pages_kernel, dim3((unsigned)(blocks < 32 ? blocks : 32)), dim3(kMapThreads),
-                     batch_bytes((int)B, p.hash_size), static_cast<hipStream_t>(stream), p);
+  p.per_page = 1.0 / (double)page_size;
+  // The pages given back are known on the device only: as many workgroups as would
+  // empty the pool in 32 rounds (an arrival costs 1.5 us, a round 0.5).
+  const int64_t blocks = n_pages / 32768;
+  const size_t lds = batch_bytes((int)B, p.hash_size);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (B <= 256 && n_pages <= 8192)
+    hipLaunchKernelGGL(release_pages_kernel<256>, dim3(1), dim3(256), lds, st, p);
+  else
+    hipLaunchKernelGGL(release_pages_kernel<1024>, dim3((unsigned)(blocks < 1 ? 1 : blocks < 32 ? blocks : 32)),
+                       dim3(1024), lds, st, p);
   return (int)hipGetLastError();
 }

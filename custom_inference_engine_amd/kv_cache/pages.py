@@ -17,7 +17,6 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from .. import _native
 from .quant import int64_index, int64_table, launch, one_device
 
 _I64 = torch.int64
@@ -86,16 +85,23 @@ def step_maps(slot_ids, new_tokens, lens, block_table, page_size: int, total_T: 
         lens, block_table = int64_index(lens), int64_table(block_table)
     slot_ids, new_tokens = int64_index(slot_ids), int64_index(new_tokens)
     if out is None:
-        out = StepMaps(torch.empty(B + 1, dtype=_I64, device=dev),
-                       *torch.empty((4, total_T), dtype=_I64, device=dev).unbind(0))
+        room = torch.empty(B + 1 + 4 * total_T, dtype=_I64, device=dev)  # (one allocation: half the time of five)
+        out = StepMaps(*room.split_with_sizes((B + 1, total_T, total_T, total_T, total_T)))
     else:
         one_device(slot_ids, *out)
-    width = block_table.shape[1]
-    launch(dev, "cie_step_maps", out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(),
-           out[4].data_ptr(), slot_ids.data_ptr(), new_tokens.data_ptr(), lens.data_ptr(), block_table.data_ptr(),
-           pages, B, total_T, page_size, n_pages, block_table.stride(0), width,
-           min(lens.shape[0], block_table.shape[0]), err=err)
+    n_slots, width = block_table.shape
+    cu, slots, positions, rows_pages, offsets = out
+    launch(dev, "cie_step_maps", cu.data_ptr(), slots.data_ptr(), positions.data_ptr(), rows_pages.data_ptr(),
+           offsets.data_ptr(), slot_ids.data_ptr(), new_tokens.data_ptr(), lens.data_ptr(), block_table.data_ptr(),
+           pages, B, total_T, page_size, n_pages, block_table.stride(0), width, min(lens.shape[0], n_slots), err=err)
     return out
+
+
+def _tokens(t: torch.Tensor, slot_ids: torch.Tensor) -> torch.Tensor:
+    if t.shape != slot_ids.shape:
+        raise AssertionError("keep and held must have one entry per sequence")
+    one_device(slot_ids, t)
+    return int64_index(t)
 
 
 def release_pages(free_list, slot_ids, lens, block_table, page_size: int, keep=None, held=None, err=None) -> None:
@@ -110,15 +116,12 @@ def release_pages(free_list, slot_ids, lens, block_table, page_size: int, keep=N
     if slot_ids.dim() != 1 or page_size < 1:
         raise AssertionError("slot_ids must be (B,) and page_size positive")
     dev = one_device(free_list, slot_ids, lens, block_table)
-    tokens = []
-    for t in (keep, held):
-        if t is not None:
-            if t.shape != slot_ids.shape:
-                raise AssertionError("keep and held must have one entry per sequence")
-            one_device(slot_ids, t)
-            t = int64_index(t)
-        tokens.append(t)
+    if keep is not None:
+        keep = _tokens(keep, slot_ids)
+    if held is not None:
+        held = _tokens(held, slot_ids)
     slot_ids = int64_index(slot_ids)
     launch(dev, "cie_release_pages", free_list.data_ptr(), slot_ids.data_ptr(), lens.data_ptr(),
-           block_table.data_ptr(), _native.ptr(tokens[0]), _native.ptr(tokens[1]), slot_ids.shape[0], page_size,
+           block_table.data_ptr(), None if keep is None else keep.data_ptr(),
+           None if held is None else held.data_ptr(), slot_ids.shape[0], page_size,
            n_pages, block_table.stride(0), block_table.shape[1], min(lens.shape[0], block_table.shape[0]), err=err)

@@ -578,7 +578,8 @@ int cie_q8_mixed(void* o, const void* q, const void* k_pool, const void* v_pool,
  * table's row: page 0, offset 0, and no new pages for its sequence; rows past T are
  * dropped, negative counts are 0 (CIE_ERRBIT_LEN).  Page ids are not checked, but
  * for those of the list (CIE_ERRBIT_PAGE, page 0 in their place).
- * lens is not advanced.  B <= 2048, T <= 2^24, n_pages and bt_width <= 2^24.
+ * lens is not advanced.  B <= 2048, T <= 2^24, n_pages and bt_width <= 2^24,
+ * page_size <= 2^30.
  */
 int cie_step_maps(int64_t* cu_seqlens, int64_t* slots, int64_t* positions, int64_t* pages,
                   int64_t* offsets, const int64_t* slot_ids, const int64_t* new_tokens,
