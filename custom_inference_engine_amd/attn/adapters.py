@@ -75,12 +75,10 @@ def adapter_plan(row_slots: Optional[torch.Tensor], slot_adapters: torch.Tensor,
 
 
 def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
-    """(T, width), or (1, T, width): the rows, dense within each."""
-    if t.dim() == 3 and t.shape[0] == 1:
-        t = t[0]
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise AssertionError(f"{name} must be (T, width) or (1, T, width), its rows dense")
-    return t
+    """The rows of (1, T, width)."""
+    if t.dim() != 3 or t.shape[0] != 1:
+        raise AssertionError(f"{name} must be (T, width) or (1, T, width)")
+    return t[0]
 
 
 def adapter_add_(y, x, a, b, scales, ranks, plan, slices, err=None):
@@ -93,38 +91,42 @@ def adapter_add_(y, x, a, b, scales, ranks, plan, slices, err=None):
     the step's ``adapter_plan``.  A plan of other rows or adapters is reported in ``err``
     (CIE_ERRBIT_PLAN), and y left as it is.
     """
-    yr, xr = _rows(y, "y"), _rows(x, "x")
-    T, d_in = xr.shape
+    yr = y if y.dim() == 2 else _rows(y, "y")
+    xr = x if x.dim() == 2 else _rows(x, "x")
+    (T, d_in), (y_T, y_w) = xr.shape, yr.shape
+    (y_row, y_one), (x_row, x_one) = yr.stride(), xr.stride()
     widths, d_out, n_slices = _widths(slices if type(slices) is tuple else tuple(slices))
     dtype = y.dtype
     kind = _TYPES.get(dtype)
-    if kind is None or x.dtype != dtype or a.dtype != dtype or b.dtype != dtype:
+    if kind is None or x.dtype is not dtype or a.dtype is not dtype or b.dtype is not dtype:
         raise AssertionError("y, x, a and b must share float16 or bfloat16")
-    if yr.shape != (T, d_out):
+    if y_T != T or y_w != d_out:
         raise AssertionError(f"y must be ({T}, {d_out}): x's rows, the slices' widths")
+    if (y_one != 1 and d_out > 1) or (x_one != 1 and d_in > 1):
+        raise AssertionError("the rows of y and x must be dense")
+    if T > 1 and y_row < d_out:
+        raise AssertionError("y's rows must not share memory")
+    y_ptr, x_ptr = y.data_ptr(), x.data_ptr()
+    if y_ptr == x_ptr and T:
+        raise AssertionError("x must not lie in y's memory")
     n, S, R, w = a.shape if a.dim() == 4 else (0,) * 4
     if S != n_slices or w != d_in or R % RANK_UNIT or not 0 < R <= MAX_RANK or not a.is_contiguous():
         raise AssertionError(f"a must be contiguous (n, {n_slices}, R, {d_in}), R a multiple of 16 up to 128")
     if b.shape != (n, d_out, R) or not b.is_contiguous():
         raise AssertionError(f"b must be contiguous ({n}, {d_out}, {R})")
-    if scales.shape != (n,) or scales.dtype != _F32 or not scales.is_contiguous():
+    if scales.dtype is not _F32 or scales.shape != (n,) or not scales.is_contiguous():
         raise AssertionError(f"scales must be contiguous float32 ({n},)")
-    if ranks.shape != (n,) or ranks.dtype != _I32 or not ranks.is_contiguous():
+    if ranks.dtype is not _I32 or ranks.shape != (n,) or not ranks.is_contiguous():
         raise AssertionError(f"ranks must be contiguous int32 ({n},)")
-    words = _plan_words(T, n)
     held = plan.numel()
-    if plan.dtype != _I32 or held < words or not plan.is_contiguous():
+    if plan.dtype is not _I32 or held < _plan_words(T, n) or not plan.is_contiguous():
         raise AssertionError("plan must come from adapter_plan for these rows and adapters")
-    y_row = yr.stride(0)
-    if T > 1 and y_row < d_out:
-        raise AssertionError("y's rows must not share memory")
     dev = one_device(y, x, a, b, scales, ranks, plan)
     if T:
-        x_row = xr.stride(0)
         if T > 1 and x_row < d_in:
             xr = xr.contiguous()
-            x_row = d_in
-        launch(dev, "cie_adapter_add", yr.data_ptr(), y_row, xr.data_ptr(), x_row, a.data_ptr(), b.data_ptr(),
+            x_ptr, x_row = xr.data_ptr(), d_in
+        launch(dev, "cie_adapter_add", y_ptr, y_row, x_ptr, x_row, a.data_ptr(), b.data_ptr(),
                scales.data_ptr(), ranks.data_ptr(), plan.data_ptr(), 4 * held, T, n, R, d_in, widths,
                n_slices, kind, err=err)
     return y

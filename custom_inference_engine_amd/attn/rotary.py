@@ -22,6 +22,7 @@ from .. import _native
 from ..kv_cache.quant import int64_index, launch, one_device
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # CIE_F16, CIE_BF16, CIE_F32
+_F64, _DENSE = torch.float64, torch.contiguous_format
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None, device=None):
@@ -85,16 +86,17 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
 
 def _positions(positions: torch.Tensor, T: int) -> torch.Tensor:
     shape = positions.shape
-    if shape != (T,) and shape != (1, T):
+    if shape[-1:] != (T,) or (len(shape) != 1 and shape != (1, T)):
         raise AssertionError("positions must have one entry per row")
     return int64_index(positions)
 
 
 def _frequencies(frequencies: torch.Tensor, d: int) -> int:
     """The dims that turn."""
-    if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
+    shape = frequencies.shape
+    if frequencies.dtype is not _F64 or len(shape) != 1 or not frequencies.is_contiguous():
         raise AssertionError("frequencies must be contiguous float64 (pairs,)")
-    rot = 2 * frequencies.shape[0]
+    rot = 2 * shape[0]
     if rot < 2 or rot > d or d % 2:
         raise AssertionError(f"2 * len(frequencies) must be in [2, head_dim = {d}], head_dim even")
     return rot
@@ -142,12 +144,12 @@ def apply_rotary(q, k, positions, frequencies, interleaved: bool = False, scale:
         dev = one_device(q, k, positions, frequencies)
     positions = _positions(positions, T)
     q, q_row, q_head = _dense_heads(q, d)
-    q_out = q.new_empty(shape)
+    q_out = torch.empty_like(q, memory_format=_DENSE)
     if k is None:
         k_out, k_ptr, to_k, h_kv, k_row, k_head = None, None, None, 0, 0, 0
     else:
         k, k_row, k_head = _dense_heads(k, d)
-        k_out = k.new_empty(k_shape)
+        k_out = torch.empty_like(k, memory_format=_DENSE)
         k_ptr, to_k = k.data_ptr(), k_out.data_ptr()
     if T and h_q + h_kv:
         _native.call(dev, "cie_rotary", q_out.data_ptr(), to_k, q.data_ptr(), k_ptr, q_row, q_head, k_row, k_head,

@@ -228,7 +228,8 @@ def test_adapters_refuse():
                  dict(scales=scales[:2]), dict(ranks=ranks.long()), dict(plan=plan[:20]), dict(plan=plan.long()),
                  dict(slices=(96,)), dict(slices=(64, 31)), dict(y=y[:1].expand(5, 96)), dict(y=y.t()),
                  dict(a=torch.zeros((3, 2, 144, 64), dtype=f16), b=torch.zeros((3, 96, 144), dtype=f16)),
-                 dict(y=y.float(), x=x.float(), a=a.float(), b=b.float())):
+                 dict(y=y.float(), x=x.float(), a=a.float(), b=b.float()), dict(y=y[None, None]), dict(x=x[None].expand(2, 5, 64)),
+                 dict(x=y[:, :64])):
         with pytest.raises(AssertionError):
             cie.adapter_add_(**{**good, **over})
     with pytest.raises(AssertionError):
