@@ -55,9 +55,11 @@ constexpr int kAdHead = 8, kAdTileHead = 4;
 constexpr int kPlanWaves = 16;
 constexpr int kPlanThreads = kPlanWaves * kWave;
 constexpr int kPlanBatch = 8;  // rows of a lane whose loads are in flight
+constexpr int kPlanKept = 16;  // and that are kept from the count for the writing
 
-// Rows of a tile: more share A's and B's reads, fewer fill the chip.
-__host__ __device__ static inline int tile_rows(int64_t T) { return T <= 2048 ? 16 : 32; }
+// Rows of a tile: more share A's and B's reads, fewer fill the chip.  (1,052 rows of
+// 1,000 at rank 64: 9.2 us with 16, 9.7 with 32; 2,048 rows of 4,096 31.2 and 23.2.)
+__host__ __device__ static inline int tile_rows(int64_t T) { return T <= 1536 ? 16 : 32; }
 static inline int64_t max_tiles(int64_t T, int64_t N, int M) {
   const int64_t groups = T < N ? T : N;  // (a group of c rows has ceil(c / M) <= (c - 1) / M + 1 tiles)
   return groups + (T - groups) / M;
@@ -81,7 +83,7 @@ struct PlanParams {
 __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p) {
   __shared__ int count[kPlanWaves * kAdMaxAdapters];  // [wave][N]: rows of a wave, then their first place
   __shared__ int tile0[kAdMaxAdapters], sums[kPlanWaves];
-  __shared__ int seen[kPlanWaves][kPlanBatch][kWave];  // a batch's adapters and places (kPlaceBits), -1: none
+  __shared__ int seen[kPlanWaves][kPlanKept][kWave];   // rows' adapters and places (kPlaceBits), -1: none
   constexpr int kPlaceBits = 21;                       // (a wave has 2^20 rows at most)
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int64_t share = (p.T + kPlanThreads - 1) / kPlanThreads * kWave;
@@ -94,12 +96,13 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p
   int mistakes = 0, before = 0, total = 0, n = 0, tiles = 0;
   int* const out = p.plan + kAdHead;
   const int words = kAdTileHead + p.M;
-  const bool again = share > kPlanBatch * kWave;  // (else a wave's places are still there the second time)
+  const bool again = share > kPlanKept * kWave;  // (else a wave's places are still there the second time)
   for (int i = tid; i < waves * p.N; i += kPlanThreads) count[i] = 0;
   __syncthreads();
   for (int pass = 0; pass < 2; ++pass) {  // counted, then written
     for (int64_t at = first; at < end; at += kPlanBatch * kWave) {
       const int batch = (int)min((end - at + kWave - 1) / kWave, (int64_t)kPlanBatch);
+      int(*const kept)[kWave] = seen[wave] + (again ? 0 : (int)(at - first) / kWave);
       if (pass == 0 || again) {
         int64_t slot[kPlanBatch];
 #pragma unroll
@@ -116,12 +119,12 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p
           const int64_t a = p.slot_adapters[max(slot[i], (int64_t)0)];
           const bool none = slot[i] < 0 || a < 0 || a >= p.N;
           if (slot[i] >= 0 && a >= p.N) mistakes |= CIE_ERRBIT_ADAPTER;
-          seen[wave][i][lane] = none ? -1 : (int)a << kPlaceBits;
+          if (i < batch) kept[i][lane] = none ? -1 : (int)a << kPlaceBits;
         }
       }
 #pragma unroll 1
       for (int i = 0; i < batch; ++i) {
-        const int was = seen[wave][i][lane], id = was >> kPlaceBits;
+        const int was = kept[i][lane], id = was >> kPlaceBits;
         const bool live = was >= 0;
         int place = was & ((1 << kPlaceBits) - 1);
         if (pass == 0 || again) {
@@ -134,7 +137,7 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p
           int from = 0;
           if (live && (same & below) == 0) from = atomicAdd(&mine[id], __popcll(same));
           place = __shfl(from, live ? __builtin_ctzll(same) : 0, kWave) + __popcll(same & below);
-          if (pass == 0 && !again && live) seen[wave][i][lane] = id << kPlaceBits | place;
+          if (pass == 0 && !again && live) kept[i][lane] = id << kPlaceBits | place;
         }
         if (pass == 1 && live) {
           const int k = place + (again ? 0 : mine[id]);
@@ -148,22 +151,22 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p
     // Adapter a's rows before each wave's, and its tiles.
     if (tid < p.N) {
 #pragma unroll 1
-      for (int w = 0; w < waves; ++w) {
-        const int c = count[w * p.N + tid];
-        count[w * p.N + tid] = n;
-        n += c;
+      for (int w0 = 0; w0 < waves; w0 += 4) {  // (four reads, then four writes: one wait for each four)
+        int c[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) c[w] = w0 + w < waves ? count[(w0 + w) * p.N + tid] : 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          if (w0 + w < waves) count[(w0 + w) * p.N + tid] = n;
+          n += c[w];
+        }
       }
     }
     tiles = (n + p.M - 1) >> p.log_m;
     const int incl = wave_inclusive_sum(tiles);
     if (lane == kWave - 1) sums[wave] = incl;
     __syncthreads();
-    before = incl - tiles;
-#pragma unroll 1
-    for (int w = 0; w < kPlanWaves; ++w) {
-      if (w < wave) before += sums[w];
-      total += sums[w];
-    }
+    before = incl - tiles + waves_before<kPlanWaves>(sums[lane % kPlanWaves], wave, total);
     if (tid < p.N) tile0[tid] = before;
     __syncthreads();
   }
@@ -190,6 +193,7 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p
 constexpr int kAdBlock = 64;   // values of x a wave takes at a time: two MFMAs
 constexpr int kAdUnits = 8;    // 16-rank units of u held at once: one slice of 128 ranks, or several of fewer
 
+constexpr int kCus = 256;
 constexpr int kAdWaves = 8;
 constexpr int kAdThreads = kAdWaves * kWave;
 
@@ -294,15 +298,26 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
   // and B then come from its L2.
   const int32_t* const head = p.plan;
   const int xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
-  int tile, chunk;
+  int tile, chunk, per_chunk = p.per_chunk;
   if constexpr (MR == 1) {
     chunk = nth % p.chunks;
     tile = nth / p.chunks * 8 + xcd;
   } else {
-    const int items = head[0] * p.chunks, share = (items + 7) / 8;
-    const int item = nth < share ? xcd * share + nth : items;
-    tile = item / p.chunks;
-    chunk = item - tile * p.chunks;
+    // Whole rounds of the CUs, a tile a workgroup; the tiles of the last round share
+    // their columns among the CUs left (258 tiles of 32 rows of 4,096 at rank 64: 87 us
+    // without this, 52 for 256).
+    const int n = head[0], round = n / kCus * (kCus / 8), left = n % kCus;
+    const int chunks = left ? min(p.chunks, kCus / left) : 1, items = left * chunks, share = (items + 7) / 8;
+    if (nth < round) {
+      tile = xcd * round + nth;
+      chunk = 0;
+      per_chunk = p.col_tiles;
+    } else {
+      const int item = nth - round < share ? xcd * share + nth - round : items;
+      tile = item < items ? round * 8 + item / chunks : n;
+      chunk = item % chunks;
+      per_chunk = (p.col_tiles + chunks - 1) / chunks;
+    }
   }
   const int32_t* const desc = p.plan + kAdHead + (int64_t)min(tile, p.max_tiles - 1) * (kAdTileHead + M);
   const int tid = threadIdx.x, lane = tid % kWave, wave = uniform(tid / kWave), m = lane % 16, g = lane / 16;
@@ -316,7 +331,8 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
     return;
   }
   if (tile >= head[0]) return;
-  const int ct0 = chunk * p.per_chunk, ct1 = min(ct0 + p.per_chunk, p.col_tiles);
+  const int ct0 = chunk * per_chunk, ct1 = min(ct0 + per_chunk, p.col_tiles);
+  if (ct0 >= ct1) return;
   // The slices' first columns and column tiles, by index: not by a load each time.
   const auto slice_of = [&](int ct) {
     return (int)(ct >= p.slice_tile[1]) + (int)(ct >= p.slice_tile[2]) + (int)(ct >= p.slice_tile[3]);
@@ -681,13 +697,20 @@ extern "C" int cie_adapter_add(void* y, int64_t y_row_stride, const void* x, int
   p.col_tiles = (int32_t)tiles;
   p.err = err;
   // Few tiles: several workgroups share one's columns (each computes u again), down to a
-  // column tile a wave.
-  const int64_t per_tile = (tiles + kAdWaves - 1) / kAdWaves;
-  int64_t chunks = 256 / p.max_tiles;
-  chunks = chunks < 1 ? 1 : chunks > per_tile ? per_tile : chunks;
-  p.per_chunk = (int32_t)((tiles + chunks - 1) / chunks);
-  p.chunks = (int32_t)((tiles + p.per_chunk - 1) / p.per_chunk);
-  const int64_t blocks = (int64_t)(p.max_tiles + 7) / 8 * 8 * p.chunks;
+  // column tile a wave and a workgroup a CU.  Tiles of 16 rows go by how many tiles there
+  // can be (their workgroups read their tile before they know how many there are).
+  const int64_t most = (tiles + kAdWaves - 1) / kAdWaves;
+  int64_t blocks;
+  if (tile_rows(T) == 16) {
+    int64_t chunks = kCus / p.max_tiles;
+    chunks = chunks < 1 ? 1 : chunks > most ? most : chunks;
+    p.per_chunk = (int32_t)((tiles + chunks - 1) / chunks);
+    p.chunks = (int32_t)((tiles + p.per_chunk - 1) / p.per_chunk);
+    blocks = (int64_t)(p.max_tiles + 7) / 8 * 8 * p.chunks;
+  } else {
+    p.chunks = (int32_t)most;
+    blocks = (int64_t)kCus * (p.max_tiles / kCus + 1);
+  }
   if (blocks > 0x7fffffff) return CIE_EUNSUPPORTED;
   const dim3 grid((unsigned)blocks);
   const int units = (int)(n_slices * (R / 16) < 5 ? n_slices * (R / 16) : 4);

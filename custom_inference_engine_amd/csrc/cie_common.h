@@ -41,6 +41,16 @@ __device__ __forceinline__ int wave_inclusive_sum(int v) {
   return v;
 }
 
+// Of a workgroup's kWaves waves: the sum over the waves before this one, and over all
+// (total).  sum: lane l holds wave l % kWaves's.  Every lane must be active.
+template <int kWaves>
+__device__ __forceinline__ int waves_before(int sum, int wave, int& total) {
+  const int lane = threadIdx.x % kWave;
+  const int incl = wave_inclusive_sum(lane < kWaves ? sum : 0);
+  total = __builtin_amdgcn_readlane(incl, kWaves - 1);
+  return __shfl(incl - sum, wave, kWave);
+}
+
 // Lane exchange l <-> l^m (ds_bpermute under the hood).
 __device__ __forceinline__ float lane_xor(float x, int m) {
   return __shfl_xor(x, m, kWave);

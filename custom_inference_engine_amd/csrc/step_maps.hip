@@ -112,17 +112,12 @@ __device__ __forceinline__ void block_exclusive(int& a, int& b, int cap_a, int c
     sm[wave][1] = min(in_b, cap_b);
   }
   __syncthreads();
-  int before_a = 0, before_b = 0;
-  total_a = total_b = 0;
-#pragma unroll 4
-  for (int w = 0; w < kThreads / kWave; ++w) {
-    if (w == wave) {
-      before_a = total_a;
-      before_b = total_b;
-    }
-    total_a = min(total_a + sm[w][0], cap_a);
-    total_b = min(total_b + sm[w][1], cap_b);
-  }
+  constexpr int kWaves = kThreads / kWave;
+  const int from = threadIdx.x % kWaves;  // (of 16 waves at most: the caps' sums fit 31 bits)
+  const int before_a = min(waves_before<kWaves>(sm[from][0], wave, total_a), cap_a);
+  const int before_b = min(waves_before<kWaves>(sm[from][1], wave, total_b), cap_b);
+  total_a = min(total_a, cap_a);
+  total_b = min(total_b, cap_b);
   a = min(before_a + min(in_a - a, cap_a), cap_a);
   b = min(before_b + min(in_b - b, cap_b), cap_b);
 }

@@ -242,8 +242,8 @@ def test_plan_sizes(native_lib):
     words = lambda T, n: native_lib.cie_adapter_plan_bytes(T, n) // 4  # noqa: E731
     assert words(1, 1) == 8 + 20 and words(5, 3) == 8 + 3 * 20
     # every dealing of T rows to at most n adapters fits: the worst is one row for all adapters but one
-    for T, n in ((1, 5), (40, 40), (100, 7), (2048, 1000), (2049, 1000), (5000, 3)):
-        m = 16 if T <= 2048 else 32
+    for T, n in ((1, 5), (40, 40), (100, 7), (1536, 1000), (1537, 1000), (5000, 3)):
+        m = 16 if T <= 1536 else 32
         g = min(T, n)
         worst = (g - 1) + -(-(T - g + 1) // m)
         assert words(T, n) >= 8 + worst * (4 + m)
