@@ -164,6 +164,13 @@ class AdapterBank(torch.nn.Module):
         self.register_buffer("scales", make((n_adapters,), dtype=torch.float32), persistent=False)
         self.register_buffer("ranks", make((n_adapters,), dtype=torch.int32), persistent=False)
 
+    def _apply(self, fn, recurse=True):
+        # (a model that is cast casts A and B; the scales stay fp32)
+        kept = self.scales
+        super()._apply(fn, recurse)
+        self.scales = kept.to(self.scales.device)
+        return self
+
     @torch.no_grad()
     def load(self, i: int, a, b, scale: float = 1.0) -> None:
         """Adapter i: for each slice A (r, in_features) and B (width, r), or None for a slice without one."""

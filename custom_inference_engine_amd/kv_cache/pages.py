@@ -20,6 +20,7 @@ import torch
 from .quant import int64_index, int64_table, launch, one_device
 
 _I64 = torch.int64
+ERR_FREE = 32  # CIE_ERRBIT_FREE
 
 
 class StepMaps(NamedTuple):

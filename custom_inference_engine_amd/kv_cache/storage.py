@@ -178,29 +178,40 @@ class KVStorage:
         self.last_generated = torch.zeros((n_slots,), dtype=torch.long, device=self.device)
 
         self.free_list = None      # block tables kept on the device (manage_pages)
+        self.page_err = None       # what its steps reported since check_pages
         self.slot_adapters = None  # each slot's low-rank adapter, -1: none (use_adapters)
         self.n_adapters = 0
 
     def manage_pages(self) -> None:
         """Block tables are kept on the device from here on: the step modules' steps take the pages that their new
-        tokens need from ``free_list`` (``pages.step_maps``), ``release`` gives them back.  Comes before the step
+        tokens need from ``free_list`` (``pages.step_maps``), ``reset`` gives them back.  Comes before the step
         modules and the scheduler, with every slot empty."""
         if bool(self.lens.any()) or bool(self.block_table.any()):
             raise AssertionError("manage_pages needs every slot empty")
         self.free_list = _pages.new_free_list(self.n_pages, self.device)
+        self.page_err = torch.zeros(1, dtype=torch.int32, device=self.device)
+
+    def check_pages(self) -> None:
+        """Raises if a step since the last check found too few free pages, or bad slots or lengths (waits for it)."""
+        bits = int(self.page_err)
+        if bits:
+            self.page_err.zero_()
+            raise RuntimeError("out of free pages: the step's tokens were not kept" if bits & _pages.ERR_FREE
+                               else f"bad slots, lengths or pages in a step (error bits {bits})")
+
+    def reset_pages(self) -> None:
+        """Every slot of a pool that manages its pages emptied, every page free, whatever a failed step left."""
+        self.lens.zero_()
+        self.block_table.zero_()
+        self.free_list.copy_(_pages.new_free_list(self.n_pages, self.device))
+        self.page_err.zero_()
+        if self.slot_adapters is not None:
+            self.slot_adapters.fill_(-1)
 
     def step_maps(self, slot_ids: torch.Tensor, new_tokens: torch.Tensor, total_T: int, out=None) -> _pages.StepMaps:
         """A packed step's maps (``pages.step_maps``), with pages for its new tokens if the pool manages them."""
         return _pages.step_maps(slot_ids, new_tokens, self.lens, self.block_table, self.page_size, total_T,
-                                free_list=self.free_list, out=out)
-
-    def release(self, slot_ids: list[int]) -> None:
-        """``reset`` of a pool that manages its pages: the slots are emptied and their pages free."""
-        if slot_ids:
-            slots = torch.tensor(slot_ids, dtype=torch.long).to(self.lens.device)
-            _pages.release_pages(self.free_list, slots, self.lens, self.block_table, self.page_size)
-            if self.slot_adapters is not None:
-                self.slot_adapters[slots] = -1
+                                free_list=self.free_list, out=out, err=self.page_err)
 
     def use_adapters(self, n_adapters: int) -> None:
         """Slots may have one of ``n_adapters`` low-rank adapters (``attn.adapters``)."""
@@ -255,7 +266,11 @@ class KVStorage:
         self.lens[self.unused_idx:self.unused_idx + 1].mul_(0)
 
     def reset(self, slot_ids: list[int]) -> None:
-        self.lens[slot_ids] = 0
-        self.block_table[slot_ids] = 0
+        if self.free_list is not None:  # the slots' pages are free again
+            slots = torch.tensor(slot_ids, dtype=torch.long).to(self.lens.device)
+            _pages.release_pages(self.free_list, slots, self.lens, self.block_table, self.page_size, err=self.page_err)
+        else:
+            self.lens[slot_ids] = 0
+            self.block_table[slot_ids] = 0
         if self.slot_adapters is not None:
             self.slot_adapters[slot_ids] = -1

@@ -50,6 +50,7 @@ class DecodeModule:
         self.metadata.slot_ids = self.slots
         self.tokens = torch.zeros((batch_size,), dtype=torch.long, device=dev)
         self.positions = torch.zeros((batch_size,), dtype=torch.long, device=dev)
+        self.managed = getattr(kv_cache, "free_list", None) is not None  # the step takes its pages itself
         self.ones = torch.ones((batch_size,), dtype=torch.long, device=dev)
         with torch.inference_mode():
             self.step = StepGraph(self._step, pool=pool, warmup=warmup_iters, device=dev)
@@ -57,9 +58,9 @@ class DecodeModule:
 
     def _step(self) -> torch.Tensor:
         kv = self.kv_cache
-        if kv.free_list is not None:  # pages for the new tokens, before the plan reads the block tables
+        if self.managed:  # pages for the new tokens, before the plan reads the block tables
             kv.step_maps(self.slots, self.ones, self.batch_size)
-        if kv.slot_adapters is not None:
+        if getattr(kv, "slot_adapters", None) is not None:
             self.metadata.adapter_plan = adapter_plan(self.slots, kv.slot_adapters, kv.n_adapters)
         # one plan for every layer's decode launch (their slots, lengths and
         # block-table rows are the step's): splits balanced by length, page
@@ -94,4 +95,6 @@ class DecodeModule:
             logits = self.replay()
             next_tokens = torch.argmax(logits[:n], dim=-1)
             self.kv_cache.last_generated[self.slots[:n]] = next_tokens
+            if self.managed:
+                self.kv_cache.check_pages()
             return next_tokens.tolist()

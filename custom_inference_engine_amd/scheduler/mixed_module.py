@@ -80,7 +80,7 @@ class MixedModule:
         self.row_slots = torch.zeros((T,), dtype=torch.long, device=dev)
         self.maps = StepMaps(self.cu_seqlens, self.row_slots, self.positions, self.metadata.pages,
                              self.metadata.offsets)
-        if kv_cache.slot_adapters is not None:  # (read by captured pieces: one address for every step)
+        if getattr(kv_cache, "slot_adapters", None) is not None:  # (read by captured pieces: one address for every step)
             self.metadata.adapter_plan = new_adapter_plan(T, kv_cache.n_adapters, dev)
         self.last_logits = None  # (n, vocab) of the last forward
 
@@ -102,7 +102,7 @@ class MixedModule:
             self.metadata.mixed_plan = make_plan(
                 kv.keys[0], self.cu_seqlens, kv.lens[self.slots], self.slots, kv.block_table, T, T,
                 self.model.config.num_attention_heads)
-            if kv.slot_adapters is not None:
+            if getattr(kv, "slot_adapters", None) is not None:
                 adapter_plan(self.row_slots, kv.slot_adapters, kv.n_adapters, out=self.metadata.adapter_plan)
 
     def _prepare_host(self, kv, B: int) -> None:
@@ -173,6 +173,8 @@ class MixedModule:
             self.last_logits = logits
             next_tokens = torch.argmax(logits, dim=-1)
             self.kv_cache.last_generated[self.slots[:n]] = next_tokens
+            if getattr(self.kv_cache, "free_list", None) is not None:
+                self.kv_cache.check_pages()
             return next_tokens.tolist()
 
 

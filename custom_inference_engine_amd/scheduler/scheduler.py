@@ -223,7 +223,7 @@ class Scheduler:
         self.model = model
         self.kv_cache = kv_cache
         # the pool keeps its block tables itself (KVStorage.manage_pages): pages are only counted here
-        self.device_pages = kv_cache.free_list is not None
+        self.device_pages = getattr(kv_cache, "free_list", None) is not None
         self.n_slots = n_slots
         self.page_size = kv_cache.page_size
         self.n_pages = kv_cache.n_pages
@@ -295,9 +295,7 @@ class Scheduler:
             self._free_slots.add(s)
             if s in self.order:
                 self.order.remove(s)
-        if slot_ids and self.device_pages:
-            self.kv_cache.release(slot_ids)
-        elif slot_ids:
+        if slot_ids:
             self.kv_cache.reset(slot_ids)
 
     # ------------------------------------------------------------------ one step
@@ -385,7 +383,7 @@ class Scheduler:
         for s, n in zip(slot_ids, budgets):
             self.slots[s].budget = n
         self._palloc(slot_ids, page_counts)
-        if slot_ids and self.kv_cache.slot_adapters is not None:
+        if slot_ids and getattr(self.kv_cache, "slot_adapters", None) is not None:
             self.kv_cache.slot_adapters[self._device_ids(slot_ids)] = self._device_ids(
                 [self.slots[s].adapter for s in slot_ids])
 
@@ -438,8 +436,8 @@ class Scheduler:
         fut: Future = Future()
         if not self.open:
             fut.set_exception(RuntimeError("Loop is not open."))
-        elif adapter != -1 and not 0 <= adapter < self.kv_cache.n_adapters:
-            fut.set_exception(ValueError(f"No adapter {adapter} of {self.kv_cache.n_adapters}."))
+        elif adapter != -1 and not 0 <= adapter < getattr(self.kv_cache, "n_adapters", 0):
+            fut.set_exception(ValueError(f"The pool has no adapter {adapter}."))
         elif len(prompt) == 0:
             fut.set_exception(ValueError("Empty prompts are not allowed."))
         elif self._required_pages(len(prompt), total=True) > self.n_pages - 1:
@@ -501,6 +499,8 @@ class Scheduler:
         while self.preempted:
             _fail(self.preempted.pop().future, exc)
         self._release(sorted(self._busy_slots))
+        if self.device_pages:  # (a step that failed may have taken pages that no slot counts)
+            self.kv_cache.reset_pages()
         self.order.clear()
         self._reset_occupancy()
 

@@ -175,13 +175,13 @@ def test_requests_with_their_own_adapters(native_lib):
             assert _rel(dec.logits[i], _logits(models[i], seqs[i])) < bar, (step, i)
             seqs[i].append(nxt[i])
     note("adapters: mixed step of decode rows, and a slot with another request's adapter")
-    kv.release([2])
+    kv.reset([2])
     kv.slot_adapters[2] = 1
     more = _prompts(30, seed=8)[0]
     nxt = eager.forward([[s[-1]] for s in (seqs[0], seqs[2])] + [more], [1, 3, 2])
     for got, model, seq in zip(eager.last_logits, (models[0], models[2], merged(theirs, 1)), (seqs[0], seqs[2], more)):
         assert _rel(got, _logits(model, seq)) < bar
-    kv.release([1, 2, 3, 5])
+    kv.reset([1, 2, 3, 5])
     assert int(kv.free_list[0]) == kv.n_pages - 1 and kv.lens.eq(0).all() and kv.block_table.eq(0).all()
 
 
@@ -234,6 +234,47 @@ def test_maps_of_the_step_modules(native_lib):
         for a, b in zip(got, (mod.cu_seqlens, mod.positions, mod.metadata.pages, mod.metadata.offsets)):
             assert torch.equal(a, b)
     assert mod.row_slots.tolist() == [4] * 17 + [2] + [5] * 30 + [0] * 16
+
+
+def test_out_of_pages(native_lib):
+    """A pool that manages its pages says when a step finds too few, keeps every token it held, and goes on when some are
+    free again; eagerly and in graphs."""
+    cfg = _config()
+    _, ours = _models(cfg)
+    kv = KVStorage(cfg, max_cache_len=6 * 16, page_size=16, n_slots=4, device=DEV, dtype=torch.float16)
+    kv.manage_pages()
+    mix, dec = MixedModule(ours, kv, token_count=64), DecodeModule(ours, kv, batch_size=2)
+    full = FullMixedModule(ours, kv, batch_size=3, token_count=64)
+    note("out of pages")
+    mix.forward([[1] * 32, [2] * 32], [1, 2])  # four of five pages
+    held = kv.keys[0][kv.block_table[1, :2]].clone()
+    for module in (mix, full):
+        with pytest.raises(RuntimeError, match="free pages"):
+            module.forward([[3] * 20], [3])
+        kv.lens[3] = 0  # (the caller drops the step)
+        assert int(kv.free_list[0]) == 1 and not kv.block_table[3].any()
+    with pytest.raises(RuntimeError, match="free pages"):
+        dec.forward([1, 2])  # a page each
+    kv.lens[1:3] = 32
+    assert torch.equal(kv.keys[0][kv.block_table[1, :2]], held)
+    kv.reset([2])
+    assert int(kv.free_list[0]) == 3
+    dec.forward([1])
+    assert kv.lens.tolist() == [0, 33, 0, 0] and int(kv.block_table[1, 2]) > 0
+    kv.reset_pages()
+    assert int(kv.free_list[0]) == 5 and not kv.lens.any() and not kv.block_table.any()
+
+
+def test_a_model_that_is_cast_keeps_its_adapters(native_lib):
+    cfg = _config()
+    _, ours = _models(cfg)
+    kv = KVStorage(cfg, max_cache_len=256, page_size=16, n_slots=3, device=DEV, dtype=torch.float16)
+    layers = use_adapters(ours, kv, 2, 8)
+    layers[0].o_adapters.load(1, torch.ones(3, 896), torch.ones(896, 3), scale=0.3)
+    ours.half()
+    bank = layers[0].o_adapters
+    assert bank.scales.dtype == torch.float32 and bank.ranks.dtype == torch.int32 and bank.a.dtype == torch.float16
+    assert bank.scales[1] == torch.tensor(0.3)
 
 
 def _run(ours, kv, prompts, theirs, bar=2e-2):

@@ -342,6 +342,14 @@ class CountingExecutor:
         return self._step(slot_ids, [len(c) for c in chunks])
 
 
+def _release(free_list, slots, lens, table, page_size, err=None):
+    li, ta, fr = lens.tolist(), table.tolist(), ref.FreeList(free_list.tolist())
+    assert ref.release_pages(fr, slots.tolist(), li, ta, page_size)
+    lens.copy_(torch.tensor(li))
+    table.copy_(torch.tensor(ta))
+    free_list.copy_(torch.tensor(fr.words()))
+
+
 def test_scheduler_with_pages_on_the_device(monkeypatch):
     """Pages are only counted on the host: the device's list never runs short, through admissions, chunked prefills and
     preemptions, each request keeps its adapter, and everything is given back."""
@@ -350,14 +358,7 @@ def test_scheduler_with_pages_on_the_device(monkeypatch):
     kv.use_adapters(4)
     before = kv.free_list[0].item()
 
-    def release(free_list, slots, lens, table, page_size):
-        li, ta, fr = lens.tolist(), table.tolist(), ref.FreeList(free_list.tolist())
-        assert ref.release_pages(fr, slots.tolist(), li, ta, page_size)
-        lens.copy_(torch.tensor(li))
-        table.copy_(torch.tensor(ta))
-        free_list.copy_(torch.tensor(fr.words()))
-
-    monkeypatch.setattr("custom_inference_engine_amd.kv_cache.pages.release_pages", release)
+    monkeypatch.setattr("custom_inference_engine_amd.kv_cache.pages.release_pages", _release)
     executor = CountingExecutor(kv)
     sched = Scheduler(None, kv, eos_token_ids={128}, max_new_tokens=16, token_budget=160, executor=executor)
     lengths, adapters = (60, 70, 50, 9, 64), [2, -1, 0, 3, -1]
@@ -369,6 +370,41 @@ def test_scheduler_with_pages_on_the_device(monkeypatch):
     assert seen == set(adapters)
     with pytest.raises(ValueError):
         sched.generate([[1]], [1, 2])
+
+
+def test_a_failed_step_leaks_no_pages(monkeypatch):
+    """A step that took pages and failed: the loop's end leaves the pool empty and its list whole."""
+    monkeypatch.setattr("custom_inference_engine_amd.kv_cache.pages.release_pages", _release)
+    kv = cie.KVStorage(_cfg(), max_cache_len=192, page_size=16, n_slots=4, device="cpu", dtype=torch.float16)
+    kv.manage_pages()
+    kv.use_adapters(1)
+    executor = CountingExecutor(kv)
+
+    def fails(chunks, slot_ids):
+        lens = kv.lens.clone()
+        executor._step(slot_ids, [len(c) for c in chunks])
+        kv.lens.copy_(lens)  # (its tokens were never counted)
+        raise ZeroDivisionError
+
+    executor.mixed = fails
+    sched = Scheduler(None, kv, eos_token_ids={128}, max_new_tokens=16, token_budget=160, executor=executor)
+    future = sched.call([1] * 40, adapter=0)
+    with pytest.raises(ZeroDivisionError):
+        sched.loop()
+    assert isinstance(future.exception(), ZeroDivisionError)
+    assert torch.equal(kv.free_list, cie.new_free_list(kv.n_pages, "cpu")) and not kv.lens.any() and not kv.block_table.any()
+    assert (kv.slot_adapters == -1).all()
+
+
+def test_pages_that_are_managed_report_errors():
+    kv = cie.KVStorage(_cfg(), max_cache_len=192, page_size=16, n_slots=4, device="cpu", dtype=torch.float16)
+    kv.manage_pages()
+    kv.check_pages()
+    for bits, text in ((32, "free pages"), (2, "bad slots"), (33, "free pages")):
+        kv.page_err.fill_(bits)
+        with pytest.raises(RuntimeError, match=text):
+            kv.check_pages()
+        kv.check_pages()
 
 
 def test_scheduler_refuses_adapters_it_has_not():
