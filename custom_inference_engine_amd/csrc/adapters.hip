@@ -70,9 +70,24 @@ struct PlanParams {
   const int64_t* row_slots;
   const int64_t* slot_adapters;
   int64_t T, n_slots;
-  int32_t N, M, log_m;
+  int64_t rows, share;  // of a workgroup, of a wave
+  int32_t* counts;      // [groups][N] rows of a workgroup, where there are several
+  int32_t N, M, log_m, groups;
   int32_t* err;
 };
+
+// Many rows are planned by several workgroups in two launches: each counts its rows,
+// then each writes its rows behind those of the workgroups before it.  One workgroup
+// does both at once, bound by what a CU reads and by the rounds of a wave: 32 rows 4.3 us,
+// 1,052 rows 5.7, 8,192 rows 12.4 (two launches 12.6); 65,536 rows 122, in two launches 27.
+constexpr int64_t kPlanAlone = 8192;
+constexpr int kPlanGroups = 64;
+static inline int64_t group_rows(int64_t T) {
+  if (T <= kPlanAlone) return T;
+  const int64_t rows = (T + kPlanGroups - 1) / kPlanGroups;
+  return (rows + kPlanThreads - 1) / kPlanThreads * kPlanThreads;
+}
+enum PlanPhase { kPlanAll, kPlanCount, kPlanWrite };
 
 // Rows are dealt to the waves in order, 64 adjacent rows at a time, and each wave
 // counts its own, so that a group's rows keep their order and the plan is the same
@@ -80,15 +95,16 @@ struct PlanParams {
 // and the first of them takes as many places as they are.  Two dependent loads, the
 // count, a scan over adapters, the rows.  The code is kept short (loops are not
 // unrolled but for the loads'): it runs once, from a cold instruction cache.
+template <PlanPhase kPhase>
 __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p) {
   __shared__ int count[kPlanWaves * kAdMaxAdapters];  // [wave][N]: rows of a wave, then their first place
   __shared__ int tile0[kAdMaxAdapters], sums[kPlanWaves];
   __shared__ int seen[kPlanWaves][kPlanKept][kWave];   // rows' adapters and places (kPlaceBits), -1: none
   constexpr int kPlaceBits = 21;                       // (a wave has 2^20 rows at most)
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int64_t share = (p.T + kPlanThreads - 1) / kPlanThreads * kWave;
-  const int64_t first = wave * share, end = min(first + share, p.T);
-  const int waves = (int)min((p.T + share - 1) / share, (int64_t)kPlanWaves);  // that have rows
+  const int64_t row0 = kPhase == kPlanAll ? 0 : blockIdx.x * p.rows, row1 = min(row0 + p.rows, p.T);
+  const int64_t share = p.share, first = row0 + wave * share, end = min(first + share, row1);
+  const int waves = (int)((row1 - row0 + share - 1) / share);  // that have rows
   const int bits = 32 - __builtin_clz(p.N);
   const uint64_t below = (1ull << lane) - 1;
   int* const mine = count + wave * p.N;
@@ -149,6 +165,18 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p
     if (pass == 1) break;
     __syncthreads();
     // Adapter a's rows before each wave's, and its tiles.
+    int rest = 0;  // rows of the workgroups from this one on
+    if (kPhase == kPlanWrite && tid < p.N) {
+#pragma unroll 8
+      for (int w = 0; w < p.groups; ++w) {
+        const int c = p.counts[w * p.N + tid];
+        if (w < (int)blockIdx.x)
+          n += c;
+        else
+          rest += c;
+      }
+      rest += n;
+    }
     if (tid < p.N) {
 #pragma unroll 1
       for (int w0 = 0; w0 < waves; w0 += 4) {  // (four reads, then four writes: one wait for each four)
@@ -162,6 +190,11 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p
         }
       }
     }
+    if constexpr (kPhase == kPlanCount) {
+      if (tid < p.N) p.counts[blockIdx.x * p.N + tid] = n;
+      break;
+    }
+    if (kPhase == kPlanWrite) n = rest;  // (all its rows)
     tiles = (n + p.M - 1) >> p.log_m;
     const int incl = wave_inclusive_sum(tiles);
     if (lane == kWave - 1) sums[wave] = incl;
@@ -170,6 +203,8 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p
     if (tid < p.N) tile0[tid] = before;
     __syncthreads();
   }
+  if (mistakes && kPhase != kPlanWrite) set_err(p.err, mistakes);  // (counted rows have been looked at)
+  if (kPhase == kPlanCount || blockIdx.x > 0) return;
   if (tid < p.N) {
 #pragma unroll 1
     for (int k = 0; k < tiles; ++k) {
@@ -185,7 +220,6 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p
     p.plan[3] = p.M;
     p.plan[4] = kAdMagic;
   }
-  if (mistakes) set_err(p.err, mistakes);
 }
 
 // ---- the products ----
@@ -624,7 +658,8 @@ using namespace cie;
 extern "C" int64_t cie_adapter_plan_bytes(int64_t T, int64_t N) {
   if (T < 0 || N <= 0 || T > kAdMaxRows || N > kAdMaxAdapters) return -1;
   const int M = tile_rows(T);
-  return 4 * (kAdHead + max_tiles(T, N, M) * (kAdTileHead + M));
+  const int64_t groups = T > kPlanAlone ? (T + group_rows(T) - 1) / group_rows(T) : 0;
+  return 4 * (kAdHead + max_tiles(T, N, M) * (kAdTileHead + M) + groups * N);
 }
 
 extern "C" int cie_adapter_plan(int32_t* plan, int64_t plan_bytes, const int64_t* row_slots,
@@ -645,7 +680,20 @@ extern "C" int cie_adapter_plan(int32_t* plan, int64_t plan_bytes, const int64_t
   p.M = tile_rows(T);
   p.log_m = p.M == 16 ? 4 : 5;
   p.err = err;
-  hipLaunchKernelGGL(adapter_plan_kernel, dim3(1), dim3(kPlanThreads), 0, static_cast<hipStream_t>(stream), p);
+  p.rows = group_rows(T);
+  p.share = (p.rows + kPlanThreads - 1) / kPlanThreads * kWave;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (T == 0) return CIE_OK;
+  if (T <= kPlanAlone) {
+    hipLaunchKernelGGL(adapter_plan_kernel<kPlanAll>, dim3(1), dim3(kPlanThreads), 0, st, p);
+    return (int)hipGetLastError();
+  }
+  p.groups = (int32_t)((T + p.rows - 1) / p.rows);
+  p.counts = plan + kAdHead + max_tiles(T, N, p.M) * (kAdTileHead + p.M);
+  hipLaunchKernelGGL(adapter_plan_kernel<kPlanCount>, dim3((unsigned)p.groups), dim3(kPlanThreads), 0, st, p);
+  const int status = (int)hipGetLastError();
+  if (status) return status;
+  hipLaunchKernelGGL(adapter_plan_kernel<kPlanWrite>, dim3((unsigned)p.groups), dim3(kPlanThreads), 0, st, p);
   return (int)hipGetLastError();
 }
 

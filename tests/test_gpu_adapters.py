@@ -86,7 +86,7 @@ def test_ranks_of_their_own(dtype):
     assert empty.any() and torch.equal(case.run()[empty], case.y[empty])  # an empty place
 
 
-@pytest.mark.parametrize("T,n", [(1536, 3), (1537, 3), (2500, 300), (4100, 1), (5000, 1024), (8200, 2)])
+@pytest.mark.parametrize("T,n", [(1536, 3), (1537, 3), (2500, 300), (4100, 1), (5000, 1024), (8200, 2), (70000, 5)])
 def test_many_rows(T, n):
     """Both tile heights; rows dealt over one, few and many adapters."""
     case = Case(spread(T, n, none=0.1), n, 16, 64, (64,), F16)
@@ -95,7 +95,7 @@ def test_many_rows(T, n):
 
 def test_plan_is_the_rows_in_order():
     """Tiles of one adapter, adapters and their rows ascending: the same plan every time."""
-    for T, n in ((1, 1), (50, 4), (700, 9), (1537, 5), (9000, 700), (17000, 40)):
+    for T, n in ((1, 1), (50, 4), (700, 9), (1537, 5), (8192, 3), (8193, 3), (9000, 700), (17000, 40), (100000, 1024)):
         ids = spread(T, n, seed=T)
         on_device = torch.tensor(ids, dtype=torch.int64, device=DEV)
         note(f"plan T={T} n={n}")
