@@ -246,19 +246,37 @@ struct AddParams {
   int32_t* err;
 };
 
-// Eight values from k on, zeros at and past n.
+// Eight values from k on, zeros at and past n.  Rows at any 2-byte address: one load all
+// the same (global memory may be read so), but for the last few values.
 template <class E, bool kAligned>
 __device__ __forceinline__ typename Lane8<E>::type load8(const E* row, int k, int n) {
   typedef typename Lane8<E>::type vec;
+  typedef vec any_vec __attribute__((aligned(2)));
   vec v = {};
   if constexpr (kAligned) {
     if (k < n) v = *reinterpret_cast<const vec*>(row + k);
+  } else if (k + 8 <= n) {
+    v = *reinterpret_cast<const any_vec*>(row + k);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < 7; ++e)
       if (k + e < n) v[e] = row[k + e];
   }
   return v;
+}
+template <class E, bool kAligned>
+__device__ __forceinline__ void store8(E* row, int k, int n, typename Lane8<E>::type v) {
+  typedef typename Lane8<E>::type vec;
+  typedef vec any_vec __attribute__((aligned(2)));
+  if constexpr (kAligned) {
+    if (k < n) *reinterpret_cast<vec*>(row + k) = v;
+  } else if (k + 8 <= n) {
+    *reinterpret_cast<any_vec*>(row + k) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (k + e < n) row[k + e] = v[e];
+  }
 }
 
 // 2^e that takes m (fp16: the largest |u| of a row) to [2^14, 2^15); 1 where there is no such.
@@ -611,13 +629,7 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
             asm volatile("" : "+v"(sum));  // (to fp32 first, in every variant: no v_fma_mixlo_f16)
             v[e] = (E)sum;
           }
-          if constexpr (kAligned) {
-            if (c < end) *reinterpret_cast<vec*>(to + c) = v;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (c + e < end) to[c + e] = v[e];
-          }
+          store8<E, kAligned>(to, c, end, v);
         }
         lds_order();
       }
@@ -630,10 +642,10 @@ static bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr
 
 template <class E, int MR, bool kAligned>
 static void launch_add(const AddParams& p, int units, dim3 grid, hipStream_t stream) {
-  // Few units in all: no registers or partial sums for more.
+  // Few units in all: no registers or partial sums for more.  (Unaligned rows: one, or any.)
   const dim3 block(kAdThreads);
-  if (kAligned && units == 1)
-    hipLaunchKernelGGL((adapter_add_kernel<E, MR, kAligned ? 1 : 4, kAligned>), grid, block, 0, stream, p);
+  if (units == 1)
+    hipLaunchKernelGGL((adapter_add_kernel<E, MR, 1, kAligned>), grid, block, 0, stream, p);
   else if (kAligned && units == 2)
     hipLaunchKernelGGL((adapter_add_kernel<E, MR, kAligned ? 2 : 4, kAligned>), grid, block, 0, stream, p);
   else if (kAligned && units == 3)
