@@ -15,7 +15,8 @@
 // angles once for several heads of the token, whose loads it issues together.
 // Few rows get a head a thread; many get fewer threads, down to a few rounds of
 // the chip, so that the angles (some 60 instructions a pair) are spread over
-// more heads.  Rows whose strides or widths leave 16-byte pieces go value by value.
+// more heads.  Rows at any address and odd widths take the same vectors, unaligned;
+// only heads that turn or copy less than a vector go value by value.
 #include "cie_common.h"
 
 namespace cie {
@@ -69,14 +70,15 @@ __device__ __forceinline__ void angles(double p, const double* f, float scale, f
   }
 }
 
-template <class E, int V>
+// V values side by side, at a multiple of their size or (global memory may be read so) of one's.
+template <class E, int V, bool kAligned>
 struct Pack {
-  E v[V] __attribute__((aligned(sizeof(E) * V)));
+  E v[V] __attribute__((aligned(sizeof(E) * (kAligned ? V : 1))));
 };
 
 // Two vectors of a head's dims (V pairs), turned.
-template <class E, int V, bool kInterleaved>
-__device__ __forceinline__ void turn(Pack<E, V>& lo, Pack<E, V>& hi, const float* c, const float* s) {
+template <class E, int V, bool kInterleaved, bool kAligned>
+__device__ __forceinline__ void turn(Pack<E, V, kAligned>& lo, Pack<E, V, kAligned>& hi, const float* c, const float* s) {
   float x[2 * V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
@@ -100,27 +102,27 @@ __device__ __forceinline__ void turn(Pack<E, V>& lo, Pack<E, V>& hi, const float
 
 constexpr int kRotHeads = 4;  // heads whose loads a thread has in flight
 
-template <class E, int V, bool kInterleaved, bool kPools>
+template <class E, int V, bool kInterleaved, bool kPools, bool kAligned>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
-  typedef Pack<E, V> vec;
+  typedef Pack<E, V, kAligned> vec;
   const uint32_t gid = blockIdx.x * 256u + threadIdx.x;  // (the host keeps the grid under 2^32 threads)
   const uint32_t rest = gid / (uint32_t)p.units;
   const int u = (int)(gid - rest * (uint32_t)p.units);
   const int64_t t = rest / (uint32_t)p.head_groups;
   const int group = (int)(rest - (uint32_t)t * (uint32_t)p.head_groups);
   if (t >= p.T) return;
-  const int pairs = p.rot / (2 * V);  // units that turn; the others copy
-  const bool turns = u < pairs;
-  int d0, d1;
+  // Units of V pairs turn, then units of 2 V dims copy.  Where they do not come out even
+  // the last unit of either kind lies back over the one before it: both write the same.
+  const int half = p.rot / 2, turning = (half + V - 1) / V;
+  const bool turns = u < turning;
+  int d0, d1, pair = 0;
   if (!turns) {
-    d0 = p.rot + 2 * V * (u - pairs);
-    d1 = d0 + V;
-  } else if (kInterleaved) {
-    d0 = 2 * V * u;
-    d1 = d0 + V;
+    d0 = p.rot + min(2 * V * (u - turning), max(p.D - p.rot - 2 * V, 0));
+    d1 = min(d0 + V, p.D - V);
   } else {
-    d0 = V * u;
-    d1 = d0 + p.rot / 2;
+    pair = min(V * u, half - V);
+    d0 = kInterleaved ? 2 * pair : pair;
+    d1 = kInterleaved ? d0 + V : d0 + half;
   }
   int64_t page = 0, off = 0;
   bool kept = true;
@@ -131,7 +133,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
   float c[V], s[V];
   // (Before the rows' loads: behind them their registers leave three waves a SIMD, and
   // 2,048 rows of 40 heads take 11.7 us, not 9.6.)
-  if (turns) angles<V>((double)p.positions[t], p.freqs + V * u, p.scale, c, s);
+  if (turns) angles<V>((double)p.positions[t], p.freqs + pair, p.scale, c, s);
   if constexpr (kPools) {
     kept = false;
     if (off < 0 || off >= p.page_size)
@@ -164,7 +166,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
     for (int i = 0; i < kRotHeads; ++i) {
       const int h = h0 + i * p.head_groups;
       if (h >= heads) continue;
-      if (turns && (!kPools || h < values)) turn<E, V, kInterleaved>(x[i][0], x[i][1], c, s);
+      if (turns && (!kPools || h < values)) turn<E, V, kInterleaved, kAligned>(x[i][0], x[i][1], c, s);
       E* to;
       if (h < keys)
         to = static_cast<E*>(p.q_out) + (t * p.H_q + h) * p.D;
@@ -184,17 +186,18 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
 
 // cos and sin of a step's positions, a value for each of the rot dims (as the
 // fused append and decode calls take them).  A thread computes V pairs.
-template <class E, int V, bool kInterleaved>
+template <class E, int V, bool kInterleaved, bool kAligned>
 __global__ __launch_bounds__(256) void rotary_tables_kernel(E* cos, E* sin, const int64_t* positions,
                                                             const double* freqs, float scale, int64_t T, int rot) {
-  typedef Pack<E, V> vec;
+  typedef Pack<E, V, kAligned> vec;
   const uint32_t gid = blockIdx.x * 256u + threadIdx.x;
-  const uint32_t units = (uint32_t)rot / (2 * V);
+  const int half = rot / 2;
+  const uint32_t units = (uint32_t)(half + V - 1) / V;
   const int64_t t = gid / units;
-  const int u = (int)(gid % units);
   if (t >= T) return;
+  const int pair = min(V * (int)(gid % units), half - V);
   float c[V], s[V];
-  angles<V>((double)positions[t], freqs + V * u, scale, c, s);
+  angles<V>((double)positions[t], freqs + pair, scale, c, s);
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
     const float* const from = part ? s : c;
@@ -205,8 +208,8 @@ __global__ __launch_bounds__(256) void rotary_tables_kernel(E* cos, E* sin, cons
       a.v[j] = (E)from[kInterleaved && V > 1 ? j / 2 : j];
       b.v[j] = (E)from[kInterleaved && V > 1 ? V / 2 + j / 2 : j];
     }
-    *reinterpret_cast<vec*>(row + (kInterleaved ? 2 * V * u : V * u)) = a;
-    *reinterpret_cast<vec*>(row + (kInterleaved ? 2 * V * u + V : V * u + rot / 2)) = b;
+    *reinterpret_cast<vec*>(row + (kInterleaved ? 2 * pair : pair)) = a;
+    *reinterpret_cast<vec*>(row + (kInterleaved ? 2 * pair + V : pair + half)) = b;
   }
 }
 
@@ -222,33 +225,37 @@ constexpr int64_t kRotThreads = 256 * 1024;
 constexpr int kRotMost = 6;
 constexpr int64_t kRotMaxBlocks = (1 << 24) - 1;  // thread indexes in 32 bits
 
-template <class E, int V, bool kPools>
+template <class E, int V, bool kPools, bool kAligned>
 static int launch_rotary(RotaryParams p, bool interleaved, hipStream_t stream) {
-  p.units = p.D / (2 * V);
+  p.units = (p.rot / 2 + V - 1) / V + (p.D - p.rot + 2 * V - 1) / (2 * V);
   const int64_t heads = (int64_t)p.H_q + (kPools ? 2 : 1) * p.H_kv, row = p.T * p.units;
   int64_t groups = 1;
   while (groups * row < kRotThreads || groups * kRotMost < heads) groups *= 2;
   p.head_groups = (int32_t)(groups < heads ? groups : heads);
   const int64_t blocks = (row * p.head_groups + 255) / 256;
   if (blocks > kRotMaxBlocks) return CIE_EUNSUPPORTED;
+  const dim3 grid((unsigned)blocks), block(256);
   if (interleaved)
-    hipLaunchKernelGGL((rotary_kernel<E, V, true, kPools>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((rotary_kernel<E, V, true, kPools, kAligned>), grid, block, 0, stream, p);
   else
-    hipLaunchKernelGGL((rotary_kernel<E, V, false, kPools>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((rotary_kernel<E, V, false, kPools, kAligned>), grid, block, 0, stream, p);
   return (int)hipGetLastError();
 }
 
+// Vectors of 16 bytes where both parts of a head hold one, aligned or not (4,000 rows of
+// 32 heads of 64, 20 dims turned: 12.0 us value by value, 9.5 so).
 template <class E, bool kPools>
 static int dispatch_rotary(const RotaryParams& p, bool interleaved, hipStream_t stream) {
   constexpr int V = VecOf<E>::kWide;
-  bool wide = multiple_of(p.rot, 2 * V) && multiple_of(p.D, 2 * V) && aligned_to(p.q, 16) && aligned_to(p.k, 16) &&
-              aligned_to(p.q_out, 16) && aligned_to(p.k_out, 16) &&
-              multiple_of(p.q_tok | p.q_head | p.k_tok | p.k_head, V);
+  if (p.rot / 2 < V || (p.D > p.rot && p.D - p.rot < V)) return launch_rotary<E, 1, kPools, true>(p, interleaved, stream);
+  bool aligned = multiple_of(p.rot, 2 * V) && multiple_of(p.D, V) && aligned_to(p.q, 16) && aligned_to(p.k, 16) &&
+                 aligned_to(p.q_out, 16) && aligned_to(p.k_out, 16) &&
+                 multiple_of(p.q_tok | p.q_head | p.k_tok | p.k_head, V);
   if (kPools)
-    wide = wide && aligned_to(p.v, 16) && aligned_to(p.v_out, 16) &&
-           multiple_of(p.v_tok | p.v_head | p.pool_page_stride | p.pool_head_stride, V);
-  return wide ? launch_rotary<E, V, kPools>(p, interleaved, stream)
-              : launch_rotary<E, 1, kPools>(p, interleaved, stream);
+    aligned = aligned && aligned_to(p.v, 16) && aligned_to(p.v_out, 16) &&
+              multiple_of(p.v_tok | p.v_head | p.pool_page_stride | p.pool_head_stride, V);
+  return aligned ? launch_rotary<E, V, kPools, true>(p, interleaved, stream)
+                 : launch_rotary<E, V, kPools, false>(p, interleaved, stream);
 }
 
 static int check_sizes(int64_t T, int64_t H_q, int64_t H_kv, int64_t D, int64_t rot, int dtype) {
@@ -258,25 +265,31 @@ static int check_sizes(int64_t T, int64_t H_q, int64_t H_kv, int64_t D, int64_t 
   return CIE_OK;
 }
 
-template <class E>
-static int launch_tables(void* cos, void* sin, const int64_t* positions, const double* freqs, float scale, int64_t T,
+template <class E, int V, bool kAligned>
+static int launch_tables(E* cos, E* sin, const int64_t* positions, const double* freqs, float scale, int64_t T,
                          int64_t rot, bool interleaved, hipStream_t stream) {
-  constexpr int V = VecOf<E>::kWide;
-  const bool wide = multiple_of(rot, 2 * V) && aligned_to(cos, 16) && aligned_to(sin, 16);
-  const int64_t blocks = (T * (rot / (wide ? 2 * V : 2)) + 255) / 256;
+  const int64_t blocks = (T * ((rot / 2 + V - 1) / V) + 255) / 256;
   if (blocks > kRotMaxBlocks) return CIE_EUNSUPPORTED;
   const dim3 grid((unsigned)blocks), block(256);
+  if (interleaved)
+    hipLaunchKernelGGL((rotary_tables_kernel<E, V, true, kAligned>), grid, block, 0, stream, cos, sin, positions, freqs,
+                       scale, T, (int)rot);
+  else
+    hipLaunchKernelGGL((rotary_tables_kernel<E, V, false, kAligned>), grid, block, 0, stream, cos, sin, positions, freqs,
+                       scale, T, (int)rot);
+  return (int)hipGetLastError();
+}
+
+template <class E>
+static int dispatch_tables(void* cos, void* sin, const int64_t* positions, const double* freqs, float scale, int64_t T,
+                           int64_t rot, bool interleaved, hipStream_t stream) {
+  constexpr int V = VecOf<E>::kWide;
   E* const c = static_cast<E*>(cos);
   E* const s = static_cast<E*>(sin);
-  if (wide && interleaved)
-    hipLaunchKernelGGL((rotary_tables_kernel<E, V, true>), grid, block, 0, stream, c, s, positions, freqs, scale, T, (int)rot);
-  else if (wide)
-    hipLaunchKernelGGL((rotary_tables_kernel<E, V, false>), grid, block, 0, stream, c, s, positions, freqs, scale, T, (int)rot);
-  else if (interleaved)
-    hipLaunchKernelGGL((rotary_tables_kernel<E, 1, true>), grid, block, 0, stream, c, s, positions, freqs, scale, T, (int)rot);
-  else
-    hipLaunchKernelGGL((rotary_tables_kernel<E, 1, false>), grid, block, 0, stream, c, s, positions, freqs, scale, T, (int)rot);
-  return (int)hipGetLastError();
+  if (rot / 2 < V) return launch_tables<E, 1, true>(c, s, positions, freqs, scale, T, rot, interleaved, stream);
+  return multiple_of(rot, 2 * V) && aligned_to(cos, 16) && aligned_to(sin, 16)
+             ? launch_tables<E, V, true>(c, s, positions, freqs, scale, T, rot, interleaved, stream)
+             : launch_tables<E, V, false>(c, s, positions, freqs, scale, T, rot, interleaved, stream);
 }
 
 }  // namespace cie
@@ -364,7 +377,7 @@ extern "C" int cie_rotary_tables(void* cos, void* sin, const int64_t* positions,
   if (T == 0) return CIE_OK;
   if (!cos || !sin || !positions || !freqs) return CIE_EINVAL;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return dtype == CIE_F16    ? launch_tables<f16>(cos, sin, positions, freqs, scale, T, rot, interleaved, st)
-         : dtype == CIE_BF16 ? launch_tables<bf16>(cos, sin, positions, freqs, scale, T, rot, interleaved, st)
-                             : launch_tables<float>(cos, sin, positions, freqs, scale, T, rot, interleaved, st);
+  return dtype == CIE_F16    ? dispatch_tables<f16>(cos, sin, positions, freqs, scale, T, rot, interleaved, st)
+         : dtype == CIE_BF16 ? dispatch_tables<bf16>(cos, sin, positions, freqs, scale, T, rot, interleaved, st)
+                             : dispatch_tables<float>(cos, sin, positions, freqs, scale, T, rot, interleaved, st);
 }

@@ -39,7 +39,8 @@ def split(qkv, h_q, h_kv, d):
 
 
 SHAPES = [(1, 14, 2, 64, 64), (5, 14, 2, 64, 32), (33, 4, 4, 128, 128), (3, 8, 1, 64, 20), (7, 2, 1, 80, 48), (2, 3, 1, 6, 2),
-          (129, 1, 1, 256, 256), (9, 5, 3, 96, 96), (64, 14, 2, 66, 66), (17, 32, 8, 128, 64)]
+          (129, 1, 1, 256, 256), (9, 5, 3, 96, 96), (64, 14, 2, 66, 66), (17, 32, 8, 128, 64), (6, 3, 2, 64, 52), (6, 3, 2, 64, 56), (6, 3, 2, 64, 60), (11, 2, 2, 40, 18),
+          (4, 2, 1, 30, 16), (4, 2, 1, 24, 14), (3, 2, 1, 42, 34)]
 
 
 @pytest.mark.parametrize("interleaved", [False, True], ids=["half", "interleaved"])
@@ -60,7 +61,8 @@ def test_apply(T, h_q, h_kv, d, rot, dtype, interleaved):
 @pytest.mark.parametrize("interleaved", [False, True], ids=["half", "interleaved"])
 @pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
 @pytest.mark.parametrize("T,h_q,h_kv,d,rot,page", [(1, 14, 2, 64, 64, 16), (77, 14, 2, 64, 32, 16), (33, 8, 8, 128, 128, 32),
-                                                   (40, 4, 2, 96, 20, 16), (5, 3, 1, 66, 66, 8)])
+                                                   (40, 4, 2, 96, 20, 16), (5, 3, 1, 66, 66, 8), (21, 3, 2, 64, 52, 16),
+                                                   (21, 3, 2, 64, 60, 16)])
 def test_append(T, h_q, h_kv, d, rot, page, dtype, interleaved):
     qkv, pos, freqs = case(T, h_q, h_kv, d, rot, dtype, seed=T)
     n_pages = 3 + -(-T // page)
