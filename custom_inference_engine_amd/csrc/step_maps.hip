@@ -21,13 +21,14 @@
 // reads the page's id from the stack, at the place that the scan gives it, not
 // from the table.  Words that other workgroups still read (the count, and a
 // release's lengths) are changed by the last workgroup to arrive.
-// Times of one call, replayed from a graph: one row 2.9 us, 32 sequences and
-// 1,056 rows 3.9 us, 496 sequences and 16,480 rows with 1,480 new pages 8 us.
+// Times of one call, replayed from a graph: one row 2.9 us, 32 sequences and 1,056
+// rows 3.5 us, 496 sequences and 16,480 rows 4.2 us; with pages and their release
+// 6.1 us for one sequence, 8.0 for 32, 14.7 for 496 with 16,480 rows and 1,480 new pages.
 #include "cie_common.h"
 
 namespace cie {
 
-constexpr int kMapMaxSeqs = 2048;          // (scans and hash table of a batch: 64 KB of LDS)
+constexpr int kMapMaxSeqs = 2048;          // (scans and hash table of a batch: at most 74 KB of LDS)
 constexpr int64_t kMapMaxRows = 1 << 24;   // sums over a batch stay below 2^31
 constexpr int64_t kMapMaxPages = 1 << 24;
 constexpr int64_t kMapMaxPage = 1 << 30;   // tokens a page: a page and a step's rows stay below 2^32
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(kThreads) void step_maps_kernel(MapParams p) {
   // New pages of a sequence whose n tokens are all mapped; 0 for the padding rows' slot and where they do not fit.
   const auto more_pages = [&](int b, int n) {
     const int64_t len = s.len[b];
-    if (s.slot[b] <= 0 || n == 0 || len < 0 || len + n > capacity) return 0;
+    if (s.slot[b] <= 0 || n == 0 || len < 0 || len > capacity - n) return 0;  // (len: any word)
     const uint32_t rest = s.rest[b];
     return (int)((rest + (uint32_t)n + P - 1) / P) - (rest > 0);
   };
@@ -232,7 +233,7 @@ __global__ __launch_bounds__(kThreads) void step_maps_kernel(MapParams p) {
       const int n = s.cu[b + 1] - s.cu[b];
       const int64_t len = s.len[b];
       if (s.slot[b] <= 0 || n == 0 || len < 0) continue;
-      if (len + n > capacity)
+      if (len > capacity - n)
         mistakes |= CIE_ERRBIT_LEN;
       else if (!add_slot(s.hash, p.hash_size, s.slot[b]))
         bad = 1;
@@ -262,7 +263,7 @@ __global__ __launch_bounds__(kThreads) void step_maps_kernel(MapParams p) {
       if (s.slot[b] >= 0) {
         slot = s.slot[b];
         const int64_t len = s.len[b];
-        pos = len + (t - s.cu[b]);
+        pos = (int64_t)((uint64_t)len + (uint64_t)(t - s.cu[b]));  // (past 2^63: negative)
         if (pos < 0 || pos >= capacity) {
           mistakes |= CIE_ERRBIT_LEN;
         } else {

@@ -172,6 +172,21 @@ def test_bad_slots_counts_and_lengths(managed):
     assert int(err) == LEN
 
 
+@pytest.mark.parametrize("page", [1, 16, 1 << 30])
+@pytest.mark.parametrize("new", [1, 3])
+def test_any_word_as_a_length(page, new):
+    """A length whose sum with the new tokens passes 63 bits takes no page and writes no table entry."""
+    lens = torch.tensor([0, (1 << 63) - 1, 2], device=DEV)
+    table = torch.full((3, 8), 5, device=DEV)
+    free, err = cie.new_free_list(8, DEV), err_word()
+    got = cie.step_maps(torch.tensor([1, 2], device=DEV), torch.tensor([new, 1], device=DEV), lens, table, page, new + 1,
+                        free_list=free, err=err)
+    assert int(err) == LEN and got.pages.tolist()[:new] == [0] * new and got.offsets.tolist()[:new] == [0] * new
+    assert int(free[0]) == (6 if page == 1 else 7)  # (the other sequence's, where it needs one)
+    table[2, 2 // page] = 5
+    assert bool((table == 5).all())
+
+
 def test_release_of_bad_sequences_leaves_them():
     pool = Pool([20, 5, 33], 16, 8, slots=6)
     err = err_word()
