@@ -89,7 +89,7 @@ def adapter_add_(y, x, a, b, scales, ranks, plan, slices, err=None):
     ``slices``: the widths of y's parts, d_out together; scales (n,) float32; ranks (n,)
     int32: an adapter's rows of rank, those behind them being zeros in a and b.  ``plan``:
     the step's ``adapter_plan``.  A plan of other rows or adapters is reported in ``err``
-    (CIE_ERRBIT_PLAN), and y left as it is.
+    (CIE_ERRBIT_PLAN), and y left as it is.  y's memory holds nothing of the other arguments'.
     """
     yr = y if y.dim() == 2 else _rows(y, "y")
     xr = x if x.dim() == 2 else _rows(x, "x")

@@ -17,8 +17,11 @@
 // left of the rounding of u is 2^-22 (bf16: 2^-16) of it; the sum with y rounds
 // once, as the plain form does.
 //
-// Bound by memory: r <= 128 ranks are 2 r flops for each value of x and y, far from
-// what the matrix cores could do.
+// Bound by memory where rows are many: r <= 128 ranks are 2 r flops for each value of x
+// and y, far from what the matrix cores could do.  8,192 rows of 4,096 take 45.6 us at
+// rank 16 (4.4 TB/s) and 53 at 64 (a workgroup fills a CU's LDS, so that its reads of x
+// and its work on y take turns).  Few rows are bound by the stages in series, header ->
+// tile -> x and A -> sums -> y: 6.2 us for one row into three slices.
 #include "cie_common.h"
 
 namespace cie {
@@ -58,7 +61,7 @@ constexpr int kPlanBatch = 8;  // rows of a lane whose loads are in flight
 constexpr int kPlanKept = 16;  // and that are kept from the count for the writing
 
 // Rows of a tile: more share A's and B's reads, fewer fill the chip.  (1,052 rows of
-// 1,000 at rank 64: 9.2 us with 16, 9.7 with 32; 2,048 rows of 4,096 31.2 and 23.2.)
+// 1,000 at rank 64: 9.3 us with 16, 9.7 with 32; 2,048 rows of 4,096 31.2 and 22.1.)
 __host__ __device__ static inline int tile_rows(int64_t T) { return T <= 1536 ? 16 : 32; }
 static inline int64_t max_tiles(int64_t T, int64_t N, int M) {
   const int64_t groups = T < N ? T : N;  // (a group of c rows has ceil(c / M) <= (c - 1) / M + 1 tiles)
@@ -78,8 +81,8 @@ struct PlanParams {
 
 // Many rows are planned by several workgroups in two launches: each counts its rows,
 // then each writes its rows behind those of the workgroups before it.  One workgroup
-// does both at once, bound by what a CU reads and by the rounds of a wave: 32 rows 4.3 us,
-// 1,052 rows 5.7, 8,192 rows 12.4 (two launches 12.6); 65,536 rows 122, in two launches 27.
+// does both at once, bound by what a CU reads and by the rounds of a wave: 32 rows 4.2 us,
+// 1,052 rows 5.6, 8,192 rows 12.4 (two launches 12.6); 65,536 rows 122, in two launches 27.
 constexpr int64_t kPlanAlone = 8192;
 constexpr int kPlanGroups = 64;
 static inline int64_t group_rows(int64_t T) {
@@ -330,8 +333,8 @@ struct AddLds {
 };
 
 // The code of small launches is kept short: each runs once, and a workgroup waits
-// some 0.25 us for each further KiB of instructions (7.3 us with loops unrolled,
-// 16 KB, for one row into three slices).
+// some 0.25 us for each further KiB of instructions (one row into three slices: 7.3 us
+// with loops unrolled, 16 KB; 6.2 so).
 template <class E, int MR, int NT, bool kAligned>
 __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
   typedef typename Lane8<E>::type vec;

@@ -1,5 +1,7 @@
 """Slot maps, rotary positions and adapters without a GPU: refusals, sizes, frequencies, and the schedulers' bookkeeping."""
 import math
+import os
+import re
 
 import pytest
 import torch
@@ -7,8 +9,10 @@ from transformers import Qwen2Config
 from transformers.models.qwen2.modeling_qwen2 import Qwen2RotaryEmbedding
 
 import custom_inference_engine_amd as cie
+from custom_inference_engine_amd import _build
 from custom_inference_engine_amd.scheduler import Scheduler
 from oracle import step as ref
+from tests import test_asm_order as asm
 
 I64 = torch.int64
 
@@ -420,7 +424,21 @@ def test_scheduler_refuses_adapters_it_has_not():
 @pytest.mark.parametrize("src,honoured", [("rotary.hip", True), ("adapters.hip", True), ("step_maps.hip", False)])
 def test_which_kernels_honour_nans(src, honoured):
     """A NaN in a row comes out of it: the last flag of the two counts."""
-    from custom_inference_engine_amd import _build
-
     flags = [f for f in _build.source_flags(src) if f in ("-fhonor-nans", "-fno-honor-nans")]
     assert (flags[-1] == "-fhonor-nans") == honoured
+
+
+@pytest.mark.skipif(not os.path.exists(asm.HIPCC), reason="hipcc not available")
+@pytest.mark.parametrize("src,kernels", [("step_maps.hip", 6), ("rotary.hip", 2), ("adapters.hip", 2)])
+def test_assembly_of_the_step_kernels(src, kernels, tmp_path, monkeypatch):
+    """Sums round to fp32 before they become 16-bit values, nothing takes the packed fp32 forms, spills registers or
+    needs the caches written back."""
+    monkeypatch.setattr(_build, "HIPCC_FLAGS", _build.source_flags(src))
+    text = asm._assembly(src, tmp_path)
+    assert "buffer_wbl2" not in text and "buffer_inv" not in text
+    assert not re.search(r"\bv_pk_(add|mul|fma)_f32\b", text)
+    assert set(re.findall(r"\.vgpr_spill_count:\s*(\d+)", text)) == {"0"}
+    bodies = asm._kernels(text)
+    assert len(bodies) >= kernels
+    for name, body in bodies.items():
+        assert not any(asm.FMA_MIX_F16.match(l) for l in body), name
