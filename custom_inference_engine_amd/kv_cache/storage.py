@@ -267,7 +267,7 @@ class KVStorage:
 
     def reset(self, slot_ids: list[int]) -> None:
         if self.free_list is not None:  # the slots' pages are free again
-            slots = torch.tensor(slot_ids, dtype=torch.long).to(self.lens.device)
+            slots = torch.tensor(list(dict.fromkeys(slot_ids)), dtype=torch.long).to(self.lens.device)  # (each once)
             _pages.release_pages(self.free_list, slots, self.lens, self.block_table, self.page_size, err=self.page_err)
         else:
             self.lens[slot_ids] = 0

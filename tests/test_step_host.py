@@ -400,6 +400,17 @@ def test_a_failed_step_leaks_no_pages(monkeypatch):
     assert (kv.slot_adapters == -1).all()
 
 
+def test_a_slot_named_twice_is_reset_once(monkeypatch):
+    monkeypatch.setattr("custom_inference_engine_amd.kv_cache.pages.release_pages", _release)
+    kv = cie.KVStorage(_cfg(), max_cache_len=192, page_size=16, n_slots=4, device="cpu", dtype=torch.float16)
+    kv.manage_pages()
+    kv.use_adapters(1)
+    CountingExecutor(kv)._step([1, 2], [20, 3])
+    kv.reset([2, 1, 2, 0, 0])
+    assert sorted(kv.free_list[2:13].tolist()) == list(range(1, 12)) and kv.free_list[0] == 11
+    assert not kv.lens.any() and not kv.block_table.any()
+
+
 def test_pages_that_are_managed_report_errors():
     kv = cie.KVStorage(_cfg(), max_cache_len=192, page_size=16, n_slots=4, device="cpu", dtype=torch.float16)
     kv.manage_pages()
