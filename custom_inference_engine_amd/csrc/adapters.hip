@@ -81,8 +81,9 @@ struct PlanParams {
 
 // Many rows are planned by several workgroups in two launches: each counts its rows,
 // then each writes its rows behind those of the workgroups before it.  One workgroup
-// does both at once, bound by what a CU reads and by the rounds of a wave: 32 rows 4.2 us,
-// 1,052 rows 5.6, 8,192 rows 12.4 (two launches 12.6); 65,536 rows 122, in two launches 27.
+// does both at once, bound by a CU's loads and the rounds of its waves: 32 rows 4.0 us,
+// 1,052 rows 5.0, 8,192 rows of four prompts 9.1 (two launches 10.2), of eight adapters at
+// random 12.3 (10.8); 16,384 rows of four prompts 15.3 and 11.1, 65,536 rows 77 and 16.6.
 constexpr int64_t kPlanAlone = 8192;
 constexpr int kPlanGroups = 64;
 static inline int64_t group_rows(int64_t T) {
@@ -95,13 +96,15 @@ enum PlanPhase { kPlanAll, kPlanCount, kPlanWrite };
 // Rows are dealt to the waves in order, 64 adjacent rows at a time, and each wave
 // counts its own, so that a group's rows keep their order and the plan is the same
 // every time.  Lanes of one adapter find each other by a ballot a bit of its number,
-// and the first of them takes as many places as they are.  Two dependent loads, the
-// count, a scan over adapters, the rows.  The code is kept short (loops are not
+// and the first of them takes as many places as they are (64 rows of one adapter need no
+// ballots: 8,192 rows of four prompts 12.2 us with, 10.3 without; and 9.1 with tiles' heads
+// written along with their first rows, not at the end).  Two dependent loads, the count, a
+// scan over adapters, the rows.  The code is kept short (loops are not
 // unrolled but for the loads'): it runs once, from a cold instruction cache.
 template <PlanPhase kPhase>
 __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p) {
   __shared__ int count[kPlanWaves * kAdMaxAdapters];  // [wave][N]: rows of a wave, then their first place
-  __shared__ int tile0[kAdMaxAdapters], sums[kPlanWaves];
+  __shared__ int tile0[kAdMaxAdapters], rows_of[kAdMaxAdapters], sums[kPlanWaves];
   __shared__ int seen[kPlanWaves][kPlanKept][kWave];   // rows' adapters and places (kPlaceBits), -1: none
   constexpr int kPlaceBits = 21;                       // (a wave has 2^20 rows at most)
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
@@ -112,7 +115,7 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p
   const uint64_t below = (1ull << lane) - 1;
   int* const mine = count + wave * p.N;
 
-  int mistakes = 0, before = 0, total = 0, n = 0, tiles = 0;
+  int mistakes = 0, total = 0, n = 0;
   int* const out = p.plan + kAdHead;
   const int words = kAdTileHead + p.M;
   const bool again = share > kPlanKept * kWave;  // (else a wave's places are still there the second time)
@@ -148,11 +151,12 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p
         int place = was & ((1 << kPlaceBits) - 1);
         if (pass == 0 || again) {
           uint64_t same = __ballot(live);
+          if (__ballot(id != uniform(id)) != 0)  // (a prompt's rows: all of one)
 #pragma unroll 1
-          for (int k = 0; k < bits; ++k) {
-            const uint64_t ones = __ballot(id >> k & 1);
-            same &= id >> k & 1 ? ones : ~ones;
-          }
+            for (int k = 0; k < bits; ++k) {
+              const uint64_t ones = __ballot(id >> k & 1);
+              same &= id >> k & 1 ? ones : ~ones;
+            }
           int from = 0;
           if (live && (same & below) == 0) from = atomicAdd(&mine[id], __popcll(same));
           place = __shfl(from, live ? __builtin_ctzll(same) : 0, kWave) + __popcll(same & below);
@@ -160,8 +164,13 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p
         }
         if (pass == 1 && live) {
           const int k = place + (again ? 0 : mine[id]);
-          out[(int64_t)(tile0[id] + (k >> p.log_m)) * words + kAdTileHead + (k & (p.M - 1))] =
-              (int)(at + i * kWave + lane);
+          int* const tile = out + (int64_t)(tile0[id] + (k >> p.log_m)) * words;
+          const int nth = k & (p.M - 1);
+          tile[kAdTileHead + nth] = (int)(at + i * kWave + lane);
+          if (nth == 0) {  // a tile's first row writes its head
+            tile[0] = id;
+            tile[1] = min(rows_of[id] - k, p.M);
+          }
         }
       }
     }
@@ -198,24 +207,19 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanParams p
       break;
     }
     if (kPhase == kPlanWrite) n = rest;  // (all its rows)
-    tiles = (n + p.M - 1) >> p.log_m;
+    const int tiles = (n + p.M - 1) >> p.log_m;
     const int incl = wave_inclusive_sum(tiles);
     if (lane == kWave - 1) sums[wave] = incl;
     __syncthreads();
-    before = incl - tiles + waves_before<kPlanWaves>(sums[lane % kPlanWaves], wave, total);
-    if (tid < p.N) tile0[tid] = before;
+    const int before = incl - tiles + waves_before<kPlanWaves>(sums[lane % kPlanWaves], wave, total);
+    if (tid < p.N) {
+      tile0[tid] = before;
+      rows_of[tid] = n;
+    }
     __syncthreads();
   }
   if (mistakes && kPhase != kPlanWrite) set_err(p.err, mistakes);  // (counted rows have been looked at)
   if (kPhase == kPlanCount || blockIdx.x > 0) return;
-  if (tid < p.N) {
-#pragma unroll 1
-    for (int k = 0; k < tiles; ++k) {
-      int* const tile = out + (int64_t)(before + k) * words;
-      tile[0] = tid;
-      tile[1] = min(n - k * p.M, p.M);
-    }
-  }
   if (tid == 0) {
     p.plan[0] = total;
     p.plan[1] = (int)p.T;
