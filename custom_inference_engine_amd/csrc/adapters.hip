@@ -10,12 +10,12 @@
 // LDS, and then each wave takes 64 columns of y at a time.  So x is read once and y
 // read and written once, and nothing goes through memory between the two products.
 //
-// u = A x is fp32.  It enters the second product as two values of the element
-// type, u = hi + lo, side by side in the MFMA's K: 16 ranks fill K = 32, and B's
-// values serve both halves.  In fp16 each row of u is first scaled by a power of two
-// to below 2^15, so that no u overflows or loses bits to fp16's range.  What is
-// left of the rounding of u is 2^-22 (bf16: 2^-16) of it; the sum with y rounds
-// once, as the plain form does.
+// u = A x is fp32.  It enters the second product as values of the element type, u = hi +
+// lo, side by side in the MFMA's K: 16 ranks fill K = 32, and B's values serve both
+// halves.  In bf16 a third value, in an MFMA of its own, takes what the 16 bits of the two
+// leave: the three hold all 24 bits of u.  In fp16 each row of u is first scaled by a power
+// of two to below 2^15, so that no u overflows or loses bits to fp16's range, and what is
+// left of its rounding is 2^-22 of it.  The sum with y rounds once, as the plain form does.
 //
 // Bound by memory where rows are many: r <= 128 ranks are 2 r flops for each value of x
 // and y, far from what the matrix cores could do.  8,192 rows of 4,096 take 45.6 us at
@@ -314,7 +314,7 @@ __device__ __forceinline__ void lds_order() { asm volatile("" : : : "memory"); }
 // LDS of an instance.  A wave has a region of its own: a stage, which holds kDepth
 // blocks of x and A on their way to the matrix cores, then the wave's partial sums of
 // u, then the products for 16 rows of 64 columns; and room for B's values.
-template <int MR, int NT>
+template <class E, int MR, int NT>
 struct AddLds {
   static constexpr int M = 16 * MR;
   static constexpr int kDepth = MR == 1 ? (NT == 1 ? 4 : NT < 4 ? 2 : 1) : (NT == 1 ? 2 : 1);
@@ -331,7 +331,10 @@ struct AddLds {
   static constexpr int kRegion = kStage + kB;
   static_assert(M * kSumRow * 4 <= kStage && kOut <= kStage, "sums and products fit the stage");
   static_assert((kGroup < 3 ? kGroup * 2048 : 8192) <= (kGroup < 3 ? kB : kRegion - kOut), "B's values fit");
-  static constexpr int kU = kAdUnits * M * 64;      // 16 ranks of u a unit: in fp32, then hi and lo
+  // 16 ranks of u a unit: in fp32, then hi and lo, and in bf16 what these leave.
+  static constexpr bool kThird = __is_same(E, bf16);
+  static constexpr int kURow = kThird ? 96 : 64;
+  static constexpr int kU = kAdUnits * M * kURow;
   static constexpr int kBytes = kAdWaves * kRegion + kU + M * 4;
   static_assert(kBytes <= 160 * 1024, "a workgroup's LDS");
 };
@@ -342,13 +345,13 @@ struct AddLds {
 template <class E, int MR, int NT, bool kAligned>
 __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
   typedef typename Lane8<E>::type vec;
-  typedef AddLds<MR, NT> L;
+  typedef AddLds<E, MR, NT> L;
   constexpr int M = L::M, NW = kAdWaves, kDepth = L::kDepth;
   constexpr int kLanes = NT == 3 ? 16 : NT * 4;  // threads that sum a row of u, four ranks each
   constexpr int kHeld = NT < 4 ? NT : kAdUnits;  // units of u (fewer than four in all: the host's choice)
   static_assert(M * 16 <= kAdThreads, "a thread sums four values of u at most, and splits one a unit");
   __shared__ __align__(16) char lds[L::kBytes];
-  char* const u_lds = lds + NW * L::kRegion;  // [unit][token]: 16 floats, or 16 his and 16 los
+  char* const u_lds = lds + NW * L::kRegion;  // [unit][token]: 16 floats, or 16 his, 16 los (and 16 thirds)
   float* const factor = reinterpret_cast<float*>(u_lds + L::kU);
 
   // Which tile, and its rows.  Small launches deal tiles to the XCDs (workgroups go
@@ -543,18 +546,18 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
 #pragma unroll
         for (int w = 0; w < NW; ++w)
           sum += reinterpret_cast<const f32x4*>(lds + w * L::kRegion)[t * (L::kSumRow / 4) + q];
-        reinterpret_cast<f32x4*>(u_lds + ((u0 + q / 4) * M + t) * 64)[q % 4] = sum;
+        reinterpret_cast<f32x4*>(u_lds + ((u0 + q / 4) * M + t) * L::kURow)[q % 4] = sum;
       }
       __syncthreads();
     }
 
-    // u = hi + lo: sixteen lanes a row, one rank of each unit.
+    // u's parts: sixteen lanes a row, one rank of each unit.
     if (tid < M * 16) {
       const int t = tid / 16, q = tid % 16;
       float v[kHeld];
 #pragma unroll
       for (int i = 0; i < kHeld; ++i)
-        v[i] = i < n_units ? reinterpret_cast<const float*>(u_lds + (i * M + t) * 64)[q] : 0.f;
+        v[i] = i < n_units ? reinterpret_cast<const float*>(u_lds + (i * M + t) * L::kURow)[q] : 0.f;
       int shift = 0;
       if constexpr (__is_same(E, f16)) {
         // The row's largest finite |u| decides its scale: an infinity stays one.
@@ -570,10 +573,12 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
 #pragma unroll
       for (int i = 0; i < kHeld; ++i) {
         if (i >= n_units) break;
-        E* const at = reinterpret_cast<E*>(u_lds + (i * M + t) * 64);
+        E* const at = reinterpret_cast<E*>(u_lds + (i * M + t) * L::kURow);
         const float u = __builtin_ldexpf(v[i], shift), left = u - (float)(E)u;
+        const float lo = __builtin_isfinite(left) ? left : 0.f;  // (of an infinity, a NaN: hi says it)
         at[q] = (E)u;
-        at[16 + q] = (E)(__builtin_isfinite(left) ? left : 0.f);  // (of an infinity, a NaN: hi says it)
+        at[16 + q] = (E)lo;
+        if constexpr (L::kThird) at[32 + q] = (E)(lo - (float)(E)lo);
       }
       if (q == 0) factor[t] = __builtin_ldexpf(scale, -shift);
     }
@@ -599,19 +604,25 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
         // 16 ranks at a time: hi and lo in one K of 32, B's values twice
 #pragma unroll 2
         for (int i = 0; i < n; ++i) {
-          vec bv[4], uv[MR];
+          vec bv[4], uv[MR], third[MR] = {};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int d = 16 * j + m, c = 2 * i + g % 2;
             bv[j] = *reinterpret_cast<const vec*>(b_room + ((d << shift) + (c ^ (d >> (3 - shift)) % pieces)) * 16);
           }
 #pragma unroll
-          for (int r = 0; r < MR; ++r)
-            uv[r] = *reinterpret_cast<const vec*>(u_lds + (((s - s0) * units + i0 + i) * M + 16 * r + m) * 64 + 16 * g);
+          for (int r = 0; r < MR; ++r) {
+            const char* const at = u_lds + (((s - s0) * units + i0 + i) * M + 16 * r + m) * L::kURow + 16 * g;
+            uv[r] = *reinterpret_cast<const vec*>(at);
+            if (L::kThird && g < 2) third[r] = *reinterpret_cast<const vec*>(at + 64);
+          }
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int r = 0; r < MR; ++r) acc[r][j] = mma(bv[j], uv[r], acc[r][j]);
+            for (int r = 0; r < MR; ++r) {
+              if constexpr (L::kThird) acc[r][j] = mma(bv[j], third[r], acc[r][j]);  // (half of K: zeros)
+              acc[r][j] = mma(bv[j], uv[r], acc[r][j]);
+            }
         }
         wait_lds_reads();
       }

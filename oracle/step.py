@@ -112,10 +112,10 @@ def adapters(y, x, a, b, scales, row_adapter, slices):
     arithmetic may be from it before the last rounding.
 
     Sums of products are bounded as chains of fp32 roundings (2^-23 of the terms' sizes for each
-    4 products that are added at once, and one for each partial sum); A x as two values of the
-    type is off by 2^-21 (bfloat16: 2^-16) of it.
+    4 products that are added at once, and one for each partial sum); A x as two values of float16
+    is off by 2^-21 of it, as three of bfloat16 not at all.
     """
-    split = 2.0 ** -16 if y.dtype == torch.bfloat16 else 2.0 ** -21
+    split = 0.0 if y.dtype == torch.bfloat16 else 2.0 ** -21
     out, off = y.double().clone(), torch.zeros(y.shape, dtype=torch.float64)
     d_in, R = a.shape[3], a.shape[2]
     for t, i in enumerate(row_adapter):

@@ -1,0 +1,43 @@
+"""Low-rank adapters where their arithmetic could lose bits or a call could reach past what it was given: sums that
+cancel, slices of different sizes, words that are no plan, plans of more rows than a wave keeps."""
+import pytest
+import torch
+
+import custom_inference_engine_amd as cie
+from oracle import step as ref
+from tests.gpu_helpers import DEV, err_word, note
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+PLAN = 16
+
+
+def add(x, a, b, scales, slices, y=None, ids=None):
+    """y (zeros) with adapter 0 added to every row, on the GPU; the error word is checked."""
+    T, n = x.shape[0], a.shape[0]
+    ids = torch.zeros(T, dtype=torch.int64) if ids is None else ids
+    y = torch.zeros(T, sum(slices), dtype=x.dtype) if y is None else y
+    ranks = torch.full((n,), a.shape[2], dtype=torch.int32)
+    note(f"adapters T={T} a={tuple(a.shape)} slices={slices} {x.dtype}")
+    err = err_word()
+    y, x, a, b, scales, ranks, ids = (t.to(DEV) for t in (y, x, a, b, scales, ranks, ids))
+    cie.adapter_add_(y, x, a, b, scales, ranks, cie.adapter_plan(None, ids, n, err=err), slices, err=err)
+    assert int(err) == 0
+    return y.cpu()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("T,R,d_in,slices", [(1, 16, 64, (64,)), (3, 64, 64, (64, 8)), (5, 16, 67, (9, 65)), (40, 128, 72, (136,)),
+                                             (2000, 16, 64, (64, 64)), (1700, 64, 72, (72,)), (1600, 32, 67, (65,))])
+def test_products_that_cancel(T, R, d_in, slices, dtype):
+    """Two ranks whose A x is 1 + 2^-9 + 2^-k and -(1 + 2^-9), added by B's ones: 2^-k is left, whole.  (Every partial
+    sum is a 24-bit value, so nothing rounds; 2^-k, beside 2^-9 and 1, is the third group of eight bits of A x.)"""
+    for k in (17, 18, 22):
+        x, a = torch.zeros(T, d_in), torch.zeros(1, len(slices), R, d_in)
+        x[:, 0], x[:, 1], x[:, 2] = 1.0, 2.0 ** -9, 2.0 ** -9
+        a[0, :, 3, 0], a[0, :, 3, 1], a[0, :, 3, 2] = 1.0, 1.0, 2.0 ** (9 - k)
+        a[0, :, R - 1, 0], a[0, :, R - 1, 1] = -1.0, -1.0
+        b = torch.zeros(1, sum(slices), R)
+        b[..., 3] = b[..., R - 1] = 1.0
+        got = add(x.to(dtype), a.to(dtype), b.to(dtype), torch.tensor([2.0 ** 10]), slices)
+        assert (got == 2.0 ** (10 - k)).all(), (k, got.unique().tolist())
