@@ -13,9 +13,10 @@
 // u = A x is fp32.  It enters the second product as values of the element type, u = hi +
 // lo, side by side in the MFMA's K: 16 ranks fill K = 32, and B's values serve both
 // halves.  In bf16 a third value, in an MFMA of its own, takes what the 16 bits of the two
-// leave: the three hold all 24 bits of u.  In fp16 each row of u is first scaled by a power
-// of two to below 2^15, so that no u overflows or loses bits to fp16's range, and what is
-// left of its rounding is 2^-22 of it.  The sum with y rounds once, as the plain form does.
+// leave: the three hold all 24 bits of u.  In fp16 each row of a slice's u is first scaled by
+// a power of two to below 2^15, so that no u overflows or loses bits to fp16's range; what is
+// left of its rounding is 2^-22 of it, or 2^-39 of the row's largest in its slice.  The sum
+// with y rounds once, as the plain form does.
 //
 // Bound by memory where rows are many: r <= 128 ranks are 2 r flops for each value of x
 // and y, far from what the matrix cores could do.  8,192 rows of 4,096 take 45.6 us at
@@ -286,7 +287,7 @@ __device__ __forceinline__ void store8(E* row, int k, int n, typename Lane8<E>::
   }
 }
 
-// 2^e that takes m (fp16: the largest |u| of a row) to [2^14, 2^15); 1 where there is no such.
+// 2^e that takes m (fp16: the largest |u| of a row's slice) to [2^14, 2^15); 1 where there is no such.
 template <class E>
 __device__ __forceinline__ int row_shift(float m) {
   if constexpr (sizeof(E) == 2 && __is_same(E, f16)) {
@@ -294,6 +295,14 @@ __device__ __forceinline__ int row_shift(float m) {
     return min(15 - __builtin_amdgcn_frexp_expf(m), 100);
   }
   return 0;
+}
+
+// The largest of a row of 16 lanes (v >= 0), in each of them: rotations by 8, 4, 2 and 1, no LDS.
+__device__ __forceinline__ float max_of_16(float v) {
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, true)));
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xf, 0xf, true)));
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x122, 0xf, 0xf, true)));
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x121, 0xf, 0xf, true)));
 }
 
 // Copies 16 bytes a lane from p to the wave's KiB at dst (LDS, lane order), without
@@ -335,7 +344,7 @@ struct AddLds {
   static constexpr bool kThird = __is_same(E, bf16);
   static constexpr int kURow = kThird ? 96 : 64;
   static constexpr int kU = kAdUnits * M * kURow;
-  static constexpr int kBytes = kAdWaves * kRegion + kU + M * 4;
+  static constexpr int kBytes = kAdWaves * kRegion + kU + kAdMaxSlices * M * 4;
   static_assert(kBytes <= 160 * 1024, "a workgroup's LDS");
 };
 
@@ -352,7 +361,7 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
   static_assert(M * 16 <= kAdThreads, "a thread sums four values of u at most, and splits one a unit");
   __shared__ __align__(16) char lds[L::kBytes];
   char* const u_lds = lds + NW * L::kRegion;  // [unit][token]: 16 floats, or 16 his, 16 los (and 16 thirds)
-  float* const factor = reinterpret_cast<float*>(u_lds + L::kU);
+  float* const factor = reinterpret_cast<float*>(u_lds + L::kU);  // [slice][token], of the slices at once
 
   // Which tile, and its rows.  Small launches deal tiles to the XCDs (workgroups go
   // to the eight in turn) one by one and read the tile's words along with the
@@ -551,36 +560,38 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
       __syncthreads();
     }
 
-    // u's parts: sixteen lanes a row, one rank of each unit.
+    // u's parts, slice by slice: sixteen lanes a row, one rank of each unit.
     if (tid < M * 16) {
       const int t = tid / 16, q = tid % 16;
-      float v[kHeld];
-#pragma unroll
-      for (int i = 0; i < kHeld; ++i)
-        v[i] = i < n_units ? reinterpret_cast<const float*>(u_lds + (i * M + t) * L::kURow)[q] : 0.f;
-      int shift = 0;
-      if constexpr (__is_same(E, f16)) {
-        // The row's largest finite |u| decides its scale: an infinity stays one.
-        float top = 0.f;
+#pragma unroll 1
+      for (int s = 0; s < s1 - s0; ++s) {
+        char* const row = u_lds + (s * units * M + t) * L::kURow;
+        float v[kHeld];
 #pragma unroll
         for (int i = 0; i < kHeld; ++i)
-          if (__builtin_fabsf(v[i]) < __builtin_huge_valf()) top = fmaxf(top, __builtin_fabsf(v[i]));
+          v[i] = i < units ? reinterpret_cast<const float*>(row + i * M * L::kURow)[q] : 0.f;
+        int shift = 0;
+        if constexpr (__is_same(E, f16)) {
+          // The largest finite |u| of the row's slice decides its scale: an infinity stays one.
+          float top = 0.f;
 #pragma unroll
-        for (int o = 1; o < 16; o *= 2) top = fmaxf(top, __shfl_xor(top, o, kWave));
-        shift = row_shift<E>(top);
-      }
-      lds_order();  // (the row's lanes are one wave's: all have read)
+          for (int i = 0; i < kHeld; ++i)
+            if (__builtin_fabsf(v[i]) < __builtin_huge_valf()) top = fmaxf(top, __builtin_fabsf(v[i]));
+          shift = row_shift<E>(max_of_16(top));
+        }
+        lds_order();  // (the row's lanes are one wave's: all have read)
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
-        if (i >= n_units) break;
-        E* const at = reinterpret_cast<E*>(u_lds + (i * M + t) * L::kURow);
-        const float u = __builtin_ldexpf(v[i], shift), left = u - (float)(E)u;
-        const float lo = __builtin_isfinite(left) ? left : 0.f;  // (of an infinity, a NaN: hi says it)
-        at[q] = (E)u;
-        at[16 + q] = (E)lo;
-        if constexpr (L::kThird) at[32 + q] = (E)(lo - (float)(E)lo);
+        for (int i = 0; i < kHeld; ++i) {
+          if (i >= units) break;
+          E* const at = reinterpret_cast<E*>(row + i * M * L::kURow);
+          const float u = __builtin_ldexpf(v[i], shift), left = u - (float)(E)u;
+          const float lo = __builtin_isfinite(left) ? left : 0.f;  // (of an infinity, a NaN: hi says it)
+          at[q] = (E)u;
+          at[16 + q] = (E)lo;
+          if constexpr (L::kThird) at[32 + q] = (E)(lo - (float)(E)lo);
+        }
+        if (q == 0) factor[s * M + t] = __builtin_ldexpf(scale, -shift);
       }
-      if (q == 0) factor[t] = __builtin_ldexpf(scale, -shift);
     }
     __syncthreads();
     if (rank <= 0) return;
@@ -638,7 +649,7 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
           const f32x4* const got = reinterpret_cast<const f32x4*>(out + t * L::kOutRow + 8 * c8);
           const f32x4 lo = got[0], hi = got[1];
           if (16 * r + t >= rows) continue;
-          const float f = factor[16 * r + t];
+          const float f = factor[(s - s0) * M + 16 * r + t];
           E* const to = static_cast<E*>(p.y) + row_of[2 * r + h] * p.y_stride;
           vec v;
 #pragma unroll

@@ -650,7 +650,8 @@ int cie_rotary_tables(void* cos, void* sin, const int64_t* positions, const doub
  * ranks (N) int32: adapter i has ranks[i] <= R rows of rank, and zeros behind them
  * in a and b.  Rows without an adapter, and rows behind T, are left as they are.
  * A x is summed in fp32 and enters the second product as two values of float16 (22
- * bits) or three of bfloat16 (all 24), that one summed in fp32 and added to y in fp32:
+ * bits, or 2^-39 of the row's largest in its slice where that is more) or three of
+ * bfloat16 (all 24), that one summed in fp32 and added to y in fp32:
  * one rounding to the element type at the end.
  *   cie_adapter_plan   once per step: which rows share an adapter, into `plan`
  *                      (cie_adapter_plan_bytes(T, N) bytes, 16-byte aligned, any

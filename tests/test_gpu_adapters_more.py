@@ -41,3 +41,39 @@ def test_products_that_cancel(T, R, d_in, slices, dtype):
         b[..., 3] = b[..., R - 1] = 1.0
         got = add(x.to(dtype), a.to(dtype), b.to(dtype), torch.tensor([2.0 ** 10]), slices)
         assert (got == 2.0 ** (10 - k)).all(), (k, got.unique().tolist())
+
+
+@pytest.mark.parametrize("T,R,d_in,widths", [(1, 16, 64, (64, 8)), (3, 64, 64, (64, 72)), (40, 32, 67, (9, 65)), (5, 128, 64, (8, 64)),
+                                             (2000, 16, 64, (64, 64)), (1700, 32, 64, (72, 8))])
+def test_a_small_slice_beside_a_large_one(T, R, d_in, widths):
+    """A slice whose A x is 2^-24 of the other's keeps its own bits, wherever it stands: of 2^-10 + 2^-28 and -2^-10, added
+    by B's ones, 2^-28 is left, whole."""
+    for small in (0, 1):
+        x, a, b = torch.zeros(T, d_in), torch.zeros(1, 2, R, d_in), torch.zeros(1, sum(widths), R)
+        x[:, 0], x[:, 1] = 1.0, 2.0 ** -14
+        a[0, 1 - small, 0, 0] = 2.0 ** 14
+        a[0, small, 3, 0], a[0, small, 3, 1], a[0, small, R - 1, 0] = 2.0 ** -10, 2.0 ** -14, -(2.0 ** -10)
+        lo = small * widths[0]
+        b[0, lo:lo + widths[small], 3] = b[0, lo:lo + widths[small], R - 1] = 1.0
+        got = add(x.half(), a.half(), b.half(), torch.tensor([2.0 ** 20]), widths)
+        want = torch.zeros(T, sum(widths))
+        want[:, lo:lo + widths[small]] = 2.0 ** -8
+        assert torch.equal(got.float(), want), small
+
+
+def test_slices_of_different_sizes():
+    """One slice's A scaled by 2^10 and another's by 2^-12 (their B scaled back), against each slice's own bound."""
+    g = torch.Generator().manual_seed(4)
+    for T, R, d_in, slices in ((9, 16, 64, (64, 64, 8)), (30, 64, 200, (136, 72, 64)), (1800, 32, 67, (65, 9, 64))):
+        T_ids = torch.randint(-1, 2, (T,), generator=g)
+        a, b = torch.randn(2, 3, R, d_in, generator=g) * d_in ** -0.5, torch.randn(2, sum(slices), R, generator=g)
+        col = 0
+        for s, e in enumerate((10, 0, -12)):
+            a[:, s] *= 2.0 ** e
+            b[:, col:col + slices[s]] *= 2.0 ** -e
+            col += slices[s]
+        a, b, x, y = a.half(), b.half(), torch.randn(T, d_in, generator=g).half(), torch.randn(T, sum(slices), generator=g).half()
+        scales = torch.tensor([0.5, 2.0])
+        got = add(x, a, b, scales, slices, y=y, ids=T_ids)
+        want, off = ref.adapters(y, x, a, b, scales, T_ids.tolist(), slices)
+        assert ((got.double() - want).abs() <= off + ref.rounding(want.abs() + off, F16)).all()
