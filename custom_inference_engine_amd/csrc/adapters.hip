@@ -367,7 +367,10 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
   // to the eight in turn) one by one and read the tile's words along with the
   // header; large ones give an XCD adjacent tiles, mostly of one adapter, whose A
   // and B then come from its L2.
+  // (Words that are no plan are found out below, after they have been used as one: the
+  // count is kept to what there can be, so that no index leaves the buffer.)
   const int32_t* const head = p.plan;
+  const int n_tiles = min(max(head[0], 0), p.max_tiles);
   const int xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
   int tile, chunk, per_chunk = p.per_chunk;
   if constexpr (MR == 1) {
@@ -377,7 +380,7 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
     // Whole rounds of the CUs, a tile a workgroup; the tiles of the last round share
     // their columns among the CUs left (258 tiles of 32 rows of 4,096 at rank 64: 87 us
     // without this, 52 for 256).
-    const int n = head[0], round = n / kCus * (kCus / 8), left = n % kCus;
+    const int n = n_tiles, round = n / kCus * (kCus / 8), left = n % kCus;
     const int chunks = left ? min(p.chunks, kCus / left) : 1, items = left * chunks, share = (items + 7) / 8;
     if (nth < round) {
       tile = xcd * round + nth;
@@ -401,7 +404,7 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
     if (tid == 0 && blockIdx.x == 0) set_err(p.err, CIE_ERRBIT_PLAN);
     return;
   }
-  if (tile >= head[0]) return;
+  if (tile >= n_tiles) return;
   const int ct0 = chunk * per_chunk, ct1 = min(ct0 + per_chunk, p.col_tiles);
   if (ct0 >= ct1) return;
   // The slices' first columns and column tiles, by index: not by a load each time.

@@ -77,3 +77,18 @@ def test_slices_of_different_sizes():
         got = add(x, a, b, scales, slices, y=y, ids=T_ids)
         want, off = ref.adapters(y, x, a, b, scales, T_ids.tolist(), slices)
         assert ((got.double() - want).abs() <= off + ref.rounding(want.abs() + off, F16)).all()
+
+
+@pytest.mark.parametrize("T", [20, 2000])
+@pytest.mark.parametrize("word", [-5, -(1 << 31), (1 << 31) - 1, 0])
+def test_words_that_are_no_plan(T, word):
+    """A buffer of the right size with anything in it: reported, nothing written."""
+    g = torch.Generator().manual_seed(0)
+    x, y = torch.randn(T, 64, generator=g).half().to(DEV), torch.randn(T, 128, generator=g).half().to(DEV)
+    a, b = torch.randn(3, 1, 16, 64, generator=g).half().to(DEV), torch.randn(3, 128, 16, generator=g).half().to(DEV)
+    scales, ranks = torch.ones(3, device=DEV), torch.full((3,), 16, dtype=torch.int32, device=DEV)
+    plan = cie.new_adapter_plan(T, 3, DEV).fill_(word)
+    err, kept = err_word(), y.clone()
+    note(f"no plan T={T} word={word}")
+    cie.adapter_add_(y, x, a, b, scales, ranks, plan, (128,), err=err)
+    assert int(err) == PLAN and torch.equal(y, kept)
