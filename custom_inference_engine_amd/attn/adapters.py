@@ -14,6 +14,7 @@ import ctypes
 import functools
 from typing import Optional
 
+import numpy as np
 import torch
 
 from .. import _native
@@ -81,6 +82,21 @@ def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
     return t[0]
 
 
+def _share(p: int, step: int, size: int, n: int, q: int, hop: int, span: int, m: int) -> bool:
+    """Whether n rows of ``size`` bytes, ``step`` apart from p on, and m of ``span`` bytes, ``hop`` apart from q on, share a byte."""
+    if n > 1 and step < size:  # (rows that lie in each other: one)
+        size, n = (n - 1) * step + size, 1
+    if m > 1 and hop < span:
+        span, m = (m - 1) * hop + span, 1
+    if n == m and step == hop and n > 1:  # views of one wider tensor: row j of the second lies behind row j + k of the first
+        k, r = divmod(q - p, step)
+        return (r < size and -n < k < n) or (r + span > step and -n < k + 1 < n)
+    rows = p + step * np.arange(n)
+    hop = max(hop, 1)
+    near = np.clip((rows - q - span) // hop + 1, 0, m - 1) * hop + q  # the first to end behind a row's start
+    return bool(((near < rows + size) & (rows < near + span)).any())
+
+
 def adapter_add_(y, x, a, b, scales, ranks, plan, slices, err=None):
     """``y`` with its rows' adapters added, in place.
 
@@ -107,7 +123,9 @@ def adapter_add_(y, x, a, b, scales, ranks, plan, slices, err=None):
     if T > 1 and y_row < d_out:
         raise AssertionError("y's rows must not share memory")
     y_ptr, x_ptr = y.data_ptr(), x.data_ptr()
-    if y_ptr == x_ptr and T:
+    y_end = y_ptr + 2 * ((T - 1) * y_row + d_out)
+    if (x_ptr < y_end and y_ptr < x_ptr + 2 * ((T - 1) * x_row + d_in)
+            and T and _share(y_ptr, 2 * y_row, 2 * d_out, T, x_ptr, 2 * x_row, 2 * d_in, T)):
         raise AssertionError("x must not lie in y's memory")
     n, S, R, w = a.shape if a.dim() == 4 else (0,) * 4
     if S != n_slices or w != d_in or R % RANK_UNIT or not 0 < R <= MAX_RANK or not a.is_contiguous():
@@ -123,12 +141,16 @@ def adapter_add_(y, x, a, b, scales, ranks, plan, slices, err=None):
         raise AssertionError("plan must come from adapter_plan for these rows and adapters")
     dev = one_device(y, x, a, b, scales, ranks, plan)
     if T:
+        a_ptr, b_ptr, s_ptr, r_ptr, p_ptr = (t.data_ptr() for t in (a, b, scales, ranks, plan))
+        for ptr, size in ((a_ptr, 2 * n * n_slices * R * d_in), (b_ptr, 2 * n * d_out * R), (s_ptr, 4 * n), (r_ptr, 4 * n),
+                          (p_ptr, 4 * held)):
+            if ptr < y_end and y_ptr < ptr + size and _share(y_ptr, 2 * y_row, 2 * d_out, T, ptr, size, size, 1):
+                raise AssertionError("a, b, scales, ranks and plan must not lie in y's memory")
         if T > 1 and x_row < d_in:
             xr = xr.contiguous()
             x_ptr, x_row = xr.data_ptr(), d_in
-        launch(dev, "cie_adapter_add", y_ptr, y_row, x_ptr, x_row, a.data_ptr(), b.data_ptr(),
-               scales.data_ptr(), ranks.data_ptr(), plan.data_ptr(), 4 * held, T, n, R, d_in, widths,
-               n_slices, kind, err=err)
+        launch(dev, "cie_adapter_add", y_ptr, y_row, x_ptr, x_row, a_ptr, b_ptr, s_ptr, r_ptr, p_ptr, 4 * held, T, n, R,
+               d_in, widths, n_slices, kind, err=err)
     return y
 
 
