@@ -12,7 +12,9 @@
 // these kernels use (zero between calls), and the pages, a stack whose top is the
 // page handed out next.  Pages are handed out in the order of the sequences and,
 // within one, of its positions, and taken back in the reverse order: giving back
-// what a call was given leaves the list as it was.
+// what a call was given leaves the list as it was.  Table entries that hold no page
+// (0: a call whose pages the list did not have) are not given back: the last workgroup
+// to arrive closes the gaps that they leave.
 //
 // Both are bound by latency, not by bytes: 40 bytes a row are written once.  So
 // one launch does it all.  Every workgroup reads the B sequences and scans them
@@ -300,17 +302,19 @@ __global__ __launch_bounds__(kThreads) void step_maps_kernel(MapParams p) {
   }
 }
 
+constexpr int64_t kNoPage = -1;  // on the stack, until the gaps are closed
+
 template <int kThreads>
 __global__ __launch_bounds__(kThreads) void release_pages_kernel(MapParams p) {
   extern __shared__ __align__(8) char lds[];
-  __shared__ int sm[kThreads / kWave][2], flag, bad;
+  __shared__ int sm[kThreads / kWave][2], flag, bad, gaps;
   const Batch s = batch_in(lds, p.B);
   const int tid = threadIdx.x, B = p.B;
   const int each = (B + kThreads - 1) / kThreads, b0 = min(tid * each, B), b1 = min(b0 + each, B);
   const int64_t capacity = p.bt_width * p.page_size, avail = p.free_list[0];
 
   for (int i = tid; i < p.hash_size; i += kThreads) s.hash[i] = -1;
-  if (tid == 0) bad = 0;
+  if (tid == 0) bad = gaps = 0;
   __syncthreads();
   int gone = 0, mistakes = 0;
 #pragma unroll 1
@@ -346,6 +350,7 @@ __global__ __launch_bounds__(kThreads) void release_pages_kernel(MapParams p) {
   // (a list of all pages but page 0 is full)
   const bool taken = !bad && avail >= 0 && avail + total < p.n_pages;
   if (!taken) mistakes |= CIE_ERRBIT_FREE;
+  int64_t* const stack = p.free_list + 2 + avail;
   if (taken) {
 #pragma unroll 1
     for (int j = blockIdx.x * kThreads + tid; j < total; j += gridDim.x * kThreads) {
@@ -354,21 +359,52 @@ __global__ __launch_bounds__(kThreads) void release_pages_kernel(MapParams p) {
       int64_t id = *entry;
       if (id <= 0 || id >= p.n_pages) {
         mistakes |= CIE_ERRBIT_PAGE;
-        id = 0;
+        if (id == 0) gaps = 1;
+        id = id == 0 ? kNoPage : 0;
       }
       *entry = 0;
-      p.free_list[2 + avail + total - 1 - j] = id;
+      // (agent scope: another CU's workgroup may close the gaps)
+      __hip_atomic_store(&stack[total - 1 - j], id, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
   if (mistakes) set_err(p.err, mistakes);
-  if (last_of_grid(p.free_list + 1, &flag)) {
-    if (taken) {
-      for (int b = tid; b < B; b += kThreads)
-        if (s.slot[b] > 0) p.lens[s.slot[b]] = s.len[b];
-      if (tid == 0) p.free_list[0] = avail + total;
+  // The last workgroup to arrive, and whether any met an entry without a page (above the arrivals' 32 bits).
+  __syncthreads();
+  bool any_gaps = gaps != 0;
+  if (gridDim.x > 1) {
+    wait_stores();
+    __syncthreads();
+    if (tid == 0) {
+      const int64_t old = __hip_atomic_fetch_add(p.free_list + 1, (int64_t)1 + ((int64_t)any_gaps << 32),
+                                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      flag = (int)(old & 0xffffffff) == (int)gridDim.x - 1 ? 1 + (any_gaps || old >> 32 != 0) : 0;
     }
-    if (tid == 0) p.free_list[1] = 0;
+    __syncthreads();
+    if (flag == 0) return;
+    any_gaps = flag == 2;
   }
+  if (taken) {
+    for (int b = tid; b < B; b += kThreads)
+      if (s.slot[b] > 0) p.lens[s.slot[b]] = s.len[b];
+    int given = total;
+    if (any_gaps) {
+      wait_stores();
+      __syncthreads();
+      given = 0;
+      for (int k0 = 0; k0 < total; k0 += kThreads) {  // (a word's new place is never behind its old one)
+        const int k = k0 + tid;
+        const int64_t id =
+            k < total ? __hip_atomic_load(&stack[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : kNoPage;
+        int place = id != kNoPage, none = 0, n, no_n;
+        block_exclusive<kThreads>(place, none, kThreads, 1, sm, n, no_n);
+        if (id != kNoPage) stack[given + place] = id;
+        given += n;
+      }
+      for (int k = given + tid; k < total; k += kThreads) stack[k] = 0;
+    }
+    if (tid == 0) p.free_list[0] = avail + given;
+  }
+  if (tid == 0) p.free_list[1] = 0;
 }
 
 static int hash_size_of(int64_t B) {

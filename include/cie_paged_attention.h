@@ -597,8 +597,10 @@ int cie_step_maps(int64_t* cu_seqlens, int64_t* slots, int64_t* positions, int64
  * A slot that comes twice, or a list that has no room for the pages: nothing is
  * done (CIE_ERRBIT_FREE).  A bad slot id (CIE_ERRBIT_PAGE) or lengths that are not
  * 0 <= keep <= held <= the table's row, lens[slot] <= held (CIE_ERRBIT_LEN): that
- * sequence is left as it is.  A bad page id goes into the list as page 0
- * (CIE_ERRBIT_PAGE).  Sizes as cie_step_maps.
+ * sequence is left as it is.  Table entries of 0 hold no page, as after a
+ * cie_step_maps whose pages the list did not have: they are not given back
+ * (CIE_ERRBIT_PAGE).  A page id outside the pool goes into the list as page 0
+ * (CIE_ERRBIT_PAGE, here and where it is handed out).  Sizes as cie_step_maps.
  */
 int cie_release_pages(int64_t* free_list, const int64_t* slot_ids, int64_t* lens,
                       int64_t* block_table, const int64_t* keep, const int64_t* held,

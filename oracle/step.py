@@ -80,12 +80,16 @@ def release_pages(free, slot_ids, lens, table, page_size, keep=None, held=None) 
         gone += [(s, i) for i in range(_ceil(k, page_size), _ceil(h, page_size))]
     if free.count + len(gone) >= free.size:
         return False
+    end = free.count + len(gone)
     for s, i in reversed(gone):
-        page = table[s][i] if 0 < table[s][i] < free.size else 0
+        page, table[s][i] = table[s][i], 0
+        if page == 0:  # no page: nothing to give back
+            continue
+        page = page if 0 < page < free.size else 0
         free.rest[len(free.stack)] = page
         free.stack.append(page)
-        table[s][i] = 0
-    free.count += len(gone)
+    free.count = len(free.stack)
+    free.rest[free.count:end] = [0] * (end - free.count)
     for s, k in kept.items():
         lens[s] = k
     return True
