@@ -191,6 +191,27 @@ class KVStorage:
         self.free_list = _pages.new_free_list(self.n_pages, self.device)
         self.page_err = torch.zeros(1, dtype=torch.int32, device=self.device)
 
+    def keep_step(self, slot_ids: torch.Tensor, new_tokens: torch.Tensor, next_tokens: torch.Tensor) -> list[int]:
+        """The end of a step that fed ``new_tokens[b]`` tokens to slot ``slot_ids[b]``: the tokens that come next, on the
+        host, and held as the slots' last.  A step that reported anything leaves lengths, pages and last tokens as they
+        were before it, and raises (``check_pages``)."""
+        *tokens, bits = torch.cat((next_tokens, self.page_err)).tolist()  # (one wait for both)
+        if bits:
+            self._drop_step(slot_ids, new_tokens)
+            self.check_pages()
+        self.last_generated[slot_ids] = next_tokens
+        return tokens
+
+    def _drop_step(self, slot_ids: torch.Tensor, new_tokens: torch.Tensor) -> None:
+        """Gives back what some sequences of a step may have got, whose lengths were not advanced."""
+        if self.free_list is None:
+            return
+        fed = new_tokens > 0
+        slot_ids, new_tokens = slot_ids[fed], new_tokens[fed]
+        keep = self.lens[slot_ids]
+        _pages.release_pages(self.free_list, slot_ids, self.lens, self.block_table, self.page_size, keep=keep,
+                             held=keep + new_tokens, err=torch.zeros_like(self.page_err))
+
     def check_pages(self) -> None:
         """Raises if a step since the last check found too few free pages, or bad slots or lengths (waits for it)."""
         bits = int(self.page_err)
@@ -257,12 +278,13 @@ class KVStorage:
     # lens[unused_idx] = 0 as a device kernel (a 1-element multiply), not a
     # host scalar copy, so a decode step that contains it can be graph-captured
     # (and no memset node lands in the graph).
+    # A step of a pool that manages its pages counts only where nothing was reported.
     def decode_advance(self, slot_ids: torch.Tensor) -> None:
-        self.lens[slot_ids] += 1
+        self.lens[slot_ids] += 1 if self.free_list is None else self.page_err == 0
         self.lens[self.unused_idx:self.unused_idx + 1].mul_(0)
 
     def mixed_advance(self, slot_ids: torch.Tensor, lens: torch.Tensor) -> None:
-        self.lens[slot_ids] += lens
+        self.lens[slot_ids] += lens if self.free_list is None else lens * (self.page_err == 0)
         self.lens[self.unused_idx:self.unused_idx + 1].mul_(0)
 
     def reset(self, slot_ids: list[int]) -> None:

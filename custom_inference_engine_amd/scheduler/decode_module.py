@@ -94,7 +94,7 @@ class DecodeModule:
             self.upload(slot_ids)
             logits = self.replay()
             next_tokens = torch.argmax(logits[:n], dim=-1)
-            self.kv_cache.last_generated[self.slots[:n]] = next_tokens
             if self.managed:
-                self.kv_cache.check_pages()
+                return self.kv_cache.keep_step(self.slots[:n], self.ones[:n], next_tokens)
+            self.kv_cache.last_generated[self.slots[:n]] = next_tokens
             return next_tokens.tolist()

@@ -1,0 +1,105 @@
+"""Steps that are refused, and state that is turned on twice or late, through the step modules and the scheduler on a
+small Qwen2."""
+import pytest
+import torch
+
+import custom_inference_engine_amd as cie
+from custom_inference_engine_amd import KVStorage, use_adapters, use_rotary
+from custom_inference_engine_amd.scheduler import DecodeModule, FullMixedModule, MixedModule, PiecewiseMixedModule, Scheduler
+from tests.gpu_helpers import DEV, note
+from tests.test_gpu_step import D, H_KV, H_Q, _adapters, _config, _logits, _models, _prompts, _rel
+
+pytestmark = pytest.mark.gpu
+
+
+def _pool(cfg, pages=6, managed=True, slots=5):
+    kv = KVStorage(cfg, max_cache_len=pages * 16, page_size=16, n_slots=slots, device=DEV, dtype=torch.float16)
+    if managed:
+        kv.manage_pages()
+    return kv
+
+
+def _state(kv):
+    words = kv.free_list.tolist()
+    return kv.lens.tolist(), kv.block_table.tolist(), words[:2 + words[0]], kv.last_generated.tolist()
+
+
+def _whole(kv):
+    """Each page of the pool is held by one slot, or free, once."""
+    held = [p for s, n in enumerate(kv.lens.tolist()) for p in kv.block_table[s, :-(-n // 16)].tolist()]
+    words = kv.free_list.tolist()
+    assert words[1] == 0 and sorted(words[2:2 + words[0]] + held) == list(range(1, kv.n_pages))
+
+
+@pytest.mark.parametrize("kind", ["eager", "graph", "piecewise"])
+def test_a_refused_step_changes_nothing(native_lib, kind):
+    """A mixed step and a decode step that find too few pages leave lengths, tables, list and last tokens as they were;
+    their slots are reset like any other, and what then runs is what runs in a pool that never refused a step."""
+    torch._dynamo.reset()
+    cfg = _config()
+    _, ours = _models(cfg)
+
+    def modules(kv):
+        if kind == "graph":
+            mix = FullMixedModule(ours, kv, batch_size=4, token_count=64)
+        elif kind == "piecewise":
+            mix = PiecewiseMixedModule(ours, kv, token_count=64,
+                                       buffer=torch.zeros(1, 64, H_Q, D, dtype=torch.float16, device=DEV))
+        else:
+            mix = MixedModule(ours, kv, token_count=64)
+        return mix, DecodeModule(ours, kv, batch_size=2)
+
+    kv, other = _pool(cfg), _pool(cfg)
+    (mix, dec), (mix2, dec2) = modules(kv), modules(other)
+    prompts = _prompts(32, 31, 20, 17)
+    note(f"refused steps: {kind}")
+    for m in (mix, mix2):
+        m.forward(prompts[:2], [1, 2])  # four of five pages
+    for _ in range(2):
+        before = _state(kv)
+        for chunks, slots in ((prompts[2:3], [3]), ([[5], prompts[3], [6]], [2, 3, 1])):
+            with pytest.raises(RuntimeError, match="free pages"):
+                mix.forward(chunks, slots)
+            assert _state(kv) == before
+        kv.reset([3])
+        assert _state(kv) == before
+        kv.check_pages()
+    for d in (dec, dec2):  # slot 1 takes the last page, slot 2 needs none yet
+        d.forward([1, 2])
+    assert _state(kv) == _state(other)
+    before = _state(kv)
+    with pytest.raises(RuntimeError, match="free pages"):
+        dec.forward([2])  # its 33rd token
+    assert _state(kv) == before
+    for pool in (kv, other):
+        pool.reset([1])
+        _whole(pool)
+    assert int(kv.free_list[0]) == 3
+    for _ in range(3):
+        got, want = dec.forward([2]), dec2.forward([2])
+        assert got == want and torch.equal(dec.logits[0], dec2.logits[0])
+    assert mix.forward([prompts[2]], [3]) == mix2.forward([prompts[2]], [3])
+    assert torch.equal(mix.last_logits, mix2.last_logits) and _state(kv) == _state(other)
+    _whole(kv)
+
+
+def test_a_step_that_some_sequences_cannot_take(native_lib):
+    """One sequence would run past its table's row while another gets a page: nothing is kept, and the page is free again."""
+    cfg = _config()
+    _, ours = _models(cfg)
+    kv = _pool(cfg, pages=5)
+    mix, dec = MixedModule(ours, kv, token_count=96), DecodeModule(ours, kv, batch_size=2)
+    note("a sequence past its table's row")
+    mix.forward([[3] * 16], [1])
+    kv.lens[2] = 80  # (a slot that a caller has set beyond its pages)
+    before = _state(kv)
+    with pytest.raises(RuntimeError, match="lengths"):
+        mix.forward([[1], [2] * 20, [4]], [2, 3, 1])
+    assert _state(kv) == before
+    with pytest.raises(RuntimeError, match="lengths"):
+        dec.forward([1, 2])
+    assert _state(kv) == before
+    kv.lens[2] = 0
+    dec.forward([1])
+    assert kv.lens.tolist() == [0, 17, 0, 0, 0] and int(kv.free_list[0]) == 2
+    _whole(kv)
