@@ -178,7 +178,8 @@ class KVStorage:
         self.last_generated = torch.zeros((n_slots,), dtype=torch.long, device=self.device)
 
         self.free_list = None      # block tables kept on the device (manage_pages)
-        self.page_err = None       # what its steps reported since check_pages
+        # what its steps reported since check_pages
+        self.page_err = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.slot_adapters = None  # each slot's low-rank adapter, -1: none (use_adapters)
         self.n_adapters = 0
 
@@ -189,7 +190,6 @@ class KVStorage:
         if bool(self.lens.any()) or bool(self.block_table.any()):
             raise AssertionError("manage_pages needs every slot empty")
         self.free_list = _pages.new_free_list(self.n_pages, self.device)
-        self.page_err = torch.zeros(1, dtype=torch.int32, device=self.device)
 
     def keep_step(self, slot_ids: torch.Tensor, new_tokens: torch.Tensor, next_tokens: torch.Tensor) -> list[int]:
         """The end of a step that fed ``new_tokens[b]`` tokens to slot ``slot_ids[b]``: the tokens that come next, on the
@@ -278,13 +278,13 @@ class KVStorage:
     # lens[unused_idx] = 0 as a device kernel (a 1-element multiply), not a
     # host scalar copy, so a decode step that contains it can be graph-captured
     # (and no memset node lands in the graph).
-    # A step of a pool that manages its pages counts only where nothing was reported.
+    # A step whose maps or pages were reported does not count.
     def decode_advance(self, slot_ids: torch.Tensor) -> None:
         self.lens[slot_ids] += 1 if self.free_list is None else self.page_err == 0
         self.lens[self.unused_idx:self.unused_idx + 1].mul_(0)
 
     def mixed_advance(self, slot_ids: torch.Tensor, lens: torch.Tensor) -> None:
-        self.lens[slot_ids] += lens if self.free_list is None else lens * (self.page_err == 0)
+        self.lens[slot_ids] += lens * (self.page_err == 0)
         self.lens[self.unused_idx:self.unused_idx + 1].mul_(0)
 
     def reset(self, slot_ids: list[int]) -> None:

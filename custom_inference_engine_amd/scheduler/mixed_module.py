@@ -172,10 +172,7 @@ class MixedModule:
             logits = self.run()[:n]
             self.last_logits = logits
             next_tokens = torch.argmax(logits, dim=-1)
-            if getattr(self.kv_cache, "free_list", None) is not None:
-                return self.kv_cache.keep_step(self.slots[:n], self.chunk_lens[:n], next_tokens)
-            self.kv_cache.last_generated[self.slots[:n]] = next_tokens
-            return next_tokens.tolist()
+            return self.kv_cache.keep_step(self.slots[:n], self.chunk_lens[:n], next_tokens)
 
 
 class FullMixedModule(MixedModule):

@@ -103,3 +103,22 @@ def test_a_step_that_some_sequences_cannot_take(native_lib):
     dec.forward([1])
     assert kv.lens.tolist() == [0, 17, 0, 0, 0] and int(kv.free_list[0]) == 2
     _whole(kv)
+
+
+@pytest.mark.parametrize("kind", ["eager", "graph"])
+def test_a_pool_whose_tables_the_caller_keeps_reports_too(native_lib, kind):
+    """A sequence past its table's row stops a mixed step with an error, and leaves the pool as it was."""
+    cfg = _config()
+    _, ours = _models(cfg)
+    kv = _pool(cfg, pages=4, managed=False)
+    mix = FullMixedModule(ours, kv, batch_size=3, token_count=32) if kind == "graph" else MixedModule(ours, kv, token_count=32)
+    kv.block_table[1, :2], kv.block_table[2, 0] = torch.tensor([1, 3], device=DEV), 2
+    note(f"past the table's row: {kind}")
+    first = mix.forward([[5] * 7, [6] * 9], [1, 2])
+    kv.lens[1] = 60
+    before = kv.lens.clone(), kv.last_generated.clone()
+    with pytest.raises(RuntimeError, match="lengths"):
+        mix.forward([[1] * 5, [2]], [1, 2])
+    assert torch.equal(kv.lens, before[0]) and torch.equal(kv.last_generated, before[1])
+    kv.lens[1], kv.lens[2] = 0, 0
+    assert mix.forward([[5] * 7, [6] * 9], [1, 2]) == first and kv.lens.tolist() == [0, 7, 9, 0, 0]
