@@ -165,6 +165,18 @@ def _(y, x, a, b, scales, ranks, plan, slices) -> None:
     return None
 
 
+# (an op of its own: torch does not take an argument that is written and may be left out)
+@torch.library.custom_op("inference::adapter_add_reported_", mutates_args=("y", "err"))
+def adapter_add_reported_op(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor,
+                            ranks: torch.Tensor, plan: torch.Tensor, slices: list[int], err: torch.Tensor) -> None:
+    adapter_add_(y, x, a, b, scales, ranks, plan, slices, err=err)
+
+
+@adapter_add_reported_op.register_fake
+def _(y, x, a, b, scales, ranks, plan, slices, err) -> None:
+    return None
+
+
 class AdapterBank(torch.nn.Module):
     """The adapters of one projection: ``n_adapters`` places for A and B of up to ``rank``, empty until ``load``.
 
@@ -228,8 +240,12 @@ class AdapterBank(torch.nn.Module):
         for t in (self.a, self.b, self.scales, self.ranks):
             t[i] = 0
 
-    def add_(self, y, x, plan) -> None:
-        adapter_add_op(y, x, self.a, self.b, self.scales, self.ranks, plan, self.slices)
+    def add_(self, y, x, plan, err=None) -> None:
+        args = (y, x, self.a, self.b, self.scales, self.ranks, plan, self.slices)
+        if err is None:
+            adapter_add_op(*args)
+        else:
+            adapter_add_reported_op(*args, err)
 
 
 def use_adapters(model, kv_cache, n_adapters: int, rank: int) -> list:

@@ -719,6 +719,8 @@ class TritonQwen2Attention(torch.nn.Module):
         if kv_manager is None:
             if self.rotary is not None:
                 raise AssertionError("the wrapped module's own path has no rotary positions of this layout")
+            if self.qkv_adapters is not None:
+                raise AssertionError("the wrapped module's own path has no adapters")
             return self.original(hidden_states, position_embeddings, attention_mask,
                                  past_key_values=past_key_values, **kwargs)
         metadata = kwargs.get("metadata")
@@ -734,11 +736,11 @@ class TritonQwen2Attention(torch.nn.Module):
             if not self.fuse_qkv:
                 raise AssertionError("adapters and use_rotary need the fused QKV projection")
         if self.rotary is not None:
-            qkv = self._project_qkv(hidden_states, metadata)
+            qkv = self._project_qkv(hidden_states, metadata, kv_manager)
             o = self._attend_rotary(qkv, *position_embeddings, kv_manager, metadata, scales)
-            return self._project_o(o.reshape(1, total_T, self.num_heads * self.head_dim), metadata), None
+            return self._project_o(o.reshape(1, total_T, self.num_heads * self.head_dim), metadata, kv_manager), None
         if self.fuse_qkv and self.fuse_rope and (self.fuse_append or not metadata.full_decode):
-            qkv = self._project_qkv(hidden_states, metadata)
+            qkv = self._project_qkv(hidden_states, metadata, kv_manager)
             cos, sin = position_embeddings
             if metadata.full_decode and scales is not None:
                 o = _q8.gqa_decode_qkv_rope_attention_q8_op(
@@ -760,10 +762,10 @@ class TritonQwen2Attention(torch.nn.Module):
                         qkv, cos, sin, keys, values, metadata.pages, metadata.offsets, self.num_heads,
                     )
                 o = self._mixed(query_states, kv_manager, metadata, scales)
-            return self._project_o(o.reshape(1, total_T, self.num_heads * self.head_dim), metadata), None
+            return self._project_o(o.reshape(1, total_T, self.num_heads * self.head_dim), metadata, kv_manager), None
 
         if self.fuse_qkv:
-            q, k, v = self._project_qkv(hidden_states, metadata).split(self.qkv_sizes, dim=-1)
+            q, k, v = self._project_qkv(hidden_states, metadata, kv_manager).split(self.qkv_sizes, dim=-1)
         else:
             q, k, v = attn.q_proj(hidden_states), attn.k_proj(hidden_states), attn.v_proj(hidden_states)
         query_states = q.view(hidden_shape)
@@ -801,22 +803,26 @@ class TritonQwen2Attention(torch.nn.Module):
             kv_manager.mixed_update(self.layer_idx, metadata.pages, metadata.offsets,
                                     key_states, value_states)
             o = self._mixed(query_states, kv_manager, metadata, scales)
-        return self._project_o(o.reshape(1, total_T, self.num_heads * self.head_dim), metadata), None
+        return self._project_o(o.reshape(1, total_T, self.num_heads * self.head_dim), metadata, kv_manager), None
 
-    def _project_qkv(self, hidden_states, metadata):
+    def _project_qkv(self, hidden_states, metadata, kv_manager):
         """The fused projection, with the adapters of the step's rows."""
         qkv = torch.nn.functional.linear(hidden_states, self.qkv_weight, self.qkv_bias)
-        plan = getattr(metadata, "adapter_plan", None)
-        if self.qkv_adapters is not None and plan is not None:
-            self.qkv_adapters.add_(qkv, hidden_states, plan)
+        self._adapt(self.qkv_adapters, qkv, hidden_states, metadata, kv_manager)
         return qkv
 
-    def _project_o(self, o, metadata):
+    def _project_o(self, o, metadata, kv_manager):
         out = self.original.o_proj(o)
-        plan = getattr(metadata, "adapter_plan", None)
-        if self.o_adapters is not None and plan is not None:
-            self.o_adapters.add_(out, o, plan)
+        self._adapt(self.o_adapters, out, o, metadata, kv_manager)
         return out
+
+    def _adapt(self, bank, y, x, metadata, kv_manager):
+        if bank is None:
+            return
+        plan = getattr(metadata, "adapter_plan", None)
+        if plan is None:
+            raise AssertionError("a layer with adapters needs the step's adapter_plan in its metadata")
+        bank.add_(y, x, plan, getattr(kv_manager, "page_err", None))
 
     def _attend_rotary(self, qkv, positions, frequencies, kv_manager, metadata, scales):
         """Append and attention of rows that are turned here (``rotary.use_rotary``)."""

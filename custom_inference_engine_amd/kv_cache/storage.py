@@ -213,12 +213,12 @@ class KVStorage:
                              held=keep + new_tokens, err=torch.zeros_like(self.page_err))
 
     def check_pages(self) -> None:
-        """Raises if a step since the last check found too few free pages, or bad slots or lengths (waits for it)."""
+        """Raises if a step since the last check found too few free pages, or bad slots, lengths or adapters (waits for it)."""
         bits = int(self.page_err)
         if bits:
             self.page_err.zero_()
             raise RuntimeError("out of free pages: the step's tokens were not kept" if bits & _pages.ERR_FREE
-                               else f"bad slots, lengths or pages in a step (error bits {bits})")
+                               else f"bad slots, lengths, pages or adapters in a step (error bits {bits})")
 
     def reset_pages(self) -> None:
         """Every slot of a pool that manages its pages emptied, every page free, whatever a failed step left."""
@@ -278,9 +278,10 @@ class KVStorage:
     # lens[unused_idx] = 0 as a device kernel (a 1-element multiply), not a
     # host scalar copy, so a decode step that contains it can be graph-captured
     # (and no memset node lands in the graph).
-    # A step whose maps or pages were reported does not count.
+    # A step that reported anything does not count.
     def decode_advance(self, slot_ids: torch.Tensor) -> None:
-        self.lens[slot_ids] += 1 if self.free_list is None else self.page_err == 0
+        reports = self.free_list is not None or self.slot_adapters is not None
+        self.lens[slot_ids] += self.page_err == 0 if reports else 1
         self.lens[self.unused_idx:self.unused_idx + 1].mul_(0)
 
     def mixed_advance(self, slot_ids: torch.Tensor, lens: torch.Tensor) -> None:

@@ -61,7 +61,7 @@ class DecodeModule:
         if self.managed:  # pages for the new tokens, before the plan reads the block tables
             kv.step_maps(self.slots, self.ones, self.batch_size)
         if getattr(kv, "slot_adapters", None) is not None:
-            self.metadata.adapter_plan = adapter_plan(self.slots, kv.slot_adapters, kv.n_adapters)
+            self.metadata.adapter_plan = adapter_plan(self.slots, kv.slot_adapters, kv.n_adapters, err=kv.page_err)
         # one plan for every layer's decode launch (their slots, lengths and
         # block-table rows are the step's): splits balanced by length, page
         # ids resolved once
@@ -94,7 +94,7 @@ class DecodeModule:
             self.upload(slot_ids)
             logits = self.replay()
             next_tokens = torch.argmax(logits[:n], dim=-1)
-            if self.managed:
+            if self.managed or self.kv_cache.slot_adapters is not None:  # (steps that may report something)
                 return self.kv_cache.keep_step(self.slots[:n], self.ones[:n], next_tokens)
             self.kv_cache.last_generated[self.slots[:n]] = next_tokens
             return next_tokens.tolist()

@@ -103,7 +103,8 @@ class MixedModule:
                 kv.keys[0], self.cu_seqlens, kv.lens[self.slots], self.slots, kv.block_table, T, T,
                 self.model.config.num_attention_heads)
             if getattr(kv, "slot_adapters", None) is not None:
-                adapter_plan(self.row_slots, kv.slot_adapters, kv.n_adapters, out=self.metadata.adapter_plan)
+                adapter_plan(self.row_slots, kv.slot_adapters, kv.n_adapters, out=self.metadata.adapter_plan,
+                             err=kv.page_err)
 
     def _prepare_host(self, kv, B: int) -> None:
         """The maps of a step prepared on the CPU (``step_maps`` in torch)."""

@@ -122,3 +122,35 @@ def test_a_pool_whose_tables_the_caller_keeps_reports_too(native_lib, kind):
     assert torch.equal(kv.lens, before[0]) and torch.equal(kv.last_generated, before[1])
     kv.lens[1], kv.lens[2] = 0, 0
     assert mix.forward([[5] * 7, [6] * 9], [1, 2]) == first and kv.lens.tolist() == [0, 7, 9, 0, 0]
+
+
+def test_adapters_that_do_not_fit_are_reported(native_lib):
+    """A bank of other adapters than the step's plan, by the op and through a layer; a slot's adapter past the last one,
+    in mixed and decode steps: an error, and no step is counted."""
+    cfg = _config()
+    _, ours = _models(cfg)
+    kv = _pool(cfg, pages=8, managed=False)
+    layers = use_adapters(ours, kv, 3, 16)
+    kv.block_table[1, :2] = torch.tensor([1, 2], device=DEV)
+    mix, dec = MixedModule(ours, kv, token_count=32), DecodeModule(ours, kv, batch_size=2)
+    kv.slot_adapters[1] = 1
+    note("adapters that do not fit")
+    mix.forward([[1] * 9], [1])
+    kv.slot_adapters[1] = 3
+    for step in (lambda: mix.forward([[1] * 9], [1]), lambda: dec.forward([1])):
+        last = kv.last_generated.clone()
+        with pytest.raises(RuntimeError, match="adapters"):
+            step()
+        assert kv.lens.tolist() == [0, 9, 0, 0, 0] and torch.equal(kv.last_generated, last)
+    kv.slot_adapters[1] = 1
+    dec.forward([1])
+    assert kv.lens.tolist() == [0, 10, 0, 0, 0]
+    other = cie.AdapterBank(2, 16, 896, 896, dtype=torch.float16, device=DEV)
+    x, y, err = torch.ones(1, 5, 896).half().to(DEV), torch.ones(1, 5, 896).half().to(DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    plan = cie.adapter_plan(None, torch.zeros(5, dtype=torch.int64, device=DEV), 300)
+    other.add_(y, x, plan, err)
+    assert int(err) == 16 and (y == 1).all()
+    layers[0].o_adapters = other
+    with pytest.raises(RuntimeError, match="adapters"):
+        mix.forward([[1] * 9], [1])
+    assert kv.lens.tolist() == [0, 10, 0, 0, 0]

@@ -4,6 +4,7 @@ import random
 
 import pytest
 import torch
+from transformers import Qwen2Config, Qwen2ForCausalLM
 
 import custom_inference_engine_amd as cie
 from custom_inference_engine_amd.attn import adapters as ad
@@ -54,3 +55,28 @@ def test_adapters_refuse_shared_memory():
             cie.adapter_add_(**adapter_args(flat, y, x))
     with pytest.raises(AssertionError):  # one row too
         cie.adapter_add_(**adapter_args(flat, flat[None, :96], flat[None, 95:159]))
+
+
+def _model():
+    cfg = Qwen2Config(hidden_size=896, num_attention_heads=14, num_key_value_heads=2, intermediate_size=256,
+                      num_hidden_layers=1, vocab_size=128, max_position_embeddings=512)
+    model = Qwen2ForCausalLM(cfg).half().eval()
+    cie.use_triton_attention(model)
+    return cfg, model
+
+
+def _pool(cfg, n_slots=4):
+    return cie.KVStorage(cfg, max_cache_len=192, page_size=16, n_slots=n_slots, device="cpu", dtype=torch.float16)
+
+
+def test_a_layer_with_adapters_wants_a_plan():
+    """A step that would leave its rows without their adapters says so: no plan in the metadata, or no cache at all."""
+    cfg, model = _model()
+    kv = _pool(cfg)
+    layer, = cie.use_adapters(model, kv, 2, 8)
+    hidden, emb = torch.zeros(1, 3, 896, dtype=torch.float16), (torch.ones(1, 3, 64).half(), torch.zeros(1, 3, 64).half())
+    meta = cie.AttentionMetadata(token_count=3, full_decode=False, device="cpu")
+    with pytest.raises(AssertionError, match="adapter_plan"):
+        layer(hidden, emb, kv_manager=kv, metadata=meta)
+    with pytest.raises(AssertionError, match="adapters"):
+        layer(hidden, emb)
