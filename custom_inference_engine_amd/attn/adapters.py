@@ -240,6 +240,12 @@ class AdapterBank(torch.nn.Module):
         for t in (self.a, self.b, self.scales, self.ranks):
             t[i] = 0
 
+    @torch.no_grad()
+    def clear_all(self) -> None:
+        """Empties every place."""
+        for t in (self.a, self.b, self.scales, self.ranks):
+            t.zero_()
+
     def add_(self, y, x, plan, err=None) -> None:
         args = (y, x, self.a, self.b, self.scales, self.ranks, plan, self.slices)
         if err is None:
@@ -252,7 +258,8 @@ def use_adapters(model, kv_cache, n_adapters: int, rank: int) -> list:
     """Places for ``n_adapters`` low-rank adapters beside every attention layer's QKV and output projections.
 
     ``use_triton_attention`` comes first, step modules and schedulers (whose graphs record
-    the adapters' launches) after.  Returns the layers: ``layer.qkv_adapters.load(i, (A_q,
+    the adapters' launches) after; again only with as many of the same rank, which
+    empties them.  Returns the layers: ``layer.qkv_adapters.load(i, (A_q,
     A_k, A_v), (B_q, B_k, B_v), scale)`` and ``layer.o_adapters.load(i, A, B, scale)``
     fill place i.  A request's adapter is its slot's, ``kv_cache.slot_adapters[slot]`` (-1:
     none), which ``Scheduler.call(prompt, adapter=i)`` sets.
@@ -262,9 +269,16 @@ def use_adapters(model, kv_cache, n_adapters: int, rank: int) -> list:
     layers = [m for m in model.modules() if isinstance(m, TritonQwen2Attention)]
     if not layers:
         raise AssertionError("use_triton_attention(model) first")
+    banks = [b for layer in layers for b in (layer.qkv_adapters, layer.o_adapters) if b is not None]
+    if any((b.n_adapters, b.rank) != (n_adapters, rank) for b in banks):
+        raise AssertionError("the layers have banks of other sizes, which graphs may hold")
+    kv_cache.use_adapters(n_adapters)
+    if banks:  # (emptied where they stand)
+        for b in banks:
+            b.clear_all()
+        return layers
     for layer in layers:
         w, o = layer.qkv_weight, layer.original.o_proj
         layer.qkv_adapters = AdapterBank(n_adapters, rank, w.shape[1], layer.qkv_sizes, w.dtype, w.device)
         layer.o_adapters = AdapterBank(n_adapters, rank, o.in_features, o.out_features, w.dtype, w.device)
-    kv_cache.use_adapters(n_adapters)
     return layers

@@ -186,10 +186,14 @@ class KVStorage:
     def manage_pages(self) -> None:
         """Block tables are kept on the device from here on: the step modules' steps take the pages that their new
         tokens need from ``free_list`` (``pages.step_maps``), ``reset`` gives them back.  Comes before the step
-        modules and the scheduler, with every slot empty."""
+        modules and the scheduler, with every slot empty.  Again, it makes every page free where the list stands."""
         if bool(self.lens.any()) or bool(self.block_table.any()):
             raise AssertionError("manage_pages needs every slot empty")
-        self.free_list = _pages.new_free_list(self.n_pages, self.device)
+        words = _pages.new_free_list(self.n_pages, self.device)
+        if self.free_list is None:
+            self.free_list = words
+        else:  # (graphs hold its address)
+            self.free_list.copy_(words)
 
     def keep_step(self, slot_ids: torch.Tensor, new_tokens: torch.Tensor, next_tokens: torch.Tensor) -> list[int]:
         """The end of a step that fed ``new_tokens[b]`` tokens to slot ``slot_ids[b]``: the tokens that come next, on the
@@ -235,9 +239,19 @@ class KVStorage:
                                 free_list=self.free_list, out=out, err=self.page_err)
 
     def use_adapters(self, n_adapters: int) -> None:
-        """Slots may have one of ``n_adapters`` low-rank adapters (``attn.adapters``)."""
-        self.slot_adapters = torch.full((self.n_slots,), -1, dtype=torch.long, device=self.device)
-        self.n_adapters = n_adapters
+        """Slots may have one of ``n_adapters`` low-rank adapters (``attn.adapters``); none has one yet.  Comes before
+        the step modules and the scheduler; again only with as many."""
+        if self.slot_adapters is None:
+            self.slot_adapters = torch.full((self.n_slots,), -1, dtype=torch.long, device=self.device)
+            self.n_adapters = n_adapters
+        elif n_adapters != self.n_adapters:
+            raise AssertionError(f"the pool's slots have one of {self.n_adapters} adapters already")
+        else:  # (graphs hold its address)
+            self.slot_adapters.fill_(-1)
+
+    def turned_on(self) -> tuple[bool, int]:
+        """What step modules and graphs are made for: whether the pool manages its pages, and its adapters."""
+        return self.free_list is not None, self.n_adapters
 
     def mixed_update(self, layer_num: int, pages: torch.Tensor, offsets: torch.Tensor,
                      k_proj: torch.Tensor, v_proj: torch.Tensor) -> None:

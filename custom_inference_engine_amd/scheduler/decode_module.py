@@ -34,6 +34,12 @@ from ..attn.metadata import AttentionMetadata
 from ..graphs import StepGraph, StepInputs
 
 
+def check_turned_on(module) -> None:
+    """The pool is what the module was made for: a step recorded before would not take pages, or leave adapters out."""
+    if module.kv_cache.turned_on() != module.turned_on:
+        raise RuntimeError("manage_pages and use_adapters come before the step modules")
+
+
 class DecodeModule:
     def __init__(self, model, kv_cache, batch_size: int, pool=None, warmup_iters: int = 3):
         self.model = model
@@ -50,7 +56,8 @@ class DecodeModule:
         self.metadata.slot_ids = self.slots
         self.tokens = torch.zeros((batch_size,), dtype=torch.long, device=dev)
         self.positions = torch.zeros((batch_size,), dtype=torch.long, device=dev)
-        self.managed = getattr(kv_cache, "free_list", None) is not None  # the step takes its pages itself
+        self.turned_on = kv_cache.turned_on()
+        self.managed = self.turned_on[0]  # the step takes its pages itself
         self.ones = torch.ones((batch_size,), dtype=torch.long, device=dev)
         with torch.inference_mode():
             self.step = StepGraph(self._step, pool=pool, warmup=warmup_iters, device=dev)
@@ -90,6 +97,7 @@ class DecodeModule:
         n = len(slot_ids)
         if n == 0:
             return []
+        check_turned_on(self)
         with torch.inference_mode():
             self.upload(slot_ids)
             logits = self.replay()

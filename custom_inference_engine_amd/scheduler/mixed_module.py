@@ -53,6 +53,7 @@ from ..attn.metadata import AttentionMetadata
 from ..graphs import StepGraph, StepInputs
 from ..kv_cache.pages import StepMaps
 from ..piecewise import get_piecewise_backend
+from .decode_module import check_turned_on
 
 
 class MixedModule:
@@ -80,6 +81,7 @@ class MixedModule:
         self.row_slots = torch.zeros((T,), dtype=torch.long, device=dev)
         self.maps = StepMaps(self.cu_seqlens, self.row_slots, self.positions, self.metadata.pages,
                              self.metadata.offsets)
+        self.turned_on = kv_cache.turned_on()
         if getattr(kv_cache, "slot_adapters", None) is not None:  # (read by captured pieces: one address for every step)
             self.metadata.adapter_plan = new_adapter_plan(T, kv_cache.n_adapters, dev)
         self.last_logits = None  # (n, vocab) of the last forward
@@ -168,6 +170,7 @@ class MixedModule:
         n = len(slot_ids)
         if n == 0:
             return []
+        check_turned_on(self)
         with torch.inference_mode():
             self.upload(prompts, slot_ids)
             logits = self.run()[:n]

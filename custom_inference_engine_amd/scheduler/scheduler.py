@@ -147,6 +147,7 @@ class ModuleExecutor:
         self.decode_modules = {b: DecodeModule(model, kv_cache, batch_size=b, pool=self.pool)
                                for b in sorted(batch_sizes, reverse=True)}
         self.max_batch = max(batch_sizes)
+        self.n_adapters = kv_cache.n_adapters  # that the graphs serve
         self.mixed_modules = {}
         piecewise = [t for t in self.token_counts if piecewise_above is not None and t > piecewise_above]
         if graph_mixed and piecewise:
@@ -436,7 +437,8 @@ class Scheduler:
         fut: Future = Future()
         if not self.open:
             fut.set_exception(RuntimeError("Loop is not open."))
-        elif adapter != -1 and not 0 <= adapter < getattr(self.kv_cache, "n_adapters", 0):
+        elif adapter != -1 and not 0 <= adapter < getattr(self.executor, "n_adapters",
+                                                          getattr(self.kv_cache, "n_adapters", 0)):
             fut.set_exception(ValueError(f"The pool has no adapter {adapter}."))
         elif len(prompt) == 0:
             fut.set_exception(ValueError("Empty prompts are not allowed."))
@@ -451,6 +453,8 @@ class Scheduler:
 
     def step(self) -> bool:
         """One scheduling round; False once the loop has nothing left to do."""
+        if self.device_pages != (getattr(self.kv_cache, "free_list", None) is not None):
+            raise RuntimeError("manage_pages comes before the scheduler")
         if self.open:
             if self._busy_slots:
                 self._admit(wait=False, only_preempted=False, left=self._plan_running())

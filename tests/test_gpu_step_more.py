@@ -154,3 +154,50 @@ def test_adapters_that_do_not_fit_are_reported(native_lib):
     with pytest.raises(RuntimeError, match="adapters"):
         mix.forward([[1] * 9], [1])
     assert kv.lens.tolist() == [0, 10, 0, 0, 0]
+
+
+def test_pages_and_adapters_turned_on_late(native_lib):
+    """Modules and schedulers made before: their steps are refused, and a scheduler takes no request whose adapter its
+    graphs would leave out."""
+    cfg = _config()
+    _, ours = _models(cfg)
+    kv = _pool(cfg, pages=16, managed=False)
+    sched = Scheduler(ours, kv, eos_token_ids={512}, max_new_tokens=4, token_budget=160)
+    mix, dec = MixedModule(ours, kv, token_count=32), DecodeModule(ours, kv, batch_size=2)
+    kv.use_adapters(2)
+    future = sched.call([1, 2, 3], adapter=1)
+    assert future.done() and isinstance(future.exception(), ValueError)
+    for step in (lambda: mix.forward([[1, 2]], [1]), lambda: dec.forward([1])):
+        with pytest.raises(RuntimeError, match="before the step modules"):
+            step()
+    assert not kv.lens.any()
+    kv = _pool(cfg, pages=16, managed=False)
+    mix, dec = FullMixedModule(ours, kv, batch_size=2, token_count=32), DecodeModule(ours, kv, batch_size=2)
+    kv.manage_pages()
+    for step in (lambda: mix.forward([[1, 2]], [1]), lambda: dec.forward([1])):
+        with pytest.raises(RuntimeError, match="before the step modules"):
+            step()
+    assert not kv.lens.any()
+
+
+def test_turned_on_twice_under_graphs(native_lib):
+    """Graphs recorded between two calls of manage_pages and use_adapters go on with the pool's own words."""
+    cfg = _config()
+    theirs, ours = _models(cfg)
+    kv = _pool(cfg, pages=16)
+    layers = use_adapters(ours, kv, 2, 16)
+    mix, dec = FullMixedModule(ours, kv, batch_size=2, token_count=32), DecodeModule(ours, kv, batch_size=2)
+    note("turned on twice")
+    kv.manage_pages()
+    assert use_adapters(ours, kv, 2, 16) == layers
+    merged = _adapters(layers, 2, 16, seed=6)
+    prompt = _prompts(20)[0]
+    kv.slot_adapters[2] = 1
+    nxt = mix.forward([prompt], [2])
+    assert _rel(mix.last_logits[0], _logits(merged(theirs, 1), prompt)) < 2e-2
+    dec.forward([2])
+    assert _rel(dec.logits[0], _logits(merged(theirs, 1), prompt + nxt)) < 2e-2
+    assert int(kv.free_list[0]) == 13
+    _whole(kv)
+    kv.reset([2])
+    assert int(kv.free_list[0]) == 15

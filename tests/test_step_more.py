@@ -8,6 +8,7 @@ from transformers import Qwen2Config, Qwen2ForCausalLM
 
 import custom_inference_engine_amd as cie
 from custom_inference_engine_amd.attn import adapters as ad
+from custom_inference_engine_amd.scheduler import Scheduler
 
 I64 = torch.int64
 
@@ -80,3 +81,49 @@ def test_a_layer_with_adapters_wants_a_plan():
         layer(hidden, emb, kv_manager=kv, metadata=meta)
     with pytest.raises(AssertionError, match="adapters"):
         layer(hidden, emb)
+
+
+def test_state_that_graphs_hold_stays_where_it_is():
+    """manage_pages and use_adapters again: the same tensors, as after the first call, or a refusal."""
+    cfg, model = _model()
+    kv = _pool(cfg)
+    kv.manage_pages()
+    held = [kv.free_list, kv.page_err]
+    kv.free_list[0] = 2
+    kv.manage_pages()
+    assert kv.free_list is held[0] and kv.page_err is held[1]
+    assert torch.equal(kv.free_list, cie.new_free_list(kv.n_pages, "cpu"))
+    layer, = cie.use_adapters(model, kv, 2, 8)
+    slots, banks = kv.slot_adapters, (layer.qkv_adapters, layer.o_adapters)
+    tensors = [t for b in banks for t in (b.a, b.b, b.scales, b.ranks)]
+    banks[1].load(1, torch.ones(3, 896), torch.ones(896, 3))
+    kv.slot_adapters[1] = 1
+    assert cie.use_adapters(model, kv, 2, 8) == [layer]
+    assert kv.slot_adapters is slots and (slots == -1).all()
+    assert (layer.qkv_adapters, layer.o_adapters) == banks
+    assert all(x is y and not y.any() for x, y in zip(tensors, [t for b in banks for t in (b.a, b.b, b.scales, b.ranks)]))
+    for n, rank in ((3, 8), (2, 16), (2, 7)):
+        with pytest.raises(AssertionError):
+            cie.use_adapters(model, kv, n, rank)
+    with pytest.raises(AssertionError):
+        kv.use_adapters(5)
+    assert kv.slot_adapters is slots and kv.n_adapters == 2
+    other = _pool(cfg)  # another pool of the same model
+    assert cie.use_adapters(model, other, 2, 8) == [layer] and other.n_adapters == 2
+
+
+def test_a_scheduler_before_manage_pages_stops():
+    """A scheduler that keeps the tables itself does not go on with a pool that keeps its own."""
+    cfg, _ = _model()
+    kv = _pool(cfg)
+    sched = Scheduler(None, kv, eos_token_ids={128}, max_new_tokens=16, token_budget=160, executor=object())
+    kv.manage_pages()
+    future = sched.call([1, 2])
+    with pytest.raises(RuntimeError, match="manage_pages"):
+        sched.loop()
+    assert future.exception() is not None
+    kv.use_adapters(2)
+    executor = type("Executor", (), {"n_adapters": 0})()  # whose graphs have none
+    sched = Scheduler(None, kv, eos_token_ids={128}, max_new_tokens=16, token_budget=160, executor=executor)
+    future = sched.call([1, 2], adapter=1)
+    assert future.done() and isinstance(future.exception(), ValueError)
