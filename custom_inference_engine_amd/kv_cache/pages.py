@@ -21,6 +21,7 @@ from .quant import int64_index, int64_table, launch, one_device
 
 _I64 = torch.int64
 ERR_FREE = 32  # CIE_ERRBIT_FREE
+MAX_SEQUENCES = 2048  # of a call
 
 
 class StepMaps(NamedTuple):
@@ -111,7 +112,8 @@ def release_pages(free_list, slot_ids, lens, block_table, page_size: int, keep=N
     ``lens[slot]`` becomes ``keep[b]`` and the released table entries 0.  ``held[b]``: the
     tokens whose pages the sequence has, where these are more than ``lens[slot]``: after
     a ``step_maps`` whose tokens ``lens`` does not count yet (keep = those of them that
-    stay).  A slot comes once, or nothing is done (CIE_ERRBIT_FREE in ``err``).
+    stay).  A slot comes once, or nothing is done (CIE_ERRBIT_FREE in ``err``).  Table
+    entries that hold no page (0) are not given back (CIE_ERRBIT_PAGE).
     """
     n_pages = _check_state(lens, block_table, free_list)
     if slot_ids.dim() != 1 or page_size < 1:

@@ -194,6 +194,7 @@ class KVStorage:
             self.free_list = words
         else:  # (graphs hold its address)
             self.free_list.copy_(words)
+            self.page_err.zero_()
 
     def keep_step(self, slot_ids: torch.Tensor, new_tokens: torch.Tensor, next_tokens: torch.Tensor) -> list[int]:
         """The end of a step that fed ``new_tokens[b]`` tokens to slot ``slot_ids[b]``: the tokens that come next, on the
@@ -305,7 +306,8 @@ class KVStorage:
     def reset(self, slot_ids: list[int]) -> None:
         if self.free_list is not None:  # the slots' pages are free again
             slots = torch.tensor(list(dict.fromkeys(slot_ids)), dtype=torch.long).to(self.lens.device)  # (each once)
-            _pages.release_pages(self.free_list, slots, self.lens, self.block_table, self.page_size, err=self.page_err)
+            for part in slots.split(_pages.MAX_SEQUENCES):
+                _pages.release_pages(self.free_list, part, self.lens, self.block_table, self.page_size, err=self.page_err)
         else:
             self.lens[slot_ids] = 0
             self.block_table[slot_ids] = 0

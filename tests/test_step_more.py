@@ -127,3 +127,18 @@ def test_a_scheduler_before_manage_pages_stops():
     sched = Scheduler(None, kv, eos_token_ids={128}, max_new_tokens=16, token_budget=160, executor=executor)
     future = sched.call([1, 2], adapter=1)
     assert future.done() and isinstance(future.exception(), ValueError)
+
+
+def test_any_number_of_slots_is_reset(monkeypatch):
+    """A call gives back the pages of 2,048 sequences at most."""
+    cfg, _ = _model()
+    kv = _pool(cfg, n_slots=5000)
+    kv.manage_pages()
+    parts = []
+    monkeypatch.setattr("custom_inference_engine_amd.kv_cache.pages.release_pages",
+                        lambda free_list, slots, *rest, err=None: parts.append(slots.tolist()))
+    kv.reset(list(range(4999, -1, -1)))
+    assert max(map(len, parts)) <= 2048 and sum(parts, []) == list(range(4999, -1, -1))
+    parts.clear()
+    kv.reset([])
+    assert not any(parts)
