@@ -25,10 +25,18 @@ _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # CIE_F16, CIE
 _F64, _DENSE = torch.float64, torch.contiguous_format
 
 
-def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None, device=None):
+# What a scaling may hold beside its type; those that a type does not use are ignored, as the model library does.
+_SCALING_KEYS = {"rope_type", "type", "rope_theta", "partial_rotary_factor", "factor", "factors", "attention_factor",
+                 "original_max_position_embeddings", "beta_fast", "beta_slow", "mscale", "mscale_all_dim", "truncate"}
+
+
+def rotary_frequencies(rotary_dim: int, base: Optional[float] = None, scaling: Optional[dict] = None, device=None):
     """(frequencies (rotary_dim / 2,) float64, scale) of a base and a scaling.
 
-    ``scaling`` is a model config's ``rope_scaling``, by its ``rope_type`` (or ``type``):
+    ``base``: the scaling's ``rope_theta`` by default, or 10,000; not another than that
+    ``rope_theta``.  ``scaling`` is a model config's ``rope_scaling``, by its
+    ``rope_type`` (or ``type``); keys not named here are refused, as is a
+    ``partial_rotary_factor`` (``rotary_dim`` says what turns).
 
     * ``default``: base ** (-2i / rotary_dim).
     * ``linear``: positions divided by ``factor``.
@@ -36,20 +44,33 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
       stretched by ``factor`` and the fastest is kept.
     * ``yarn``: pairs that turn more than ``beta_fast`` (32) times within
       ``original_max_position_embeddings`` are kept, those under ``beta_slow`` (1) are
-      stretched by ``factor``, with a ramp between; ``scale`` is ``attention_factor``, or
-      0.1 ln(factor) + 1.
+      stretched by ``factor``, with a ramp between, from a whole pair to a whole pair unless
+      ``truncate`` is false; ``scale`` is ``attention_factor``; or where ``mscale`` and
+      ``mscale_all_dim`` are set m(mscale) / m(mscale_all_dim), m(x) = 0.1 x ln(factor) + 1 (1
+      for factors up to 1); or m(1).
     * ``factors``: each frequency divided by its own ``factors[i]``; ``scale`` is
       ``attention_factor``, or 1.
     """
+    scaling = {k: v for k, v in (scaling or {}).items() if v is not None}
+    unknown = set(scaling) - _SCALING_KEYS
+    if unknown:
+        raise AssertionError(f"rope scaling has keys that are not understood: {sorted(unknown)}")
+    if scaling.get("partial_rotary_factor", 1) != 1:
+        raise AssertionError("rotary_dim says how much of a head turns: leave out 'partial_rotary_factor'")
+    theta = scaling.get("rope_theta")
+    if base is None:
+        base = 10000.0 if theta is None else theta
+    elif theta is not None and theta != base:
+        raise AssertionError(f"base {base} is not the scaling's rope_theta {theta}")
+    base = float(base)
     if rotary_dim < 2 or rotary_dim % 2 or not base > 0:
         raise AssertionError("rotary_dim must be even and positive, base positive")
     n = rotary_dim // 2
-    scaling = dict(scaling or {})
     kind = scaling.get("rope_type", scaling.get("type", "default"))
     scale = 1.0
 
     def need(name):
-        if scaling.get(name) is None:
+        if name not in scaling:
             raise AssertionError(f"rope scaling '{kind}' needs '{name}'")
         return scaling[name]
 
@@ -62,23 +83,35 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
         freqs = [f / float(need("factor")) for f in freqs]
     elif kind == "yarn":
         factor, trained = float(need("factor")), need("original_max_position_embeddings")
+        fast, slow = scaling.get("beta_fast") or 32, scaling.get("beta_slow") or 1
         if base == 1.0:
             raise AssertionError("rope scaling 'yarn' needs a base other than 1")
+        if not fast > slow:
+            raise AssertionError("rope scaling 'yarn' needs beta_fast over beta_slow")
 
         def pair_that_turns(times):  # (a real number) within the trained positions
             return rotary_dim * math.log(trained / (times * 2 * math.pi)) / (2 * math.log(base))
 
-        low = max(math.floor(pair_that_turns(scaling.get("beta_fast") or 32)), 0)
-        high = min(math.ceil(pair_that_turns(scaling.get("beta_slow") or 1)), rotary_dim - 1)
+        def m(x):
+            return 0.1 * x * math.log(factor) + 1 if factor > 1 else 1.0
+
+        low, high = pair_that_turns(fast), pair_that_turns(slow)
+        if scaling.get("truncate", True):
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, rotary_dim - 1)
         stretched = [min(max((i - low) / max(high - low, 1e-3), 0.0), 1.0) for i in range(n)]
         freqs = [f / factor * s + f * (1 - s) for f, s in zip(freqs, stretched)]
-        scale = scaling.get("attention_factor") or (0.1 * math.log(factor) + 1 if factor > 1 else 1.0)
+        if scaling.get("mscale") and scaling.get("mscale_all_dim"):
+            scale = m(scaling["mscale"]) / m(scaling["mscale_all_dim"])
+        else:
+            scale = m(1)
+        scale = scaling.get("attention_factor", scale)
     elif kind == "factors":
         factors = need("factors")
         if len(factors) != n:
             raise AssertionError(f"'factors' must have {n} entries")
         freqs = [f / float(x) for f, x in zip(freqs, factors)]
-        scale = scaling.get("attention_factor") or 1.0
+        scale = scaling.get("attention_factor", 1.0)
     elif kind not in ("default", "linear", "ntk"):
         raise AssertionError(f"unknown rope scaling '{kind}': default, linear, ntk, yarn or factors")
     return torch.tensor(freqs, dtype=torch.float64, device=device), float(scale)

@@ -5,6 +5,7 @@ import random
 import pytest
 import torch
 from transformers import Qwen2Config, Qwen2ForCausalLM
+from transformers.models.qwen2.modeling_qwen2 import Qwen2RotaryEmbedding
 
 import custom_inference_engine_amd as cie
 from custom_inference_engine_amd.attn import adapters as ad
@@ -142,3 +143,46 @@ def test_any_number_of_slots_is_reset(monkeypatch):
     parts.clear()
     kv.reset([])
     assert not any(parts)
+
+
+# ---- rotary ----
+
+YARN = {"rope_type": "yarn", "factor": 40.0, "original_max_position_embeddings": 4096}
+
+
+@pytest.mark.parametrize("scaling", [
+    dict(YARN, mscale=1.0, mscale_all_dim=1.0), dict(YARN, mscale=0.707, mscale_all_dim=1.0), dict(YARN, mscale=0.7),
+    dict(YARN, mscale_all_dim=0.7), dict(YARN, mscale=0.7, mscale_all_dim=0.0),
+    dict(YARN, mscale=0.7, mscale_all_dim=0.5, attention_factor=1.1), dict(YARN, attention_factor=0.0),
+    dict(YARN, truncate=False), dict(YARN, truncate=True), dict(YARN, truncate=False, beta_fast=4, beta_slow=2), dict(YARN, beta_fast=None),
+    dict(YARN, factor=1.0, mscale=2.0, mscale_all_dim=1.0), dict(YARN, factor=0.5),
+    dict(YARN, rope_theta=1e4), {"rope_type": "linear", "factor": 2.0, "rope_theta": 5e5}, {"rope_type": "default", "rope_theta": 1e6},
+    {"rope_type": "linear", "factor": 2.0, "partial_rotary_factor": 1.0}, {"rope_type": "linear", "factor": 2.0, "attention_factor": 3.0},
+], ids=str)
+@pytest.mark.parametrize("d", [64, 128])
+def test_every_key_of_a_scaling_counts(scaling, d):
+    """The config's own rope_scaling, as the model library keeps it, against its rotary embedding's fp32 frequencies:
+    three roundings and a power (ln(base) < 14 times the exponent's), and a ramp of four more of the unscaled frequency."""
+    cfg = Qwen2Config(hidden_size=14 * d, num_attention_heads=14, num_key_value_heads=2, rope_theta=1e6,
+                      max_position_embeddings=32768, rope_scaling=dict(scaling))
+    emb = Qwen2RotaryEmbedding(cfg)
+    held = dict(cfg.rope_scaling)
+    assert held["rope_theta"] == scaling.get("rope_theta", 1e6)
+    freqs, scale = cie.rotary_frequencies(d, scaling=held)
+    plain = held["rope_theta"] ** (-torch.arange(0, d, 2).double() / d)
+    want = emb.inv_freq.double()
+    assert ((freqs - want).abs() <= (20 * want + 4 * plain) * 2.0 ** -23).all()
+    assert abs(scale - emb.attention_scaling) <= 1e-6
+    again, _ = cie.rotary_frequencies(d, held["rope_theta"], held)
+    assert torch.equal(again, freqs)
+
+
+@pytest.mark.parametrize("base,scaling", [
+    (None, dict(YARN, short_factor=[1.0])), (None, dict(YARN, llama_4_scaling_beta=0.1)), (1e4, dict(YARN, rope_theta=1e6)),
+    (None, {"rope_type": "linear", "factor": 2.0, "partial_rotary_factor": 0.5}), (None, {"partial_rotary_factor": 0.5}),
+    (None, {"rope_type": "default", "mrope_section": [8, 12, 12]}), (None, dict(YARN, beta_fast=1, beta_slow=32)),
+    (None, {"rope_type": "linear", "factor": None}), (-1.0, None), (None, {"rope_theta": 0.0}),
+])
+def test_keys_that_are_not_understood_are_refused(base, scaling):
+    with pytest.raises(AssertionError):
+        cie.rotary_frequencies(64, base, scaling)
