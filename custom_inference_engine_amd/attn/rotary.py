@@ -294,9 +294,13 @@ class RotaryPositions(torch.nn.Module):
         return self
 
     def forward(self, x, position_ids):
-        if self.tables:
+        if not self.tables:
+            return position_ids, self.frequencies
+        if position_ids.dim() < 2 or position_ids.shape[0] == 1:
             return rotary_tables_op(position_ids, self.frequencies, x.dtype, self.interleaved, self.scale)
-        return position_ids, self.frequencies
+        # several rows of tokens (the wrapped modules' own path): side by side, and dealt to the rows again
+        cos, sin = rotary_tables_op(position_ids.flatten(), self.frequencies, x.dtype, self.interleaved, self.scale)
+        return cos.view(*position_ids.shape, -1), sin.view(*position_ids.shape, -1)
 
 
 def use_rotary(model, frequencies, scale: float = 1.0, interleaved: bool = False) -> None:

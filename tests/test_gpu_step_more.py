@@ -201,3 +201,27 @@ def test_turned_on_twice_under_graphs(native_lib):
     _whole(kv)
     kv.reset([2])
     assert int(kv.free_list[0]) == 15
+
+
+def test_the_wrapped_modules_path_after_use_rotary(native_lib):
+    """A model that is called without a cache, on one row of tokens and on several (padded or not): as before use_rotary,
+    up to the tables' rounding."""
+    cfg = _config()
+    _, ours = _models(cfg)
+    g = torch.Generator().manual_seed(1)
+    calls = [dict(input_ids=torch.randint(0, 512, (b, n), generator=g).to(DEV)) for b, n in ((1, 7), (3, 7), (2, 1))]
+    mask = torch.ones(3, 7, dtype=torch.int64, device=DEV)
+    mask[1, :4] = 0
+    calls.append(dict(calls[1], attention_mask=mask, position_ids=(mask.cumsum(1) - 1).clamp(min=0)))
+    with torch.inference_mode():
+        want = [ours(**c, use_cache=False).logits for c in calls]
+        use_rotary(ours, *cie.rotary_frequencies(D, 1e6))
+        note("the wrapped modules' path")
+        for c, w in zip(calls, want):
+            got = ours(**c, use_cache=False).logits
+            assert got.shape == w.shape and _rel(got, w.float().cpu()) < 2e-2
+        rows = torch.tensor([[0, 1, 2], [70000, 5, 9]], device=DEV)
+        cos, sin = ours.model.rotary_emb(want[0], rows)
+        for t, one in ((cos, 0), (sin, 1)):
+            assert t.shape == (2, 3, D)
+            assert torch.equal(t, torch.cat([cie.rotary_tables(r, ours.model.rotary_emb.frequencies)[one] for r in rows]))
