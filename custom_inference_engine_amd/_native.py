@@ -175,17 +175,17 @@ _SIGNATURES = {
     "cie_rotary": (
         ctypes.c_int,
         [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64p, _c_ptr,
-         ctypes.c_float, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int, _c_ptr],
+         ctypes.c_double, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int, _c_ptr],
     ),
     "cie_kv_append_tokens_qkv_rotary": (
         ctypes.c_int,
-        [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64p, _c_ptr, ctypes.c_float, _c_i64p, _c_i64p,
+        [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64p, _c_ptr, ctypes.c_double, _c_i64p, _c_i64p,
          _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int,
          ctypes.c_int, _c_ptr, _c_ptr],
     ),
     "cie_rotary_tables": (
         ctypes.c_int,
-        [_c_ptr, _c_ptr, _c_i64p, _c_ptr, ctypes.c_float, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int,
+        [_c_ptr, _c_ptr, _c_i64p, _c_ptr, ctypes.c_double, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int,
          _c_ptr],
     ),
     "cie_adapter_plan_bytes": (_c_i64, [_c_i64, _c_i64]),
@@ -200,7 +200,7 @@ _SIGNATURES = {
     ),
 }
 
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 

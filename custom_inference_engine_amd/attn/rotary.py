@@ -6,7 +6,8 @@ operators turn rows by their positions themselves.  Pair i of the first ``2 *
 len(frequencies)`` dims of a head, (x, y), becomes ``scale * (x cos a - y sin a,
 y cos a + x sin a)`` with ``a = position * frequencies[i]``: dims (i, i + half) or, with
 ``interleaved``, (2i, 2i + 1); the other dims are copied.  Angles are computed in 64 bits,
-so far positions keep them; products and sums in fp32, rounded once.
+so far positions keep them, and for fp32 rows and tables their cos and sin too; products and
+sums in fp32, rounded once.
 
 ``rotary_frequencies`` makes the table of a base and a long-context scaling; any other is
 a float64 tensor of radians a position.

@@ -6,9 +6,10 @@
 // copied.  The f_i are radians a position in fp64, so any base and any stretching
 // for long contexts is a table of them.
 //
-// Angles: p * f_i in fp64, in turns, less the nearest whole turn (exact), and only
-// then fp32: at position 2^31 the angle is off by 2^-20 rad, where an fp32 product
-// is off by whole turns.  Products and sums are fp32, rounded once at the end.
+// Angles: p * f_i in fp64, in turns, less the nearest whole turn (exact): at position
+// 2^31 the angle is off by 2^-20 rad, where an fp32 product is off by whole turns.  cos
+// and sin of what is left are taken in fp32 for 16-bit rows, whose rounding hides the 2^-22
+// that this costs, and in fp64 for fp32 rows, rounded once.  Products and sums are fp32.
 //
 // Bound by memory: each row is read and written once.  A thread takes 16 bytes of
 // each half of a pair's dims (two vectors of V values) and computes their V
@@ -16,7 +17,8 @@
 // Few rows get a head a thread; many get fewer threads, down to a few rounds of
 // the chip, so that the angles (some 60 instructions a pair) are spread over
 // more heads.  8,192 rows of 48 heads of 128 into the pools: 40.7 us, 5.0 TB/s, what a copy
-// reaches.  Rows at any address and odd widths take the same vectors, unaligned;
+// reaches; 8,192 rows of 40 heads of 128 in fp32 61.4 us, 5.5 TB/s (their tables 3.9 us, with cos
+// and sin in fp32 3.7).  Rows at any address and odd widths take the same vectors, unaligned;
 // only heads that turn or copy less than a vector go value by value.
 #include "cie_common.h"
 
@@ -53,21 +55,28 @@ struct RotaryParams {
   const int64_t* offsets;
   int64_t pool_page_stride, pool_head_stride, n_pages;
   int64_t T;
-  float scale;
+  double scale;
   int32_t H_q, H_kv, D, rot, units, head_groups, page_size;
   int32_t* err;
 };
 
-// cos and sin of position p at V pairs from pair i on, times scale.
-template <int V>
-__device__ __forceinline__ void angles(double p, const double* f, float scale, float* c, float* s) {
+// cos and sin of position p at V pairs from pair i on, times scale, for rows of E.
+template <class E, int V>
+__device__ __forceinline__ void angles(double p, const double* f, double scale, float* c, float* s) {
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const double turns = p * f[j] * 0.15915494309189533577;  // 1 / 2 pi
-    const float half_turns = 2.0f * (float)(turns - __builtin_rint(turns));
-    sincospif(half_turns, &s[j], &c[j]);
-    c[j] *= scale;
-    s[j] *= scale;
+    const double left = turns - __builtin_rint(turns);
+    if constexpr (sizeof(E) == 4) {
+      double sin, cos;
+      sincospi(2.0 * left, &sin, &cos);
+      c[j] = (float)(cos * scale);
+      s[j] = (float)(sin * scale);
+    } else {
+      sincospif(2.0f * (float)left, &s[j], &c[j]);
+      c[j] *= (float)scale;
+      s[j] *= (float)scale;
+    }
   }
 }
 
@@ -134,7 +143,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
   float c[V], s[V];
   // (Before the rows' loads: behind them their registers leave three waves a SIMD, and
   // 2,048 rows of 40 heads take 11.7 us, not 9.6.)
-  if (turns) angles<V>((double)p.positions[t], p.freqs + pair, p.scale, c, s);
+  if (turns) angles<E, V>((double)p.positions[t], p.freqs + pair, p.scale, c, s);
   if constexpr (kPools) {
     kept = false;
     if (off < 0 || off >= p.page_size)
@@ -189,7 +198,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
 // fused append and decode calls take them).  A thread computes V pairs.
 template <class E, int V, bool kInterleaved, bool kAligned>
 __global__ __launch_bounds__(256) void rotary_tables_kernel(E* cos, E* sin, const int64_t* positions,
-                                                            const double* freqs, float scale, int64_t T, int rot) {
+                                                            const double* freqs, double scale, int64_t T, int rot) {
   typedef Pack<E, V, kAligned> vec;
   const uint32_t gid = blockIdx.x * 256u + threadIdx.x;
   const int half = rot / 2;
@@ -198,7 +207,7 @@ __global__ __launch_bounds__(256) void rotary_tables_kernel(E* cos, E* sin, cons
   if (t >= T) return;
   const int pair = min(V * (int)(gid % units), half - V);
   float c[V], s[V];
-  angles<V>((double)positions[t], freqs + pair, scale, c, s);
+  angles<E, V>((double)positions[t], freqs + pair, scale, c, s);
 #pragma unroll
   for (int j = 0; j < V; ++j) asm volatile("" : "+v"(c[j]), "+v"(s[j]));  // (to fp32 first, as above)
 #pragma unroll
@@ -269,7 +278,7 @@ static int check_sizes(int64_t T, int64_t H_q, int64_t H_kv, int64_t D, int64_t 
 }
 
 template <class E, int V, bool kAligned>
-static int launch_tables(E* cos, E* sin, const int64_t* positions, const double* freqs, float scale, int64_t T,
+static int launch_tables(E* cos, E* sin, const int64_t* positions, const double* freqs, double scale, int64_t T,
                          int64_t rot, bool interleaved, hipStream_t stream) {
   const int64_t blocks = (T * ((rot / 2 + V - 1) / V) + 255) / 256;
   if (blocks > kRotMaxBlocks) return CIE_EUNSUPPORTED;
@@ -284,7 +293,7 @@ static int launch_tables(E* cos, E* sin, const int64_t* positions, const double*
 }
 
 template <class E>
-static int dispatch_tables(void* cos, void* sin, const int64_t* positions, const double* freqs, float scale, int64_t T,
+static int dispatch_tables(void* cos, void* sin, const int64_t* positions, const double* freqs, double scale, int64_t T,
                            int64_t rot, bool interleaved, hipStream_t stream) {
   constexpr int V = VecOf<E>::kWide;
   E* const c = static_cast<E*>(cos);
@@ -301,7 +310,7 @@ using namespace cie;
 
 extern "C" int cie_rotary(void* q_out, void* k_out, const void* q, const void* k, int64_t q_tok_stride,
                           int64_t q_head_stride, int64_t k_tok_stride, int64_t k_head_stride,
-                          const int64_t* positions, const double* freqs, float scale, int64_t T, int64_t H_q,
+                          const int64_t* positions, const double* freqs, double scale, int64_t T, int64_t H_q,
                           int64_t H_kv, int64_t D, int64_t rot, int interleaved, int dtype, void* stream) {
   const int bad = check_sizes(T, H_q, H_kv, D, rot, dtype);
   if (bad) return bad;
@@ -332,7 +341,7 @@ extern "C" int cie_rotary(void* q_out, void* k_out, const void* q, const void* k
 
 extern "C" int cie_kv_append_tokens_qkv_rotary(
     void* q_out, void* k_pool, void* v_pool, const void* qkv, int64_t qkv_row_stride, const int64_t* positions,
-    const double* freqs, float scale, const int64_t* pages, const int64_t* offsets, int64_t T, int64_t H_q,
+    const double* freqs, double scale, const int64_t* pages, const int64_t* offsets, int64_t T, int64_t H_q,
     int64_t H_kv, int64_t page_size, int64_t D, int64_t n_pages, int64_t pool_page_stride, int64_t pool_head_stride,
     int64_t rot, int interleaved, int dtype, int32_t* err, void* stream) {
   const int bad = check_sizes(T, H_q, H_kv, D, rot, dtype);
@@ -373,7 +382,7 @@ extern "C" int cie_kv_append_tokens_qkv_rotary(
                           : dispatch_rotary<bf16, true>(p, interleaved, st);
 }
 
-extern "C" int cie_rotary_tables(void* cos, void* sin, const int64_t* positions, const double* freqs, float scale,
+extern "C" int cie_rotary_tables(void* cos, void* sin, const int64_t* positions, const double* freqs, double scale,
                                  int64_t T, int64_t rot, int interleaved, int dtype, void* stream) {
   if (T < 0 || rot < 2 || rot % 2) return CIE_EINVAL;
   if (dtype < 0 || dtype > 2 || rot > 65536 || T > 0x7fffffff) return CIE_EUNSUPPORTED;

@@ -613,7 +613,8 @@ int cie_release_pages(int64_t* free_list, const int64_t* slot_ids, int64_t* lens
  *   scale * (x cos a - y sin a, y cos a + x sin a),  a = positions[t] * freqs[i]
  * with freqs[i] in radians a position (rot / 2 doubles).  Pairs are dims
  * (i, i + rot / 2), or (2i, 2i + 1) where interleaved; dims from rot on are copied.
- * Angles are computed in fp64, products and sums in fp32, outputs rounded once.
+ * Angles are computed in fp64 (for 16-bit types their cos and sin in fp32), products
+ * and sums in fp32, outputs rounded once.
  * Beside apply_rotary_pos_emb of the reference's layer (attn/core.py:193-198).
  *   cie_rotary         q (T, H_q, D) and k (T, H_kv, D) views, their own token and
  *                      head strides (elements), dims dense; either may have no
@@ -629,19 +630,19 @@ int cie_release_pages(int64_t* free_list, const int64_t* slot_ids, int64_t* lens
 int cie_rotary(void* q_out, void* k_out, const void* q, const void* k,
                int64_t q_tok_stride, int64_t q_head_stride,
                int64_t k_tok_stride, int64_t k_head_stride,
-               const int64_t* positions, const double* freqs, float scale,
+               const int64_t* positions, const double* freqs, double scale,
                int64_t T, int64_t H_q, int64_t H_kv, int64_t D, int64_t rot,
                int interleaved, int dtype, void* stream);
 int cie_kv_append_tokens_qkv_rotary(void* q_out, void* k_pool, void* v_pool, const void* qkv,
                                     int64_t qkv_row_stride, const int64_t* positions,
-                                    const double* freqs, float scale,
+                                    const double* freqs, double scale,
                                     const int64_t* pages, const int64_t* offsets,
                                     int64_t T, int64_t H_q, int64_t H_kv, int64_t page_size,
                                     int64_t D, int64_t n_pages, int64_t pool_page_stride,
                                     int64_t pool_head_stride, int64_t rot, int interleaved,
                                     int dtype, int32_t* err, void* stream);
 int cie_rotary_tables(void* cos, void* sin, const int64_t* positions, const double* freqs,
-                      float scale, int64_t T, int64_t rot, int interleaved, int dtype,
+                      double scale, int64_t T, int64_t rot, int interleaved, int dtype,
                       void* stream);
 
 /*
