@@ -200,16 +200,21 @@ class KVStorage:
         """The end of a step that fed ``new_tokens[b]`` tokens to slot ``slot_ids[b]``: the tokens that come next, on the
         host, and held as the slots' last.  A step that reported anything leaves lengths, pages and last tokens as they
         were before it, and raises (``check_pages``)."""
+        held = self.last_generated[slot_ids]
+        self.last_generated[slot_ids] = next_tokens  # (behind the wait it would cost the step 10 us)
         *tokens, bits = torch.cat((next_tokens, self.page_err)).tolist()  # (one wait for both)
         if bits:
+            self.last_generated[slot_ids] = held
             self._drop_step(slot_ids, new_tokens)
             self.check_pages()
-        self.last_generated[slot_ids] = next_tokens
         return tokens
 
     def _drop_step(self, slot_ids: torch.Tensor, new_tokens: torch.Tensor) -> None:
-        """Gives back what some sequences of a step may have got, whose lengths were not advanced."""
+        """Lengths as before a step; of a pool that manages its pages, whose lengths were not advanced, what some of its
+        sequences may have got is given back."""
         if self.free_list is None:
+            self.lens[slot_ids] -= new_tokens
+            self.lens[self.unused_idx] = 0
             return
         fed = new_tokens > 0
         slot_ids, new_tokens = slot_ids[fed], new_tokens[fed]
@@ -293,14 +298,14 @@ class KVStorage:
     # lens[unused_idx] = 0 as a device kernel (a 1-element multiply), not a
     # host scalar copy, so a decode step that contains it can be graph-captured
     # (and no memset node lands in the graph).
-    # A step that reported anything does not count.
+    # In a pool that manages its pages a step that reported anything does not count, so that
+    # steps that follow it unseen find the same lengths.
     def decode_advance(self, slot_ids: torch.Tensor) -> None:
-        reports = self.free_list is not None or self.slot_adapters is not None
-        self.lens[slot_ids] += self.page_err == 0 if reports else 1
+        self.lens[slot_ids] += 1 if self.free_list is None else self.page_err == 0
         self.lens[self.unused_idx:self.unused_idx + 1].mul_(0)
 
     def mixed_advance(self, slot_ids: torch.Tensor, lens: torch.Tensor) -> None:
-        self.lens[slot_ids] += lens * (self.page_err == 0)
+        self.lens[slot_ids] += lens if self.free_list is None else lens * (self.page_err == 0)
         self.lens[self.unused_idx:self.unused_idx + 1].mul_(0)
 
     def reset(self, slot_ids: list[int]) -> None:
