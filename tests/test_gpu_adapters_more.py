@@ -92,3 +92,35 @@ def test_words_that_are_no_plan(T, word):
     note(f"no plan T={T} word={word}")
     cie.adapter_add_(y, x, a, b, scales, ranks, plan, (128,), err=err)
     assert int(err) == PLAN and torch.equal(y, kept)
+
+
+def test_a_plan_of_more_rows_than_a_wave_keeps():
+    """Past about a million rows a wave counts its rows anew when it writes them: the same order, each row once."""
+    T, n = 1_200_007, 37
+    g = torch.Generator().manual_seed(0)
+    row_slots = torch.randint(0, 90, (T,), generator=g)
+    row_slots[300_000:700_000] = 5  # (a long prompt's)
+    by_slot = torch.randint(-1, n, (90,), generator=g)
+    by_slot[5] = 11
+    err = err_word()
+    note(f"plan T={T} n={n}")
+    plan = cie.adapter_plan(row_slots.to(DEV), by_slot.to(DEV), n, err=err)
+    assert int(err) == 0
+    ids = by_slot[row_slots]
+    rows = torch.sort(ids, stable=True).indices[int((ids < 0).sum()):]
+    counts = torch.bincount(ids[ids >= 0], minlength=n)
+    tiles_of = (counts + 31) // 32
+    tiles = int(tiles_of.sum())
+    words = plan.cpu()
+    assert words[:4].tolist() == [tiles, T, n, 32]
+    got = words[8:8 + 36 * tiles].view(tiles, 36)
+    assert torch.equal(got[:, 0].long(), torch.repeat_interleave(torch.arange(n), tiles_of))
+    live = torch.arange(32) < got[:, 1:2]
+    assert torch.equal(got[:, 4:][live].long(), rows)
+    x, y = torch.randn(T, 8, generator=g).half(), torch.zeros(T, 8).half()
+    a, b = torch.randn(n, 1, 16, 8, generator=g).half(), torch.randn(n, 8, 16, generator=g).half()
+    ranks = torch.full((n,), 16, dtype=torch.int32)
+    out = cie.adapter_add_(y.to(DEV), x.to(DEV), a.to(DEV), b.to(DEV), torch.ones(n, device=DEV), ranks.to(DEV), plan, (8,))
+    some = torch.randint(0, T, (400,), generator=g)
+    want, off = ref.adapters(y[some], x[some], a, b, torch.ones(n), ids[some].tolist(), (8,))
+    assert ((out.cpu()[some].double() - want).abs() <= off + ref.rounding(want.abs() + off, F16)).all()
