@@ -571,8 +571,8 @@ __global__ __launch_bounds__(kAdThreads) void adapter_add_kernel(AddParams p) {
         char* const row = u_lds + (s * units * M + t) * L::kURow;
         float v[kHeld];
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i)
-          v[i] = i < units ? reinterpret_cast<const float*>(row + i * M * L::kURow)[q] : 0.f;
+        for (int i = 0; i < kHeld; ++i)  // (past the slice's units: its last again, so that all loads go at once)
+          v[i] = reinterpret_cast<const float*>(row + min(i, units - 1) * M * L::kURow)[q];
         int shift = 0;
         if constexpr (__is_same(E, f16)) {
           // The largest finite |u| of the row's slice decides its scale: an infinity stays one.
