@@ -141,11 +141,14 @@ def adapter_add_(y, x, a, b, scales, ranks, plan, slices, err=None):
         raise AssertionError("plan must come from adapter_plan for these rows and adapters")
     dev = one_device(y, x, a, b, scales, ranks, plan)
     if T:
-        a_ptr, b_ptr, s_ptr, r_ptr, p_ptr = (t.data_ptr() for t in (a, b, scales, ranks, plan))
-        for ptr, size in ((a_ptr, 2 * n * n_slices * R * d_in), (b_ptr, 2 * n * d_out * R), (s_ptr, 4 * n), (r_ptr, 4 * n),
-                          (p_ptr, 4 * held)):
-            if ptr < y_end and y_ptr < ptr + size and _share(y_ptr, 2 * y_row, 2 * d_out, T, ptr, size, size, 1):
-                raise AssertionError("a, b, scales, ranks and plan must not lie in y's memory")
+        a_ptr, b_ptr, s_ptr, r_ptr, p_ptr = a.data_ptr(), b.data_ptr(), scales.data_ptr(), ranks.data_ptr(), plan.data_ptr()
+        if (y_ptr < a_ptr + 2 * n * n_slices * R * d_in and a_ptr < y_end or y_ptr < b_ptr + 2 * n * d_out * R and b_ptr < y_end
+                or y_ptr < s_ptr + 4 * n and s_ptr < y_end or y_ptr < r_ptr + 4 * n and r_ptr < y_end
+                or y_ptr < p_ptr + 4 * held and p_ptr < y_end):  # (between y's rows, or in them)
+            for t in (a, b, scales, ranks, plan):
+                size = t.numel() * t.element_size()
+                if _share(y_ptr, 2 * y_row, 2 * d_out, T, t.data_ptr(), size, size, 1):
+                    raise AssertionError("a, b, scales, ranks and plan must not lie in y's memory")
         if T > 1 and x_row < d_in:
             xr = xr.contiguous()
             x_ptr, x_row = xr.data_ptr(), d_in

@@ -124,3 +124,21 @@ def test_a_plan_of_more_rows_than_a_wave_keeps():
     some = torch.randint(0, T, (400,), generator=g)
     want, off = ref.adapters(y[some], x[some], a, b, torch.ones(n), ids[some].tolist(), (8,))
     assert ((out.cpu()[some].double() - want).abs() <= off + ref.rounding(want.abs() + off, F16)).all()
+
+
+def test_weights_in_y_are_refused():
+    """A bank whose tensors lie in y's rows, and one between them, which is taken."""
+    room = torch.zeros(64 * 1024, dtype=F16, device=DEV)
+    y = room[:20 * 2048].view(20, 2048)[:, 100:164]
+    x, plan = torch.ones(20, 8).half().to(DEV), cie.adapter_plan(None, torch.zeros(20, dtype=torch.int64, device=DEV), 1)
+    scales, ranks = torch.ones(1, device=DEV), torch.full((1,), 16, dtype=torch.int32, device=DEV)
+    a, b = torch.ones(1, 1, 16, 8).half().to(DEV), torch.ones(1, 64, 16).half().to(DEV)
+    for lo in (0, 60, 163, 2048, 19 * 2048 + 40):
+        for bad in (dict(a=room[lo:lo + 128].view(1, 1, 16, 8)), dict(b=room[lo:lo + 1024].view(1, 64, 16))):
+            args = {**dict(a=a, b=b), **bad}
+            with pytest.raises(AssertionError, match="y's memory"):
+                cie.adapter_add_(y, x, args["a"], args["b"], scales, ranks, plan, (64,))
+    room[2048 + 200:2048 + 328] = 1.0  # (an A of ones between two rows)
+    between = room[2048 + 200:2048 + 328].view(1, 1, 16, 8)
+    cie.adapter_add_(y, x, between, b, scales, ranks, plan, (64,))
+    assert (y == 16 * 8).all() and (between == 1).all()
