@@ -206,7 +206,8 @@ def append_tokens_qkv_rotary(qkv, positions, frequencies, k_cache, v_cache, page
 
     Row t of ``qkv`` (1, T, (H_q + 2 H_kv) D) is turned by ``positions[t]``; its k and v
     go to ``(pages[t], :, offsets[t])`` of the 16-bit pools (qkv's type), and the turned
-    q is returned, (1, T, H_q, D).  Of rows with the same page and offset any one is kept.
+    q is returned, (1, T, H_q, D).  Rows with the same page and offset (padding's) leave some of
+    each: any value held there is one of theirs.
     """
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
         raise AssertionError("K/V pools must both be (n_pages, H_kv, page_size, D), with identical strides")

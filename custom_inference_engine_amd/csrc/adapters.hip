@@ -19,9 +19,10 @@
 // with y rounds once, as the plain form does.
 //
 // Bound by memory where rows are many: r <= 128 ranks are 2 r flops for each value of x
-// and y, far from what the matrix cores could do.  8,192 rows of 4,096 take 45.6 us at
-// rank 16 (4.4 TB/s) and 53 at 64 (a workgroup fills a CU's LDS, so that its reads of x
-// and its work on y take turns).  Few rows are bound by the stages in series, header ->
+// and y, far from what the matrix cores could do.  8,192 rows of 4,096 take 45.9 us at
+// rank 16 (4.4 TB/s), 54 at 64 and 80 at 128 (a workgroup fills a CU's LDS, so that its reads
+// of x and its work on y take turns); in bf16, with the third value's MFMAs, 45.9, 56.4 and
+// 84.  Few rows are bound by the stages in series, header ->
 // tile -> x and A -> sums -> y: 6.2 us for one row into three slices.
 #include "cie_common.h"
 
@@ -85,6 +86,8 @@ struct PlanParams {
 // does both at once, bound by a CU's loads and the rounds of its waves: 32 rows 4.0 us,
 // 1,052 rows 5.0, 8,192 rows of four prompts 9.1 (two launches 10.2), of eight adapters at
 // random 12.3 (10.8); 16,384 rows of four prompts 15.3 and 11.1, 65,536 rows 77 and 16.6.
+// (Prompts decide: thousands of rows are prompts, each with one adapter, as a decoding
+// request has a row or a few.)
 constexpr int64_t kPlanAlone = 8192;
 constexpr int kPlanGroups = 64;
 static inline int64_t group_rows(int64_t T) {

@@ -25,7 +25,7 @@
 // release's lengths) are changed by the last workgroup to arrive.
 // Times of one call, replayed from a graph: one row 2.9 us, 32 sequences and 1,056
 // rows 3.5 us, 496 sequences and 16,480 rows 4.2 us; with pages and their release
-// 6.1 us for one sequence, 8.0 for 32, 14.7 for 496 with 16,480 rows and 1,480 new pages.
+// 6.2 us for one sequence, 8.3 for 32, 14.9 for 496 with 16,480 rows and 1,480 new pages.
 #include "cie_common.h"
 
 namespace cie {
