@@ -275,13 +275,14 @@ def use_adapters(model, kv_cache, n_adapters: int, rank: int) -> list:
     banks = [b for layer in layers for b in (layer.qkv_adapters, layer.o_adapters) if b is not None]
     if any((b.n_adapters, b.rank) != (n_adapters, rank) for b in banks):
         raise AssertionError("the layers have banks of other sizes, which graphs may hold")
-    kv_cache.use_adapters(n_adapters)
-    if banks:  # (emptied where they stand)
-        for b in banks:
-            b.clear_all()
-        return layers
-    for layer in layers:
+    new = []
+    for layer in layers if not banks else ():
         w, o = layer.qkv_weight, layer.original.o_proj
-        layer.qkv_adapters = AdapterBank(n_adapters, rank, w.shape[1], layer.qkv_sizes, w.dtype, w.device)
-        layer.o_adapters = AdapterBank(n_adapters, rank, o.in_features, o.out_features, w.dtype, w.device)
+        new.append((AdapterBank(n_adapters, rank, w.shape[1], layer.qkv_sizes, w.dtype, w.device),
+                    AdapterBank(n_adapters, rank, o.in_features, o.out_features, w.dtype, w.device)))
+    kv_cache.use_adapters(n_adapters)  # (nothing has changed until here: what is refused leaves all as it was)
+    for b in banks:
+        b.clear_all()
+    for layer, pair in zip(layers, new):
+        layer.qkv_adapters, layer.o_adapters = pair
     return layers

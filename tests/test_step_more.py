@@ -186,3 +186,17 @@ def test_every_key_of_a_scaling_counts(scaling, d):
 def test_keys_that_are_not_understood_are_refused(base, scaling):
     with pytest.raises(AssertionError):
         cie.rotary_frequencies(64, base, scaling)
+
+
+def test_adapters_that_are_refused_leave_the_pool_alone():
+    cfg, model = _model()
+    kv = _pool(cfg)
+    for n, rank in ((2, 500), (2, 0), (5000, 8)):
+        with pytest.raises(AssertionError):
+            cie.use_adapters(model, kv, n, rank)
+        assert kv.slot_adapters is None and kv.n_adapters == 0
+    kv.use_adapters(2)
+    with pytest.raises(AssertionError):
+        cie.use_adapters(model, kv, 3, 8)
+    layer, = cie.use_adapters(model, kv, 2, 8)
+    assert layer.qkv_adapters.n_adapters == 2
