@@ -310,6 +310,7 @@ def use_rotary(model, frequencies, scale: float = 1.0, interleaved: bool = False
 
     ``rotary_frequencies`` makes them: a longer context than the model's own, part of the
     head (fewer pairs than head_dim / 2), or the interleaved layout of its checkpoint.
+    Comes before step modules and schedulers, whose graphs turn rows by what they found.
     """
     from .core import TritonQwen2Attention
 

@@ -34,10 +34,18 @@ from ..attn.metadata import AttentionMetadata
 from ..graphs import StepGraph, StepInputs
 
 
+def positions_of(model):
+    """The model's rotary embedding: a graph holds its tensors' addresses, so its module keeps it."""
+    return getattr(getattr(model, "model", None), "rotary_emb", None)
+
+
 def check_turned_on(module) -> None:
-    """The pool is what the module was made for: a step recorded before would not take pages, or leave adapters out."""
+    """Pool and model are what the module was made for: a step recorded before would not take pages, leave adapters out
+    or turn its rows by the positions of then."""
     if module.kv_cache.turned_on() != module.turned_on:
         raise RuntimeError("manage_pages and use_adapters come before the step modules")
+    if hasattr(module, "rotary_emb") and module.rotary_emb is not positions_of(module.model):
+        raise RuntimeError("use_rotary comes before the step modules")
 
 
 class DecodeModule:
@@ -56,7 +64,7 @@ class DecodeModule:
         self.metadata.slot_ids = self.slots
         self.tokens = torch.zeros((batch_size,), dtype=torch.long, device=dev)
         self.positions = torch.zeros((batch_size,), dtype=torch.long, device=dev)
-        self.turned_on = kv_cache.turned_on()
+        self.turned_on, self.rotary_emb = kv_cache.turned_on(), positions_of(model)
         self.managed = self.turned_on[0]  # the step takes its pages itself
         self.ones = torch.ones((batch_size,), dtype=torch.long, device=dev)
         with torch.inference_mode():

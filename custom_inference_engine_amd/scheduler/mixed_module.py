@@ -53,7 +53,7 @@ from ..attn.metadata import AttentionMetadata
 from ..graphs import StepGraph, StepInputs
 from ..kv_cache.pages import StepMaps
 from ..piecewise import get_piecewise_backend
-from .decode_module import check_turned_on
+from .decode_module import check_turned_on, positions_of
 
 
 class MixedModule:
@@ -185,6 +185,7 @@ class FullMixedModule(MixedModule):
     def __init__(self, model, kv_cache, batch_size: int, token_count: int, pool=None,
                  warmup_iters: int = 3):
         super().__init__(model, kv_cache, token_count, batch_size=batch_size)
+        self.rotary_emb = positions_of(model)
         with torch.inference_mode():
             self.step = StepGraph(self._step, pool=pool, warmup=warmup_iters, device=self.device)
 
@@ -207,6 +208,7 @@ class PiecewiseMixedModule(MixedModule):
     def __init__(self, model, kv_cache, token_count: int, buffer: torch.Tensor, pool=None,
                  batch_size: int | None = None):
         super().__init__(model, kv_cache, token_count, batch_size=batch_size)
+        self.rotary_emb = positions_of(model)
         self.backend = get_piecewise_backend(buffer[:, :token_count], pool)
         self.compiled = torch.compile(self._forward, backend=self.backend, fullgraph=True,
                                       dynamic=False)

@@ -225,3 +225,33 @@ def test_the_wrapped_modules_path_after_use_rotary(native_lib):
         for t, one in ((cos, 0), (sin, 1)):
             assert t.shape == (2, 3, D)
             assert torch.equal(t, torch.cat([cie.rotary_tables(r, ours.model.rotary_emb.frequencies)[one] for r in rows]))
+
+
+@pytest.mark.parametrize("kind", ["decode", "graph", "piecewise", "eager"])
+def test_other_positions_after_a_module_was_made(native_lib, kind):
+    """Recorded steps keep the frequencies that they read and are refused; an eager module turns by the new ones."""
+    torch._dynamo.reset()
+    cfg = _config()
+    theirs, ours = _models(cfg)
+    kv = _pool(cfg, pages=16)
+    use_rotary(ours, *cie.rotary_frequencies(D, 1e4))
+    mix = MixedModule(ours, kv, token_count=32)
+    if kind == "decode":
+        made = DecodeModule(ours, kv, batch_size=1)
+    elif kind == "graph":
+        made = FullMixedModule(ours, kv, batch_size=2, token_count=32)
+    elif kind == "piecewise":
+        made = PiecewiseMixedModule(ours, kv, token_count=32, buffer=torch.zeros(1, 32, H_Q, D, dtype=torch.float16, device=DEV))
+    first = ours.model.rotary_emb.frequencies.data_ptr()
+    use_rotary(ours, *cie.rotary_frequencies(D, 1e6))
+    note(f"other positions: {kind}")
+    prompt = _prompts(20)[0]
+    nxt = mix.forward([prompt], [1])
+    assert _rel(mix.last_logits[0], _logits(theirs, prompt)) < 2e-2
+    if kind == "eager":
+        return
+    assert made.rotary_emb.frequencies.data_ptr() == first
+    lens = kv.lens.clone()
+    with pytest.raises(RuntimeError, match="use_rotary"):
+        made.forward([1]) if kind == "decode" else made.forward([nxt], [1])
+    assert torch.equal(kv.lens, lens)
